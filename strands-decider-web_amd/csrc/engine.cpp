@@ -38,6 +38,15 @@ int fail(int code, const std::string& msg) {
   return code;
 }
 
+}  // namespace
+
+namespace ha {
+// the other host files' errors (kv_host.cpp) go to the same message
+int set_error(int code, const std::string& msg) { return fail(code, msg); }
+}  // namespace ha
+
+namespace {
+
 #define HA_HIP(expr)                                                                          \
   do {                                                                                        \
     hipError_t e_ = (expr);                                                                   \

@@ -42,6 +42,18 @@ class HaMnbFormat(ctypes.Structure):
     _fields_ = [("bits", ctypes.c_int), ("group", ctypes.c_int), ("asym", ctypes.c_int)]
 
 
+class HaKvConfig(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("n_layers", "n_pages", "page_size", "max_ctx", "HQ", "HK", "HD", "rot_dim",
+                                            "gated", "dtype")] + \
+               [("rope_theta", ctypes.c_float), ("eps", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
+class HaKvBatch(ctypes.Structure):
+    _fields_ = [("n_seqs", ctypes.c_int), ("n_rows", ctypes.c_int), ("max_rows", ctypes.c_int), ("max_len", ctypes.c_int),
+                ("row_start", ctypes.c_void_p), ("len", ctypes.c_void_p), ("pages", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int)]
+
+
 class HaForwardOpts(ctypes.Structure):
     _fields_ = [("recurrence", ctypes.c_int), ("timestamps", ctypes.c_int), ("sync", ctypes.c_int),
                 ("gpu_ms", ctypes.c_float), ("layer_ms", ctypes.POINTER(ctypes.c_float)),
@@ -89,6 +101,12 @@ def load_library(path=LIB_PATH):
         "ha_add_norm": ([i, i, i, vp, vp, vp, vp, i, vp, ctypes.c_float, i, vp], i),
         "ha_silu_mul": ([i, i, vp, vp, i, vp], i),
         "ha_add_bias": ([i, i, vp, vp, i, vp], i),
+        "ha_kv_page_bytes": ([ctypes.POINTER(HaKvConfig), ctypes.POINTER(sz)], i),
+        "ha_kv_create": ([ctypes.POINTER(HaKvConfig), vp, i, ctypes.POINTER(vp)], i),
+        "ha_kv_set_param": ([vp, i, ctypes.c_char_p, ctypes.POINTER(ctypes.c_float), sz], i),
+        "ha_kv_append": ([vp, i, ctypes.POINTER(HaKvBatch), vp, ctypes.c_long, vp, vp, vp], i),
+        "ha_kv_attention": ([vp, i, ctypes.POINTER(HaKvBatch), vp, vp, ctypes.c_long, vp, vp], i),
+        "ha_kv_destroy": ([vp], i),
         "ha_timer_create": ([i, i, ctypes.POINTER(vp)], i),
         "ha_timer_mark": ([vp, i, vp], i),
         "ha_timer_elapsed": ([vp, i, i, ctypes.POINTER(ctypes.c_float)], i),
@@ -306,6 +324,72 @@ def add_bias(L, N, y, c, device=0, stream=None):
     """y[t][j] += c[j] (y f16, c f32; wgsl.js:113-121)."""
     load_library()
     _check(_lib.ha_add_bias(L, N, _ptr(y), _ptr(c), device, _st(stream)))
+
+
+class KVBatch:
+    """A call's sequences on a :class:`PagedKV` (ha_kv_batch): int32 device arrays ``row_start`` [n_seqs + 1], ``lens``
+    [n_seqs] and ``pages`` [n_seqs][table_stride], and the host's bounds on them. The arrays are read when a call runs; this
+    object keeps a reference to them."""
+
+    def __init__(self, n_seqs, n_rows, max_rows, max_len, row_start, lens, pages, table_stride):
+        self._held = (row_start, lens, pages)
+        self.c = HaKvBatch(n_seqs, n_rows, max_rows, max_len, _ptr(row_start), _ptr(lens), _ptr(pages), table_stride)
+
+
+class PagedKV:
+    """A paged cache of 4-bit keys and values (ha_kv_*): ``pages`` is the device memory of [n_layers][n_pages] pages of
+    ``page_bytes`` bytes, which this object keeps a reference to. ``append`` puts a batch's fused rows into the cache and
+    gives the queries, ``attention`` reads it. Calls on one object must be ordered (one stream, or synchronised)."""
+
+    def __init__(self, pages, n_pages, page_size=64, n_layers=1, max_ctx=4096, HQ=8, HK=2, HD=256, rot_dim=64, gated=True,
+                 dtype=F16, rope_theta=1e7, eps=1e-6, scale=0.0, device=0):
+        lib = load_library()
+        self._h = None
+        self.cfg = HaKvConfig(n_layers, n_pages, page_size, max_ctx, HQ, HK, HD, rot_dim, int(bool(gated)), dtype,
+                              rope_theta, eps, scale)
+        h = ctypes.c_void_p()
+        _check(lib.ha_kv_create(ctypes.byref(self.cfg), _ptr(pages), device, ctypes.byref(h)))
+        self._h = h
+        self._borrowed = pages
+
+    @staticmethod
+    def page_bytes(page_size=64, HK=2, HD=256):
+        """Bytes of one page of one layer."""
+        lib = load_library()
+        c = HaKvConfig(1, 1, page_size, 1, HK, HK, HD, 0, 0, F16, 1.0, 1e-6, 0.0)
+        n = ctypes.c_size_t()
+        _check(lib.ha_kv_page_bytes(ctypes.byref(c), ctypes.byref(n)))
+        return n.value
+
+    def set_param(self, layer, name, values):
+        import numpy as np
+        a = np.ascontiguousarray(values, dtype=np.float32).ravel()
+        _check(_lib.ha_kv_set_param(self._h, layer, name.encode(), a.ctypes.data_as(ctypes.POINTER(ctypes.c_float)),
+                                    a.size))
+
+    def append(self, layer, batch, rows, row_stride, q=None, values=None, stream=None):
+        """Norm, rotate and store the batch's rows [n_rows][row_stride]; q [n_rows][HQ][HD] and values
+        [n_rows][2][HK][HD] (both f16, may be None) take the queries and the rows as the cache holds them."""
+        _check(_lib.ha_kv_append(self._h, layer, ctypes.byref(batch.c), _ptr(rows), row_stride, _ptr(q), _ptr(values),
+                                 _st(stream)))
+
+    def attention(self, layer, batch, q, rows, row_stride, out, stream=None):
+        """out [n_rows][HQ][HD] f16 = gated causal attention of q over the cache (rows, row_stride: the fused rows that
+        hold the gates; None, 0 without gates)."""
+        _check(_lib.ha_kv_attention(self._h, layer, ctypes.byref(batch.c), _ptr(q), _ptr(rows), row_stride, _ptr(out),
+                                    _st(stream)))
+
+    def close(self):
+        if self._h:
+            _check(_lib.ha_kv_destroy(self._h))
+            self._h = None
+            self._borrowed = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 class Timer:
