@@ -34,7 +34,8 @@ struct KvArgs {
 
 hipError_t launch_kv_rope(float* rope, const double* theta_pow, int max_ctx, int rot, hipStream_t s);
 hipError_t launch_kv_append(const KvArgs& a, hipStream_t s);
-hipError_t launch_kv_attention(const KvArgs& a, hipStream_t s);
+size_t kv_workspace_bytes();  // of partial results, whatever the call
+hipError_t launch_kv_attention(const KvArgs& a, void* ws, size_t ws_bytes, hipStream_t s);
 
 // Sets the calling thread's ha_last_error() message; returns the code.
 int set_error(int code, const std::string& msg);

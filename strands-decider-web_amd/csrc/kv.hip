@@ -9,49 +9,10 @@
 // channels of one group, so a lane that reads 8 bytes of a row has 4 channels of each group.
 #include <cmath>
 
-#include "kv.h"
+#include "kv_common.h"
 
 namespace ha {
 namespace {
-
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h4 __attribute__((ext_vector_type(4)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-
-// ---- a batch's sequences ----
-
-// Sequence b's rows [r0, r0 + n) and its context, positions [len - n, len) of which are the rows'. A sequence whose
-// numbers do not fit the call's (ok false) stores nothing; the rows of it that lie in the call come out as NaN.
-struct Seq {
-  int r0, n, len;
-  bool ok;
-};
-__device__ __forceinline__ Seq seq_of(const KvArgs& a, int b) {
-  const int r0 = a.row_start[b], r1 = a.row_start[b + 1], len = a.len[b];
-  Seq s;
-  s.ok = r0 >= 0 && r1 >= r0 && r1 <= a.n_rows && r1 - r0 <= a.max_rows && len >= r1 - r0 && len <= a.max_len;
-  s.r0 = min(max(r0, 0), a.n_rows);
-  s.n = min(min(max(r1, s.r0), a.n_rows) - s.r0, a.max_rows);
-  s.len = s.ok ? len : 0;
-  return s;
-}
-
-// The block of (sequence b, KV head, which) that holds token t, or nullptr where the table names no page of the pool.
-__device__ __forceinline__ unsigned char* block_of(const KvArgs& a, int b, int t, int kh, int which) {
-  const int p = a.table[(size_t)b * a.table_stride + (t >> a.page_log2)];
-  if ((unsigned)p >= (unsigned)a.n_pages) return nullptr;
-  return a.pool + (((size_t)p * a.HK + kh) * 2 + which) * kv_block_bytes(a.page, a.HD);
-}
-// f16 index of (token slot, group, 0: scale, 1: zero) among a block's parameters
-__device__ __forceinline__ int param_at(int slot, int g, int which) { return ((slot >> 2) * kKvGroups + g) * 8 + which * 4 + (slot & 3); }
-
-__device__ __forceinline__ f4 ld4(const float* p) { return *reinterpret_cast<const f4*>(p); }
-__device__ __forceinline__ f4 ld4(const _Float16* p) {
-  const h4 x = *reinterpret_cast<const h4*>(p);
-  return f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
-}
-__device__ __forceinline__ h4 to_h4(const f4& x) { return h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]}; }
 
 __global__ void kv_rope_kernel(float* rope, const double* theta_pow, int n, int half) {
   const long i = (long)blockIdx.x * 256 + threadIdx.x;
@@ -184,69 +145,6 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a) {
   }
 }
 
-// ---- attention ----
-
-// One wave per (row, query head): 64 keys at a time, a key a lane for the scores, then 4 (2) channels a lane for the values.
-template <int HD, typename T>
-__global__ __launch_bounds__(64) void kv_attend_kernel(KvArgs a) {
-  constexpr int kC = HD / 64;
-  __shared__ float ql[HD];
-  const int lane = threadIdx.x, h = blockIdx.y, i = blockIdx.x, b = blockIdx.z, kh = h / (a.HQ / a.HK);
-  const Seq sq = seq_of(a, b);
-  if (i >= sq.n) return;
-  const int t = sq.r0 + i, last = sq.len - sq.n + i;
-  for (int c = lane; c < HD; c += 64) ql[c] = (float)a.q[((size_t)t * a.HQ + h) * HD + c] * a.scale;
-  __syncthreads();
-  float m = -INFINITY, sum = 0.0f, o[kC] = {};
-  for (int j0 = 0; sq.ok && j0 <= last; j0 += 64) {
-    const int j = j0 + lane;
-    float sc = -INFINITY;
-    if (j <= last) {
-      const unsigned char* blk = block_of(a, b, j, kh, 0);
-      const int ps = j & (a.page - 1);
-      if (!blk) {
-        sc = __builtin_nanf("");
-      } else {
-        const _Float16* par = reinterpret_cast<const _Float16*>(blk + (size_t)a.page * (HD / 2));
-        const unsigned short* cd = reinterpret_cast<const unsigned short*>(blk + (size_t)ps * (HD / 2));
-        sc = 0.0f;
-        for (int g = 0; g < 4; g++) {
-          const float s = (float)par[param_at(ps, g, 0)], z = (float)par[param_at(ps, g, 1)];
-          for (int gi = 0; gi < HD / 16; gi++) {
-            const unsigned u = cd[4 * gi + g];
-            for (int e = 0; e < 4; e++) sc += ql[g * (HD / 4) + 4 * gi + e] * fmaf(s, (float)((int)((u >> (4 * e)) & 15u) - 8), z);
-          }
-        }
-      }
-    }
-    float mx = sc;
-    for (int d = 32; d >= 1; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d));
-    const float mn = fmaxf(m, mx), al = mn == m ? 1.0f : __expf(m - mn);
-    const float p = j <= last ? __expf(sc - (mn == -INFINITY ? 0.0f : mn)) : 0.0f;
-    sum = sum * al + xor_sum<64>(p);
-    for (int c = 0; c < kC; c++) o[c] *= al;
-    m = mn;
-    for (int k = 0; k < 64 && j0 + k <= last; k++) {
-      const float pk = __shfl(p, k);
-      const unsigned char* blk = block_of(a, b, j0 + k, kh, 1);
-      if (!blk) continue;  // (its score was NaN)
-      const int ps = (j0 + k) & (a.page - 1);
-      const _Float16* par = reinterpret_cast<const _Float16*>(blk + (size_t)a.page * (HD / 2));
-      for (int c = 0; c < kC; c++) {
-        const int ch = kC * lane + c, g = ch / (HD / 4), w = ch % (HD / 4), nib = 16 * (w / 4) + 4 * g + w % 4;
-        const int code = (blk[(size_t)ps * (HD / 2) + nib / 2] >> (4 * (nib & 1))) & 15;
-        o[c] += pk * fmaf((float)par[param_at(ps, g, 0)], (float)(code - 8), (float)par[param_at(ps, g, 1)]);
-      }
-    }
-  }
-  for (int c = 0; c < kC; c++) {
-    const int ch = kC * lane + c;
-    float v = sq.ok ? o[c] / sum : __builtin_nanf("");
-    if (a.gated) v /= 1.0f + __expf(-(float)static_cast<const T*>(a.rows)[(size_t)t * a.stride + (size_t)h * 2 * HD + HD + ch]);
-    a.out[((size_t)t * a.HQ + h) * HD + ch] = (_Float16)v;
-  }
-}
-
 }  // namespace
 
 hipError_t launch_kv_rope(float* rope, const double* theta_pow, int max_ctx, int rot, hipStream_t s) {
@@ -264,18 +162,6 @@ hipError_t launch_kv_append(const KvArgs& a, hipStream_t s) {
   } else {
     if (a.dtype == 0) hipLaunchKernelGGL((kv_append_kernel<128, float>), grid, block, 0, s, a);
     else hipLaunchKernelGGL((kv_append_kernel<128, _Float16>), grid, block, 0, s, a);
-  }
-  return hipGetLastError();
-}
-
-hipError_t launch_kv_attention(const KvArgs& a, hipStream_t s) {
-  const dim3 grid(a.max_rows, a.HQ, a.n_seqs), block(64);
-  if (a.HD == 256) {
-    if (a.dtype == 0) hipLaunchKernelGGL((kv_attend_kernel<256, float>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((kv_attend_kernel<256, _Float16>), grid, block, 0, s, a);
-  } else {
-    if (a.dtype == 0) hipLaunchKernelGGL((kv_attend_kernel<128, float>), grid, block, 0, s, a);
-    else hipLaunchKernelGGL((kv_attend_kernel<128, _Float16>), grid, block, 0, s, a);
   }
   return hipGetLastError();
 }

@@ -1,0 +1,55 @@
+// Shared by the kernels of the paged 4-bit K/V cache (kv.hip, kv_attn.hip), gfx950.
+#pragma once
+#include "kv.h"
+
+namespace ha {
+namespace {
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+// ---- a batch's sequences ----
+
+// Sequence b's rows [r0, r0 + n) and its context, positions [len - n, len) of which are the rows'. A sequence whose
+// numbers do not fit the call's (ok false) stores nothing; the rows of it that lie in the call come out as NaN.
+struct Seq {
+  int r0, n, len;
+  bool ok;
+};
+__device__ __forceinline__ Seq seq_of(const KvArgs& a, int b) {
+  const int r0 = a.row_start[b], r1 = a.row_start[b + 1], len = a.len[b];
+  Seq s;
+  s.ok = r0 >= 0 && r1 >= r0 && r1 <= a.n_rows && r1 - r0 <= a.max_rows && len >= r1 - r0 && len <= a.max_len;
+  s.r0 = min(max(r0, 0), a.n_rows);
+  s.n = min(min(max(r1, s.r0), a.n_rows) - s.r0, a.max_rows);
+  s.len = s.ok ? len : 0;
+  return s;
+}
+
+// The block of (sequence b, KV head, which) that holds token t, or nullptr where the table names no page of the pool.
+__device__ __forceinline__ unsigned char* block_of(const KvArgs& a, int b, int t, int kh, int which) {
+  const int p = a.table[(size_t)b * a.table_stride + (t >> a.page_log2)];
+  if ((unsigned)p >= (unsigned)a.n_pages) return nullptr;
+  return a.pool + (((size_t)p * a.HK + kh) * 2 + which) * kv_block_bytes(a.page, a.HD);
+}
+// f16 index of (token slot, group, 0: scale, 1: zero) among a block's parameters
+__device__ __forceinline__ int param_at(int slot, int g, int which) { return ((slot >> 2) * kKvGroups + g) * 8 + which * 4 + (slot & 3); }
+
+template <typename T>
+using gptr = const __attribute__((address_space(1))) T*;
+template <typename T>
+__device__ __forceinline__ gptr<T> gp(const void* p) { return (gptr<T>)(p); }
+template <typename T>
+__device__ __forceinline__ __attribute__((address_space(1))) T* gpw(void* p) { return (__attribute__((address_space(1))) T*)(p); }
+
+__device__ __forceinline__ f4 ld4(const float* p) { return *gp<f4>(p); }
+__device__ __forceinline__ f4 ld4(const _Float16* p) {
+  const h4 x = *gp<h4>(p);
+  return f4{(float)x[0], (float)x[1], (float)x[2], (float)x[3]};
+}
+__device__ __forceinline__ h4 to_h4(const f4& x) { return h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]}; }
+
+}  // namespace
+}  // namespace ha

@@ -61,6 +61,7 @@ struct ha_kv {
   size_t layer_bytes = 0;
   float* rope = nullptr;
   float* norms = nullptr;          // [n_layers][2][HD]: q_norm, k_norm
+  void* ws = nullptr;              // partial results of attention calls
 };
 
 namespace {
@@ -71,7 +72,7 @@ bool kv_ok(const ha_kv* k) {
 }
 
 void free_kv(ha_kv* k) {
-  for (void* p : {(void*)k->rope, (void*)k->norms})
+  for (void* p : {(void*)k->rope, (void*)k->norms, k->ws})
     if (p) (void)hipFree(p);
   k->magic = 0xdeadbeefu;
   delete k;
@@ -148,6 +149,7 @@ int ha_kv_create(const ha_kv_config* cfg, void* pages, int device, ha_kv** out) 
     const size_t nn = (size_t)cfg->n_layers * 2 * cfg->HD;
     const std::vector<float> ones(nn, 1.0f);
     if (hipMalloc(reinterpret_cast<void**>(&k->norms), nn * sizeof(float)) != hipSuccess) return bail(set_error(HA_ERR_NOMEM, "hipMalloc of the norms failed"));
+    if (hipMalloc(&k->ws, ha::kv_workspace_bytes()) != hipSuccess) return bail(set_error(HA_ERR_NOMEM, "hipMalloc of the workspace failed"));
     hipError_t he = hipMemcpy(k->norms, ones.data(), nn * sizeof(float), hipMemcpyHostToDevice);
     if (he != hipSuccess) return bail(hip_error("norms", he));
     if (cfg->rot_dim) {
@@ -212,7 +214,7 @@ int ha_kv_attention(ha_kv* k, int layer, const ha_kv_batch* batch, const void* q
   a.rows = rows; a.stride = row_stride; a.q = static_cast<_Float16*>(const_cast<void*>(q)); a.out = static_cast<_Float16*>(out);
   OnDevice on(k->device);
   if (on.rc != hipSuccess) return hip_error("hipSetDevice", on.rc);
-  const hipError_t he = ha::launch_kv_attention(a, static_cast<hipStream_t>(stream));
+  const hipError_t he = ha::launch_kv_attention(a, k->ws, ha::kv_workspace_bytes(), static_cast<hipStream_t>(stream));
   return he == hipSuccess ? HA_OK : hip_error("attention launch", he);
 }
 
