@@ -20,6 +20,8 @@ struct KvArgs {
   const int* len;        // [n_seqs]
   const int* table;      // [n_seqs][table_stride]
   int n_pages, page, page_log2, HQ, HK, HD, rot, gated, dtype;
+  int ratio;             // HQ / HK
+  unsigned ratio_inv;    // ceil(2^32 / ratio), 0 for 1
   float eps, scale;
   unsigned char* pool;   // the layer's pages
   const float* rope;     // [max_ctx][rot / 2] (cos, sin)
@@ -30,12 +32,14 @@ struct KvArgs {
   _Float16* q;           // [n_rows][HQ][HD]: written by append, read by attention
   _Float16* values;      // [n_rows][2][HK][HD] or nullptr
   _Float16* out;         // [n_rows][HQ][HD]
+  // x / ratio of 0 <= x < 2^28 (with ratio <= 16, x ratio_inv is less than 2^32 too large)
+  __host__ __device__ int by_ratio(int x) const { return ratio_inv ? (int)(((unsigned long long)(unsigned)x * ratio_inv) >> 32) : x; }
 };
 
 hipError_t launch_kv_rope(float* rope, const double* theta_pow, int max_ctx, int rot, hipStream_t s);
 hipError_t launch_kv_append(const KvArgs& a, hipStream_t s);
 size_t kv_workspace_bytes();  // of partial results, whatever the call
-hipError_t launch_kv_attention(const KvArgs& a, void* ws, size_t ws_bytes, hipStream_t s);
+hipError_t launch_kv_attention(const KvArgs& a, void* ws, hipStream_t s);
 
 // Sets the calling thread's ha_last_error() message; returns the code.
 int set_error(int code, const std::string& msg);

@@ -28,7 +28,8 @@ typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
 constexpr float kRaise = 8.0f;  // log2 headroom before a column's maximum is raised
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kCols = 16, kWaves = 4, kStep = 32;
+constexpr int kCols = 16, kWaves = 4, kStep = 32;  // few columns: of a workgroup; waves; keys a wave's step
+constexpr int kBigCols = 128, kTile = 32;          // many columns
 
 // x combined over the four lanes l, l ^ 16, l ^ 32, l ^ 48
 template <typename F>
@@ -48,6 +49,13 @@ __device__ __forceinline__ float sum_halves(float x) {
 }
 __device__ __forceinline__ float max_quads(float x) { return over_quads(x, [](float u, float v) { return fmaxf(u, v); }); }
 __device__ __forceinline__ float sum_quads(float x) { return over_quads(x, [](float u, float v) { return u + v; }); }
+
+// Orders a wave's LDS accesses before its later ones to other lanes' entries (no workgroup barrier).
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 // the low (high) half-words of u and v, u's first
 __device__ __forceinline__ unsigned halves(unsigned u, unsigned v, bool high) {
@@ -88,28 +96,204 @@ __device__ __forceinline__ f4 gate4(const KvArgs& a, int t, int h, int ch) {
 }
 __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
-// Partial results: for each (sequence, KV head, column block, piece, column) O (unnormalised) [HD], maximum, sum.
-struct Parts {
-  float* p;
-  int cols, ns;  // columns a block has, pieces
-  __device__ __forceinline__ float* column(const KvArgs& a, int ncb, int b, int kh, int cb, int piece, int c) const {
-    return p + ((((((size_t)b * a.HK + kh) * ncb + cb) * ns + piece) * cols) + c) * (a.HD + 4);
-  }
+// ---- who does what ----
+//
+// The host knows neither how long the sequences are nor which of them have many rows, so the device shares the work out. A
+// sequence has lo < columns <= hi of one of two kinds (few, many); its (column block, KV head)s are units. Units of few columns
+// are cut into pieces of `chunk` keys, chosen so that all of them make about `want` pieces; those of many columns, which are only
+// used where they fill the chip, are not. A workgroup's index is its place in the list of all pieces of all sequences, which
+// each wave finds by a prefix sum with a sequence a lane. A batch of more than kScanMost sequences with few columns, and one of
+// equal sequences with many, are laid out in a grid instead (`direct`), with the host's bounds.
+struct Kind {
+  float* p;  // results of the pieces of cut units: for each piece and column O (unnormalised) [HD], maximum, sum
+  int cols;  // columns a block has, at most
+  int lo, hi, want, direct, chunk, ncb, ns;
 };
+struct Item {
+  int b, kh, cb, piece, chunk, slot;  // slot: of the piece, where there is more than one
+  int row;                            // of the sequence (merge)
+  Seq sq;
+};
+constexpr int kScanMost = 128;
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }  // (for the compiler)
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, true); }
+template <int kCtrl, int kRows>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, kRows, 0xf, true));
+}
+// inclusive prefix sum over the wave
+template <typename F>
+__device__ __forceinline__ F scan64(F v) {
+  v = dpp_add<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+  v = dpp_add<0x112, 0xf>(v);
+  v = dpp_add<0x114, 0xf>(v);
+  v = dpp_add<0x118, 0xf>(v);
+  v = dpp_add<0x142, 0xa>(v);  // row_bcast 15, 31
+  return dpp_add<0x143, 0xc>(v);
+}
+__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+__device__ __forceinline__ Seq lane_value(const Seq& s, int lane) {
+  return Seq{lane_value(s.r0, lane), lane_value(s.n, lane), lane_value(s.len, lane), lane_value((int)s.ok, lane) != 0};
+}
+
+// a lane's sequence: its rows and units
+struct Lane {
+  Seq sq;
+  int ncb;
+};
+template <int BC>
+__device__ __forceinline__ Lane lane_of(const KvArgs& a, const Kind& k, int s) {
+  Lane l{};
+  if (s < a.n_seqs) {
+    l.sq = seq_of(a, s);
+    const int cols = l.sq.n * a.ratio;
+    if (cols > k.lo && cols <= k.hi) l.ncb = l.sq.ok ? (cols + BC - 1) / BC : 1;  // (one unit writes all rows of a sequence that does not fit)
+  }
+  return l;
+}
+__device__ __forceinline__ int pieces_of(int len, int chunk) { return len > chunk ? (len + chunk - 1) / chunk : 1; }
+constexpr int kUnit = kStep * kWaves;  // keys that a piece has at least
+// keys a piece: the units' keys over `want`
+__device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, const Lane& first, int lane) {
+  float w = (float)first.ncb * (float)first.sq.len;
+  for (int s0 = 64; s0 < a.n_seqs; s0 += 64) {
+    const Lane l = lane_of<kCols>(a, k, s0 + lane);
+    w += (float)l.ncb * (float)l.sq.len;
+  }
+  w = __builtin_bit_cast(float, lane_value(__builtin_bit_cast(int, scan64(w)), 63)) * (float)a.HK;
+  return uniform(kUnit * max(1, (int)fminf(ceilf(w / (float)(k.want * kUnit)), 1e6f)));
+}
+
+// Piece x of few columns, or false where there is none.
+__device__ __forceinline__ bool find_piece(const KvArgs& a, const Kind& k, int x, Item& it) {
+  const int lane = threadIdx.x & 63;
+  if (k.direct) {
+    it.b = blockIdx.z;
+    it.chunk = k.chunk;
+    it.sq = seq_of(a, it.b);
+    const int cols = it.sq.n * a.ratio;
+    it.piece = blockIdx.x;
+    it.kh = blockIdx.y / k.ncb;
+    it.cb = blockIdx.y - it.kh * k.ncb;
+    it.slot = ((it.b * a.HK + it.kh) * k.ncb + it.cb) * k.ns + it.piece;
+    return cols > k.lo && cols <= k.hi && it.cb * kCols < cols && (it.sq.ok || it.cb == 0);
+  }
+  Lane l = lane_of<kCols>(a, k, lane);
+  it.chunk = chunk_of(a, k, l, lane);
+  int base = 0, slots = 0;
+  for (int s0 = 0;; s0 += 64) {
+    if (s0) l = lane_of<kCols>(a, k, s0 + lane);
+    const int n = pieces_of(l.sq.len, it.chunk), items = l.ncb * n * a.HK, cut = n > 1 ? items : 0, sum = scan64(items), csum = scan64(cut);
+    const unsigned long long past = __ballot(base + sum > x);
+    if (past) {
+      const int at = __builtin_ctzll(past), rel = x - base - lane_value(sum, at) + lane_value(items, at), ns = lane_value(n, at);
+      it.b = s0 + at;
+      it.slot = slots + lane_value(csum, at) - lane_value(cut, at) + rel;
+      it.sq = lane_value(l.sq, at);
+      const int unit = uniform(rel / ns), row = uniform(unit / a.HK);
+      it.piece = rel - unit * ns;
+      it.kh = unit - row * a.HK;
+      it.cb = row;
+      return true;
+    }
+    base += lane_value(sum, 63);
+    slots += lane_value(csum, 63);
+    if (s0 + 64 >= a.n_seqs) return false;
+  }
+}
+// Column block x of many columns, or false where there is none: the last blocks, which have the most keys, first.
+__device__ __forceinline__ bool find_block(const KvArgs& a, const Kind& k, int x, Item& it) {
+  const int lane = threadIdx.x & 63;
+  if (k.direct) {  // a pair's workgroups share an XCD
+    const int pairs = a.n_seqs * a.HK, row = x / pairs, pair = x - row * pairs;
+    it.b = pair / a.HK;
+    it.kh = pair - it.b * a.HK;
+    it.cb = k.ncb - 1 - row;
+    it.sq = seq_of(a, it.b);
+    return it.cb * kBigCols < it.sq.n * a.ratio && (it.sq.ok || it.cb == 0);
+  }
+  for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+    const Lane l = lane_of<kBigCols>(a, k, s0 + lane);
+    const int all = lane_value(scan64(l.ncb), 63) * a.HK;
+    if (x >= all) {
+      x -= all;
+      continue;
+    }
+    for (int level = 0;; level++) {  // the last block of all 64 sequences, the last but one, ...
+      const unsigned long long has = __ballot(l.ncb > level);
+      const int n = __popcll(has) * a.HK;
+      if (x >= n) {
+        x -= n;
+        continue;
+      }
+      const int nth = uniform(x / a.HK), rank = __builtin_amdgcn_mbcnt_hi((unsigned)(has >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has, 0));
+      const int at = __builtin_ctzll(__ballot(l.ncb > level && rank == nth));
+      it.b = s0 + at;
+      it.kh = x - nth * a.HK;
+      it.cb = lane_value(l.ncb, at) - 1 - level;
+      it.sq = lane_value(l.sq, at);
+      return true;
+    }
+  }
+  return false;
+}
+// (row, head) x of the sequences of few columns that are cut, or false where there is none; it.slot: of its unit's first piece.
+__device__ __forceinline__ bool find_row(const KvArgs& a, const Kind& k, int x, int& h, Item& it) {
+  const int lane = threadIdx.x & 63;
+  int rel = x, ns = k.ns, slot = 0;
+  if (k.direct) {
+    it.b = blockIdx.y;
+    it.chunk = k.chunk;
+    it.sq = seq_of(a, it.b);
+    const int cols = it.sq.n * a.ratio;
+    if (cols <= k.lo || cols > k.hi || !it.sq.ok || rel >= it.sq.n * a.HQ) return false;
+  } else {
+    Lane l = lane_of<kCols>(a, k, lane);
+    it.chunk = chunk_of(a, k, l, lane);
+    int base = 0;
+    for (int s0 = 0;; s0 += 64) {
+      if (s0) l = lane_of<kCols>(a, k, s0 + lane);
+      const int n = pieces_of(l.sq.len, it.chunk), rows = n > 1 && l.ncb ? l.sq.n * a.HQ : 0, cut = n > 1 ? l.ncb * n * a.HK : 0;
+      const int sum = scan64(rows), csum = scan64(cut);
+      const unsigned long long past = __ballot(base + sum > x);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        it.b = s0 + at;
+        rel = x - base - lane_value(sum, at) + lane_value(rows, at);
+        slot += lane_value(csum, at) - lane_value(cut, at);
+        ns = lane_value(n, at);
+        it.sq = lane_value(l.sq, at);
+        break;
+      }
+      base += lane_value(sum, 63);
+      slot += lane_value(csum, 63);
+      if (s0 + 64 >= a.n_seqs) return false;
+    }
+  }
+  it.row = uniform(rel / a.HQ);
+  h = rel - it.row * a.HQ;
+  it.kh = a.by_ratio(h);
+  it.cb = (it.row * a.ratio + h - it.kh * a.ratio) / kCols;
+  it.slot = k.direct ? ((it.b * a.HK + it.kh) * k.ncb + it.cb) * k.ns : slot + (it.cb * a.HK + it.kh) * ns;
+  return true;
+}
+__device__ __forceinline__ float* column_of(const KvArgs& a, const Kind& k, int slot, int c) { return k.p + ((size_t)slot * k.cols + c) * (a.HD + 4); }
 
 // The rows of a sequence that does not fit its batch.
 template <int HD>
-__device__ __forceinline__ void nan_rows(const KvArgs& a, const Seq& sq, int kh, int c0, int cols, int threads) {
-  const int ratio = a.HQ / a.HK;
-  for (int k = threadIdx.x; k < cols * HD; k += threads) {
-    const int r = c0 + k / HD;
-    a.out[((size_t)(sq.r0 + r / ratio) * a.HQ + kh * ratio + r % ratio) * HD + k % HD] = (_Float16)__builtin_nanf("");
+__device__ __forceinline__ void nan_rows(const KvArgs& a, const Seq& sq, int kh, int threads) {
+  const _Float16 x = (_Float16)__builtin_nanf("");
+  for (int r = threadIdx.x / (HD / 4); r < sq.n * a.ratio; r += threads / (HD / 4)) {
+    const int i = a.by_ratio(r);
+    *gpw<h4>(a.out + ((size_t)(sq.r0 + i) * a.HQ + kh * a.ratio + r - i * a.ratio) * HD + 4 * (threadIdx.x % (HD / 4))) = h4{x, x, x, x};
   }
 }
 // Channels ch .. + 3 of column r: O / l, the gate, f16.
 template <int HD>
 __device__ __forceinline__ void finish(const KvArgs& a, const Seq& sq, int kh, int r, int ch, f4 v, float inv) {
-  const int ratio = a.HQ / a.HK, t = sq.r0 + r / ratio, h = kh * ratio + r % ratio;
+  const int i = a.by_ratio(r), t = sq.r0 + i, h = kh * a.ratio + r - i * a.ratio;
   v *= inv;
   if (a.gated) {
     const f4 gt = gate4(a, t, h, ch);
@@ -120,47 +304,95 @@ __device__ __forceinline__ void finish(const KvArgs& a, const Seq& sq, int kh, i
 }
 
 template <int HD>
-__global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, int chunk, int ncb, Parts parts) {
+__global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind kind) {
   constexpr int G = HD / 4, kH = HD / 128, kE = HD / 64, kRow = HD / 2;
   constexpr int kPitch = HD + 4;
-  __shared__ float ol[kWaves * kCols * kPitch];
+  __shared__ __attribute__((aligned(16))) float ol[kWaves * (kCols / 2) * kPitch];
   __shared__ float ml[kWaves][kCols][2];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, j = lane & 15, kg = lane >> 4;
-  const int ratio = a.HQ / a.HK;
-  // the last column blocks first: they have the most keys; (sequence, KV head) pairs cycle fastest, so that the workgroups of
-  // a pair share an XCD and its cache
-  int id = blockIdx.x;
-  const int pairs = a.n_seqs * a.HK, pair = id % pairs;
-  id /= pairs;
-  const int piece = id % parts.ns, cb = ncb - 1 - id / parts.ns, b = pair / a.HK, kh = pair % a.HK;
-  const int k0 = piece * chunk;
-  const int* table = a.table + (size_t)b * a.table_stride;
-  const int page_log2 = a.page_log2, top_page = a.table_stride - 1;
-  // lane k: the page of tokens k0 + 1024 seg + 16 k .. + 15
-  int ids = gp<int>(table)[min((k0 + 16 * lane) >> page_log2, top_page)], seg = 0;
-  const Seq sq = seq_of(a, b);
-  const int c0 = cb * kCols, cols = min(kCols, sq.n * ratio - c0);
-  if (cols <= 0) return;
+  const int ratio = a.ratio;
+  Item it;
+  if (!find_piece(a, kind, blockIdx.x, it)) return;
+  const Seq sq = it.sq;
+  const int kh = it.kh, b = it.b, k0 = it.piece * it.chunk, c0 = it.cb * kCols, cols = min(kCols, sq.n * ratio - c0);
   if (!sq.ok) {
-    if (piece == 0) nan_rows<HD>(a, sq, kh, c0, cols, 64 * kWaves);
+    if (it.piece == 0) nan_rows<HD>(a, sq, kh, 64 * kWaves);
     return;
   }
+  const int* table = a.table + (size_t)b * a.table_stride;
+  const int page_log2 = a.page_log2, top_page = a.table_stride - 1;
+  int ids = gp<int>(table)[min((k0 + 16 * lane) >> page_log2, top_page)];  // lane k: the page of tokens seg + 16 k .. + 15
   const int before = sq.len - sq.n;
-  const int keys = before + (c0 + cols - 1) / ratio + 1, ns = (keys + chunk - 1) / chunk;
-  if (piece >= ns) return;
-  const int k1 = min(k0 + chunk, keys);
-  const int all = before + c0 / ratio + 1;  // keys below this are seen by every column
-  const int r = c0 + min(j, cols - 1), last = before + r / ratio;  // columns behind the last one repeat it
+  const int keys = before + a.by_ratio(c0 + cols - 1) + 1;
+  if (k0 >= keys) return;
+  const int k1 = min(k0 + it.chunk, keys);
+  const int all = before + a.by_ratio(c0) + 1;  // keys below this are seen by every column
+  const int r = c0 + min(j, cols - 1), ri = a.by_ratio(r), last = before + ri;  // columns behind the last one repeat it
   h8 q[kH][4];
-  float qs[4], qc[4];  // over each group: sum of the column's q, and what the codes' offsets add to its products
-  const Magic mg;
   {
-    const _Float16* qp = a.q + ((size_t)(sq.r0 + r / ratio) * a.HQ + kh * ratio + r % ratio) * HD + 8 * kg;
+    const _Float16* qp = a.q + ((size_t)(sq.r0 + ri) * a.HQ + kh * ratio + r - ri * ratio) * HD + 8 * kg;
 #pragma unroll
     for (int h = 0; h < kH; h++)
 #pragma unroll
       for (int g = 0; g < 4; g++) q[h][g] = *gp<h8>(qp + G * g + 32 * h);
   }
+  // A step's 32 keys are two tiles of 16, each in one page. Its codes wait in registers: K's of the next step are fetched when
+  // the scores are done, V's when the outputs are. The parameters (16 bytes a lane: tile and K or V, key quad, group) go through
+  // the wave's part of LDS, where each lane finds those of its keys.
+  const size_t blk_bytes = kv_block_bytes(a.page, HD);
+  const unsigned par_off = (unsigned)a.page * kRow;
+  u4 kc[2][kH], pr;
+  u2 vc[2][4];
+  bool gone[2];
+  const unsigned char* blk[2];
+  int slot[2];
+  auto locate = [&](int seg, int t0) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      int page = __builtin_amdgcn_readlane(ids, ((t0 - seg) / 16 + i) & 63);
+      if (t0 + 16 * i >= k1) page = 0;  // (behind the last key: any page)
+      gone[i] = (unsigned)page >= (unsigned)a.n_pages;
+      blk[i] = a.pool + ((size_t)(gone[i] ? 0 : page) * a.HK + kh) * 2 * blk_bytes;
+      slot[i] = (t0 + 16 * i) & (a.page - 1);
+    }
+  };
+  auto fetch_k = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int h = 0; h < kH; h++) kc[i][h] = *gp<u4>(blk[i] + (unsigned)((slot[i] + j) * kRow + 64 * h + 16 * kg));
+    const bool second = lane & 16;
+    pr = *gp<u4>((second ? blk[1] : blk[0]) + (lane & 32 ? blk_bytes : 0) + par_off + (unsigned)((second ? slot[1] : slot[0]) * kKvParamBytes + 16 * (lane & 15)));
+  };
+  auto fetch_v = [&]() {
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+        vc[i][k] = *gp<u2>(blk[i] + blk_bytes + (unsigned)((slot[i] + 4 * kg + k) * kRow + 8 * (HD == 256 ? j : j & 7)));
+  };
+  unsigned char* params = reinterpret_cast<unsigned char*>(ol + wave * (kCols / 2) * kPitch);
+  auto put_params = [&](int t0) {
+    const bool lost = lane & 16 ? gone[1] : gone[0];
+    // beyond the sequence, and in no page: parameters of any bits (a score of no page is NaN)
+    if (lost) pr = lane & 32 ? u4{} : u4{0x7E007E00u, 0x7E007E00u, 0u, 0u};
+    if (t0 + kStep > keys) {
+      const int t = t0 + (lane & 16) + (lane & 12);
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (t + e >= keys) {
+          pr[e >> 1] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+          pr[2 + (e >> 1)] &= e & 1 ? 0x0000FFFFu : 0xFFFF0000u;
+        }
+    }
+    *reinterpret_cast<u4*>(params + 16 * lane) = pr;
+    wave_sync();
+  };
+  locate(k0, k0 + kStep * wave);  // (a wave without keys: any page)
+  fetch_k();
+  fetch_v();
+  const Magic mg;
+  float qs[4], qc[4];  // over each group: sum of the column's q, and what the codes' offsets add to its products
 #pragma unroll
   for (int g = 0; g < 4; g++) {
     float s0 = 0.0f, s1 = 0.0f;
@@ -180,51 +412,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, int ch
     qc[g] = -1032.0f * s0 - 72.0f * s1;
   }
   const float scale = a.scale * kLog2e;
-  f4 o[4][kE], zs[4];
-  float m = -INFINITY, sum = 0.0f;
+  f4 o[4][kE], zs = {};  // zs[g]: sum P z_g (row 4 i + g of A is group g's zeros)
+  float m = -INFINITY, sum = 0.0f, cs[4] = {};  // cs[g]: the lane's part of -24 sum P s_g
 #pragma unroll
-  for (int g = 0; g < 4; g++) {
-    zs[g] = f4{};
+  for (int g = 0; g < 4; g++)
 #pragma unroll
     for (int e = 0; e < kE; e++) o[g][e] = f4{};
-  }
-  const size_t blk_bytes = kv_block_bytes(a.page, HD);
-  const unsigned par_off = (unsigned)a.page * kRow;
 
-  for (int t0 = k0 + kStep * wave; t0 < k1; t0 += kStep * kWaves) {
-    if ((t0 - k0) >> 10 != seg) {
-      seg = (t0 - k0) >> 10;
-      ids = gp<int>(table)[min((k0 + 1024 * seg + 16 * lane) >> page_log2, top_page)];
-    }
-    // this step's 32 keys: two tiles of 16, each in one page (any page for a tile behind the last key)
-    const unsigned char* blk[2];
-    int slot[2];
-    bool gone[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-      int page = __builtin_amdgcn_readlane(ids, ((t0 - k0) & 1023) / 16 + i);
-      if (t0 + 16 * i >= k1) page = 0;
-      gone[i] = (unsigned)page >= (unsigned)a.n_pages;
-      blk[i] = a.pool + ((size_t)(gone[i] ? 0 : page) * a.HK + kh) * 2 * blk_bytes;
-      slot[i] = (t0 + 16 * i) & (a.page - 1);
-    }
-    u4 kc[2][kH], kp[2][4], vp[2][4];
-    u2 vc[2][4];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-#pragma unroll
-      for (int h = 0; h < kH; h++) kc[i][h] = *gp<u4>(blk[i] + (unsigned)((slot[i] + j) * kRow + 64 * h + 16 * kg));
-#pragma unroll
-      for (int g = 0; g < 4; g++) kp[i][g] = *gp<u4>(blk[i] + par_off + (unsigned)((slot[i] + 4 * kg) * kKvParamBytes + 16 * g));
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-#pragma unroll
-      for (int k = 0; k < 4; k++)
-        vc[i][k] = *gp<u2>(blk[i] + blk_bytes + (unsigned)((slot[i] + 4 * kg + k) * kRow + 8 * (HD == 256 ? j : j & 7)));
-#pragma unroll
-      for (int g = 0; g < 4; g++) vp[i][g] = *gp<u4>(blk[i] + blk_bytes + par_off + (unsigned)((slot[i] + 4 * kg) * kKvParamBytes + 16 * g));
-    }
+  // The keys t0 .. t0 + 31. `more`: the wave's next step is one of the segment's (a template argument: with a branch the compiler
+  // would not know how many loads are in flight, and wait for all of them).
+  auto step = [&](int seg, int t0, auto more_c) {
+    constexpr bool more = decltype(more_c)::value;
+    put_params(t0);
+    const u4* par = reinterpret_cast<const u4*>(params) + 4 * kg;  // [tile and K or V: 16][group]
     // scores of tokens t0 + 16 i + 4 kg + k
     float sc[2][4];
 #pragma unroll
@@ -237,32 +437,24 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, int ch
           const u4 op = codes_k(mg, halves(kc[i][h][g >> 1], kc[i][h][(g >> 1) + 2], g & 1));
           acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, op), q[h][g], acc, 0, 0, 0);
         }
-        const h8 p = __builtin_bit_cast(h8, kp[i][g]);
+        const h8 p = __builtin_bit_cast(h8, par[16 * i + g]);
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           const float z = g ? fmaf((float)p[4 + k], qs[g], sc[i][k]) : (float)p[4 + k] * qs[g];
           sc[i][k] = fmaf((float)p[k], acc[k], z);
         }
       }
-    const bool edge = t0 + kStep > all || gone[0] || gone[1];
+    if constexpr (more) {
+      locate(seg, t0 + kStep * kWaves);
+      fetch_k();
+    }
+    const bool edge = t0 + kStep > all;
     if (edge) {
 #pragma unroll
       for (int i = 0; i < 2; i++)
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-          const int tok = t0 + 16 * i + 4 * kg + k;
-          if (gone[i]) sc[i][k] = __builtin_nanf("");
-          if (tok > last) sc[i][k] = -INFINITY;
-          // beyond the sequence, and in no page: scales and zeros of any bits
-          if (tok >= keys || gone[i]) {
-            const unsigned clear = k & 1 ? 0x0000FFFFu : 0xFFFF0000u;
-#pragma unroll
-            for (int g = 0; g < 4; g++) {
-              vp[i][g][k >> 1] &= clear;
-              vp[i][g][2 + (k >> 1)] &= clear;
-            }
-          }
-        }
+        for (int k = 0; k < 4; k++)
+          if (t0 + 16 * i + 4 * kg + k > last) sc[i][k] = -INFINITY;
     }
     float mx = -INFINITY;
 #pragma unroll
@@ -272,13 +464,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, int ch
     mx = max_quads(mx) * scale;
     const float mn = mx > m + kRaise ? mx : m;
     if (__any(mn != m)) {
-      const float al = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-      sum *= al;
+      if (__any(m != -INFINITY)) {  // (else O is zero)
+        const float al = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        sum *= al;
+        zs *= al;
 #pragma unroll
-      for (int g = 0; g < 4; g++) {
-        zs[g] *= al;
+        for (int g = 0; g < 4; g++) {
+          cs[g] *= al;
 #pragma unroll
-        for (int e = 0; e < kE; e++) o[g][e] *= al;
+          for (int e = 0; e < kE; e++) o[g][e] *= al;
+        }
       }
       m = mn;
     }
@@ -294,12 +489,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, int ch
         sum += p0 + p1;
         p[2 * i + k / 2] = as_u(h2{(_Float16)p0, (_Float16)p1});
       }
-    const _Float16 off = (_Float16)-24.0f;
+    {
+      const u2 z0 = reinterpret_cast<const u2*>(par + 32 + (j & 3))[1], z1 = reinterpret_cast<const u2*>(par + 48 + (j & 3))[1];
+      zs = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, u4{z0[0], z0[1], z1[0], z1[1]}), __builtin_bit_cast(h8, p), zs, 0, 0, 0);
+    }
+    const h2 off = {(_Float16)-24.0f, (_Float16)-24.0f};
 #pragma unroll
     for (int g = 0; g < 4; g++) {
+      const u2 vs[2] = {*reinterpret_cast<const u2*>(par + 32 + g), *reinterpret_cast<const u2*>(par + 48 + g)};
       u4 w;  // P s_g
 #pragma unroll
-      for (int k = 0; k < 4; k++) w[k] = scale2(sc[k >> 1][2 * (k & 1)], sc[k >> 1][2 * (k & 1) + 1], vp[k >> 1][g][k & 1]);
+      for (int k = 0; k < 4; k++) w[k] = scale2(sc[k >> 1][2 * (k & 1)], sc[k >> 1][2 * (k & 1) + 1], vs[k >> 1][k & 1]);
       if (edge) {  // a masked token's scale may be NaN
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -308,9 +508,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, int ch
         }
       }
       const h8 wh = __builtin_bit_cast(h8, w);
-      const u4 z = {vp[0][g][2], vp[0][g][3], vp[1][g][2], vp[1][g][3]};
-      zs[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, z), __builtin_bit_cast(h8, p), zs[g], 0, 0, 0);
-      zs[g] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h8{off, off, off, off, off, off, off, off}, wh, zs[g], 0, 0, 0);
+#pragma unroll
+      for (int k = 0; k < 4; k++) cs[g] = __builtin_amdgcn_fdot2(as_h2(w[k]), off, cs[g], false);
       unsigned x[4];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
@@ -323,128 +522,213 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, int ch
         o[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, op), wh, o[g][e], 0, 0, 0);
       }
     }
+    if constexpr (more) fetch_v();
+    wave_sync();  // (the parameters' place is used again)
+  };
+  for (int seg = k0;;) {  // segments of 1024 keys, whose pages the lanes hold
+    const int end = min(seg + 1024, k1);
+    int t0 = seg + kStep * wave;
+#pragma clang loop unroll(disable)
+    for (; t0 + kStep * kWaves < end; t0 += kStep * kWaves) step(seg, t0, std::true_type{});
+    if (t0 < end) step(seg, t0, std::false_type{});
+    seg += 1024;
+    if (seg >= k1) break;
+    ids = gp<int>(table)[min((seg + 16 * lane) >> page_log2, top_page)];
+    locate(seg, seg + kStep * wave);
+    fetch_k();
+    fetch_v();
   }
   // the four waves' sums: O^T row 4 kg + k of (g, e) is channel G g + 16 kg + 4 k + e (HD 256), G g + 4 (row & 7) + 2 (row >> 3) + e
   // (HD 128)
   sum = sum_quads(sum);
+#pragma unroll
+  for (int g = 0; g < 4; g++) zs[g] += sum_quads(cs[g]);
   if (kg == 0) {
     ml[wave][j][0] = m;
     ml[wave][j][1] = sum;
   }
-  if (j < cols) {
-    float* d = ol + (wave * kCols + j) * kPitch;
+  for (int h0 = 0; h0 < cols; h0 += kCols / 2) {  // half of the columns at a time (LDS)
+    if (h0) __syncthreads();
+    if (j >= h0 && j < min(h0 + kCols / 2, cols)) {
+      float* d = ol + (wave * (kCols / 2) + j - h0) * kPitch;
 #pragma unroll
-    for (int g = 0; g < 4; g++)
+      for (int g = 0; g < 4; g++)
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        if constexpr (HD == 256) {
-          *reinterpret_cast<f4*>(d + G * g + 16 * kg + 4 * k) = f4{o[g][0][k], o[g][1][k], o[g][2][k], o[g][3][k]} + zs[g][k];
-        } else {
-          const int ii = 4 * kg + k;
-          *reinterpret_cast<float2*>(d + G * g + 4 * (ii & 7) + 2 * (ii >> 3)) = float2{o[g][0][k] + zs[g][k], o[g][1][k] + zs[g][k]};
+        for (int k = 0; k < 4; k++) {
+          if constexpr (HD == 256) {
+            *reinterpret_cast<f4*>(d + G * g + 16 * kg + 4 * k) = f4{o[g][0][k], o[g][1][k], o[g][2][k], o[g][3][k]} + zs[g];
+          } else {
+            const int ii = 4 * kg + k;
+            *reinterpret_cast<float2*>(d + G * g + 4 * (ii & 7) + 2 * (ii >> 3)) = float2{o[g][0][k] + zs[g], o[g][1][k] + zs[g]};
+          }
         }
-      }
-  }
-  __syncthreads();
-  for (int k = tid; k < cols * (HD / 4); k += 64 * kWaves) {
-    const int c = k / (HD / 4), ch = 4 * (k % (HD / 4));
-    float mm = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) mm = fmaxf(mm, ml[w][c][0]);
-    f4 v = {};
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) {
-      const float f = ml[w][c][0] == mm ? 1.0f : __builtin_amdgcn_exp2f(ml[w][c][0] - mm);
-      l += f * ml[w][c][1];
-      v += f * *reinterpret_cast<const f4*>(ol + (w * kCols + c) * kPitch + ch);
     }
-    if (ns > 1) {
-      float* s = parts.column(a, ncb, b, kh, cb, piece, c);
-      *gpw<f4>(s + ch) = v;
-      if (ch == 0) {
-        s[HD] = mm;
-        s[HD + 1] = l;
+    __syncthreads();
+    for (int k = tid; k < min(kCols / 2, cols - h0) * (HD / 4); k += 64 * kWaves) {
+      const int c = h0 + k / (HD / 4), ch = 4 * (k % (HD / 4));
+      float mm = -INFINITY, l = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) mm = fmaxf(mm, ml[w][c][0]);
+      f4 v = {};
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        const float f = ml[w][c][0] == mm ? 1.0f : __builtin_amdgcn_exp2f(ml[w][c][0] - mm);
+        l += f * ml[w][c][1];
+        v += f * *reinterpret_cast<const f4*>(ol + (w * (kCols / 2) + c - h0) * kPitch + ch);
       }
-    } else {
-      finish<HD>(a, sq, kh, c0 + c, ch, v, 1.0f / l);
+      if (keys > it.chunk) {
+        float* s = column_of(a, kind, it.slot, c);
+        *gpw<f4>(s + ch) = v;
+        if (ch == 0) {
+          s[HD] = mm;
+          s[HD + 1] = l;
+        }
+      } else {
+        finish<HD>(a, sq, kh, c0 + c, ch, v, 1.0f / l);
+      }
     }
   }
 }
 
 // ---- many columns ----
 
-constexpr int kBigCols = 128, kTile = 32;
 typedef float f16v __attribute__((ext_vector_type(16)));
 
 // LDS of kv_many_kernel, each part twice: K tile [32][HD] and V^T tile [HD][32] as f16 (rows 16 bytes longer, so that eight rows
-// of an operand lie in different banks), K's scales [4][32] and zeros [32][4] twice each, V's scales and zeros [4][32], P f32 in
-// the lanes' order, the columns' factors and the waves' flags.
+// of an operand lie in different banks), K's scales [4][32] and zeros [32][4] twice each, P f32 in the lanes' order, the columns'
+// factors and the waves' flags; V's scales and zeros [4][32] each of four tiles.
 template <int HD>
 struct ManyLds {
   static constexpr int kKPitch = HD * 2 + 16, kVPitch = kTile * 2 + 16;
-  static constexpr int kKs = kTile * kKPitch, kKz = kKs + 256, kV = kKz + 512, kVs = kV + HD * kVPitch, kVz = kVs + 256, kP = kVz + 256;
+  static constexpr int kKs = kTile * kKPitch, kKz = kKs + 256, kV = kKz + 512, kP = kV + HD * kVPitch;
   static constexpr int kAl = kP + kBigCols * kTile * 4, kFlag = kAl + kBigCols * 4, kBuf = kFlag + 16;
+  static constexpr int kParam = 2 * kBuf, kAll = kParam + 4 * 512;
 };
 
 // A workgroup has 128 columns and walks the keys in tiles of 32. Four of its eight waves compute P (32 columns each: S^T = K Q^T on
-// v_mfma_f32_32x32x16_f16, scales and zeros, online softmax), the other four the outputs of the tile before (64 columns and half
-// the channels each: O^T = V^T P^T) and unpack the next codes, as f16 numbers c - 8, into LDS; each SIMD has one of either
-// kind, so the matrix products of the one run beside the vector instructions of the other. One barrier a tile. Scales and
-// zeros stay apart from the codes, so that both operands are exact: S = sum_g s_g (q . (c - 8))_g + sum_g z_g sum(q_g), the last
+// v_mfma_f32_32x32x16_f16, scales and zeros, online softmax) and unpack the next tile's keys into LDS, the other four the outputs
+// of the tile before (64 columns and half the channels each: O^T = V^T P^T) and this tile's values; each SIMD has one of either
+// kind, so the matrix products of the one run beside the vector instructions of the other. One barrier a tile. Scales and zeros
+// stay apart from the codes, so that both operands are exact: S = sum_g s_g (q . (c - 8))_g + sum_g z_g sum(q_g), the last
 // as one more product (with sum(q_g) / G as two f16), and O takes P s_g, rounded to f16 once, and sum P z_g.
 template <int HD>
-__global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, int chunk, int ncb, Parts parts) {
+__global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
   constexpr int G = HD / 4, U = HD / 16, kRow = HD / 2, kKs = G / 16, kDt = HD / 64;  // kKs: k-steps of a group; kDt: 32-row blocks of V^T a wave
   typedef ManyLds<HD> M;
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c32 = lane & 31, half = lane >> 5;
-  const int ratio = a.HQ / a.HK;
-  int id = blockIdx.x;  // (the order of kv_attend_kernel)
-  const int pairs = a.n_seqs * a.HK, pair = id % pairs;
-  id /= pairs;
-  const int piece = id % parts.ns, cb = ncb - 1 - id / parts.ns, b = pair / a.HK, kh = pair % a.HK;
-  const Seq sq = seq_of(a, b);
-  const int c0 = cb * kBigCols, cols = min(kBigCols, sq.n * ratio - c0);
-  if (cols <= 0) return;
+  const int ratio = a.ratio;
+  Item it;
+  if (!find_block(a, kind, blockIdx.x, it)) return;
+  const Seq sq = it.sq;
+  const int kh = it.kh, b = it.b, c0 = it.cb * kBigCols, cols = min(kBigCols, sq.n * ratio - c0);
   if (!sq.ok) {
-    if (piece == 0) nan_rows<HD>(a, sq, kh, c0, cols, 512);
+    nan_rows<HD>(a, sq, kh, 512);
     return;
   }
-  const int before = sq.len - sq.n, keys = before + (c0 + cols - 1) / ratio + 1, ns = (keys + chunk - 1) / chunk;
-  if (piece >= ns) return;
-  const int k0 = piece * chunk, k1 = min(k0 + chunk, keys), tiles = (k1 - k0 + kTile - 1) / kTile;
-  const int all = before + c0 / ratio + 1;  // keys below this are seen by every column
+  const int before = sq.len - sq.n, keys = before + a.by_ratio(c0 + cols - 1) + 1;
+  const int tiles = (keys + kTile - 1) / kTile;
+  const int all = before + a.by_ratio(c0) + 1;  // keys below this are seen by every column
   const float scale = a.scale * kLog2e;
-  float* stats = reinterpret_cast<float*>(lds);  // after the last tile: [128] maxima, [128] sums
+  float* stats = reinterpret_cast<float*>(lds);  // after the last tile: the columns' sums
+
+  // the codes: a wave of either kind takes its quarter of a tile's keys (values)
+  const int u = tid & 255;
+  const size_t blk_bytes = kv_block_bytes(a.page, HD);
+  const int* table = a.table + (size_t)b * a.table_stride;
+  const unsigned par_off = (unsigned)a.page * kRow;
+  const int page_log2 = a.page_log2, top_page = a.table_stride - 1;
+  int ids = 0;  // lane k: the page of tokens 1024 seg + 16 k .. + 15, seg that of the tile fetched last
+  // the block (K: 0, V: 1) of the half of the tile at t0 that `second` says, and whether its page is none; a half behind the last
+  // key lies in any page
+  auto block_at = [&](int t0, bool second, int which, bool& gone) {
+    const int n = (t0 & 1023) / 16;
+    int p0 = __builtin_amdgcn_readlane(ids, n), p1 = __builtin_amdgcn_readlane(ids, n + 1);
+    p0 = t0 < keys ? p0 : 0;
+    p1 = t0 + 16 < keys ? p1 : 0;
+    const int p = second ? p1 : p0;
+    gone = (unsigned)p >= (unsigned)a.n_pages;
+    return a.pool + ((size_t)(gone ? 0 : p) * a.HK + kh) * 2 * blk_bytes + which * blk_bytes;
+  };
+  auto load_ids = [&](int t0) {
+    if ((t0 & 1023) == 0) ids = gp<int>(table)[min((t0 + 16 * lane) >> page_log2, top_page)];
+  };
+  const Magic mg;
 
   if (wave < 4) {
     // ---- P of columns 32 wave .. + 31 ----
-    const int w0 = 32 * wave, r = c0 + min(w0 + c32, cols - 1), last = before + r / ratio;
+    const int kkey = HD == 256 ? u >> 3 : (u >> 2) & 31, kpos = HD == 256 ? u & 7 : u & 3;
+    const bool unpacks = HD == 256 || u < 128;
+    // two keys' parameters of K or of V: word pdw of key quad pquad: (g, s or z, key pair)
+    const int pwhich = u >> 7, pquad = (u >> 4) & 7, pdw = u & 15, pg = pdw >> 2, ppart = (pdw >> 1) & 1, pkey = 4 * pquad + 2 * (pdw & 1);
+    u4 raw = {};
+    unsigned praw = 0;
+    bool pgone = false;
+    auto fetch = [&](int t0) {
+      load_ids(t0);
+      bool gone;
+      const unsigned char* p = block_at(t0, kkey >= 16, 0, gone);
+      if (unpacks) raw = *gp<u4>(p + (unsigned)(((t0 + kkey) & (a.page - 1)) * kRow + 16 * kpos));
+      p = block_at(t0, pquad >= 4, pwhich, pgone) + par_off;
+      praw = *gp<unsigned>(p + (unsigned)(((t0 + 4 * pquad) & (a.page - 1)) * kKvParamBytes + 4 * pdw));
+    };
+    auto unpack = [&](int t0, unsigned char* buf) {
+      if (unpacks) {
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+          *reinterpret_cast<u4*>(buf + kkey * M::kKPitch + 16 * ((G / 8) * g + kpos)) = codes_k(mg, halves(raw[g >> 1], raw[(g >> 1) + 2], g & 1));
+      }
+      // behind the sequence, and in no page: parameters of any bits (a score of no page is NaN)
+      unsigned w = pgone ? (pwhich || ppart ? 0u : 0x7E007E00u) : praw;
+      if (t0 + pkey >= keys) w = 0;
+      else if (t0 + pkey + 1 >= keys) w &= 0xFFFFu;
+      if (pwhich) {
+        *reinterpret_cast<unsigned*>(lds + M::kParam + ((t0 / kTile) & 3) * 512 + ppart * 256 + pg * 64 + pkey * 2) = w;
+      } else {
+        if (ppart) {
+          *reinterpret_cast<unsigned*>(buf + M::kKz + pkey * 16 + 4 * pg) = (w & 0xFFFFu) * 0x10001u;
+          *reinterpret_cast<unsigned*>(buf + M::kKz + pkey * 16 + 16 + 4 * pg) = (w >> 16) * 0x10001u;
+        } else {
+          *reinterpret_cast<unsigned*>(buf + M::kKs + pg * 64 + pkey * 2) = w;
+        }
+      }
+    };
+    const int w0 = 32 * wave, r = c0 + min(w0 + c32, cols - 1), ri = a.by_ratio(r), last = before + ri;
     const bool idle = w0 >= cols;
+    fetch(0);
     // the B operand of k-step ks of group g is channels G g + 16 ks + 8 half .. + 7, in the order of K's chunks
     h8 q[4][kKs], qz;
+    f16v qc[4];  // what the codes' offsets add to a column's products, in every row
     {
-      const _Float16* qp = a.q + ((size_t)(sq.r0 + r / ratio) * a.HQ + kh * ratio + r % ratio) * HD + 8 * half;
+      const _Float16* qp = a.q + ((size_t)(sq.r0 + ri) * a.HQ + kh * ratio + r - ri * ratio) * HD + 8 * half;
 #pragma unroll
       for (int g = 0; g < 4; g++)
 #pragma unroll
         for (int ks = 0; ks < kKs; ks++) q[g][ks] = *gp<h8>(qp + G * g + 16 * ks);
 #pragma unroll
       for (int g = 0; g < 4; g++) {
-        float s = 0.0f;
+        float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
         for (int ks = 0; ks < kKs; ks++) {
           const h8 x = q[g][ks];
 #pragma unroll
-          for (int e = 0; e < 8; e++) s += (float)x[e];
+          for (int e = 0; e < 8; e += 2) {
+            s0 += (float)x[e];
+            s1 += (float)x[e + 1];
+          }
           q[g][ks] = h8{x[0], x[4], x[1], x[5], x[2], x[6], x[3], x[7]};
         }
-        s = sum_halves(s) * (1.0f / G);
+        s0 = sum_halves(s0);
+        s1 = sum_halves(s1);
+        qc[g] = f16v{} + (-1032.0f * s0 - 72.0f * s1);
+        const float s = (s0 + s1) * (1.0f / G);
         const _Float16 hi = (_Float16)s;
         qz[2 * g] = half ? (_Float16)0.0f : hi;
         qz[2 * g + 1] = half ? (_Float16)0.0f : (_Float16)(s - (float)hi);
       }
     }
+    unpack(0, lds);
+    if (tiles > 1) fetch(kTile);
     float m = -INFINITY, sum = 0.0f;
     // S^T row i holds key pi(i) (bits 2 and 3 of i swapped): the lane's values 8 kb .. 8 kb + 7 are then keys 16 kb + 8 half .. + 7,
     // which is P^T's operand of k-step kb
@@ -452,16 +736,16 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, int chunk, in
     __syncthreads();
 #pragma unroll 1
     for (int i = 0; i <= tiles; i++) {
+      const int t0 = kTile * i;
+      unsigned char* buf = lds + (i & 1) * M::kBuf;
       if (i < tiles && !idle) {
-        const int t0 = k0 + kTile * i;
-        unsigned char* buf = lds + (i & 1) * M::kBuf;
         const unsigned char* kr = buf + pr * M::kKPitch + 16 * half;
         f16v st = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8*>(buf + M::kKz + pr * 16), qz, f16v{}, 0, 0, 0);
 #pragma unroll
         for (int v = 0; v < 16; v++) st[v] *= (float)G;
 #pragma unroll
         for (int g = 0; g < 4; g++) {
-          f16v acc = f16v{};
+          f16v acc = qc[g];
 #pragma unroll
           for (int ks = 0; ks < kKs; ks++)
             acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(*reinterpret_cast<const h8*>(kr + 16 * ((G / 8) * g + 2 * ks)), q[g][ks], acc, 0, 0, 0);
@@ -472,7 +756,7 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, int chunk, in
             for (int e = 0; e < 8; e++) st[8 * kb + e] = fmaf((float)s[e], acc[8 * kb + e], st[8 * kb + e]);
           }
         }
-        if (t0 + kTile > all || t0 + kTile > k1) {
+        if (t0 + kTile > all) {
           const int tok = t0 + 8 * half;
 #pragma unroll
           for (int v = 0; v < 16; v++) st[v] = tok + 16 * (v >> 3) + (v & 7) <= last ? st[v] : -INFINITY;
@@ -503,146 +787,127 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, int chunk, in
           pl[64 * k] = p;
         }
       }
+      if (i + 1 < tiles) {
+        unpack(t0 + kTile, lds + ((i + 1) & 1) * M::kBuf);
+        if (i + 2 < tiles) fetch(t0 + 2 * kTile);
+      }
       __syncthreads();
     }
     sum = sum_halves(sum);
-    if (half == 0) {
-      stats[w0 + c32] = m;
-      stats[kBigCols + w0 + c32] = sum;
-    }
+    if (half == 0) stats[w0 + c32] = sum;
     __syncthreads();
     return;
   }
 
   // ---- outputs of columns 64 cp .. + 63 and groups 2 dh, 2 dh + 1 ----
-  const int u = tid - 256, cp = wave & 1, dh = (wave >> 1) & 1;
+  const int cp = wave & 1, dh = (wave >> 1) & 1;
   const bool idle = 64 * cp >= cols;
-  const size_t blk_bytes = kv_block_bytes(a.page, HD);
-  const int* table = a.table + (size_t)b * a.table_stride;
-  const unsigned par_off = (unsigned)a.page * kRow;
-  // what this thread unpacks: 16 bytes of a key, 4 bytes of four keys' values, two keys' parameters of K or of V
+  const int vquad = HD == 256 ? u >> 5 : (u >> 4) & 7, vpos = HD == 256 ? u & 31 : u & 15;  // 4 bytes of four keys' values
   const bool unpacks = HD == 256 || u < 128;
-  const int kkey = HD == 256 ? u >> 3 : (u >> 2) & 31, kpos = HD == 256 ? u & 7 : u & 3;
-  const int vquad = HD == 256 ? u >> 5 : (u >> 4) & 7, vpos = HD == 256 ? u & 31 : u & 15;
-  const int pwhich = u >> 7, pquad = (u >> 4) & 7, pdw = u & 15;  // parameter word pdw of key quad pquad: (g, s or z, key pair)
-  auto block_at = [&](int tok, bool& gone) {
-    const int p = gp<int>(table)[min(tok, keys - 1) >> a.page_log2];
-    gone = (unsigned)p >= (unsigned)a.n_pages;
-    return a.pool + ((size_t)(gone ? 0 : p) * a.HK + kh) * 2 * blk_bytes;
-  };
-  u4 kraw = {}, vraw = {};
-  unsigned praw = 0;
-  bool pgone = false;
-  // K of the tile at tk, V of the tile at tv
-  auto fetch = [&](int tk, int tv) {
+  u4 raw = {};
+  auto fetch = [&](int t0) {
+    load_ids(t0);
     bool gone;
+    const unsigned char* p = block_at(t0, vquad >= 4, 1, gone) + (unsigned)(((t0 + 4 * vquad) & (a.page - 1)) * kRow + 4 * vpos);
     if (unpacks) {
-      kraw = *gp<u4>(block_at(tk + kkey, gone) + (unsigned)(((tk + kkey) & (a.page - 1)) * kRow + 16 * kpos));
-      const unsigned char* p = block_at(tv + 4 * vquad, gone) + blk_bytes + (unsigned)(((tv + 4 * vquad) & (a.page - 1)) * kRow + 4 * vpos);
 #pragma unroll
-      for (int k = 0; k < 4; k++) vraw[k] = *gp<unsigned>(p + k * kRow);
+      for (int k = 0; k < 4; k++) raw[k] = *gp<unsigned>(p + k * kRow);
     }
-    const int tok = (pwhich ? tv : tk) + 4 * pquad;
-    praw = *gp<unsigned>(block_at(tok, pgone) + pwhich * blk_bytes + par_off + (unsigned)((tok & (a.page - 1)) * kKvParamBytes + 4 * pdw));
   };
-  const Magic mg;
   const h2 m24 = {(_Float16)-24.0f, (_Float16)-24.0f};
-  auto unpack = [&](int tk, int tv, unsigned char* kb, unsigned char* vb) {
+  auto unpack = [&](unsigned char* buf) {
     if (unpacks) {
-#pragma unroll
-      for (int g = 0; g < 4; g++) {
-        const unsigned x = halves(kraw[g >> 1], kraw[(g >> 1) + 2], g & 1);
-        u4 w;
-#pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = as_u(as_h2(code_v(mg, x, e)) + m24);
-        *reinterpret_cast<u4*>(kb + kkey * M::kKPitch + 16 * ((G / 8) * g + kpos)) = w;
-      }
 #pragma unroll
       for (int gg = 0; gg < 2; gg++) {
-        const unsigned x0 = halves(vraw[0], vraw[1], gg), x1 = halves(vraw[2], vraw[3], gg);
+        const unsigned x0 = halves(raw[0], raw[1], gg), x1 = halves(raw[2], raw[3], gg);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const u2 w = {as_u(as_h2(code_v(mg, x0, e)) + m24), as_u(as_h2(code_v(mg, x1, e)) + m24)};
           const int R = 4 * U * (2 * (vpos & 1) + gg) + U * e + (vpos >> 1);
-          *reinterpret_cast<u2*>(vb + M::kV + R * M::kVPitch + 8 * vquad) = w;
+          *reinterpret_cast<u2*>(buf + M::kV + R * M::kVPitch + 8 * vquad) = w;
         }
       }
     }
-    const int g = pdw >> 2, part = (pdw >> 1) & 1, key = 4 * pquad + 2 * (pdw & 1), t0 = pwhich ? tv : tk;
-    // behind the sequence, and in no page: parameters of any bits (a score of no page is NaN)
-    unsigned w = pgone ? (pwhich == 0 && part == 0 ? 0x7E007E00u : 0u) : praw;
-    if (t0 + key >= keys) w = 0;
-    else if (t0 + key + 1 >= keys) w &= 0xFFFFu;
-    if (pwhich) {
-      *reinterpret_cast<unsigned*>(vb + (part ? M::kVz : M::kVs) + g * 64 + key * 2) = w;
-    } else if (part) {
-      *reinterpret_cast<unsigned*>(kb + M::kKz + key * 16 + 4 * g) = (w & 0xFFFFu) * 0x10001u;
-      *reinterpret_cast<unsigned*>(kb + M::kKz + key * 16 + 16 + 4 * g) = (w >> 16) * 0x10001u;
-    } else {
-      *reinterpret_cast<unsigned*>(kb + M::kKs + g * 64 + key * 2) = w;
-    }
   };
-  f16v o[2][kDt], zacc[2];
+  f16v o[2][kDt];
+  float zs[2][2] = {};  // the lane's part of sum P z_g
   int last[2];
 #pragma unroll
   for (int n = 0; n < 2; n++) {
-    last[n] = before + (c0 + min(64 * cp + 32 * n + c32, cols - 1)) / ratio;
-    zacc[n] = f16v{};
+    last[n] = before + a.by_ratio(c0 + min(64 * cp + 32 * n + c32, cols - 1));
 #pragma unroll
     for (int d = 0; d < kDt; d++) o[n][d] = f16v{};
   }
-  fetch(k0, k0);
-  unpack(k0, k0, lds, lds);
-  fetch(k0 + kTile, k0);
+  fetch(0);
   __syncthreads();
-  // step i: P of tile i, outputs of tile i - 1; K of tile i + 1 and V of tile i go to LDS (while the other waves are busy with their
-  // products), the next codes are fetched (K's behind the last tile: any)
+  // step i: the values of tile i are unpacked (while the other waves compute its P), the outputs take tile i - 1
 #pragma unroll 1
   for (int i = 0; i <= tiles; i++) {
-    if (i < tiles) {
-      unpack(k0 + kTile * (i + 1), k0 + kTile * i, lds + ((i + 1) & 1) * M::kBuf, lds + (i & 1) * M::kBuf);
-      if (i + 1 < tiles) fetch(k0 + kTile * (i + 2), k0 + kTile * (i + 1));
-    }
-    if (i > 0 && !idle) {
-      const int t0 = k0 + kTile * (i - 1);
-      const unsigned char* buf = lds + ((i - 1) & 1) * M::kBuf;
+    const bool takes = i > 0 && !idle;
+    const int t0 = kTile * (i - 1);
+    const unsigned char* buf = lds + ((i & 1) ^ 1) * M::kBuf;
+    // what the outputs need first is on its way while the codes are unpacked
+    f4 p[2][4];
+    u4 ps[2][2], pz[2][2];
+    bool f0 = false, f1 = false;
+    const unsigned char* par = lds + M::kParam + ((i - 1) & 3) * 512 + 16 * half;
+    if (takes) {
       const int* flag = reinterpret_cast<const int*>(buf + M::kFlag) + 2 * cp;
-      const bool f0 = flag[0], f1 = flag[1] && 64 * cp + 32 < cols;
+      f0 = flag[0];
+      f1 = flag[1] && 64 * cp + 32 < cols;
+      const f4* pl = reinterpret_cast<const f4*>(buf + M::kP) + 2 * cp * 256 + lane;
+#pragma unroll
+      for (int k = 0; k < 4; k++)
+#pragma unroll
+        for (int n = 0; n < 2; n++) p[n][k] = pl[256 * n + 64 * k];
+#pragma unroll
+      for (int kb = 0; kb < 2; kb++)
+#pragma unroll
+        for (int gg = 0; gg < 2; gg++) {
+          ps[kb][gg] = *reinterpret_cast<const u4*>(par + (2 * dh + gg) * 64 + 32 * kb);
+          pz[kb][gg] = *reinterpret_cast<const u4*>(par + 256 + (2 * dh + gg) * 64 + 32 * kb);
+        }
+    }
+    if (i < tiles) {
+      unpack(lds + (i & 1) * M::kBuf);
+      if (i + 1 < tiles) fetch(kTile * (i + 1));
+    }
+    if (takes) {
       if (f0 || f1) {
 #pragma unroll
         for (int n = 0; n < 2; n++) {
           const float al = (n ? f1 : f0) ? *reinterpret_cast<const float*>(buf + M::kAl + 4 * (64 * cp + 32 * n + c32)) : 1.0f;
-          zacc[n] *= al;
+          zs[n][0] *= al;
+          zs[n][1] *= al;
 #pragma unroll
           for (int d = 0; d < kDt; d++) o[n][d] *= al;
         }
       }
-      const bool edge = t0 + kTile > all || t0 + kTile > k1;
-      const f4* pl = reinterpret_cast<const f4*>(buf + M::kP) + 2 * cp * 256 + lane;
+      const bool edge = t0 + kTile > all;
       const unsigned char* vr = buf + M::kV + (2 * dh * G + c32) * M::kVPitch + 16 * half;
 #pragma unroll
       for (int kb = 0; kb < 2; kb++) {
-        f4 p[2][2];
+        unsigned ph[2][4];
 #pragma unroll
         for (int n = 0; n < 2; n++)
 #pragma unroll
-          for (int k = 0; k < 2; k++) p[n][k] = pl[256 * n + 64 * (2 * kb + k)];
-        const h8 z = *reinterpret_cast<const h8*>(buf + M::kVz + (2 * dh + (c32 & 1)) * 64 + 32 * kb + 16 * half);
-#pragma unroll
-        for (int n = 0; n < 2; n++) {
-          const h8 ph = {(_Float16)p[n][0][0], (_Float16)p[n][0][1], (_Float16)p[n][0][2], (_Float16)p[n][0][3],
-                         (_Float16)p[n][1][0], (_Float16)p[n][1][1], (_Float16)p[n][1][2], (_Float16)p[n][1][3]};
-          zacc[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(z, ph, zacc[n], 0, 0, 0);
-        }
+          for (int k = 0; k < 4; k++) {
+            const f4 x = p[n][2 * kb + (k >> 1)];
+            ph[n][k] = as_u(h2{(_Float16)x[2 * (k & 1)], (_Float16)x[2 * (k & 1) + 1]});
+          }
 #pragma unroll
         for (int gg = 0; gg < 2; gg++) {
-          const u4 s = *reinterpret_cast<const u4*>(buf + M::kVs + (2 * dh + gg) * 64 + 32 * kb + 16 * half);
+          const u4 s = ps[kb][gg];
+#pragma unroll
+          for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) zs[n][gg] = __builtin_amdgcn_fdot2(as_h2(ph[n][k]), as_h2(pz[kb][gg][k]), zs[n][gg], false);
           h8 wh[2];
 #pragma unroll
           for (int n = 0; n < 2; n++) {
             u4 w;
 #pragma unroll
-            for (int k = 0; k < 4; k++) w[k] = scale2(p[n][k >> 1][2 * (k & 1)], p[n][k >> 1][2 * (k & 1) + 1], s[k]);
+            for (int k = 0; k < 4; k++) w[k] = scale2(p[n][2 * kb + (k >> 1)][2 * (k & 1)], p[n][2 * kb + (k >> 1)][2 * (k & 1) + 1], s[k]);
             if (edge) {  // a masked token's scale may be NaN
 #pragma unroll
               for (int k = 0; k < 4; k++) {
@@ -669,10 +934,10 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, int chunk, in
 #pragma unroll
   for (int n = 0; n < 2; n++) {
     const int c = 64 * cp + 32 * n + c32;
+    const float zz[2] = {sum_halves(zs[n][0]), sum_halves(zs[n][1])};
     if (c >= cols) continue;
-    const float mm = stats[c], l = stats[kBigCols + c], inv = 1.0f / l;
+    const float inv = 1.0f / stats[c];
     // O^T row rho of dt is V^T row R = 32 dt + rho: channel G g + 4 i + e with R = 4 U g + U e + i
-    float* pp = ns > 1 ? parts.column(a, ncb, b, kh, cb, piece, c) : nullptr;
 #pragma unroll
     for (int gg = 0; gg < 2; gg++)
 #pragma unroll
@@ -686,44 +951,36 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, int chunk, in
           i = 4 * half + k;
           v = f4{o[n][gg][k], o[n][gg][k + 4], o[n][gg][k + 8], o[n][gg][k + 12]};
         }
-        v += zacc[n][gg];
+        v += zz[gg];
         const int ch = G * (2 * dh + gg) + 4 * i;
-        if (ns > 1) {
-          *gpw<f4>(pp + ch) = v;
-        } else {
-          finish<HD>(a, sq, kh, c0 + c, ch, v, inv);
-        }
+        finish<HD>(a, sq, kh, c0 + c, ch, v, inv);
       }
-    if (ns > 1 && half == 0 && dh == 0) {
-      pp[HD] = mm;
-      pp[HD + 1] = l;
-    }
   }
 }
 
 // out of one (row, head) from its pieces: thread (k, c) adds pieces k, k + blockDim / (HD / 4), ... of channels 4 c .. + 3.
 constexpr int kMergeMost = 2048;  // pieces
 template <int HD>
-__global__ __launch_bounds__(1024) void kv_merge_kernel(KvArgs a, int chunk, int ncb, int block_cols, Parts parts) {
+__global__ __launch_bounds__(1024) void kv_merge_kernel(KvArgs a, Kind kind) {
   constexpr int C = HD / 4;
   __shared__ float wl[kMergeMost], red[2][16];
   __shared__ f4 vl[1024];
-  const int tid = threadIdx.x, i = blockIdx.x, h = blockIdx.y, b = blockIdx.z, ratio = a.HQ / a.HK, kh = h / ratio;
-  const Seq sq = seq_of(a, b);
-  if (i >= sq.n || !sq.ok) return;
-  const int col = i * ratio + h % ratio, cb = col / block_cols, c = col % block_cols;
-  const int end = min(block_cols, sq.n * ratio - cb * block_cols);
-  const int keys = sq.len - sq.n + (cb * block_cols + end - 1) / ratio + 1, ns = (keys + chunk - 1) / chunk;
+  const int tid = threadIdx.x;
+  Item it;
+  int h;
+  if (!find_row(a, kind, blockIdx.x, h, it)) return;
+  const Seq sq = it.sq;
+  const int t = sq.r0 + it.row, c = it.row * a.ratio + h - it.kh * a.ratio - it.cb * kCols, end = min((it.cb + 1) * kCols, sq.n * a.ratio);
+  const int keys = sq.len - sq.n + a.by_ratio(end - 1) + 1, ns = pieces_of(keys, it.chunk);
   if (ns <= 1) return;
-  const float* p = parts.column(a, ncb, b, kh, cb, 0, c);
-  const size_t step = (size_t)parts.cols * (HD + 4);
+  const float* p = column_of(a, kind, it.slot, c);
+  const size_t step = (size_t)kind.cols * (HD + 4);
   const int k = tid / C, n = blockDim.x / C, ch = 4 * (tid % C), wave = tid >> 6, waves = blockDim.x >> 6;
   // the first pieces' O and the gate go out before the maxima are waited for
   constexpr int kAhead = 4;
   f4 ahead[kAhead];
 #pragma unroll
   for (int x = 0; x < kAhead; x++) ahead[x] = ld4(p + min(k + x * n, ns - 1) * step + ch);
-  const int t = sq.r0 + i;
   const f4 gt = a.gated && k == 0 ? gate4(a, t, h, ch) : f4{};
   float mm = -INFINITY, l = 0.0f, mine[kMergeMost / 256], suml[kMergeMost / 256];
   const int per = (ns + (int)blockDim.x - 1) / (int)blockDim.x;
@@ -775,53 +1032,65 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvArgs a, int chunk, int
   *gpw<h4>(a.out + ((size_t)t * a.HQ + h) * HD + ch) = to_h4(v);
 }
 
-// The pieces of a call of `units` (column block, KV head, sequence): `want` workgroups in all, of at least `unit` keys each, as
-// long as the pieces' results fit the workspace.
-int pieces(long units, int max_len, int want, int unit, size_t unit_bytes, size_t ws_bytes, int* chunk) {
-  long c = std::max<long>((units * max_len / want + unit - 1) / unit * unit, unit);
-  while ((max_len + c - 1) / c > 1 && ((size_t)units * ((max_len + c - 1) / c) * unit_bytes > ws_bytes || (max_len + c - 1) / c > kMergeMost)) c *= 2;
-  *chunk = (int)std::min<long>(c, 1 << 30);
-  return (int)((max_len + c - 1) / c);
-}
+// Which kernel serves a sequence. A unit of many columns is one workgroup that walks all its keys, so they pay where there are
+// enough for the chip. Measured, us, few columns' kernel / many columns': 2048 rows of 2, 3, 4, 8 sequences (256, 384, 512, 1024
+// units) 128 / 120, 176 / 125, 229 / 152, 458 / 284; 4096 rows of one (256) 210 / 220; ragged, 7777 rows of 4 (486) 249 / 258;
+// heads of 128: 2048 rows of one (512) 152 / 108, 100 rows after 500 of 16 sequences (400) 83 / 67, prefills and decode steps in
+// one batch (296) 81 / 131. Up to kFewCols columns a sequence stays with the first also beside others that do not.
+constexpr int kFewCols = 256, kManyUnits = 384;
+constexpr int kWant = 512;                // pieces: two workgroups a CU
+constexpr size_t kSlots = 2 * kWant;      // (cut units have less than 2 kWant pieces)
+constexpr size_t kSlotBytes = (size_t)kCols * (256 + 4) * sizeof(float);
 
-template <int HD, bool MANY>
-hipError_t launch(const KvArgs& a, float* ws, size_t ws_bytes, int want, hipStream_t s) {
-  constexpr int block_cols = MANY ? kBigCols : kCols;
-  const int most = a.max_rows * (a.HQ / a.HK), ncb = (most + block_cols - 1) / block_cols;
-  Parts parts{ws, std::min(block_cols, most), 1};
-  const long units = (long)a.n_seqs * a.HK * ncb;
-  int chunk;
-  parts.ns = pieces(units, a.max_len, want, MANY ? 2 * kTile : kStep * kWaves, (size_t)parts.cols * (HD + 4) * sizeof(float), ws_bytes, &chunk);
-  if constexpr (MANY) {
-    constexpr int lds = 2 * ManyLds<HD>::kBuf;
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kv_many_kernel<HD>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-    if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((kv_many_kernel<HD>), dim3((unsigned)(units * parts.ns)), dim3(512), lds, s, a, chunk, ncb, parts);
-  } else {
-    hipLaunchKernelGGL((kv_few_kernel<HD>), dim3((unsigned)(units * parts.ns)), dim3(64 * kWaves), 0, s, a, chunk, ncb, parts);
-  }
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess || parts.ns == 1) return e;
-  hipLaunchKernelGGL((kv_merge_kernel<HD>), dim3(a.max_rows, a.HQ, a.n_seqs), dim3(parts.ns > 16 ? 1024 : 256), 0, s, a, chunk, ncb, block_cols, parts);
-  return hipGetLastError();
-}
-
-#ifndef KV_FEW_COLS
-#define KV_FEW_COLS 16
-#endif
 template <int HD>
-hipError_t attend(const KvArgs& a, float* ws, size_t ws_bytes, hipStream_t s) {
-  const int most = a.max_rows * (a.HQ / a.HK);
-  if (most > KV_FEW_COLS) return launch<HD, true>(a, ws, ws_bytes, 512, s);
-  return launch<HD, false>(a, ws, ws_bytes, 1024, s);
+hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
+  const int most = a.max_rows * a.ratio;  // columns a sequence has, at most
+  const bool equal = (long)a.n_rows == (long)a.n_seqs * a.max_rows;
+  const bool use_many = most > kFewCols && (long)a.n_rows * a.ratio / kBigCols * a.HK >= kManyUnits;
+  Kind few{}, many{};
+  few.p = ws;
+  few.hi = !use_many ? 0x7fffffff : equal ? 0 : kFewCols;
+  few.cols = std::min(kCols, most);
+  few.want = kWant;
+  many.lo = few.hi;
+  many.hi = 0x7fffffff;
+  hipError_t e = hipSuccess;
+  if (use_many) {
+    many.direct = equal;
+    many.ncb = (most + kBigCols - 1) / kBigCols;
+    const long grid = equal ? (long)a.n_seqs * a.HK * many.ncb : ((long)a.n_rows * a.ratio / kBigCols + a.n_seqs) * a.HK;
+    constexpr int lds = ManyLds<HD>::kAll;
+    e = hipFuncSetAttribute(reinterpret_cast<const void*>(kv_many_kernel<HD>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((kv_many_kernel<HD>), dim3((unsigned)grid), dim3(512), lds, s, a, many);
+    if ((e = hipGetLastError()) != hipSuccess || equal) return e;
+  }
+  few.ncb = (std::min(most, few.hi) + kCols - 1) / kCols;
+  const long units = std::min<long>((long)a.n_seqs * few.ncb, (long)a.n_rows * a.ratio / kCols + a.n_seqs) * a.HK;
+  dim3 grid((unsigned)(units + (a.max_len > kUnit ? kSlots : 0)));
+  dim3 merge((unsigned)std::min<long>((long)a.n_rows * a.HQ, (long)kWant * kCols));  // a unit that is cut has kCols columns at most
+  if (a.n_seqs > kScanMost && few.ncb == 1) {
+    few.direct = 1;
+    const long all = (long)a.n_seqs * a.HK;
+    long c = std::max<long>((all * a.max_len / (2 * kWant) + kUnit - 1) / kUnit * kUnit, kUnit);
+    while ((a.max_len + c - 1) / c > 1 && ((size_t)all * ((a.max_len + c - 1) / c) > kSlots || (a.max_len + c - 1) / c > kMergeMost)) c *= 2;
+    few.chunk = (int)std::min<long>(c, 1 << 30);
+    few.ns = (int)((a.max_len + c - 1) / c);
+    grid = dim3(few.ns, a.HK, a.n_seqs);
+    merge = dim3(most * a.HK, a.n_seqs);
+  }
+  hipLaunchKernelGGL((kv_few_kernel<HD>), grid, dim3(64 * kWaves), 0, s, a, few);
+  if ((e = hipGetLastError()) != hipSuccess || a.max_len <= kUnit || (few.direct && few.ns == 1)) return e;
+  hipLaunchKernelGGL((kv_merge_kernel<HD>), merge, dim3(a.max_len > 16 * kUnit && !few.direct ? 1024 : 256), 0, s, a, few);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-size_t kv_workspace_bytes() { return (size_t)64 << 20; }
+size_t kv_workspace_bytes() { return kSlots * kSlotBytes; }
 
-hipError_t launch_kv_attention(const KvArgs& a, void* ws, size_t ws_bytes, hipStream_t s) {
-  return a.HD == 256 ? attend<256>(a, static_cast<float*>(ws), ws_bytes, s) : attend<128>(a, static_cast<float*>(ws), ws_bytes, s);
+hipError_t launch_kv_attention(const KvArgs& a, void* ws, hipStream_t s) {
+  return a.HD == 256 ? attend<256>(a, static_cast<float*>(ws), s) : attend<128>(a, static_cast<float*>(ws), s);
 }
 
 }  // namespace ha

@@ -85,6 +85,7 @@ int call_args(ha_kv* k, int layer, const ha_kv_batch* b, ha::KvArgs* a) {
   if (!b || !b->row_start || !b->len || !b->pages) return set_error(HA_ERR_ARG, "batch, row_start, len and pages must be non-NULL");
   if (b->n_seqs < 1 || b->n_seqs > 65535) return set_error(HA_ERR_ARG, "n_seqs must be in [1, 65535]");
   if (b->n_rows < 0 || b->max_rows < 0 || b->max_rows > b->n_rows) return set_error(HA_ERR_ARG, "max_rows must be in [0, n_rows]");
+  if ((long)b->n_rows * (c.HQ / c.HK) > 1l << 27) return set_error(HA_ERR_ARG, "too many rows: n_rows * HQ / HK must be at most 2^27");
   if (b->max_len < b->max_rows || b->table_stride < 1) return set_error(HA_ERR_ARG, "max_len must be >= max_rows and table_stride > 0");
   if (b->max_len > c.max_ctx)
     return set_error(HA_ERR_CONTEXT, "context " + std::to_string(b->max_len) + " exceeds " + std::to_string(c.max_ctx));
@@ -95,6 +96,7 @@ int call_args(ha_kv* k, int layer, const ha_kv_batch* b, ha::KvArgs* a) {
   a->row_start = b->row_start; a->len = b->len; a->table = b->pages;
   a->n_pages = c.n_pages; a->page = c.page_size; a->page_log2 = __builtin_ctz((unsigned)c.page_size);
   a->HQ = c.HQ; a->HK = c.HK; a->HD = c.HD; a->rot = c.rot_dim; a->gated = c.gated ? 1 : 0; a->dtype = c.dtype;
+  a->ratio = c.HQ / c.HK; a->ratio_inv = a->ratio > 1 ? (unsigned)((0x100000000ull + a->ratio - 1) / a->ratio) : 0u;
   a->eps = c.eps; a->scale = c.scale > 0.0f ? c.scale : (float)(1.0 / std::sqrt((double)c.HD));
   a->pool = k->pages + (size_t)layer * k->layer_bytes;
   a->rope = k->rope;
@@ -214,7 +216,7 @@ int ha_kv_attention(ha_kv* k, int layer, const ha_kv_batch* batch, const void* q
   a.rows = rows; a.stride = row_stride; a.q = static_cast<_Float16*>(const_cast<void*>(q)); a.out = static_cast<_Float16*>(out);
   OnDevice on(k->device);
   if (on.rc != hipSuccess) return hip_error("hipSetDevice", on.rc);
-  const hipError_t he = ha::launch_kv_attention(a, k->ws, ha::kv_workspace_bytes(), static_cast<hipStream_t>(stream));
+  const hipError_t he = ha::launch_kv_attention(a, k->ws, static_cast<hipStream_t>(stream));
   return he == hipSuccess ? HA_OK : hip_error("attention launch", he);
 }
 
