@@ -38,7 +38,7 @@ struct KvArgs {
 
 hipError_t launch_kv_rope(float* rope, const double* theta_pow, int max_ctx, int rot, hipStream_t s);
 hipError_t launch_kv_append(const KvArgs& a, hipStream_t s);
-size_t kv_workspace_bytes();  // of partial results, whatever the call
+size_t kv_workspace_bytes();  // of partial results, whatever the call; zero at first
 hipError_t launch_kv_attention(const KvArgs& a, void* ws, hipStream_t s);
 
 // Sets the calling thread's ha_last_error() message; returns the code.

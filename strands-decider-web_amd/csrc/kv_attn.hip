@@ -50,13 +50,6 @@ __device__ __forceinline__ float sum_halves(float x) {
 __device__ __forceinline__ float max_quads(float x) { return over_quads(x, [](float u, float v) { return fmaxf(u, v); }); }
 __device__ __forceinline__ float sum_quads(float x) { return over_quads(x, [](float u, float v) { return u + v; }); }
 
-// Orders a wave's LDS accesses before its later ones to other lanes' entries (no workgroup barrier).
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
 // the low (high) half-words of u and v, u's first
 __device__ __forceinline__ unsigned halves(unsigned u, unsigned v, bool high) {
   return __builtin_amdgcn_perm(v, u, high ? 0x07060302u : 0x05040100u);
@@ -104,8 +97,12 @@ __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf
 // used where they fill the chip, are not. A workgroup's index is its place in the list of all pieces of all sequences, which
 // each wave finds by a prefix sum with a sequence a lane. A batch of more than kScanMost sequences with few columns, and one of
 // equal sequences with many, are laid out in a grid instead (`direct`), with the host's bounds.
+constexpr int kWant = 512;                // pieces: two workgroups a CU
+constexpr size_t kSlots = 2 * kWant;      // (cut units have less than 2 kWant pieces)
+constexpr size_t kSlotBytes = (size_t)kCols * (256 + 4) * sizeof(float);
 struct Kind {
   float* p;  // results of the pieces of cut units: for each piece and column O (unnormalised) [HD], maximum, sum
+  int* count;  // of a cut unit's pieces that are done, at its first piece's slot; zero between calls
   int cols;  // columns a block has, at most
   int lo, hi, want, direct, chunk, ncb, ns;
 };
@@ -279,7 +276,21 @@ __device__ __forceinline__ bool find_row(const KvArgs& a, const Kind& k, int x, 
   it.slot = k.direct ? ((it.b * a.HK + it.kh) * k.ncb + it.cb) * k.ns : slot + (it.cb * a.HK + it.kh) * ns;
   return true;
 }
-__device__ __forceinline__ float* column_of(const KvArgs& a, const Kind& k, int slot, int c) { return k.p + ((size_t)slot * k.cols + c) * (a.HD + 4); }
+// byte offset of a piece's column among the results: O [HD], maximum, sum, padding
+template <int HD>
+__device__ __forceinline__ unsigned column_at(const Kind& k, int slot, int c) { return (unsigned)(slot * k.cols + c) * (HD + 4) * 4; }
+constexpr int kCacheSc1 = 16;  // cache-policy operand of buffer instructions: device-coherent (sc1)
+typedef int i4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t rs, unsigned at, f4 v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i4, v), rs, at, 0, kCacheSc1);
+}
+__device__ __forceinline__ f4 get4(__amdgpu_buffer_rsrc_t rs, unsigned at) {
+  return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, kCacheSc1));
+}
+// Whether a unit's ns pieces are joined by the last of them, and not by kv_merge_kernel: one workgroup's loads.
+constexpr int kJoinMost = 32;
+template <int HD>
+__host__ __device__ inline bool joins(const Kind& k, int ns) { return ns * ((k.cols * (HD / 4) + 64 * kWaves - 1) / (64 * kWaves)) <= kJoinMost; }
 
 // The rows of a sequence that does not fit its batch.
 template <int HD>
@@ -313,6 +324,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
   const int ratio = a.ratio;
   Item it;
   if (!find_piece(a, kind, blockIdx.x, it)) return;
+  const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(kind.p, 0, (int)(kSlots * kSlotBytes), 0x00020000);
   const Seq sq = it.sq;
   const int kh = it.kh, b = it.b, k0 = it.piece * it.chunk, c0 = it.cb * kCols, cols = min(kCols, sq.n * ratio - c0);
   if (!sq.ok) {
@@ -577,16 +589,46 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
         v += f * *reinterpret_cast<const f4*>(ol + (w * (kCols / 2) + c - h0) * kPitch + ch);
       }
       if (keys > it.chunk) {
-        float* s = column_of(a, kind, it.slot, c);
-        *gpw<f4>(s + ch) = v;
-        if (ch == 0) {
-          s[HD] = mm;
-          s[HD + 1] = l;
-        }
+        const unsigned at = column_at<HD>(kind, it.slot, c);
+        put4(rs, at + 4 * ch, v);
+        if (ch == 0) put4(rs, at + 4 * HD, f4{mm, l, 0.0f, 0.0f});
       } else {
         finish<HD>(a, sq, kh, c0 + c, ch, v, 1.0f / l);
       }
     }
+  }
+  const int ns = pieces_of(keys, it.chunk);
+  if (ns <= 1 || !joins<HD>(kind, ns)) return;
+
+  // The last of a unit's pieces to get here joins them. Their results go past the XCDs' caches (sc1), and the count of those that
+  // are written is taken when they are there; the last one clears it for the next call. Nobody waits.
+  const int first = it.slot - it.piece;
+  __shared__ int is_last;
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (tid == 0) is_last = __hip_atomic_fetch_add(kind.count + first, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ns - 1;
+  __syncthreads();
+  if (!is_last) return;
+  if (tid == 0) __hip_atomic_store(kind.count + first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  f4* wl = reinterpret_cast<f4*>(ol);  // [column][piece]: maximum, sum
+  for (int k = tid; k < cols * ns; k += 64 * kWaves) {
+    const int c = k / ns;
+    wl[k] = get4(rs, column_at<HD>(kind, first + k - c * ns, c) + 4 * HD);
+  }
+  __syncthreads();
+  for (int k = tid; k < cols * (HD / 4); k += 64 * kWaves) {
+    const int c = k / (HD / 4), ch = 4 * (k % (HD / 4));
+    float mm = -INFINITY, l = 0.0f;
+    for (int s = 0; s < ns; s++) mm = fmaxf(mm, wl[c * ns + s][0]);
+    f4 v = {};
+#pragma unroll 8
+    for (int s = 0; s < ns; s++) {
+      const f4 w = wl[c * ns + s];
+      const float f = w[0] == mm ? 1.0f : __builtin_amdgcn_exp2f(w[0] - mm);
+      l += f * w[1];
+      v += f * get4(rs, column_at<HD>(kind, first + s, c) + 4 * ch);
+    }
+    finish<HD>(a, sq, kh, c0 + c, ch, v, 1.0f / l);
   }
 }
 
@@ -972,8 +1014,8 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvArgs a, Kind kind) {
   const Seq sq = it.sq;
   const int t = sq.r0 + it.row, c = it.row * a.ratio + h - it.kh * a.ratio - it.cb * kCols, end = min((it.cb + 1) * kCols, sq.n * a.ratio);
   const int keys = sq.len - sq.n + a.by_ratio(end - 1) + 1, ns = pieces_of(keys, it.chunk);
-  if (ns <= 1) return;
-  const float* p = column_of(a, kind, it.slot, c);
+  if (ns <= 1 || joins<HD>(kind, ns)) return;
+  const float* p = kind.p + column_at<HD>(kind, it.slot, c) / 4;
   const size_t step = (size_t)kind.cols * (HD + 4);
   const int k = tid / C, n = blockDim.x / C, ch = 4 * (tid % C), wave = tid >> 6, waves = blockDim.x >> 6;
   // the first pieces' O and the gate go out before the maxima are waited for
@@ -1038,10 +1080,6 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvArgs a, Kind kind) {
 // heads of 128: 2048 rows of one (512) 152 / 108, 100 rows after 500 of 16 sequences (400) 83 / 67, prefills and decode steps in
 // one batch (296) 81 / 131. Up to kFewCols columns a sequence stays with the first also beside others that do not.
 constexpr int kFewCols = 256, kManyUnits = 384;
-constexpr int kWant = 512;                // pieces: two workgroups a CU
-constexpr size_t kSlots = 2 * kWant;      // (cut units have less than 2 kWant pieces)
-constexpr size_t kSlotBytes = (size_t)kCols * (256 + 4) * sizeof(float);
-
 template <int HD>
 hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
   const int most = a.max_rows * a.ratio;  // columns a sequence has, at most
@@ -1049,6 +1087,7 @@ hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
   const bool use_many = most > kFewCols && (long)a.n_rows * a.ratio / kBigCols * a.HK >= kManyUnits;
   Kind few{}, many{};
   few.p = ws;
+  few.count = reinterpret_cast<int*>(ws + kSlots * kSlotBytes / sizeof(float));
   few.hi = !use_many ? 0x7fffffff : equal ? 0 : kFewCols;
   few.cols = std::min(kCols, most);
   few.want = kWant;
@@ -1081,13 +1120,14 @@ hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
   }
   hipLaunchKernelGGL((kv_few_kernel<HD>), grid, dim3(64 * kWaves), 0, s, a, few);
   if ((e = hipGetLastError()) != hipSuccess || a.max_len <= kUnit || (few.direct && few.ns == 1)) return e;
+  if (joins<HD>(few, (a.max_len + kUnit - 1) / kUnit)) return e;  // whatever the chunk
   hipLaunchKernelGGL((kv_merge_kernel<HD>), merge, dim3(a.max_len > 16 * kUnit && !few.direct ? 1024 : 256), 0, s, a, few);
   return hipGetLastError();
 }
 
 }  // namespace
 
-size_t kv_workspace_bytes() { return kSlots * kSlotBytes; }
+size_t kv_workspace_bytes() { return kSlots * (kSlotBytes + sizeof(int)); }
 
 hipError_t launch_kv_attention(const KvArgs& a, void* ws, hipStream_t s) {
   return a.HD == 256 ? attend<256>(a, static_cast<float*>(ws), s) : attend<128>(a, static_cast<float*>(ws), s);

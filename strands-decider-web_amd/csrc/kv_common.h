@@ -51,5 +51,12 @@ __device__ __forceinline__ f4 ld4(const _Float16* p) {
 }
 __device__ __forceinline__ h4 to_h4(const f4& x) { return h4{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]}; }
 
+// Orders a wave's LDS accesses before its later ones to other lanes' entries (no workgroup barrier).
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 }  // namespace
 }  // namespace ha

@@ -152,7 +152,9 @@ int ha_kv_create(const ha_kv_config* cfg, void* pages, int device, ha_kv** out) 
     const std::vector<float> ones(nn, 1.0f);
     if (hipMalloc(reinterpret_cast<void**>(&k->norms), nn * sizeof(float)) != hipSuccess) return bail(set_error(HA_ERR_NOMEM, "hipMalloc of the norms failed"));
     if (hipMalloc(&k->ws, ha::kv_workspace_bytes()) != hipSuccess) return bail(set_error(HA_ERR_NOMEM, "hipMalloc of the workspace failed"));
-    hipError_t he = hipMemcpy(k->norms, ones.data(), nn * sizeof(float), hipMemcpyHostToDevice);
+    hipError_t he = hipMemset(k->ws, 0, ha::kv_workspace_bytes());
+    if (he != hipSuccess) return bail(hip_error("workspace", he));
+    he = hipMemcpy(k->norms, ones.data(), nn * sizeof(float), hipMemcpyHostToDevice);
     if (he != hipSuccess) return bail(hip_error("norms", he));
     if (cfg->rot_dim) {
       // angle t / theta^(2 i / rot) in f64, its cosine and sine stored as f32, as the engine's table
