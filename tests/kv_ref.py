@@ -55,6 +55,17 @@ class Pool:
         par = blk[self.page * self.HD // 2:].view(np.float16).reshape(self.page // 4, 4, 2, 4)
         par[slot // 4, :, 0, slot % 4], par[slot // 4, :, 1, slot % 4] = s, z
 
+    def put_rows(self, page, slot, kh, which, rows):
+        """put() of rows [n][HD] at (page[n], slot[n])."""
+        c, s, z = quantise(rows.astype(np.float32))
+        nib = np.zeros(rows.shape, np.uint8)
+        nib[:, nibble_of(self.HD)] = c
+        self.codes()[page, kh, which, slot] = nib[:, 0::2] | nib[:, 1::2] << 4
+        half = self.data[..., self.page * self.HD // 2:].view(np.float16)
+        par = half.reshape(half.shape[:-1] + (self.page // 4, 4, 2, 4))
+        assert np.shares_memory(par, self.data)
+        par[page, kh, which, slot // 4, :, 0, slot % 4], par[page, kh, which, slot // 4, :, 1, slot % 4] = s, z
+
     def read(self, page, slot, kh, which):
         """Values [n][HD] (f64) of tokens at (page[n], slot[n])."""
         b = self.codes()[page, kh, which, slot].astype(np.int64)

@@ -1,0 +1,114 @@
+"""ha_kv_attention and ha_kv_append on batches whose work is shared out in other ways (csrc/kv_attn.hip, "who does what"): many rows a
+sequence, equal and ragged, beside single tokens; more sequences than one wave has lanes, and more than are listed; long pieces.
+Tolerances: tests/test_gpu_kv.py."""
+import numpy as np
+import pytest
+
+import kv_ref as kr
+from test_gpu_kv import Call, check, check_append
+
+pytestmark = pytest.mark.gpu
+H16 = (16, 1, 256, 64)   # 16 query heads on one KV head: 8 rows are a block of 128 columns
+H8 = (16, 2, 128, 128)
+MODEL = (8, 2, 256, 64)
+
+
+def some(c, n=40, seed=0):
+    """Rows to check: the first and last of every sequence, and n others."""
+    rng = np.random.default_rng(seed)
+    ends = {int(t) for b in range(len(c.seqs)) if c.seqs[b][1] for t in (c.start[b], c.start[b + 1] - 1)}
+    if len(ends) > 60:
+        ends = set(rng.permutation(sorted(ends))[:60].tolist())
+    return ends | set(rng.integers(0, c.T, n).tolist())
+
+
+# columns x KV heads / 128 is at least 384 in all of these: the kernel of many columns
+@pytest.mark.parametrize("seqs,heads,page,gated", [
+    ([(0, 800)] * 4, H8, 16, False),                                   # equal
+    ([(37, 1600)] * 2, H16, 64, True),                                 # behind a prefix
+    ([(0, 3100)], H16, 32, False),                                     # one
+    ([(0, 1), (5, 900), (0, 1333), (700, 1), (64, 1000), (3, 0), (31, 17)], H16, 16, True),   # ragged, single tokens among them
+    ([(100, 6300)], MODEL, 128, True)])
+def test_many_rows(seqs, heads, page, gated):
+    c = Call(seqs, heads, page, gated, seed=1, extra=2)
+    got = c.attention()
+    check(got[:c.T], c.expected(rows=some(c)))
+    assert np.isfinite(got[:c.T].astype(np.float32)).all() and (got[c.T:] == 7).all()
+
+
+def test_many_rows_of_more_than_64_sequences():
+    rng = np.random.default_rng(2)
+    c = Call([(int(p), int(n)) for p, n in zip(rng.integers(0, 40, 90), rng.integers(0, 90, 90))], H16, 16, seed=2)
+    assert c.T * 16 // 128 >= 384
+    check(c.attention(), c.expected(rows=some(c)))
+
+
+@pytest.mark.parametrize("n", [64, 65, 100, 128, 129, 140])
+def test_single_tokens_of_many_sequences(n):
+    rng = np.random.default_rng(n)
+    c = Call([(int(p), 1) for p in rng.integers(0, 300, n)], (3, 1, 256, 0), 16, False, seed=n)
+    check(c.attention(), c.expected())
+
+
+@pytest.mark.parametrize("n,heads", [(30, MODEL), (130, (3, 1, 256, 0)), (200, (4, 4, 128, 64))])
+def test_some_long_sequences(n, heads):
+    """A few sequences are cut into pieces, the others are shorter than one."""
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, 60, n)
+    lens[[1, n // 2, n - 1]] = [2600, 1500, 2047]
+    c = Call([(int(p), 1 + int(i % 5 == 0)) for i, p in enumerate(lens)], heads, 16, seed=n)
+    rows = some(c, 20) | {int(c.start[b]) for b in (1, n // 2, n - 1)}
+    check(c.attention(), c.expected(rows=rows))
+
+
+@pytest.mark.parametrize("P,n,heads", [(40000, 1, (16, 1, 128, 8)), (33000, 2, (2, 2, 128, 8)), (9000, 20, MODEL)])
+def test_pieces_of_a_long_context(P, n, heads):
+    """Pieces longer than 1024 keys (the first two: 40000 x 1 unit over 512 is one step a wave; the same over few units is not)."""
+    c = Call([(P, n)], heads, 256, seed=3)
+    check(c.attention(), c.expected(rows={0, n - 1}))
+
+
+def test_long_pieces_of_many_sequences():
+    """130 equal sequences in a grid of pieces of 1024 keys and more."""
+    c = Call([(2300, 1)] * 130, (4, 4, 128, 8), 256, False, seed=4)
+    check(c.attention(), c.expected(rows={0, 64, 129}))
+
+
+def test_append_many_rows():
+    c = Call([(0, 2100), (5, 1500)], (16, 2, 128, 128), 32, False, seed=5, extra=1)
+    check_append(c, *c.append())
+    c = Call([(0, 700), (33, 1200), (7, 1)], MODEL, 16, True, True, seed=6)
+    check_append(c, *c.append())
+
+
+@pytest.mark.parametrize("heads", [H8, H16])
+def test_sequences_that_do_not_fit_among_many_rows(heads):
+    c = Call([(0, 1100), (10, 1300), (0, 40), (20, 1), (0, 900)], heads, 16, seed=7)
+    start, lens = c.start.copy(), c.lens.copy()
+    lens[1] = 900         # fewer tokens than rows
+    lens[3] = -4
+    c.dev[1].copy_(c.torch.from_numpy(lens))
+    got = c.attention()
+    bad = np.r_[start[1]:start[2], start[3]:start[4]]
+    assert np.isnan(got[bad].astype(np.float32)).all()
+    check(got, {t: w for t, w in c.expected(rows=some(c)).items() if t not in set(bad.tolist())})
+
+
+def test_bad_page_among_many_rows():
+    c = Call([(0, 3200)], H16, 16, seed=8)
+    c.table[0, 150] = -1  # tokens 2400 .. 2415
+    c.dev[2].copy_(c.torch.from_numpy(c.table))
+    got = c.attention()
+    assert np.isnan(got[2400:].astype(np.float32)).all()
+    check(got, kr.attend(c.pool, c.table % c.n_pages, c.lens, c.start, c.q, c.gates(), c.HQ, rows={0, 5, 1000, 2399}))
+
+
+@pytest.mark.parametrize("seqs,heads", [([(3000, 1)], MODEL), ([(900, 3), (40, 1), (1700, 2)], MODEL), ([(0, 3200)], H16), ([(2000, 60)], MODEL)])
+def test_the_same_call_gives_the_same_bits(seqs, heads):
+    """Also after a call of another shape, which leaves other results in the workspace."""
+    c = Call(seqs, heads, 64, seed=9)
+    first = c.attention()
+    small = c.make_batch(n_seqs=1, n_rows=min(c.T, 5), max_rows=min(c.T, 5))
+    for _ in range(3):
+        c.attention(batch=small)
+        np.testing.assert_array_equal(c.attention().view(np.uint16), first.view(np.uint16))
