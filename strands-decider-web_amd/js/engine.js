@@ -85,7 +85,7 @@ class DeviceBuffer {
     this._engine = engine;
     this.bytes = bytes;
     this.ptr = native.deviceAlloc(engine._h, bytes);
-    this._borrows = 0;  // MatMulNBits handles reading this buffer (the C handle keeps only its address)
+    this._borrows = 0;  // MatMulNBits and PagedKV handles on this buffer (the C handle keeps only its address)
   }
   upload(typedArray) {
     if (typedArray.byteLength > this.bytes) throw new RangeError('upload larger than the buffer');
@@ -102,11 +102,11 @@ class DeviceBuffer {
     native.copyToHost(this._engine._h, typedArray, this.ptr);
     return typedArray;
   }
-  // Frees the device memory. Refused while a MatMulNBits handle borrows the buffer: the handle would go on reading
-  // memory already returned to the allocator.
+  // Frees the device memory. Refused while a MatMulNBits or PagedKV handle borrows the buffer: the handle would go on
+  // using memory already returned to the allocator.
   free() {
     if (this._borrows > 0) {
-      const e = new Error('device buffer is borrowed by ' + this._borrows + ' MatMulNBits handle(s); destroy them first');
+      const e = new Error('device buffer is borrowed by ' + this._borrows + ' handle(s); destroy them first');
       e.code = 'HA_BORROWED';
       throw e;
     }
@@ -269,6 +269,61 @@ class MatMulNBits {
       this._borrowed = [];
     }
   }
+}
+
+/*
+ * A paged cache of 4-bit keys and values for full-attention layers (ha_kv_*, include/ha.h): pages is the device memory
+ * of [nLayers][nPages] pages of PagedKV.pageBytes(config) bytes, borrowed as MatMulNBits borrows its weights. config:
+ * {nLayers, nPages, pageSize, maxCtx, HQ, HK, HD, rotDim, gated, dtype, ropeTheta, eps, scale}. A batch is {nSeqs, nRows,
+ * maxRows, maxLen, rowStart, lens, pages, tableStride} with int32 device arrays rowStart [nSeqs + 1], lens [nSeqs] and
+ * pages [nSeqs][tableStride]. The calls run on the engine's stream, in order with its token mixers.
+ */
+class PagedKV {
+  constructor(engine, pages, config) {
+    this.engine = engine;
+    this.config = kvConfig(config);
+    this._h = native.kvCreate(this.config, ptrOf(pages), engine ? engine.device : pick(config, 'device', 0));
+    this._borrowed = [pages].map((x) => (x instanceof DeviceView ? x.buf : x)).filter((x) => x instanceof DeviceBuffer);
+    this._borrowed.forEach((x) => { x._borrows++; });
+  }
+  static pageBytes(config) {
+    return native.kvPageBytes(Object.assign({ nPages: 1 }, kvConfig(config)));
+  }
+  setParam(layer, name, data) {
+    native.kvSetParam(this._h, layer, name, data);
+  }
+  // Puts the batch's fused rows [nRows][rowStride] into the layer's pages; q [nRows][HQ][HD] and values
+  // [nRows][2][HK][HD] (f16, may be null) take the queries and the rows as the cache holds them.
+  append(layer, batch, rows, rowStride, q, values) {
+    native.kvAppend(this._h, layer, kvBatch(batch), ptrOf(rows), rowStride, optPtrOf(q), optPtrOf(values), this._stream());
+  }
+  // out [nRows][HQ][HD] (f16) = causal attention of q over the cache, gated by the fused rows of a gated cache.
+  attention(layer, batch, q, rows, rowStride, out) {
+    native.kvAttention(this._h, layer, kvBatch(batch), ptrOf(q), optPtrOf(rows), rowStride, ptrOf(out), this._stream());
+  }
+  _stream() {
+    return this.engine ? this.engine._h : null;
+  }
+  destroy() {
+    if (this._h) {
+      native.kvDestroy(this._h);
+      this._h = null;
+      this._borrowed.forEach((x) => { x._borrows--; });
+      this._borrowed = [];
+    }
+  }
+}
+
+function kvConfig(c) {
+  return Object.assign({}, c, { gated: pick(c, 'gated', true) ? 1 : 0, dtype: dtypeCode(pick(c, 'dtype', null), F16) });
+}
+
+function kvBatch(b) {
+  return Object.assign({}, b, { rowStart: ptrOf(b.rowStart), lens: ptrOf(b.lens), pages: ptrOf(b.pages) });
+}
+
+function optPtrOf(x) {
+  return x === undefined || x === null ? null : ptrOf(x);
 }
 
 // In-place orthonormal Walsh-Hadamard transform of every n-block of an f16 device buffer of `elems` values: the
@@ -520,6 +575,7 @@ module.exports = {
   Engine: Engine,
   Torso: Torso,
   MatMulNBits: MatMulNBits,
+  PagedKV: PagedKV,
   fwht: fwht,
   Snapshot: Snapshot,
   DeviceBuffer: DeviceBuffer,

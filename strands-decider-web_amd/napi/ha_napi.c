@@ -16,7 +16,7 @@
 #include "ha.h"
 
 /* Every external holds one of these boxes; `kind` tells them apart, so a handle of the wrong kind is a TypeError. */
-enum { BOX_ENGINE = 0x45, BOX_SNAPSHOT = 0x53, BOX_MNB = 0x4d, BOX_TIMER = 0x54 };
+enum { BOX_ENGINE = 0x45, BOX_SNAPSHOT = 0x53, BOX_MNB = 0x4d, BOX_KV = 0x4b, BOX_TIMER = 0x54 };
 
 typedef struct engine_box {
   int kind;
@@ -40,6 +40,11 @@ typedef struct {
   int kind;
   ha_mnb* w;
 } mnb_box;
+
+typedef struct {
+  int kind;
+  ha_kv* k;
+} kv_box;
 
 typedef struct {
   int kind;
@@ -138,6 +143,7 @@ static void* get_box(napi_env env, napi_value v, int kind) {
 static engine_box* get_engine(napi_env env, napi_value v) { return (engine_box*)get_box(env, v, BOX_ENGINE); }
 static snap_box* get_snap(napi_env env, napi_value v) { return (snap_box*)get_box(env, v, BOX_SNAPSHOT); }
 static mnb_box* get_mnb(napi_env env, napi_value v) { return (mnb_box*)get_box(env, v, BOX_MNB); }
+static kv_box* get_kv(napi_env env, napi_value v) { return (kv_box*)get_box(env, v, BOX_KV); }
 static timer_box* get_timer(napi_env env, napi_value v) { return (timer_box*)get_box(env, v, BOX_TIMER); }
 
 /* host bytes of a TypedArray / ArrayBuffer view */
@@ -220,6 +226,13 @@ static void mnb_finalize(napi_env env, void* data, void* hint) {
   (void)env; (void)hint;
   mnb_box* b = (mnb_box*)data;
   if (b->w) ha_mnb_destroy(b->w);
+  free(b);
+}
+
+static void kv_finalize(napi_env env, void* data, void* hint) {
+  (void)env; (void)hint;
+  kv_box* b = (kv_box*)data;
+  if (b->k) ha_kv_destroy(b->k);
   free(b);
 }
 
@@ -661,6 +674,161 @@ static napi_value js_mnb_destroy(napi_env env, napi_callback_info info) {
   return NULL;
 }
 
+/* the fields of a cache's config, defaults as in hybrid_attention.PagedKV */
+static int kv_config(napi_env env, napi_value v, ha_kv_config* c) {
+  memset(c, 0, sizeof(*c));
+  return !is_nullish(env, v) && get_int(env, v, "nLayers", 1, &c->n_layers) && get_int(env, v, "nPages", 0, &c->n_pages) &&
+         get_int(env, v, "pageSize", 64, &c->page_size) && get_int(env, v, "maxCtx", 4096, &c->max_ctx) &&
+         get_int(env, v, "HQ", 8, &c->HQ) && get_int(env, v, "HK", 2, &c->HK) && get_int(env, v, "HD", 256, &c->HD) &&
+         get_int(env, v, "rotDim", 64, &c->rot_dim) && get_int(env, v, "gated", 1, &c->gated) &&
+         get_int(env, v, "dtype", HA_F16, &c->dtype) && get_float(env, v, "ropeTheta", 1e7f, &c->rope_theta) &&
+         get_float(env, v, "eps", 1e-6f, &c->eps) && get_float(env, v, "scale", 0.0f, &c->scale);
+}
+
+/* kvPageBytes({pageSize, HK, HD, ...}) -> bytes of one page of one layer */
+static napi_value js_kv_page_bytes(napi_env env, napi_callback_info info) {
+  napi_value argv[1];
+  if (!get_args(env, info, 1, argv)) return NULL;
+  ha_kv_config c;
+  if (!kv_config(env, argv[0], &c)) return type_error(env, "invalid cache config field");
+  size_t n = 0;
+  CHECK_HA(ha_kv_page_bytes(&c, &n));
+  napi_value r;
+  CHECK_NAPI(napi_create_double(env, (double)n, &r));
+  return r;
+}
+
+/* kvCreate(cfg, pages: BigInt, device) -> handle */
+static napi_value js_kv_create(napi_env env, napi_callback_info info) {
+  napi_value argv[3];
+  if (!get_args(env, info, 3, argv)) return NULL;
+  ha_kv_config c;
+  if (!kv_config(env, argv[0], &c)) return type_error(env, "invalid cache config field");
+  void* pages;
+  int32_t device = 0;
+  if (!get_ptr(env, argv[1], &pages)) return type_error(env, "pages must be a BigInt");
+  if (!is_nullish(env, argv[2]) && napi_get_value_int32(env, argv[2], &device) != napi_ok)
+    return type_error(env, "device must be an integer");
+  ha_kv* k = NULL;
+  CHECK_HA(ha_kv_create(&c, pages, device, &k));
+  kv_box* b = (kv_box*)malloc(sizeof(kv_box));
+  if (!b) {
+    ha_kv_destroy(k);
+    return type_error(env, "out of host memory");
+  }
+  b->kind = BOX_KV;
+  b->k = k;
+  napi_value r;
+  if (napi_create_external(env, b, kv_finalize, NULL, &r) != napi_ok) {
+    ha_kv_destroy(k);
+    free(b);
+    napi_throw_error(env, NULL, "napi_create_external failed");
+    return NULL;
+  }
+  return r;
+}
+
+#define KV_ARG(v)                                          \
+  kv_box* kb = get_kv(env, v);                             \
+  if (!kb) return type_error(env, "not a PagedKV handle"); \
+  if (!kb->k) return type_error(env, "PagedKV handle was destroyed")
+
+/* kvSetParam(handle, layer, name, Float32Array) */
+static napi_value js_kv_set_param(napi_env env, napi_callback_info info) {
+  napi_value argv[4];
+  if (!get_args(env, info, 4, argv)) return NULL;
+  KV_ARG(argv[0]);
+  int32_t layer;
+  char name[64];
+  size_t nlen = 0, len, off;
+  napi_typedarray_type type;
+  napi_value ab;
+  void* d;
+  bool is_ta = false;
+  if (napi_get_value_int32(env, argv[1], &layer) != napi_ok) return type_error(env, "layer must be an integer");
+  if (napi_get_value_string_utf8(env, argv[2], name, sizeof(name), &nlen) != napi_ok)
+    return type_error(env, "name must be a string");
+  if (napi_is_typedarray(env, argv[3], &is_ta) != napi_ok || !is_ta ||
+      napi_get_typedarray_info(env, argv[3], &type, &len, &d, &ab, &off) != napi_ok || type != napi_float32_array)
+    return type_error(env, "data must be a Float32Array");
+  CHECK_HA(ha_kv_set_param(kb->k, layer, name, (const float*)d, len));
+  return NULL;
+}
+
+/* {nSeqs, nRows, maxRows, maxLen, rowStart: BigInt, lens: BigInt, pages: BigInt, tableStride} */
+static int kv_batch(napi_env env, napi_value v, ha_kv_batch* b) {
+  napi_value x[3];
+  void *start, *len, *pages;
+  if (is_nullish(env, v) || !get_int(env, v, "nSeqs", 0, &b->n_seqs) || !get_int(env, v, "nRows", 0, &b->n_rows) ||
+      !get_int(env, v, "maxRows", 0, &b->max_rows) || !get_int(env, v, "maxLen", 0, &b->max_len) ||
+      !get_int(env, v, "tableStride", 0, &b->table_stride) ||
+      napi_get_named_property(env, v, "rowStart", &x[0]) != napi_ok ||
+      napi_get_named_property(env, v, "lens", &x[1]) != napi_ok ||
+      napi_get_named_property(env, v, "pages", &x[2]) != napi_ok || !get_ptr(env, x[0], &start) ||
+      !get_ptr(env, x[1], &len) || !get_ptr(env, x[2], &pages))
+    return 0;
+  b->row_start = (const int*)start;
+  b->len = (const int*)len;
+  b->pages = (const int*)pages;
+  return 1;
+}
+
+static int opt_ptr(napi_env env, napi_value v, void** out) {
+  *out = NULL;
+  return is_nullish(env, v) || get_ptr(env, v, out);
+}
+
+/* kvAppend(handle, layer, batch, rows: BigInt, rowStride, q: BigInt|null, values: BigInt|null, engine|null) */
+static napi_value js_kv_append(napi_env env, napi_callback_info info) {
+  napi_value argv[8];
+  if (!get_args(env, info, 8, argv)) return NULL;
+  KV_ARG(argv[0]);
+  int32_t layer;
+  int64_t stride;
+  ha_kv_batch b;
+  void *rows, *q, *values, *st;
+  if (napi_get_value_int32(env, argv[1], &layer) != napi_ok || napi_get_value_int64(env, argv[4], &stride) != napi_ok)
+    return type_error(env, "layer and rowStride must be integers");
+  if (!kv_batch(env, argv[2], &b)) return type_error(env, "invalid batch field");
+  if (!get_ptr(env, argv[3], &rows) || !opt_ptr(env, argv[5], &q) || !opt_ptr(env, argv[6], &values))
+    return type_error(env, "rows must be a BigInt, q and values a BigInt or null");
+  if (!stream_of(env, argv[7], &st)) return type_error(env, "the last argument must be an engine handle or null");
+  CHECK_HA(ha_kv_append(kb->k, layer, &b, rows, (long)stride, q, values, st));
+  return NULL;
+}
+
+/* kvAttention(handle, layer, batch, q: BigInt, rows: BigInt|null, rowStride, out: BigInt, engine|null) */
+static napi_value js_kv_attention(napi_env env, napi_callback_info info) {
+  napi_value argv[8];
+  if (!get_args(env, info, 8, argv)) return NULL;
+  KV_ARG(argv[0]);
+  int32_t layer;
+  int64_t stride;
+  ha_kv_batch b;
+  void *rows, *q, *out, *st;
+  if (napi_get_value_int32(env, argv[1], &layer) != napi_ok || napi_get_value_int64(env, argv[5], &stride) != napi_ok)
+    return type_error(env, "layer and rowStride must be integers");
+  if (!kv_batch(env, argv[2], &b)) return type_error(env, "invalid batch field");
+  if (!get_ptr(env, argv[3], &q) || !opt_ptr(env, argv[4], &rows) || !get_ptr(env, argv[6], &out))
+    return type_error(env, "q and out must be BigInt, rows a BigInt or null");
+  if (!stream_of(env, argv[7], &st)) return type_error(env, "the last argument must be an engine handle or null");
+  CHECK_HA(ha_kv_attention(kb->k, layer, &b, q, rows, (long)stride, out, st));
+  return NULL;
+}
+
+static napi_value js_kv_destroy(napi_env env, napi_callback_info info) {
+  napi_value argv[1];
+  if (!get_args(env, info, 1, argv)) return NULL;
+  kv_box* kb = get_kv(env, argv[0]);
+  if (!kb) return type_error(env, "not a PagedKV handle");
+  if (kb->k) {
+    ha_kv* k = kb->k;
+    kb->k = NULL;
+    CHECK_HA(ha_kv_destroy(k));
+  }
+  return NULL;
+}
+
 /* timerCreate(device, n): n GPU timestamps (a WebGPU timestamp query set's counterpart) */
 static napi_value js_timer_create(napi_env env, napi_callback_info info) {
   napi_value argv[2];
@@ -873,6 +1041,9 @@ static napi_value init(napi_env env, napi_value exports) {
       {"synchronize", js_synchronize},
       {"mnbCreate", js_mnb_create},         {"mnbForward", js_mnb_forward},
       {"mnbDestroy", js_mnb_destroy},       {"fwht", js_fwht},
+      {"kvPageBytes", js_kv_page_bytes},    {"kvCreate", js_kv_create},
+      {"kvSetParam", js_kv_set_param},      {"kvAppend", js_kv_append},
+      {"kvAttention", js_kv_attention},     {"kvDestroy", js_kv_destroy},
       {"embed", js_embed},                  {"addNorm", js_add_norm},
       {"siluMul", js_silu_mul},             {"addBias", js_add_bias},
       {"shareStream", js_share_stream},
