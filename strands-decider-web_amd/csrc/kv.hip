@@ -12,7 +12,6 @@
 
 #include "kv_common.h"
 
-
 namespace ha {
 namespace {
 
@@ -176,22 +175,55 @@ __device__ __forceinline__ unsigned short nibbles(const float* c) {
   return (unsigned short)(unsigned)fmaf(fmaf(fmaf(c[3], 16.0f, c[2]), 16.0f, c[1]), 16.0f, c[0] + (float)0x8888);
 }
 
+// Block x of `rows` rows among those of all sequences, or false where there is none. A sequence that does not fit its batch is
+// one block, from row 0.
+__device__ __forceinline__ bool find_rows(const KvArgs& a, int rows, int x, int& b, int& b0, Seq& sq) {
+  const int lane = threadIdx.x & 63;
+  for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
+    Seq l{};
+    if (s0 + lane < a.n_seqs) l = seq_of(a, s0 + lane);
+    const int n = l.n == 0 ? 0 : l.ok ? (l.n + rows - 1) / rows : 1, sum = scan64(n);
+    const unsigned long long past = __ballot(sum > x);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      b = s0 + at;
+      b0 = (x - lane_value(sum, at) + lane_value(n, at)) * rows;
+      sq = lane_value(l, at);
+      return true;
+    }
+    x -= lane_value(sum, 63);
+  }
+  return false;
+}
+
 // A wave has one head slot (the query heads, then the keys', then the values') of NR x 64 / (HD / 8) rows of a sequence. A query
 // head's rotated channels, which are in few of a row's lanes, are done for all its rows at once, by lanes of their own.
 template <int HD, typename T, int NR>
-__global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a) {
+__global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int listed) {
   constexpr int kLanes = HD / 8, kRows = 64 / kLanes, kBlock = NR * kRows;
   __shared__ float invs[4][kBlock];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, l = lane % kLanes, c = 8 * l, lr = lane / kLanes;
-  const int slot = blockIdx.y * 4 + wave, b = blockIdx.z;
+  const int slot = blockIdx.y * 4 + wave;
   if (slot >= a.HQ + 2 * a.HK || (slot < a.HQ && !a.q)) return;
-  const Seq sq = seq_of(a, b);
-  const int b0 = blockIdx.x * kBlock;  // rows b0 + lr, b0 + lr + kRows, ... of the sequence
-  if (b0 >= sq.n) return;
+  int b = blockIdx.z, b0 = blockIdx.x * kBlock;  // rows b0 + lr, b0 + lr + kRows, ... of sequence b
+  Seq sq;
+  if (listed) {
+    if (!find_rows(a, kBlock, blockIdx.x, b, b0, sq)) return;
+  } else {
+    sq = seq_of(a, b);
+    if (b0 >= sq.n) return;
+  }
+  const h8 nan8 = h8{} + (_Float16)__builtin_nanf("");
+  if (!sq.ok) {
+    for (int i = b0 + lr; i < (listed ? sq.n : min(b0 + kBlock, sq.n)); i += kRows) {
+      if (slot < a.HQ) *gpw<h8>(a.q + ((size_t)(sq.r0 + i) * a.HQ + slot) * HD + c) = nan8;
+      else if (a.values) *gpw<h8>(a.values + ((size_t)(sq.r0 + i) * 2 * a.HK + slot - a.HQ) * HD + c) = nan8;
+    }
+    return;
+  }
   const int per = a.gated ? 2 * HD : HD, which = slot >= a.HQ + a.HK, kh = slot - a.HQ - which * a.HK;
   const T* base = static_cast<const T*>(a.rows) + (slot < a.HQ ? (size_t)slot * per : (size_t)a.HQ * per + (size_t)(slot - a.HQ) * HD) + (size_t)sq.r0 * a.stride;
-  const int first_pos = sq.ok ? sq.len - sq.n : 0;
-  const h8 nan8 = h8{} + (_Float16)__builtin_nanf("");
+  const int first_pos = sq.len - sq.n;
   auto row_of = [&](int n) { return min(b0 + lr + n * kRows, sq.n - 1); };
   Eight<T> x[NR];
 #pragma unroll
@@ -208,7 +240,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a) {
       h8 o;
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] = (_Float16)(x[n][e] * (inv * w[e >> 2][e & 3]));
-      if (c >= a.rot && i < sq.n) *gpw<h8>(q + (size_t)i * a.HQ * HD + c) = sq.ok ? o : nan8;
+      if (c >= a.rot && i < sq.n) *gpw<h8>(q + (size_t)i * a.HQ * HD + c) = o;
     }
     wave_sync();
     const int chunks = a.rot / 8, share = min(kBlock, sq.n - b0) * chunks;  // 8 channels of a row a lane
@@ -217,7 +249,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a) {
       const int r = (int)((unsigned)k * by_chunks >> 16), c = 8 * (k - r * chunks), i = b0 + r;
       const Turn tn(c, a.rot);
       const T* row = base + (size_t)i * a.stride;
-      const float* rope = a.rope + (size_t)(first_pos + (sq.ok ? i : 0)) * a.rot;
+      const float* rope = a.rope + (size_t)(first_pos + i) * a.rot;
       Eight<T> x;
       x.load(row + c);
       f4 w[2], py[2], wp[2], cs[4];
@@ -234,14 +266,14 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a) {
       h8 o;
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] = (_Float16)y[e];
-      *gpw<h8>(q + (size_t)i * a.HQ * HD + c) = sq.ok ? o : nan8;
+      *gpw<h8>(q + (size_t)i * a.HQ * HD + c) = o;
     }
     return;
   }
 
   int page[NR];
 #pragma unroll
-  for (int n = 0; n < NR; n++) page[n] = sq.ok ? gp<int>(a.table)[(size_t)b * a.table_stride + ((first_pos + row_of(n)) >> a.page_log2)] : -1;
+  for (int n = 0; n < NR; n++) page[n] = gp<int>(a.table)[(size_t)b * a.table_stride + ((first_pos + row_of(n)) >> a.page_log2)];
   // the values of a row (channels c .. + 7 of the lane) into their page
   auto put = [&](int n, const float* v) {
     _Float16 s, z;
@@ -281,7 +313,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a) {
 #pragma unroll
   for (int n = 0; n < NR; n++) {
     const T* row = base + (size_t)row_of(n) * a.stride;
-    const float* rope = a.rope + (size_t)(first_pos + (sq.ok ? row_of(n) : 0)) * a.rot;
+    const float* rope = a.rope + (size_t)(first_pos + row_of(n)) * a.rot;
     f4 py[2], wp[2], cs[4];
 #pragma unroll
     for (int k = 0; k < 2; k++)
@@ -310,10 +342,18 @@ hipError_t launch_kv_rope(float* rope, const double* theta_pow, int max_ctx, int
   return hipGetLastError();
 }
 
+// A workgroup's place is in a grid of (rows, sequences), or, where most of that would be empty, in a list that the wave goes through.
+// Measured, us, grid / list, the model's heads: one new row each of 8 sequences 4.7 / 4.0, 2048 rows each 48.8 / 51.4; 2048 rows and 47
+// single ones 46.4 / 11.1, 400 rows and 200 single ones 58.8 / 7.7; 20 rows and 500 single ones 14.0 / 11.5, 8 rows and 1000 single
+// ones (the list is 16 loads deep, the grid a quarter full) 21.2 / 27.3.
+constexpr int kListFrom = 2;
 template <int HD, typename T, int NR>
 hipError_t append_rows(const KvArgs& a, hipStream_t s) {
   constexpr int kBlock = NR * 64 / (HD / 8);
-  hipLaunchKernelGGL((kv_append_kernel<HD, T, NR>), dim3((a.max_rows + kBlock - 1) / kBlock, (a.HQ + 2 * a.HK + 3) / 4, a.n_seqs), dim3(256), 0, s, a);
+  const long grid = (long)a.n_seqs * ((a.max_rows + kBlock - 1) / kBlock), list = a.n_rows / kBlock + a.n_seqs;
+  const bool listed = grid > kListFrom * list;
+  hipLaunchKernelGGL((kv_append_kernel<HD, T, NR>), dim3((unsigned)(listed ? list : (a.max_rows + kBlock - 1) / kBlock), (a.HQ + 2 * a.HK + 3) / 4, listed ? 1 : a.n_seqs),
+                     dim3(256), 0, s, a, (int)listed);
   return hipGetLastError();
 }
 // More rows a wave where there are enough waves. Measured, us, 1 / 2 / 4 times 64 / (HD / 8) rows a wave, the model's heads: 256 rows

@@ -113,28 +113,6 @@ struct Item {
 };
 constexpr int kScanMost = 128;
 
-__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }  // (for the compiler)
-template <int kCtrl, int kRows>
-__device__ __forceinline__ int dpp_add(int v) { return v + __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, true); }
-template <int kCtrl, int kRows>
-__device__ __forceinline__ float dpp_add(float v) {
-  return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, kRows, 0xf, true));
-}
-// inclusive prefix sum over the wave
-template <typename F>
-__device__ __forceinline__ F scan64(F v) {
-  v = dpp_add<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
-  v = dpp_add<0x112, 0xf>(v);
-  v = dpp_add<0x114, 0xf>(v);
-  v = dpp_add<0x118, 0xf>(v);
-  v = dpp_add<0x142, 0xa>(v);  // row_bcast 15, 31
-  return dpp_add<0x143, 0xc>(v);
-}
-__device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
-__device__ __forceinline__ Seq lane_value(const Seq& s, int lane) {
-  return Seq{lane_value(s.r0, lane), lane_value(s.n, lane), lane_value(s.len, lane), lane_value((int)s.ok, lane) != 0};
-}
-
 // a lane's sequence: its rows and units
 struct Lane {
   Seq sq;

@@ -112,3 +112,28 @@ def test_the_same_call_gives_the_same_bits(seqs, heads):
     for _ in range(3):
         c.attention(batch=small)
         np.testing.assert_array_equal(c.attention().view(np.uint16), first.view(np.uint16))
+
+
+# one sequence has most of the rows: append's rows are found in a list (csrc/kv.hip, find_rows)
+@pytest.mark.parametrize("seqs,heads", [
+    ([(7, 1)] * 5 + [(3, 90), (0, 0), (9, 3)] + [(30, 1)] * 4, MODEL),
+    ([(int(p), 1) for p in range(70)] + [(11, 200)] + [(4, 2), (0, 0)] * 10, H8),
+    ([(2, 130)] + [(5, 1)] * 150, (3, 1, 256, 0))])
+def test_append_of_one_long_sequence(seqs, heads):
+    c = Call(seqs, heads, 16, True, seed=10, extra=2)
+    check_append(c, *c.append())
+
+
+def test_append_of_one_long_sequence_that_does_not_fit():
+    c = Call([(7, 1)] * 6 + [(3, 90), (9, 3)], MODEL, 16, True, seed=11)
+    lens = c.lens.copy()
+    lens[[2, 6]] = 0
+    c.dev[1].copy_(c.torch.from_numpy(lens))
+    before = c.dpool.cpu().numpy()
+    q, v, pool = c.append()
+    bad = np.zeros(c.T, bool)
+    bad[2] = bad[6:96] = True
+    for x in (q, v):
+        assert np.isnan(x[bad]).all() and np.isfinite(x[~bad]).all()
+    changed = set(np.nonzero((pool != before).any(axis=(1, 2, 3)))[0])
+    assert changed == {int(c.table[b, p // 16]) for b in (0, 1, 3, 4, 5, 7) for p in range(c.lens[b] - (c.start[b + 1] - c.start[b]), c.lens[b])}
