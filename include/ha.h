@@ -268,7 +268,7 @@ int ha_add_bias(int L, int N, void* y, const float* c, int device, void* stream)
    Format: a row (one token and KV head) is 4 groups of G = HD / 4 consecutive channels, each value s (c - 8) + z with a code
    c of 4 bits and an f16 scale s and zero z for each group:
      z = f16(lo + (hi - lo) 8/15), s = f16(max((hi - z)/7, (z - lo)/8)), c = clamp(rint((x - z)/s) + 8, 0, 15)
-   in f32 of the group's least and largest values lo, hi (all values equal: s = 0, c = 8). A group with a value that is not
+   in f32 of the group's least and largest values lo, hi (c = 8 where s = 0). A group with a value that is not
    finite, or whose s or z is not, reads as NaN.
    Pages: a layer's pool is n_pages pages of ha_kv_page_bytes bytes; a page holds page_size tokens as [HK][keys, values]
    blocks of page_size rows of HD / 2 bytes (channel c in nibble 16 ((c % G) / 4) + 4 (c / G) + c % 4, low nibble first), then
@@ -279,7 +279,7 @@ typedef struct ha_kv_config {
   int n_layers;     /* full-attention layers; each has a pool of its own, all share the page tables */
   int n_pages;      /* pages of a layer's pool */
   int page_size;    /* tokens a page: 16, 32, 64, 128 or 256 */
-  int max_ctx;      /* positions a sequence may have */
+  int max_ctx;      /* positions a sequence may have, up to 2^24 */
   int HQ, HK, HD;   /* heads, KV heads (HQ a multiple of HK, up to 16 times), head_dim 128 or 256 */
   int rot_dim;      /* rotated channels, a multiple of 8 (0: none) */
   int gated;        /* 1: fused rows are [q | gate] x HQ | k x HK | v x HK and the output takes sigmoid(gate); 0: q x HQ | ... */
@@ -293,8 +293,8 @@ typedef struct ha_kv_config {
    row_start[b + 1] - 1 of the call, its context with them len[b] tokens: they are its last positions. Token t stands in page
    pages[b][t / page_size], slot t % page_size; entries behind the last token's are not read. */
 typedef struct ha_kv_batch {
-  int n_seqs;            /* up to 65535 */
-  int n_rows;            /* rows of q, values and outputs */
+  int n_seqs;            /* up to 65535 (n_seqs HK up to 2^22) */
+  int n_rows;            /* rows of q, values and outputs (n_rows HQ up to 2^27) */
   int max_rows;          /* no sequence has more new rows */
   int max_len;           /* no sequence has a longer context (at most max_ctx and table_stride pages) */
   const int* row_start;  /* device [n_seqs + 1] */
@@ -311,13 +311,14 @@ int ha_kv_set_param(ha_kv* k, int layer, const char* name, const float* host, si
 /* Puts a batch's new tokens into the layer's pages, from its fused rows [n_rows][row_stride]: keys after norm and rotation at
    their positions, values as they are. q (or NULL) takes the normed and rotated queries, [n_rows][HQ][HD] f16; values (or
    NULL) the new rows as the cache now holds them, [n_rows][keys, values][HK][HD] f16. Rows of no sequence are left as they
-   were. A sequence whose row_start or len does not fit the batch stores nothing and its rows of q and values are NaN; a token
-   whose table entry is no page of the pool is not stored and its values are NaN. Two sequences must not append to one slot. */
+   were. A sequence whose row_start or len does not fit the batch stores nothing and its rows of q and values (the first
+   max_rows of them) are NaN; a token whose table entry is no page of the pool is not stored and its values are NaN. Two
+   sequences must not append to one slot. */
 int ha_kv_append(ha_kv* k, int layer, const ha_kv_batch* batch, const void* rows, long row_stride, void* q, void* values, void* stream);
 /* out[n_rows][HQ][HD] (f16) = causal attention of the queries q (as append gives them) over their sequences' contexts, times
    sigmoid(gate) with the gates of the fused rows where the cache is gated (rows may be NULL otherwise). A row that sees a token
-   whose table entry is no page of the pool is NaN, and so is every row of a sequence that does not fit the batch; rows of no
-   sequence are left as they were. Uses a workspace of the handle: calls on one handle must be ordered. Neither call
+   whose table entry is no page of the pool is NaN, and so are the (first max_rows) rows of a sequence that does not fit the
+   batch; rows of no sequence are left as they were. q and out must not overlap. Uses a workspace of the handle: calls on one handle must be ordered. Neither call
    allocates or synchronises, and both can be captured into a HIP graph. */
 int ha_kv_attention(ha_kv* k, int layer, const ha_kv_batch* batch, const void* q, const void* rows, long row_stride, void* out,
                     void* stream);

@@ -38,7 +38,8 @@ int hip_error(const char* what, hipError_t e) { return set_error(HA_ERR_DEVICE, 
 int check_config(const ha_kv_config* c) {
   auto bad = [](const char* m) { return set_error(HA_ERR_ARG, m); };
   if (!c) return bad("config is NULL");
-  if (c->n_layers < 1 || c->n_pages < 1 || c->max_ctx < 1) return bad("n_layers, n_pages and max_ctx must be > 0");
+  if (c->n_layers < 1 || c->n_pages < 1) return bad("n_layers and n_pages must be > 0");
+  if (c->max_ctx < 1 || c->max_ctx > 1 << 24) return bad("max_ctx must be in [1, 2^24]");
   if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1))) return bad("page_size must be 16, 32, 64, 128 or 256");
   if (c->HD != 128 && c->HD != 256) return bad("head_dim must be 128 or 256");
   if (c->HK < 1 || c->HQ < 1 || c->HQ % c->HK || c->HQ / c->HK > ha::kKvMaxRatio || c->HQ > 1024)
@@ -83,9 +84,10 @@ int call_args(ha_kv* k, int layer, const ha_kv_batch* b, ha::KvArgs* a) {
   const ha_kv_config& c = k->cfg;
   if (layer < 0 || layer >= c.n_layers) return set_error(HA_ERR_ARG, "layer index out of range");
   if (!b || !b->row_start || !b->len || !b->pages) return set_error(HA_ERR_ARG, "batch, row_start, len and pages must be non-NULL");
-  if (b->n_seqs < 1 || b->n_seqs > 65535) return set_error(HA_ERR_ARG, "n_seqs must be in [1, 65535]");
+  if (b->n_seqs < 1 || b->n_seqs > 65535 || (long)b->n_seqs * c.HK > 1l << 22)
+    return set_error(HA_ERR_ARG, "n_seqs must be in [1, 65535] and n_seqs * HK at most 2^22");
   if (b->n_rows < 0 || b->max_rows < 0 || b->max_rows > b->n_rows) return set_error(HA_ERR_ARG, "max_rows must be in [0, n_rows]");
-  if ((long)b->n_rows * (c.HQ / c.HK) > 1l << 27) return set_error(HA_ERR_ARG, "too many rows: n_rows * HQ / HK must be at most 2^27");
+  if ((long)b->n_rows * c.HQ > 1l << 27) return set_error(HA_ERR_ARG, "too many rows: n_rows * HQ must be at most 2^27");
   if (b->max_len < b->max_rows || b->table_stride < 1) return set_error(HA_ERR_ARG, "max_len must be >= max_rows and table_stride > 0");
   if (b->max_len > c.max_ctx)
     return set_error(HA_ERR_CONTEXT, "context " + std::to_string(b->max_len) + " exceeds " + std::to_string(c.max_ctx));
@@ -165,11 +167,12 @@ int ha_kv_create(const ha_kv_config* cfg, void* pages, int device, ha_kv** out) 
         return bail(set_error(HA_ERR_NOMEM, "hipMalloc of the RoPE table failed"));
       he = hipMemcpy(pow_dev, pw.data(), sizeof(double) * pw.size(), hipMemcpyHostToDevice);
       if (he == hipSuccess) he = ha::launch_kv_rope(k->rope, pow_dev, cfg->max_ctx, cfg->rot_dim, nullptr);
-      if (he == hipSuccess) he = hipStreamSynchronize(nullptr);
       if (he != hipSuccess) return bail(hip_error("RoPE table", he));
-      (void)hipFree(pow_dev);
-      pow_dev = nullptr;
     }
+    he = hipStreamSynchronize(nullptr);  // the calls may come on streams that do not wait for the null stream
+    if (he != hipSuccess) return bail(hip_error("tables", he));
+    if (pow_dev) (void)hipFree(pow_dev);
+    pow_dev = nullptr;
     std::lock_guard<std::mutex> lock(g_kv_mu);
     g_live_kvs.insert(k);
   } catch (const std::bad_alloc&) {

@@ -12,7 +12,8 @@ import hybrid_attention as ha
     (dict(HK=0), "multiple of HK"), (dict(HQ=2048, HK=128), "1024"), (dict(rot_dim=12), "rotary_dim"), (dict(rot_dim=264), "rotary_dim"),
     (dict(rot_dim=-8), "rotary_dim"), (dict(dtype=2), "dtype"), (dict(rope_theta=0.0), "rope_theta"),
     (dict(rope_theta=float("nan")), "rope_theta"), (dict(eps=0.0), "eps"), (dict(scale=-1.0), "scale"),
-    (dict(scale=float("inf")), "scale"), (dict(n_pages=0), "n_pages"), (dict(n_layers=0), "n_layers"), (dict(max_ctx=0), "max_ctx")])
+    (dict(scale=float("inf")), "scale"), (dict(n_pages=0), "n_pages"), (dict(n_layers=0), "n_layers"), (dict(max_ctx=0), "max_ctx"),
+    (dict(max_ctx=(1 << 24) + 1), "max_ctx")])
 def test_configs(over, msg):
     with pytest.raises(ha.HAError) as ei:
         ha.PagedKV(16, **{"n_pages": 4, **over})
