@@ -7,15 +7,21 @@
 //
 // kv_few_kernel: a workgroup has 16 columns and a piece of the keys, its four waves 32 keys each in turn, with nothing shared
 // until the end. It computes S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16, straight from the codes:
-//   - a code c in bits 6..9 of an f16 whose exponent is 2^4 is the number 16 + c: with one v_perm for eight codes, a shift and
-//     an and-or for two, the operands need no arithmetic. The dot product starts at -24 sum(q) (C operand), which leaves
-//     sum(q (c - 8)) with f32 roundings only; the scale and zero of a group come in afterwards, on its 16 x 16 sums:
-//     S = sum_g s_g (q . (c - 8))_g + z_g sum(q_g).
+//   - a code c in the low bits of an f16 whose exponent is 2^10 (2^6, 2^4) is the number 1024 + c (64 + c, 16 + c): with a v_perm
+//     and an and-or for two codes, the operands need no arithmetic. K's products start at -1032 sum(q) (-72 sum(q) for the
+//     others), as the C operand, which leaves sum(q (c - 8)) with f32 roundings only; the scale and zero of a group come in
+//     afterwards, on its 16 x 16 sums: S = sum_g s_g (q . (c - 8))_g + z_g sum(q_g).
 //   - K's operand is 16 bytes of a token's row a lane, V's 8 bytes of 8 tokens' rows, two tokens' half-words joined by
 //     v_perm; S^T's layout (a column a lane) is that of P^T as an operand, so P goes from registers to registers.
-//   - V's scales go onto P (P s_g, f16), and its zeros and the -24 into one more sum for each group: Z_g = sum P z_g - 24 sum P s_g.
+//   - V's scales go onto P (P s_g, f16), and its zeros and the codes' offset into one more sum for each group:
+//     Z_g = sum P z_g - 24 sum P s_g.
 //   - a column's maximum is the wave's own; it is raised only when a score exceeds it by 2^8.
-// Pieces leave their O, maximum and sum in the workspace, and kv_merge_kernel joins them.
+// P, at most 2^8, and P s_g are rounded to f16 once each, the roundings that q and the outputs have too; everything that is summed
+// is f32. Pieces leave their O, maximum and sum in the workspace; the last of a unit's pieces joins them, or kv_merge_kernel where
+// they are many. Two workgroups a CU (228 registers for HD 256) and codes fetched a step ahead keep memory busy where there are
+// few columns: 8 sequences of 32768 tokens, 2 x 4 heads of 256, 151 MB: 35 us, 4.3 TB/s (a copy of that size 4.8). With 16 columns
+// and more it is bound by the vector instructions that unpack codes (2048 rows of 8 sequences: 458 us), which kv_many_kernel shares
+// among 128 columns (284 us, 480 TFLOP/s).
 #include <algorithm>
 #include <cmath>
 
@@ -95,23 +101,26 @@ __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf
 // sequence has lo < columns <= hi of one of two kinds (few, many); its (column block, KV head)s are units. Units of few columns
 // are cut into pieces of `chunk` keys, chosen so that all of them make about `want` pieces; those of many columns, which are only
 // used where they fill the chip, are not. A workgroup's index is its place in the list of all pieces of all sequences, which
-// each wave finds by a prefix sum with a sequence a lane. A batch of more than kScanMost sequences with few columns, and one of
-// equal sequences with many, are laid out in a grid instead (`direct`), with the host's bounds.
+// each wave finds by a prefix sum with a sequence a lane. Of more than kScanMost sequences the sums are taken once, by
+// kv_plan_kernel, and searched. Short contexts of that many sequences, and equal sequences with many columns, are laid out in a
+// grid instead (`direct`), with the host's bounds.
 constexpr int kWant = 512;                // pieces: two workgroups a CU
 constexpr size_t kSlots = 2 * kWant;      // (cut units have less than 2 kWant pieces)
 constexpr size_t kSlotBytes = (size_t)kCols * (256 + 4) * sizeof(float);
 struct Kind {
   float* p;  // results of the pieces of cut units: for each piece and column O (unnormalised) [HD], maximum, sum
   int* count;  // of a cut unit's pieces that are done, at its first piece's slot; zero between calls
+  int* plan;   // or nullptr: keys a piece; then for each sequence the sums up to and with it of its pieces, of those of them that
+               // are cut, and of its (row, head)s to be merged
   int cols;  // columns a block has, at most
-  int lo, hi, want, direct, chunk, ncb, ns;
+  int lo, hi, want, direct, ncb;
 };
 struct Item {
-  int b, kh, cb, piece, chunk, slot;  // slot: of the piece, where there is more than one
+  int b, kh, cb, piece, size, slot;  // size: keys a piece; slot: of the piece, where there is more than one
   int row;                            // of the sequence (merge)
   Seq sq;
 };
-constexpr int kScanMost = 128;
+constexpr int kScanMost = 128, kPlanMost = 65536;
 
 // a lane's sequence: its rows and units
 struct Lane {
@@ -128,57 +137,156 @@ __device__ __forceinline__ Lane lane_of(const KvArgs& a, const Kind& k, int s) {
   }
   return l;
 }
-__device__ __forceinline__ int pieces_of(int len, int chunk) { return len > chunk ? (len + chunk - 1) / chunk : 1; }
 constexpr int kUnit = kStep * kWaves;  // keys that a piece has at least
-// keys a piece: the units' keys over `want`
+constexpr int kEven = 4;               // times that, from which pieces are made even
+// a / s of 0 <= a < 2^21, s > 0: (a + 1/2) / s is 1 / (2 s) away from the next integer, its error at most a 2^-22 / s
+__device__ __forceinline__ int small_div(int a, int s) { return (int)(((float)a + 0.5f) * __builtin_amdgcn_rcpf((float)s)); }
+// Keys a piece of a sequence, a multiple of kUnit: `chunk` where that is short, else as near to it as pieces of one size come.
+// (240 sequences of 3001 tokens, us: 88 so, 135 with a short last piece.)
+__device__ __forceinline__ int size_of(int len, int chunk) {
+  const int c = chunk / kUnit, u = (len + kUnit - 1) / kUnit;
+  if (c < kEven) return chunk;
+  const int n = max(1, small_div(u + c / 2, c));
+  return small_div(u + n - 1, n) * kUnit;
+}
+__device__ __forceinline__ int pieces_of(int len, int size) {
+  const int s = size / kUnit;
+  return len > size ? small_div((len + kUnit - 1) / kUnit + s - 1, s) : 1;
+}
+// keys a piece: the keys of one KV head's units, w, over `want`
+__device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, float w) {
+  return uniform(kUnit * max(1, (int)fminf(ceilf(w * (float)a.HK / (float)(k.want * kUnit)), 1e6f)));
+}
 __device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, const Lane& first, int lane) {
   float w = (float)first.ncb * (float)first.sq.len;
   for (int s0 = 64; s0 < a.n_seqs; s0 += 64) {
     const Lane l = lane_of<kCols>(a, k, s0 + lane);
     w += (float)l.ncb * (float)l.sq.len;
   }
-  w = __builtin_bit_cast(float, lane_value(__builtin_bit_cast(int, scan64(w)), 63)) * (float)a.HK;
-  return uniform(kUnit * max(1, (int)fminf(ceilf(w / (float)(k.want * kUnit)), 1e6f)));
+  return chunk_of(a, k, __builtin_bit_cast(float, lane_value(__builtin_bit_cast(int, scan64(w)), 63)));
+}
+// Whether a unit's ns pieces are joined by the last of them, and not by kv_merge_kernel: one workgroup's loads.
+constexpr int kJoinMost = 32;
+__host__ __device__ inline bool joins(const KvArgs& a, const Kind& k, int ns) { return ns * ((k.cols * (a.HD / 4) + 64 * kWaves - 1) / (64 * kWaves)) <= kJoinMost; }
+// a sequence's pieces (with all its column blocks and KV heads), those of them that are cut, and its (row, head)s to be merged
+struct Counts {
+  int items, cut, rows;
+  int size, ns;  // of a unit's pieces
+};
+__device__ __forceinline__ Counts counts_of(const KvArgs& a, const Kind& k, const Lane& l, int chunk) {
+  const int size = size_of(l.sq.len, chunk), n = pieces_of(l.sq.len, size), items = l.ncb * n * a.HK;
+  return Counts{items, n > 1 ? items : 0, l.ncb && !joins(a, k, n) ? l.sq.n * a.HQ : 0, size, n};
+}
+
+// Kind::plan: a thread has neighbouring sequences.
+__global__ __launch_bounds__(1024) void kv_plan_kernel(KvArgs a, Kind k) {
+  __shared__ float ws[16];
+  __shared__ int tot[16][3];
+  const int tid = threadIdx.x, wave = tid >> 6, per = (a.n_seqs + 1023) / 1024, s0 = tid * per, s1 = min(s0 + per, a.n_seqs);
+  float w = 0.0f;
+  for (int s = s0; s < s1; s++) {
+    const Lane l = lane_of<kCols>(a, k, s);
+    w += (float)l.ncb * (float)l.sq.len;
+  }
+  w = scan64(w);
+  if ((tid & 63) == 63) ws[wave] = w;
+  __syncthreads();
+  w = 0.0f;
+  for (int x = 0; x < 16; x++) w += ws[x];
+  const int chunk = chunk_of(a, k, w);
+  Counts c{};
+  for (int s = s0; s < s1; s++) {
+    const Counts x = counts_of(a, k, lane_of<kCols>(a, k, s), chunk);
+    c = Counts{c.items + x.items, c.cut + x.cut, c.rows + x.rows, 0, 0};
+  }
+  const Counts in = {scan64(c.items), scan64(c.cut), scan64(c.rows), 0, 0};
+  if ((tid & 63) == 63) {
+    tot[wave][0] = in.items;
+    tot[wave][1] = in.cut;
+    tot[wave][2] = in.rows;
+  }
+  __syncthreads();
+  Counts at = {in.items - c.items, in.cut - c.cut, in.rows - c.rows, 0, 0};
+  for (int x = 0; x < wave; x++) at = Counts{at.items + tot[x][0], at.cut + tot[x][1], at.rows + tot[x][2], 0, 0};
+  if (tid == 0) k.plan[0] = chunk;
+  int* sums = k.plan + 1;
+  for (int s = s0; s < s1; s++) {
+    const Counts x = counts_of(a, k, lane_of<kCols>(a, k, s), chunk);
+    at = Counts{at.items + x.items, at.cut + x.cut, at.rows + x.rows, 0, 0};
+    sums[s] = at.items;
+    sums[kPlanMost + s] = at.cut;
+    sums[2 * kPlanMost + s] = at.rows;
+  }
+}
+// the first of n sums, in order, that is more than x, or n
+__device__ __forceinline__ int search(const int* sums, int n, int x) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  for (int step = n > 4096 ? 4096 : n > 64 ? 64 : 1; step; step >>= 6) {
+    const int last = lo + (lane + 1) * step - 1;  // of the lane's block
+    const unsigned long long past = __ballot(gp<int>(sums)[min(last, n - 1)] > x);
+    if (!past) return n;
+    lo += __builtin_ctzll(past) * step;
+  }
+  return uniform(lo);
 }
 
 // Piece x of few columns, or false where there is none.
 __device__ __forceinline__ bool find_piece(const KvArgs& a, const Kind& k, int x, Item& it) {
   const int lane = threadIdx.x & 63;
   if (k.direct) {
-    it.b = blockIdx.z;
-    it.chunk = k.chunk;
+    it.b = x;
+    it.kh = blockIdx.y;
+    it.cb = it.piece = it.slot = 0;
+    it.size = 0x7fffffff;
     it.sq = seq_of(a, it.b);
-    const int cols = it.sq.n * a.ratio;
-    it.piece = blockIdx.x;
-    it.kh = blockIdx.y / k.ncb;
-    it.cb = blockIdx.y - it.kh * k.ncb;
-    it.slot = ((it.b * a.HK + it.kh) * k.ncb + it.cb) * k.ns + it.piece;
-    return cols > k.lo && cols <= k.hi && it.cb * kCols < cols && (it.sq.ok || it.cb == 0);
+    return it.sq.n > 0;
   }
-  Lane l = lane_of<kCols>(a, k, lane);
-  it.chunk = chunk_of(a, k, l, lane);
-  int base = 0, slots = 0;
-  for (int s0 = 0;; s0 += 64) {
-    if (s0) l = lane_of<kCols>(a, k, s0 + lane);
-    const int n = pieces_of(l.sq.len, it.chunk), items = l.ncb * n * a.HK, cut = n > 1 ? items : 0, sum = scan64(items), csum = scan64(cut);
-    const unsigned long long past = __ballot(base + sum > x);
-    if (past) {
-      const int at = __builtin_ctzll(past), rel = x - base - lane_value(sum, at) + lane_value(items, at), ns = lane_value(n, at);
-      it.b = s0 + at;
-      it.slot = slots + lane_value(csum, at) - lane_value(cut, at) + rel;
-      it.sq = lane_value(l.sq, at);
-      const int unit = uniform(rel / ns), row = uniform(unit / a.HK);
-      it.piece = rel - unit * ns;
-      it.kh = unit - row * a.HK;
-      it.cb = row;
-      return true;
+  int rel, ns;  // rel: piece of the sequence; ns: pieces of a unit
+  if (k.plan) {
+    const int *sums = k.plan + 1, s = search(sums, a.n_seqs, x);
+    if (s == a.n_seqs) return false;
+    it.b = s;
+    const Lane l = lane_of<kCols>(a, k, s);
+    const Counts c = counts_of(a, k, l, gp<int>(k.plan)[0]);
+    it.size = uniform(c.size);
+    ns = uniform(c.ns);
+    rel = uniform(x - gp<int>(sums)[s] + c.items);
+    it.slot = uniform(gp<int>(sums)[kPlanMost + s] - c.cut + rel);
+    it.sq = l.sq;
+  } else {
+    Lane l = lane_of<kCols>(a, k, lane);
+    const int chunk = chunk_of(a, k, l, lane);
+    int base = 0, slots = 0;
+    for (int s0 = 0;; s0 += 64) {
+      if (s0) l = lane_of<kCols>(a, k, s0 + lane);
+      const Counts c = counts_of(a, k, l, chunk);
+      const int sum = scan64(c.items), csum = scan64(c.cut);
+      const unsigned long long past = __ballot(base + sum > x);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        rel = x - base - lane_value(sum, at) + lane_value(c.items, at);
+        it.b = s0 + at;
+        it.slot = slots + lane_value(csum, at) - lane_value(c.cut, at) + rel;
+        it.sq = lane_value(l.sq, at);
+        it.size = lane_value(c.size, at);
+        ns = lane_value(c.ns, at);
+        break;
+      }
+      base += lane_value(sum, 63);
+      slots += lane_value(csum, 63);
+      if (s0 + 64 >= a.n_seqs) return false;
     }
-    base += lane_value(sum, 63);
-    slots += lane_value(csum, 63);
-    if (s0 + 64 >= a.n_seqs) return false;
   }
+  const int unit = uniform(rel / ns);
+  it.cb = uniform(unit / a.HK);
+  it.piece = rel - unit * ns;
+  it.kh = unit - it.cb * a.HK;
+  return true;
 }
-// Column block x of many columns, or false where there is none: the last blocks, which have the most keys, first.
+// Column block x of many columns, or false where there is none: those with the most keys first (each of 64 sequences, in
+// kOrder steps of the longest; 3000, 1777, 2000 and 1000 rows of 4 sequences, us: 172 so, 246 by the blocks' numbers).
+constexpr int kOrder = 16;
 __device__ __forceinline__ bool find_block(const KvArgs& a, const Kind& k, int x, Item& it) {
   const int lane = threadIdx.x & 63;
   if (k.direct) {  // a pair's workgroups share an XCD
@@ -196,50 +304,59 @@ __device__ __forceinline__ bool find_block(const KvArgs& a, const Kind& k, int x
       x -= all;
       continue;
     }
-    for (int level = 0;; level++) {  // the last block of all 64 sequences, the last but one, ...
-      const unsigned long long has = __ballot(l.ncb > level);
-      const int n = __popcll(has) * a.HK;
+    const int before = l.sq.len - l.sq.n;
+    int left = l.ncb;  // the lane's blocks that are not yet in the list
+    for (int step = kOrder - 1;; step--) {
+      // blocks whose first row sees more than step / kOrder of the longest context (all, at last)
+      const int from = (int)((long)a.max_len * step / kOrder), low = step == 0 ? 0 : min(l.ncb, (max(from - before, 0) * a.ratio + kBigCols - 1) / kBigCols);
+      const int here = max(left - low, 0), sum = scan64(here), n = lane_value(sum, 63) * a.HK;
       if (x >= n) {
         x -= n;
+        left -= here;
         continue;
       }
-      const int nth = uniform(x / a.HK), rank = __builtin_amdgcn_mbcnt_hi((unsigned)(has >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has, 0));
-      const int at = __builtin_ctzll(__ballot(l.ncb > level && rank == nth));
+      const int nth = uniform(x / a.HK), at = __builtin_ctzll(__ballot(sum > nth));
       it.b = s0 + at;
       it.kh = x - nth * a.HK;
-      it.cb = lane_value(l.ncb, at) - 1 - level;
+      it.cb = lane_value(left, at) - 1 - (nth - lane_value(sum, at) + lane_value(here, at));
       it.sq = lane_value(l.sq, at);
       return true;
     }
   }
   return false;
 }
-// (row, head) x of the sequences of few columns that are cut, or false where there is none; it.slot: of its unit's first piece.
+// (row, head) x of those that kv_merge_kernel merges, or false where there is none; it.slot: of its unit's first piece.
 __device__ __forceinline__ bool find_row(const KvArgs& a, const Kind& k, int x, int& h, Item& it) {
   const int lane = threadIdx.x & 63;
-  int rel = x, ns = k.ns, slot = 0;
-  if (k.direct) {
-    it.b = blockIdx.y;
-    it.chunk = k.chunk;
-    it.sq = seq_of(a, it.b);
-    const int cols = it.sq.n * a.ratio;
-    if (cols <= k.lo || cols > k.hi || !it.sq.ok || rel >= it.sq.n * a.HQ) return false;
+  int rel, ns, slot = 0;
+  if (k.plan) {
+    const int *sums = k.plan + 1, s = search(sums + 2 * kPlanMost, a.n_seqs, x);
+    if (s == a.n_seqs) return false;
+    it.b = s;
+    const Lane l = lane_of<kCols>(a, k, s);
+    const Counts c = counts_of(a, k, l, gp<int>(k.plan)[0]);
+    it.size = uniform(c.size);
+    ns = uniform(c.ns);
+    rel = uniform(x - gp<int>(sums)[2 * kPlanMost + s] + c.rows);
+    slot = uniform(gp<int>(sums)[kPlanMost + s] - c.cut);
+    it.sq = l.sq;
   } else {
     Lane l = lane_of<kCols>(a, k, lane);
-    it.chunk = chunk_of(a, k, l, lane);
+    const int chunk = chunk_of(a, k, l, lane);
     int base = 0;
     for (int s0 = 0;; s0 += 64) {
       if (s0) l = lane_of<kCols>(a, k, s0 + lane);
-      const int n = pieces_of(l.sq.len, it.chunk), rows = n > 1 && l.ncb ? l.sq.n * a.HQ : 0, cut = n > 1 ? l.ncb * n * a.HK : 0;
-      const int sum = scan64(rows), csum = scan64(cut);
+      const Counts c = counts_of(a, k, l, chunk);
+      const int sum = scan64(c.rows), csum = scan64(c.cut);
       const unsigned long long past = __ballot(base + sum > x);
       if (past) {
         const int at = __builtin_ctzll(past);
         it.b = s0 + at;
-        rel = x - base - lane_value(sum, at) + lane_value(rows, at);
-        slot += lane_value(csum, at) - lane_value(cut, at);
-        ns = lane_value(n, at);
+        rel = x - base - lane_value(sum, at) + lane_value(c.rows, at);
+        slot += lane_value(csum, at) - lane_value(c.cut, at);
         it.sq = lane_value(l.sq, at);
+        it.size = lane_value(c.size, at);
+        ns = lane_value(c.ns, at);
         break;
       }
       base += lane_value(sum, 63);
@@ -251,7 +368,7 @@ __device__ __forceinline__ bool find_row(const KvArgs& a, const Kind& k, int x, 
   h = rel - it.row * a.HQ;
   it.kh = a.by_ratio(h);
   it.cb = (it.row * a.ratio + h - it.kh * a.ratio) / kCols;
-  it.slot = k.direct ? ((it.b * a.HK + it.kh) * k.ncb + it.cb) * k.ns : slot + (it.cb * a.HK + it.kh) * ns;
+  it.slot = slot + (it.cb * a.HK + it.kh) * ns;
   return true;
 }
 // byte offset of a piece's column among the results: O [HD], maximum, sum, padding
@@ -265,11 +382,6 @@ __device__ __forceinline__ void put4(__amdgpu_buffer_rsrc_t rs, unsigned at, f4 
 __device__ __forceinline__ f4 get4(__amdgpu_buffer_rsrc_t rs, unsigned at) {
   return __builtin_bit_cast(f4, __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, kCacheSc1));
 }
-// Whether a unit's ns pieces are joined by the last of them, and not by kv_merge_kernel: one workgroup's loads.
-constexpr int kJoinMost = 32;
-template <int HD>
-__host__ __device__ inline bool joins(const Kind& k, int ns) { return ns * ((k.cols * (HD / 4) + 64 * kWaves - 1) / (64 * kWaves)) <= kJoinMost; }
-
 // The rows of a sequence that does not fit its batch.
 template <int HD>
 __device__ __forceinline__ void nan_rows(const KvArgs& a, const Seq& sq, int kh, int threads) {
@@ -304,7 +416,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
   if (!find_piece(a, kind, blockIdx.x, it)) return;
   const __amdgpu_buffer_rsrc_t rs = __builtin_amdgcn_make_buffer_rsrc(kind.p, 0, (int)(kSlots * kSlotBytes), 0x00020000);
   const Seq sq = it.sq;
-  const int kh = it.kh, b = it.b, k0 = it.piece * it.chunk, c0 = it.cb * kCols, cols = min(kCols, sq.n * ratio - c0);
+  const int kh = it.kh, b = it.b, k0 = it.piece * it.size, c0 = it.cb * kCols, cols = min(kCols, sq.n * ratio - c0);
   if (!sq.ok) {
     if (it.piece == 0) nan_rows<HD>(a, sq, kh, 64 * kWaves);
     return;
@@ -315,7 +427,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
   const int before = sq.len - sq.n;
   const int keys = before + a.by_ratio(c0 + cols - 1) + 1;
   if (k0 >= keys) return;
-  const int k1 = min(k0 + it.chunk, keys);
+  const int k1 = min(k0 + it.size, keys);
   const int all = before + a.by_ratio(c0) + 1;  // keys below this are seen by every column
   const int r = c0 + min(j, cols - 1), ri = a.by_ratio(r), last = before + ri;  // columns behind the last one repeat it
   h8 q[kH][4];
@@ -566,7 +678,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
         l += f * ml[w][c][1];
         v += f * *reinterpret_cast<const f4*>(ol + (w * (kCols / 2) + c - h0) * kPitch + ch);
       }
-      if (keys > it.chunk) {
+      if (keys > it.size) {
         const unsigned at = column_at<HD>(kind, it.slot, c);
         put4(rs, at + 4 * ch, v);
         if (ch == 0) put4(rs, at + 4 * HD, f4{mm, l, 0.0f, 0.0f});
@@ -575,8 +687,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
       }
     }
   }
-  const int ns = pieces_of(keys, it.chunk);
-  if (ns <= 1 || !joins<HD>(kind, ns)) return;
+  const int ns = pieces_of(keys, it.size);
+  if (ns <= 1 || !joins(a, kind, ns)) return;
 
   // The last of a unit's pieces to get here joins them. Their results go past the XCDs' caches (sc1), and the count of those that
   // are written is taken when they are there; the last one clears it for the next call. Nobody waits.
@@ -628,7 +740,10 @@ struct ManyLds {
 // A workgroup has 128 columns and walks the keys in tiles of 32. Four of its eight waves compute P (32 columns each: S^T = K Q^T on
 // v_mfma_f32_32x32x16_f16, scales and zeros, online softmax) and unpack the next tile's keys into LDS, the other four the outputs
 // of the tile before (64 columns and half the channels each: O^T = V^T P^T) and this tile's values; each SIMD has one of either
-// kind, so the matrix products of the one run beside the vector instructions of the other. One barrier a tile. Scales and zeros
+// kind, so the matrix products of the one run beside the vector instructions of the other. One barrier a tile, which takes about
+// 3700 cycles (HD 256): matrix products 1060 of them a SIMD, vector instructions about 2150, LDS about 2000 (250 KB read and
+// written), each waiting for the others at times; with 64 columns a wave that compute P, or the values unpacked by both kinds,
+// it took longer (spills; 311 us instead of 296 for 2048 rows of 8 sequences). Scales and zeros
 // stay apart from the codes, so that both operands are exact: S = sum_g s_g (q . (c - 8))_g + sum_g z_g sum(q_g), the last
 // as one more product (with sum(q_g) / G as two f16), and O takes P s_g, rounded to f16 once, and sum P z_g.
 template <int HD>
@@ -979,7 +1094,7 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
 }
 
 // out of one (row, head) from its pieces: thread (k, c) adds pieces k, k + blockDim / (HD / 4), ... of channels 4 c .. + 3.
-constexpr int kMergeMost = 2048;  // pieces
+constexpr int kMergeMost = kSlots;  // pieces
 template <int HD>
 __global__ __launch_bounds__(1024) void kv_merge_kernel(KvArgs a, Kind kind) {
   constexpr int C = HD / 4;
@@ -991,8 +1106,8 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvArgs a, Kind kind) {
   if (!find_row(a, kind, blockIdx.x, h, it)) return;
   const Seq sq = it.sq;
   const int t = sq.r0 + it.row, c = it.row * a.ratio + h - it.kh * a.ratio - it.cb * kCols, end = min((it.cb + 1) * kCols, sq.n * a.ratio);
-  const int keys = sq.len - sq.n + a.by_ratio(end - 1) + 1, ns = pieces_of(keys, it.chunk);
-  if (ns <= 1 || joins<HD>(kind, ns)) return;
+  const int keys = sq.len - sq.n + a.by_ratio(end - 1) + 1, ns = pieces_of(keys, it.size);
+  if (joins(a, kind, ns)) return;
   const float* p = kind.p + column_at<HD>(kind, it.slot, c) / 4;
   const size_t step = (size_t)kind.cols * (HD + 4);
   const int k = tid / C, n = blockDim.x / C, ch = 4 * (tid % C), wave = tid >> 6, waves = blockDim.x >> 6;
@@ -1053,16 +1168,25 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvArgs a, Kind kind) {
 }
 
 // Which kernel serves a sequence. A unit of many columns is one workgroup that walks all its keys, so they pay where there are
-// enough for the chip. Measured, us, few columns' kernel / many columns': 2048 rows of 2, 3, 4, 8 sequences (256, 384, 512, 1024
-// units) 128 / 120, 176 / 125, 229 / 152, 458 / 284; 4096 rows of one (256) 210 / 220; ragged, 7777 rows of 4 (486) 249 / 258;
-// heads of 128: 2048 rows of one (512) 152 / 108, 100 rows after 500 of 16 sequences (400) 83 / 67, prefills and decode steps in
-// one batch (296) 81 / 131. Up to kFewCols columns a sequence stays with the first also beside others that do not.
-constexpr int kFewCols = 256, kManyUnits = 384;
+// enough units for the longest of them, about 1.5 us for 32 keys, to end with the others: units x (mean keys / most keys) is at
+// least kManyUnits, with the mean as in a batch of equal sequences, or half of the most where they are not. Measured, us, few
+// columns' kernel / many columns', with that product: the model's heads, rows of n sequences without a prefix, 4096 of 1 (128)
+// 197 / 219, 2048 of 2 (128) 126 / 121, of 3 (192) 175 / 120, of 8 (512) 430 / 281; 300, 500 rows after 1000 of 8 (133, 208)
+// 81 / 83, 132 / 94; 3000, 1777, 2000, 1000 rows (243) 218 / 172; 2 or 4 of 1500 rows after 500, 2 of 600, 30 single ones (132,
+// 226) 120 / 133, 205 / 163; 32 heads of 128 on 8: 1000, 1200, 1500 rows of one (125, 150, 187) 50 / 55, 69 / 64, 95 / 78; 777
+// rows, 130 after 2000, 300 after 64, 8 single ones (152) 71 / 118; 100 rows after 500 of 16 (366) 86 / 76. Up to kFewCols columns
+// a sequence stays with the first also beside others that do not.
+constexpr int kFewCols = 256, kManyUnits = 160;
+// Contexts up to which more than kScanMost sequences are neither cut nor planned. Measured, us, in a grid / planned: single rows of
+// 140 sequences of 100, 1000, 3000 tokens 8.2 / 12.2, 25.6 / 31.6, 64.6 / 62.8, of 1000 sequences of 10 tokens 22 / 30, of 200 of
+// 300 and one of 20000 250 / 26.
+constexpr int kDirectKeys = 1024;
 template <int HD>
 hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
   const int most = a.max_rows * a.ratio;  // columns a sequence has, at most
   const bool equal = (long)a.n_rows == (long)a.n_seqs * a.max_rows;
-  const bool use_many = most > kFewCols && (long)a.n_rows * a.ratio / kBigCols * a.HK >= kManyUnits;
+  const double units_of_many = (double)a.n_rows * a.ratio / kBigCols * a.HK;
+  const bool use_many = most > kFewCols && units_of_many * (equal ? 1.0 - 0.5 * a.max_rows / a.max_len : 0.5) >= kManyUnits;
   Kind few{}, many{};
   few.p = ws;
   few.count = reinterpret_cast<int*>(ws + kSlots * kSlotBytes / sizeof(float));
@@ -1085,27 +1209,28 @@ hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
   few.ncb = (std::min(most, few.hi) + kCols - 1) / kCols;
   const long units = std::min<long>((long)a.n_seqs * few.ncb, (long)a.n_rows * a.ratio / kCols + a.n_seqs) * a.HK;
   dim3 grid((unsigned)(units + (a.max_len > kUnit ? kSlots : 0)));
-  dim3 merge((unsigned)std::min<long>((long)a.n_rows * a.HQ, (long)kWant * kCols));  // a unit that is cut has kCols columns at most
-  if (a.n_seqs > kScanMost && few.ncb == 1) {
-    few.direct = 1;
-    const long all = (long)a.n_seqs * a.HK;
-    long c = std::max<long>((all * a.max_len / (2 * kWant) + kUnit - 1) / kUnit * kUnit, kUnit);
-    while ((a.max_len + c - 1) / c > 1 && ((size_t)all * ((a.max_len + c - 1) / c) > kSlots || (a.max_len + c - 1) / c > kMergeMost)) c *= 2;
-    few.chunk = (int)std::min<long>(c, 1 << 30);
-    few.ns = (int)((a.max_len + c - 1) / c);
-    grid = dim3(few.ns, a.HK, a.n_seqs);
-    merge = dim3(most * a.HK, a.n_seqs);
+  if (a.n_seqs > kScanMost) {
+    if (few.ncb == 1 && a.max_len <= kDirectKeys) {
+      few.direct = 1;
+      grid = dim3((unsigned)a.n_seqs, (unsigned)a.HK);
+    } else {
+      few.plan = few.count + kSlots;
+      hipLaunchKernelGGL(kv_plan_kernel, dim3(1), dim3(1024), 0, s, a, few);
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+    }
   }
   hipLaunchKernelGGL((kv_few_kernel<HD>), grid, dim3(64 * kWaves), 0, s, a, few);
-  if ((e = hipGetLastError()) != hipSuccess || a.max_len <= kUnit || (few.direct && few.ns == 1)) return e;
-  if (joins<HD>(few, (a.max_len + kUnit - 1) / kUnit)) return e;  // whatever the chunk
-  hipLaunchKernelGGL((kv_merge_kernel<HD>), merge, dim3(a.max_len > 16 * kUnit && !few.direct ? 1024 : 256), 0, s, a, few);
+  if ((e = hipGetLastError()) != hipSuccess || a.max_len <= kUnit || few.direct) return e;
+  if (joins(a, few, (a.max_len + kUnit - 1) / kUnit)) return e;  // whatever the chunk
+  // units of c columns that are not joined have more than 128 / c pieces of less than kSlots in all: at most 8 c^2 (row, head)s
+  const long rows = std::min<long>((long)a.n_rows * a.HQ, 8 * kCols * kCols);
+  hipLaunchKernelGGL((kv_merge_kernel<HD>), dim3((unsigned)rows), dim3(a.max_len > 16 * kUnit && rows <= 512 ? 1024 : 256), 0, s, a, few);
   return hipGetLastError();
 }
 
 }  // namespace
 
-size_t kv_workspace_bytes() { return kSlots * (kSlotBytes + sizeof(int)); }
+size_t kv_workspace_bytes() { return kSlots * (kSlotBytes + sizeof(int)) + sizeof(int) * (1 + 3 * (size_t)kPlanMost); }
 
 hipError_t launch_kv_attention(const KvArgs& a, void* ws, hipStream_t s) {
   return a.HD == 256 ? attend<256>(a, static_cast<float*>(ws), s) : attend<128>(a, static_cast<float*>(ws), s);

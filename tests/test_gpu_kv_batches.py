@@ -137,3 +137,26 @@ def test_append_of_one_long_sequence_that_does_not_fit():
         assert np.isnan(x[bad]).all() and np.isfinite(x[~bad]).all()
     changed = set(np.nonzero((pool != before).any(axis=(1, 2, 3)))[0])
     assert changed == {int(c.table[b, p // 16]) for b in (0, 1, 3, 4, 5, 7) for p in range(c.lens[b] - (c.start[b + 1] - c.start[b]), c.lens[b])}
+
+
+# more than 128 sequences: contexts of up to 1024 keys in a grid, others by a plan of the pieces
+@pytest.mark.parametrize("n,heads,long,rows", [
+    (129, MODEL, 1100, 1), (300, (3, 1, 256, 0), 5000, 1), (150, H8, 2100, 5), (200, (4, 4, 128, 64), 300, 7), (1500, H8, 1500, 1),
+    (5000, (16, 1, 128, 8), 1700, 1), (4500, (16, 1, 128, 8), 20, 1), (140, H16, 3100, 40)])
+def test_plans(n, heads, long, rows):
+    """Some sequences longer than a piece, some without rows, some that do not fit."""
+    rng = np.random.default_rng(n)
+    seqs = [(int(p), int(r)) for p, r in zip(rng.integers(0, 30, n), rng.integers(0, 2, n))]
+    for at in (0, 3, n // 2, n - 1):
+        seqs[at] = (int(long * rng.uniform(0.4, 1.0)), rows)
+    c = Call(seqs, heads, 16, heads[2] == 256, seed=n)
+    lens = c.lens.copy()
+    bad = [b for b in (2, n // 3, n - 2) if seqs[b][1]]
+    lens[bad] = -1
+    c.dev[1].copy_(c.torch.from_numpy(lens))
+    got = c.attention()
+    out = np.zeros(c.T, bool)
+    for b in bad:
+        out[c.start[b]:c.start[b + 1]] = True
+    assert np.isnan(got[out]).all() and np.isfinite(got[~out]).all()
+    check(got, c.expected(rows={t for t in some(c) if not out[t]}))
