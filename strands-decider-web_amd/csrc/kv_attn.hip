@@ -165,7 +165,9 @@ __device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, const La
   }
   return chunk_of(a, k, __builtin_bit_cast(float, lane_value(__builtin_bit_cast(int, scan64(w)), 63)));
 }
-// Whether a unit's ns pieces are joined by the last of them, and not by kv_merge_kernel: one workgroup's loads.
+// Whether a unit's ns pieces are joined by the last of them, and not by kv_merge_kernel: the loads that a thread would make. Measured,
+// us, joined / merged: 61 rows after 500 (5 pieces of 16 columns) 14.5 / 19.2, after 1531 (13) 23.0 / 16.7; one row after 4000 (32
+// pieces of 4 columns) 11.6 / 12.4, after 8000 (63) 15.3 / 12.6.
 constexpr int kJoinMost = 32;
 __host__ __device__ inline bool joins(const KvArgs& a, const Kind& k, int ns) { return ns * ((k.cols * (a.HD / 4) + 64 * kWaves - 1) / (64 * kWaves)) <= kJoinMost; }
 // a sequence's pieces (with all its column blocks and KV heads), those of them that are cut, and its (row, head)s to be merged
@@ -391,13 +393,16 @@ __device__ __forceinline__ void nan_rows(const KvArgs& a, const Seq& sq, int kh,
     *gpw<h4>(a.out + ((size_t)(sq.r0 + i) * a.HQ + kh * a.ratio + r - i * a.ratio) * HD + 4 * (threadIdx.x % (HD / 4))) = h4{x, x, x, x};
   }
 }
-// Channels ch .. + 3 of column r: O / l, the gate, f16.
+// Channels ch .. + 3 of column r: the gate, and with it O / l as f16.
+__device__ __forceinline__ f4 gate_of(const KvArgs& a, const Seq& sq, int kh, int r, int ch) {
+  const int i = a.by_ratio(r);
+  return a.gated ? gate4(a, sq.r0 + i, kh * a.ratio + r - i * a.ratio, ch) : f4{};
+}
 template <int HD>
-__device__ __forceinline__ void finish(const KvArgs& a, const Seq& sq, int kh, int r, int ch, f4 v, float inv) {
+__device__ __forceinline__ void finish(const KvArgs& a, const Seq& sq, int kh, int r, int ch, f4 v, float inv, const f4& gt) {
   const int i = a.by_ratio(r), t = sq.r0 + i, h = kh * a.ratio + r - i * a.ratio;
   v *= inv;
   if (a.gated) {
-    const f4 gt = gate4(a, t, h, ch);
 #pragma unroll
     for (int e = 0; e < 4; e++) v[e] *= sigmoid(gt[e]);
   }
@@ -651,6 +656,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
   }
   for (int h0 = 0; h0 < cols; h0 += kCols / 2) {  // half of the columns at a time (LDS)
     if (h0) __syncthreads();
+    constexpr int kEach = (kCols / 2) * (HD / 4) / (64 * kWaves);
+    const int left = min(kCols / 2, cols - h0) * (HD / 4);
+    f4 gt[kEach];
+    if (keys <= it.size) {  // (loaded before the others are waited for)
+#pragma unroll
+      for (int n = 0; n < kEach; n++) {
+        const int k = min(tid + n * 64 * kWaves, left - 1);
+        gt[n] = gate_of(a, sq, kh, c0 + h0 + k / (HD / 4), 4 * (k % (HD / 4)));
+      }
+    }
     if (j >= h0 && j < min(h0 + kCols / 2, cols)) {
       float* d = ol + (wave * (kCols / 2) + j - h0) * kPitch;
 #pragma unroll
@@ -666,7 +681,10 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
         }
     }
     __syncthreads();
-    for (int k = tid; k < min(kCols / 2, cols - h0) * (HD / 4); k += 64 * kWaves) {
+#pragma unroll
+    for (int n = 0; n < kEach; n++) {
+      const int k = tid + n * 64 * kWaves;
+      if (k >= left) break;
       const int c = h0 + k / (HD / 4), ch = 4 * (k % (HD / 4));
       float mm = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -683,7 +701,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
         put4(rs, at + 4 * ch, v);
         if (ch == 0) put4(rs, at + 4 * HD, f4{mm, l, 0.0f, 0.0f});
       } else {
-        finish<HD>(a, sq, kh, c0 + c, ch, v, 1.0f / l);
+        finish<HD>(a, sq, kh, c0 + c, ch, v, 1.0f / l, gt[n]);
       }
     }
   }
@@ -700,25 +718,35 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
   __syncthreads();
   if (!is_last) return;
   if (tid == 0) __hip_atomic_store(kind.count + first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  f4* wl = reinterpret_cast<f4*>(ol);  // [column][piece]: maximum, sum
-  for (int k = tid; k < cols * ns; k += 64 * kWaves) {
-    const int c = k / ns;
-    wl[k] = get4(rs, column_at<HD>(kind, first + k - c * ns, c) + 4 * HD);
-  }
-  __syncthreads();
   for (int k = tid; k < cols * (HD / 4); k += 64 * kWaves) {
     const int c = k / (HD / 4), ch = 4 * (k % (HD / 4));
+    const f4 gt = gate_of(a, sq, kh, c0 + c, ch);
     float mm = -INFINITY, l = 0.0f;
-    for (int s = 0; s < ns; s++) mm = fmaxf(mm, wl[c * ns + s][0]);
     f4 v = {};
-#pragma unroll 8
-    for (int s = 0; s < ns; s++) {
-      const f4 w = wl[c * ns + s];
-      const float f = w[0] == mm ? 1.0f : __builtin_amdgcn_exp2f(w[0] - mm);
-      l += f * w[1];
-      v += f * get4(rs, column_at<HD>(kind, first + s, c) + 4 * ch);
+    constexpr int kAt = 8;  // pieces whose maxima, sums and O are loaded at once
+    for (int s0 = 0; s0 < ns; s0 += kAt) {
+      f4 w[kAt], x[kAt];
+#pragma unroll
+      for (int n = 0; n < kAt; n++) {
+        const unsigned at = column_at<HD>(kind, first + min(s0 + n, ns - 1), c);
+        w[n] = get4(rs, at + 4 * HD);
+        x[n] = get4(rs, at + 4 * ch);
+      }
+      float mx = mm;
+#pragma unroll
+      for (int n = 0; n < kAt; n++) mx = fmaxf(mx, w[n][0]);
+      const float al = mm == mx ? 1.0f : __builtin_amdgcn_exp2f(mm - mx);
+      mm = mx;
+      l *= al;
+      v *= al;
+#pragma unroll
+      for (int n = 0; n < kAt; n++) {
+        const float f = s0 + n >= ns ? 0.0f : w[n][0] == mm ? 1.0f : __builtin_amdgcn_exp2f(w[n][0] - mm);
+        l += f * w[n][1];
+        v += f * x[n];
+      }
     }
-    finish<HD>(a, sq, kh, c0 + c, ch, v, 1.0f / l);
+    finish<HD>(a, sq, kh, c0 + c, ch, v, 1.0f / l, gt);
   }
 }
 
@@ -1088,7 +1116,7 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
         }
         v += zz[gg];
         const int ch = G * (2 * dh + gg) + 4 * i;
-        finish<HD>(a, sq, kh, c0 + c, ch, v, inv);
+        finish<HD>(a, sq, kh, c0 + c, ch, v, inv, gate_of(a, sq, kh, c0 + c, ch));
       }
   }
 }
