@@ -109,7 +109,7 @@ constexpr size_t kSlots = 2 * kWant;      // (cut units have less than 2 kWant p
 constexpr size_t kSlotBytes = (size_t)kCols * (256 + 4) * sizeof(float);
 struct Kind {
   float* p;  // results of the pieces of cut units: for each piece and column O (unnormalised) [HD], maximum, sum
-  int* count;  // of a cut unit's pieces that are done, at its first piece's slot; zero between calls
+  int* count;  // of a cut unit's pieces (a group's) that are done, at the first one's slot, then of its groups; zero between calls
   int* plan;   // or nullptr: keys a piece; then for each sequence the sums up to and with it of its pieces, of those of them that
                // are cut, and of its (row, head)s to be merged
   int cols;  // columns a block has, at most
@@ -165,11 +165,17 @@ __device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, const La
   }
   return chunk_of(a, k, __builtin_bit_cast(float, lane_value(__builtin_bit_cast(int, scan64(w)), 63)));
 }
-// Whether a unit's ns pieces are joined by the last of them, and not by kv_merge_kernel: the loads that a thread would make. Measured,
-// us, joined / merged: 61 rows after 500 (5 pieces of 16 columns) 14.5 / 19.2, after 1531 (13) 23.0 / 16.7; one row after 4000 (32
-// pieces of 4 columns) 11.6 / 12.4, after 8000 (63) 15.3 / 12.6.
+// A unit's ns pieces are joined by the last of them, or by the last of each group of neighbours and then the last of the groups, or
+// by kv_merge_kernel. The pieces of a group (ns: one group), or 0 for the merge: joining costs what a thread loads one after the other.
+// Measured, us, joined / merged: 61 rows after 500 (5 pieces of 16 columns) 14.5 / 19.2, after 1531 (13) 23.0 / 16.7; 2 after 8000
+// (63 of 8 columns, groups of 16) 16.0 / 12.9; one row (4 columns) after 8000 (63) 10.7 / 12.9, after 20000 (157) 15.3 / 16.5, after
+// 131071 (512) 24.8 / 26.8; 4 sequences of 8000 (63) 13.7 / 15.5; after 4000 (32) 10.3 in groups, 11.6 at once.
 constexpr int kJoinMost = 32;
-__host__ __device__ inline bool joins(const KvArgs& a, const Kind& k, int ns) { return ns * ((k.cols * (a.HD / 4) + 64 * kWaves - 1) / (64 * kWaves)) <= kJoinMost; }
+__host__ __device__ inline int group_of(const KvArgs& a, const Kind& k, int ns) {
+  const int per = (k.cols * (a.HD / 4) + 64 * kWaves - 1) / (64 * kWaves);  // columns' channels a thread
+  if (per > 1) return ns * per <= kJoinMost ? ns : 0;
+  return ns <= 16 ? ns : ns <= 64 ? 8 : ns <= 256 ? 16 : 32;
+}
 // a sequence's pieces (with all its column blocks and KV heads), those of them that are cut, and its (row, head)s to be merged
 struct Counts {
   int items, cut, rows;
@@ -177,7 +183,7 @@ struct Counts {
 };
 __device__ __forceinline__ Counts counts_of(const KvArgs& a, const Kind& k, const Lane& l, int chunk) {
   const int size = size_of(l.sq.len, chunk), n = pieces_of(l.sq.len, size), items = l.ncb * n * a.HK;
-  return Counts{items, n > 1 ? items : 0, l.ncb && !joins(a, k, n) ? l.sq.n * a.HQ : 0, size, n};
+  return Counts{items, n > 1 ? items : 0, l.ncb && !group_of(a, k, n) ? l.sq.n * a.HQ : 0, size, n};
 }
 
 // Kind::plan: a thread has neighbouring sequences.
@@ -705,47 +711,80 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
       }
     }
   }
-  const int ns = pieces_of(keys, it.size);
-  if (ns <= 1 || !joins(a, kind, ns)) return;
+  const int ns = pieces_of(keys, it.size), group = group_of(a, kind, ns);
+  if (ns <= 1 || !group) return;
 
-  // The last of a unit's pieces to get here joins them. Their results go past the XCDs' caches (sc1), and the count of those that
-  // are written is taken when they are there; the last one clears it for the next call. Nobody waits.
+  // The last of a group's pieces to get here joins them, and the last of the groups those. What they write goes past the XCDs' caches
+  // (sc1), and is counted when it is there; the last one clears the count for the next call. Nobody waits.
   const int first = it.slot - it.piece;
   __shared__ int is_last;
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (tid == 0) is_last = __hip_atomic_fetch_add(kind.count + first, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == ns - 1;
-  __syncthreads();
-  if (!is_last) return;
-  if (tid == 0) __hip_atomic_store(kind.count + first, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  for (int k = tid; k < cols * (HD / 4); k += 64 * kWaves) {
-    const int c = k / (HD / 4), ch = 4 * (k % (HD / 4));
-    const f4 gt = gate_of(a, sq, kh, c0 + c, ch);
-    float mm = -INFINITY, l = 0.0f;
+  auto last_of = [&](int* count, int n) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (tid == 0) {
+      const bool x = __hip_atomic_fetch_add(count, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == n - 1;
+      if (x) __hip_atomic_store(count, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      is_last = x;
+    }
+    __syncthreads();
+    return is_last != 0;
+  };
+  // channels ch .. + 3 of column c over the results s0, s0 + stride, ... (n of them): O, maximum, sum
+  auto join = [&](int s0, int stride, int n, int c, int ch, float& mm, float& l) {
     f4 v = {};
-    constexpr int kAt = 8;  // pieces whose maxima, sums and O are loaded at once
-    for (int s0 = 0; s0 < ns; s0 += kAt) {
+    mm = -INFINITY;
+    l = 0.0f;
+    constexpr int kAt = 8;  // loaded at once
+    for (int x0 = 0; x0 < n; x0 += kAt) {
       f4 w[kAt], x[kAt];
 #pragma unroll
-      for (int n = 0; n < kAt; n++) {
-        const unsigned at = column_at<HD>(kind, first + min(s0 + n, ns - 1), c);
-        w[n] = get4(rs, at + 4 * HD);
-        x[n] = get4(rs, at + 4 * ch);
+      for (int e = 0; e < kAt; e++) {
+        const unsigned at = column_at<HD>(kind, s0 + min(x0 + e, n - 1) * stride, c);
+        w[e] = get4(rs, at + 4 * HD);
+        x[e] = get4(rs, at + 4 * ch);
       }
       float mx = mm;
 #pragma unroll
-      for (int n = 0; n < kAt; n++) mx = fmaxf(mx, w[n][0]);
+      for (int e = 0; e < kAt; e++) mx = fmaxf(mx, w[e][0]);
       const float al = mm == mx ? 1.0f : __builtin_amdgcn_exp2f(mm - mx);
       mm = mx;
       l *= al;
       v *= al;
 #pragma unroll
-      for (int n = 0; n < kAt; n++) {
-        const float f = s0 + n >= ns ? 0.0f : w[n][0] == mm ? 1.0f : __builtin_amdgcn_exp2f(w[n][0] - mm);
-        l += f * w[n][1];
-        v += f * x[n];
+      for (int e = 0; e < kAt; e++) {
+        const float f = x0 + e >= n ? 0.0f : w[e][0] == mm ? 1.0f : __builtin_amdgcn_exp2f(w[e][0] - mm);
+        l += f * w[e][1];
+        v += f * x[e];
       }
     }
+    return v;
+  };
+  int s0 = first, stride = 1, n = ns;
+  if (group < ns) {
+    s0 = first + it.piece / group * group;
+    n = min(group, first + ns - s0);
+    if (!last_of(kind.count + s0, n)) return;
+    for (int k0 = 0; k0 < cols * (HD / 4); k0 += 64 * kWaves) {
+      const int k = k0 + tid, c = min(k / (HD / 4), cols - 1), ch = 4 * (k % (HD / 4));
+      float mm, l;
+      const f4 v = join(s0, 1, n, c, ch, mm, l);
+      __syncthreads();  // (the sum is written over one of those that were read)
+      if (k < cols * (HD / 4)) {
+        const unsigned at = column_at<HD>(kind, s0, c);
+        put4(rs, at + 4 * ch, v);
+        if (ch == 0) put4(rs, at + 4 * HD, f4{mm, l, 0.0f, 0.0f});
+      }
+    }
+    s0 = first;
+    stride = group;
+    n = (ns + group - 1) / group;
+  }
+  if (!last_of(kind.count + (group < ns ? (int)kSlots : 0) + first, n)) return;
+  for (int k = tid; k < cols * (HD / 4); k += 64 * kWaves) {
+    const int c = k / (HD / 4), ch = 4 * (k % (HD / 4));
+    const f4 gt = gate_of(a, sq, kh, c0 + c, ch);
+    float mm, l;
+    const f4 v = join(s0, stride, n, c, ch, mm, l);
     finish<HD>(a, sq, kh, c0 + c, ch, v, 1.0f / l, gt);
   }
 }
@@ -1135,7 +1174,7 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvArgs a, Kind kind) {
   const Seq sq = it.sq;
   const int t = sq.r0 + it.row, c = it.row * a.ratio + h - it.kh * a.ratio - it.cb * kCols, end = min((it.cb + 1) * kCols, sq.n * a.ratio);
   const int keys = sq.len - sq.n + a.by_ratio(end - 1) + 1, ns = pieces_of(keys, it.size);
-  if (joins(a, kind, ns)) return;
+  if (group_of(a, kind, ns)) return;
   const float* p = kind.p + column_at<HD>(kind, it.slot, c) / 4;
   const size_t step = (size_t)kind.cols * (HD + 4);
   const int k = tid / C, n = blockDim.x / C, ch = 4 * (tid % C), wave = tid >> 6, waves = blockDim.x >> 6;
@@ -1242,15 +1281,15 @@ hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
       few.direct = 1;
       grid = dim3((unsigned)a.n_seqs, (unsigned)a.HK);
     } else {
-      few.plan = few.count + kSlots;
+      few.plan = few.count + 2 * kSlots;
       hipLaunchKernelGGL(kv_plan_kernel, dim3(1), dim3(1024), 0, s, a, few);
       if ((e = hipGetLastError()) != hipSuccess) return e;
     }
   }
   hipLaunchKernelGGL((kv_few_kernel<HD>), grid, dim3(64 * kWaves), 0, s, a, few);
   if ((e = hipGetLastError()) != hipSuccess || a.max_len <= kUnit || few.direct) return e;
-  if (joins(a, few, (a.max_len + kUnit - 1) / kUnit)) return e;  // whatever the chunk
-  // units of c columns that are not joined have more than 128 / c pieces of less than kSlots in all: at most 8 c^2 (row, head)s
+  if (group_of(a, few, (int)std::min<size_t>((a.max_len + kUnit - 1) / kUnit, kSlots))) return e;  // whatever the chunk: more pieces, more loads
+  // units of c columns that are not joined have more than 128 / c pieces, of at most kSlots in all: 8 c^2 (row, head)s
   const long rows = std::min<long>((long)a.n_rows * a.HQ, 8 * kCols * kCols);
   hipLaunchKernelGGL((kv_merge_kernel<HD>), dim3((unsigned)rows), dim3(a.max_len > 16 * kUnit && rows <= 512 ? 1024 : 256), 0, s, a, few);
   return hipGetLastError();
@@ -1258,7 +1297,7 @@ hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
 
 }  // namespace
 
-size_t kv_workspace_bytes() { return kSlots * (kSlotBytes + sizeof(int)) + sizeof(int) * (1 + 3 * (size_t)kPlanMost); }
+size_t kv_workspace_bytes() { return kSlots * (kSlotBytes + 2 * sizeof(int)) + sizeof(int) * (1 + 3 * (size_t)kPlanMost); }
 
 hipError_t launch_kv_attention(const KvArgs& a, void* ws, hipStream_t s) {
   return a.HD == 256 ? attend<256>(a, static_cast<float*>(ws), s) : attend<128>(a, static_cast<float*>(ws), s);

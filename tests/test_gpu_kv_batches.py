@@ -160,3 +160,19 @@ def test_plans(n, heads, long, rows):
         out[c.start[b]:c.start[b + 1]] = True
     assert np.isnan(got[out]).all() and np.isfinite(got[~out]).all()
     check(got, c.expected(rows={t for t in some(c) if not out[t]}))
+
+
+# pieces joined in groups (one row of up to 4 columns of 256 channels, 8 of 128), by the last one, and merged
+@pytest.mark.parametrize("P,n,heads", [
+    (1900, 1, MODEL), (2100, 1, MODEL), (2500, 1, H8), (8200, 1, MODEL), (12000, 1, H8), (33500, 1, MODEL), (40000, 1, (1, 1, 256, 64)),
+    (2100, 2, MODEL), (1000, 4, MODEL), (8200, 2, H8), (900, 9, H16)])
+def test_joins(P, n, heads):
+    """Three times, with a shorter call between: the counts are zero again, what the workspace holds does not matter."""
+    c = Call([(P, n)], heads, 64, seed=12)
+    first = c.attention()
+    check(first, c.expected(rows={0, n - 1}))
+    for _ in range(2):
+        c.dev[1].fill_(P // 2 + n)
+        c.attention()
+        c.dev[1].fill_(P + n)
+        np.testing.assert_array_equal(c.attention().view(np.uint16), first.view(np.uint16))
