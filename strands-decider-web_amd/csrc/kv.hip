@@ -196,6 +196,14 @@ __device__ __forceinline__ bool find_rows(const KvArgs& a, int rows, int x, int&
   return false;
 }
 
+// q and values of the largest calls (NR 4) do not stay in the caches, which leaves those to the rows: 16384 rows 46.6 us instead of 52.8,
+// and the attention after them takes as long as before.
+template <int NR>
+__device__ __forceinline__ void put8(_Float16* p, h8 v) {
+  if constexpr (NR == 4) __builtin_nontemporal_store(v, gpw<h8>(p));
+  else *gpw<h8>(p) = v;
+}
+
 // A wave has one head slot (the query heads, then the keys', then the values') of NR x 64 / (HD / 8) rows of a sequence. A query
 // head's rotated channels, which are in few of a row's lanes, are done for all its rows at once, by lanes of their own.
 template <int HD, typename T, int NR>
@@ -240,7 +248,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int listed) {
       h8 o;
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] = (_Float16)(x[n][e] * (inv * w[e >> 2][e & 3]));
-      if (c >= a.rot && i < sq.n) *gpw<h8>(q + (size_t)i * a.HQ * HD + c) = o;
+      if (c >= a.rot && i < sq.n) put8<NR>(q + (size_t)i * a.HQ * HD + c, o);
     }
     wave_sync();
     const int chunks = a.rot / 8, share = min(kBlock, sq.n - b0) * chunks;  // 8 channels of a row a lane
@@ -266,7 +274,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int listed) {
       h8 o;
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] = (_Float16)y[e];
-      *gpw<h8>(q + (size_t)i * a.HQ * HD + c) = o;
+      put8<NR>(q + (size_t)i * a.HQ * HD + c, o);
     }
     return;
   }
@@ -295,7 +303,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int listed) {
       h8 o;
 #pragma unroll
       for (int e = 0; e < 8; e++) o[e] = (_Float16)fmaf((float)s, code[e], (float)z);
-      *gpw<h8>(a.values + (((size_t)(sq.r0 + i) * 2 + which) * a.HK + kh) * HD + c) = in_pool ? o : nan8;
+      put8<NR>(a.values + (((size_t)(sq.r0 + i) * 2 + which) * a.HK + kh) * HD + c, in_pool ? o : nan8);
     }
   };
   if (which) {
@@ -357,7 +365,7 @@ hipError_t append_rows(const KvArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 // More rows a wave where there are enough waves. Measured, us, 1 / 2 / 4 times 64 / (HD / 8) rows a wave, the model's heads: 256 rows
-// 5.0 / 4.7 / 7.0, 1024 rows 7.1 / 6.2 / 8.1, 4096 rows 18.5 / 17.6 / 18.4, 16384 rows 66.5 / 58.4 / 52.5.
+// 5.0 / 4.7 / 7.0, 1024 rows 7.1 / 6.2 / 8.1, 4096 rows 18.5 / 17.6 / 18.4, 16384 rows 66.5 / 58.4 / 52.5 (without streaming stores).
 template <int HD, typename T>
 hipError_t append(const KvArgs& a, hipStream_t s) {
   constexpr int kRows = 64 / (HD / 8);
