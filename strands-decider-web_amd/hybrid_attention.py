@@ -329,9 +329,13 @@ def add_bias(L, N, y, c, device=0, stream=None):
 class KVBatch:
     """A call's sequences on a :class:`PagedKV` (ha_kv_batch): int32 device arrays ``row_start`` [n_seqs + 1], ``lens``
     [n_seqs] and ``pages`` [n_seqs][table_stride], and the host's bounds on them. The arrays are read when a call runs; this
-    object keeps a reference to them."""
+    object keeps a reference to them. Tensors (not plain addresses) of another type or device, or too few elements, raise."""
 
     def __init__(self, n_seqs, n_rows, max_rows, max_len, row_start, lens, pages, table_stride):
+        for x, n in ((row_start, n_seqs + 1), (lens, n_seqs), (pages, n_seqs * table_stride)):
+            if hasattr(x, "data_ptr") and not (x.is_cuda and x.is_contiguous() and str(x.dtype) == "torch.int32" and x.numel() >= n):
+                raise TypeError("row_start, lens and pages must be contiguous int32 device tensors of n_seqs + 1, n_seqs and "
+                                "n_seqs * table_stride elements")
         self._held = (row_start, lens, pages)
         self.c = HaKvBatch(n_seqs, n_rows, max_rows, max_len, _ptr(row_start), _ptr(lens), _ptr(pages), table_stride)
 
@@ -348,8 +352,15 @@ class PagedKV:
         self.cfg = HaKvConfig(n_layers, n_pages, page_size, max_ctx, HQ, HK, HD, rot_dim, int(bool(gated)), dtype,
                               rope_theta, eps, scale)
         h = ctypes.c_void_p()
+        tensor = hasattr(pages, "data_ptr")
+        if tensor and not (pages.is_cuda and pages.is_contiguous()):
+            raise ValueError("pages must be a contiguous device tensor")
         _check(lib.ha_kv_create(ctypes.byref(self.cfg), _ptr(pages), device, ctypes.byref(h)))
         self._h = h
+        need = n_layers * n_pages * self.page_bytes(page_size, HK, HD)
+        if tensor and pages.numel() * pages.element_size() < need:
+            self.close()
+            raise ValueError("pages must be a device tensor of n_layers * n_pages * page_bytes = %d bytes" % need)
         self._borrowed = pages
 
     @staticmethod

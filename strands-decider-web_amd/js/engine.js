@@ -282,6 +282,9 @@ class PagedKV {
   constructor(engine, pages, config) {
     this.engine = engine;
     this.config = kvConfig(config);
+    const need = PagedKV.pageBytes(config) * pick(config, 'nPages', 0) * pick(config, 'nLayers', 1);
+    const have = pages instanceof DeviceView ? pages.buf.bytes - pages.offset : pages instanceof DeviceBuffer ? pages.bytes : need;
+    if (have < need) throw new RangeError('pages of ' + have + ' bytes, the cache needs ' + need);
     this._h = native.kvCreate(this.config, ptrOf(pages), engine ? engine.device : pick(config, 'device', 0));
     this._borrowed = [pages].map((x) => (x instanceof DeviceView ? x.buf : x)).filter((x) => x instanceof DeviceBuffer);
     this._borrowed.forEach((x) => { x._borrows++; });

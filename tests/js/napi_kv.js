@@ -53,6 +53,7 @@ expect('rows that are too short', 'HA_1', () => kv.append(0, batch, bufs[3], spe
 expect('no gates', 'HA_1', () => kv.attention(0, batch, q, null, 0, out));
 expect('a batch without arrays', 'HA_1', () => kv.attention(0, spec.batch, q, bufs[3], spec.rowStride, out));
 expect('no Float32Array', 'TypeError', () => kv.setParam(0, 'q_norm', new Float64Array(c.HD)));
+expect('too few pages', 'RangeError', () => new ha.PagedKV(engine, new ha.DeviceView(pages, 16), c));
 expect('borrowed pages', 'HA_BORROWED', () => pages.free());
 kv.destroy();
 kv.destroy();  // idempotent

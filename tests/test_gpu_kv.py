@@ -69,6 +69,8 @@ class Call:
     def make_batch(self, **kw):
         d = dict(n_seqs=len(self.seqs), n_rows=self.n_rows, max_rows=self.max_rows, max_len=self.max_len, row_start=self.dev[0],
                  lens=self.dev[1], pages=self.dev[2], table_stride=self.width)
+        if "n_seqs" in kw:  # (as plain addresses: KVBatch refuses tensors that end too early, the library the number)
+            d.update({k: d[k].data_ptr() for k in ("row_start", "lens", "pages")})
         d.update(kw)
         return ha.KVBatch(**d)
 

@@ -179,3 +179,46 @@ def test_two_handles_on_two_streams():
     t.cuda.synchronize()
     np.testing.assert_array_equal(oa.cpu().numpy(), wa)
     np.testing.assert_array_equal(ob.cpu().numpy(), wb)
+
+
+# every way of sharing out the work (csrc/kv_attn.hip): in a list, planned, in a grid, both kernels, joined and merged
+@pytest.mark.parametrize("seqs,heads,page", [
+    ([(700, 1), (30, 40), (0, 0)], (8, 2, 256, 64), 16), ([(2000, 20)], (8, 2, 256, 64), 64), ([(0, 3200)], (16, 1, 256, 64), 16),
+    ([(40, 1), (0, 1700), (0, 1650), (9, 3)], (16, 1, 256, 64), 32), ([(3, 1)] * 140, (16, 2, 128, 128), 16),
+    ([(30, 1)] * 139 + [(3000, 2)], (16, 2, 128, 128), 16)])
+def test_captured_calls(seqs, heads, page):
+    """Other lengths in the same arrays between replays: a sequence becomes shorter, and long again."""
+    import torch as t
+    from test_gpu_kv import Call
+    c = Call(seqs, heads, page, seed=21)
+    st = t.cuda.Stream()
+    q, out = t.zeros_like(c.dq), t.zeros_like(c.dq)
+    at = max(range(len(seqs)), key=lambda b: seqs[b][0])
+    full = int(c.lens[at])
+    short = max(full // 2, seqs[at][1])
+
+    def call():
+        c.kv.append(0, c.batch, c.drows, c.stride, q, stream=st.cuda_stream)
+        c.kv.attention(0, c.batch, q, c.drows, c.stride, out, stream=st.cuda_stream)
+
+    want = {}
+    with t.cuda.stream(st):
+        for n in (short, full):
+            c.dev[1][at] = n
+            call()
+            st.synchronize()
+            want[n] = out.clone(), q.clone(), c.dpool.clone()
+        g = t.cuda.CUDAGraph()
+        with t.cuda.graph(g, stream=st):
+            call()
+        for k, n in enumerate([full, short, full, full, short, full]):
+            if k in (1, 4):
+                call()
+            c.dev[1][at] = n
+            c.dpool.copy_(want[n][2])
+            for x in (q, out):
+                x.fill_(float("nan"))
+            g.replay()
+            st.synchronize()
+            for x, w in zip((out, q, c.dpool), want[n]):
+                assert t.equal(x, w), "replay %d" % k

@@ -55,3 +55,34 @@ def test_handles():
     assert lib.ha_kv_create(None, None, 0, None) == ha.HA_ERR_ARG
     assert lib.ha_kv_page_bytes(None, None) == ha.HA_ERR_ARG
     assert buf[0] == 0x48414B56
+
+
+def test_tensors():
+    """Tensors that the device could not read, or that end too early, are refused before a call."""
+    torch = pytest.importorskip("torch")
+    i32 = torch.zeros(8, dtype=torch.int32)
+    for args in [(i32, 16, 16), (16, i32, 16), (16, 16, i32)]:  # (host memory)
+        with pytest.raises(TypeError):
+            ha.KVBatch(2, 2, 1, 1, *args, 4)
+    assert ha.KVBatch(2, 2, 1, 1, 16, 32, 48, 4).c.table_stride == 4
+    with pytest.raises(ValueError):
+        ha.PagedKV(torch.zeros(1 << 20, dtype=torch.uint8), 4)
+
+
+@pytest.mark.gpu
+def test_device_tensors():
+    torch = pytest.importorskip("torch")
+    ok = [torch.zeros(n, dtype=torch.int32, device="cuda:0") for n in (3, 2, 8)]
+    ha.KVBatch(2, 2, 1, 1, *ok, 4)
+    for k in range(3):
+        for x in (ok[k][:-1], ok[k].long(), ok[k].cpu(), torch.zeros(32, dtype=torch.int32, device="cuda:0")[::2]):
+            with pytest.raises(TypeError):
+                ha.KVBatch(2, 2, 1, 1, *[x if j == k else ok[j] for j in range(3)], 4)
+    nb = ha.PagedKV.page_bytes()
+    pool = torch.zeros(3 * nb + 16, dtype=torch.uint8, device="cuda:0")
+    ha.PagedKV(pool, 3).close()
+    for bad in (pool[:3 * nb - 1], pool.cpu()):
+        with pytest.raises(ValueError):
+            ha.PagedKV(bad, 3)
+    with pytest.raises(ValueError):
+        ha.PagedKV(pool, 2, n_layers=2)
