@@ -176,3 +176,22 @@ def test_joins(P, n, heads):
         c.attention()
         c.dev[1].fill_(P + n)
         np.testing.assert_array_equal(c.attention().view(np.uint16), first.view(np.uint16))
+
+
+@pytest.mark.parametrize("size", [2e-4, 0.05, 300.0, 2e4])
+@pytest.mark.parametrize("seqs,heads", [([(900, 3), (40, 1)], MODEL), ([(300, 20)], H8), ([(0, 3200)], H16)])
+def test_sizes_of_values(seqs, heads, size):
+    """Values from f16's subnormal scales to its largest: P times a scale stays an f16."""
+    c = Call(seqs, heads, 16, False, seed=14)
+    for b in range(len(seqs)):
+        t = np.arange(c.lens[b])
+        for h in range(c.HK):
+            c.pool.put_rows(c.table[b, t // 16], t % 16, h, 1, np.clip(size * c.rng.standard_normal((len(t), c.HD)), -6e4, 6e4))
+    c.dpool.copy_(c.torch.from_numpy(c.pool.data))
+    c.q[:] = c.q * np.float16(3)  # (maxima that rise)
+    c.dq = c.torch.from_numpy(c.q).to("cuda:0")
+    got, want = c.attention(), c.expected(rows=some(c))
+    e = np.stack([got[t].astype(np.float64) - want[t] for t in sorted(want)])
+    w = np.stack([want[t] for t in sorted(want)])
+    # as check(), and f16's steps of 2^-24 in the output and in the products P s, which stand against P of 1 and more and up to 8 codes
+    assert np.isfinite(e).all() and np.linalg.norm(e) <= 2 ** -9 * np.linalg.norm(w) + 9 * 2 ** -25 * np.sqrt(e.size)
