@@ -28,7 +28,7 @@ __global__ void kv_rope_kernel(float* rope, const double* theta_pow, int n, int 
 // A lane has 8 consecutive channels of a row, HD / 8 lanes a row, a wave 64 / (HD / 8) rows of one head at a time; a group's
 // channels are in HD / 32 neighbouring lanes. All sums and extremes are DPP steps, and a rotated channel's partner is loaded
 // once more instead of exchanged, so that only the norms' factors go through LDS. It is bound by memory where there are many rows
-// (16384 of the model's heads, 211 MB: 46.6 us, 4.5 TB/s, where a copy reaches 4.8) and by a chain of loads where there are few (one
+// (16384 of the model's heads, 211 MB: 53.8 us, 3.9 TB/s, on new buffers, 46.6 on the same ones again, where a copy reaches 4.8) and by a chain of loads where there are few (one
 // row each of 8 sequences: 4.4 us).
 
 typedef unsigned u2v __attribute__((ext_vector_type(2)));
@@ -198,8 +198,8 @@ __device__ __forceinline__ bool find_rows(const KvArgs& a, int rows, int x, int&
   return false;
 }
 
-// q and values of the largest calls (NR 4) do not stay in the caches, which leaves those to the rows: 16384 rows 46.6 us instead of 52.8,
-// and the attention after them takes as long as before.
+// q and values of the largest calls (NR 4) do not stay in the caches, which leaves those to the rows: 16384 rows 46.6 us instead of
+// 52.8 (on new buffers 53.8 and 57.7), and the attention after them takes as long as before.
 template <int NR>
 __device__ __forceinline__ void put8(_Float16* p, h8 v) {
   if constexpr (NR == 4) __builtin_nontemporal_store(v, gpw<h8>(p));
