@@ -52,7 +52,7 @@ class Call:
         self.n_rows = self.T + extra
         self.max_rows = max([n for _, n in seqs] + [0])
         self.max_len = int(max(list(self.lens) + [1]))
-        self.stride = self.HQ * self.HD * (2 if gated else 1) + 2 * self.HK * self.HD
+        self.stride = self.HQ * self.HD * (2 if gated else 1) + 2 * self.HK * self.HD + (0 if gated else 8)  # (some rows with padding)
         self.rows = rng.standard_normal((max(self.n_rows, 1), self.stride)).astype(np.float32 if f32 else np.float16)
         self.qw, self.kw = ((1 + 0.1 * rng.standard_normal(self.HD)).astype(np.float32) for _ in "qk")
         self.dpool = torch.from_numpy(self.pool.data.copy()).to(DEV)
