@@ -290,8 +290,9 @@ typedef struct ha_kv_config {
 } ha_kv_config;
 /* A call's sequences. row_start, len and pages are read on the device when the call runs, so a captured call may be
    replayed with other contents within the same n_rows, max_rows and max_len. Sequence b's new rows are rows row_start[b] ..
-   row_start[b + 1] - 1 of the call, its context with them len[b] tokens: they are its last positions. Token t stands in page
-   pages[b][t / page_size], slot t % page_size; entries behind the last token's are not read. */
+   row_start[b + 1] - 1 of the call, its context with them len[b] tokens: they are its last positions. row_start does not fall:
+   rows that two sequences claim get the results of one of them or NaN, and no others are touched by that. Token t stands in
+   page pages[b][t / page_size], slot t % page_size; entries behind the last token's are not read. */
 typedef struct ha_kv_batch {
   int n_seqs;            /* up to 65535 (n_seqs HK up to 2^22) */
   int n_rows;            /* rows of q, values and outputs (n_rows HQ up to 2^27) */

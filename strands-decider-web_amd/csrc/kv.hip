@@ -181,9 +181,9 @@ __device__ __forceinline__ unsigned short nibbles(const float* c) {
 // one block, from row 0.
 __device__ __forceinline__ bool find_rows(const KvArgs& a, int rows, int x, int& b, int& b0, Seq& sq) {
   const int lane = threadIdx.x & 63;
+  int top = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
-    Seq l{};
-    if (s0 + lane < a.n_seqs) l = seq_of(a, s0 + lane);
+    const Seq l = seq_in_order(a, s0 + lane, top);
     const int n = l.n == 0 ? 0 : l.ok ? (l.n + rows - 1) / rows : 1, sum = scan64(n);
     const unsigned long long past = __ballot(sum > x);
     if (past) {
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int listed) {
   if (listed) {
     if (!find_rows(a, kBlock, blockIdx.x, b, b0, sq)) return;
   } else {
-    sq = seq_of(a, b);
+    sq = seq_alone(a, b);
     if (b0 >= sq.n) return;
   }
   const h8 nan8 = h8{} + (_Float16)__builtin_nanf("");

@@ -113,7 +113,7 @@ struct Kind {
   float* p;  // results of the pieces of cut units: for each piece and column O (unnormalised) [HD], maximum, sum
   int* count;  // of a cut unit's pieces (a group's) that are done, at the first one's slot, then of its groups; zero between calls
   int* plan;   // or nullptr: keys a piece; then for each sequence the sums up to and with it of its pieces, of those of them that
-               // are cut, and of its (row, head)s to be merged
+               // are cut, and of its (row, head)s to be merged, and the greatest row_start up to its own
   int cols;  // columns a block has, at most
   int lo, hi, want, direct, ncb;
 };
@@ -130,15 +130,14 @@ struct Lane {
   int ncb;
 };
 template <int BC>
-__device__ __forceinline__ Lane lane_of(const KvArgs& a, const Kind& k, int s) {
-  Lane l{};
-  if (s < a.n_seqs) {
-    l.sq = seq_of(a, s);
-    const int cols = l.sq.n * a.ratio;
-    if (cols > k.lo && cols <= k.hi) l.ncb = l.sq.ok ? (cols + BC - 1) / BC : 1;  // (one unit writes all rows of a sequence that does not fit)
-  }
+__device__ __forceinline__ Lane lane_of(const KvArgs& a, const Kind& k, const Seq& sq) {
+  Lane l{sq, 0};
+  const int cols = sq.n * a.ratio;
+  if (cols > k.lo && cols <= k.hi) l.ncb = sq.ok ? (cols + BC - 1) / BC : 1;  // (one unit writes all rows of a sequence that does not fit)
   return l;
 }
+template <int BC>
+__device__ __forceinline__ Lane lane_of(const KvArgs& a, const Kind& k, int s, int& top) { return lane_of<BC>(a, k, seq_in_order(a, s, top)); }
 constexpr int kUnit = kStep * kWaves;  // keys that a piece has at least
 constexpr int kEven = 4;               // times that, from which pieces are made even
 // a / s of 0 <= a < 2^21, s > 0: (a + 1/2) / s is 1 / (2 s) away from the next integer, its error at most a 2^-22 / s
@@ -159,10 +158,10 @@ __device__ __forceinline__ int pieces_of(int len, int size) {
 __device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, float w) {
   return uniform(kUnit * max(1, (int)fminf(ceilf(w * (float)a.HK / (float)(k.want * kUnit)), 1e6f)));
 }
-__device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, const Lane& first, int lane) {
+__device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, const Lane& first, int lane, int top) {
   float w = (float)first.ncb * (float)first.sq.len;
   for (int s0 = 64; s0 < a.n_seqs; s0 += 64) {
-    const Lane l = lane_of<kCols>(a, k, s0 + lane);
+    const Lane l = lane_of<kCols>(a, k, s0 + lane, top);
     w += (float)l.ncb * (float)l.sq.len;
   }
   return chunk_of(a, k, __builtin_bit_cast(float, lane_value(__builtin_bit_cast(int, scan64(w)), 63)));
@@ -191,11 +190,22 @@ __device__ __forceinline__ Counts counts_of(const KvArgs& a, const Kind& k, cons
 // Kind::plan: a thread has neighbouring sequences.
 __global__ __launch_bounds__(1024) void kv_plan_kernel(KvArgs a, Kind k) {
   __shared__ float ws[16];
-  __shared__ int tot[16][3];
+  __shared__ int tot[16][3], tops[16];
   const int tid = threadIdx.x, wave = tid >> 6, per = (a.n_seqs + 1023) / 1024, s0 = tid * per, s1 = min(s0 + per, a.n_seqs);
+  int* sums = k.plan + 1;
+  int top = 0;  // of the thread's sequences, then of those before them
+  for (int s = s0; s < s1; s++) top = max(top, a.row_start[s]);
+  top = max64(top);
+  if ((tid & 63) == 63) tops[wave] = top;
+  top = __shfl_up(top, 1);
+  if ((tid & 63) == 0) top = 0;
+  __syncthreads();
+  for (int x = 0; x < wave; x++) top = max(top, tops[x]);
   float w = 0.0f;
   for (int s = s0; s < s1; s++) {
-    const Lane l = lane_of<kCols>(a, k, s);
+    top = max(top, a.row_start[s]);
+    sums[3 * kPlanMost + s] = top;
+    const Lane l = lane_of<kCols>(a, k, seq_of(a, s, top));
     w += (float)l.ncb * (float)l.sq.len;
   }
   w = scan64(w);
@@ -206,7 +216,7 @@ __global__ __launch_bounds__(1024) void kv_plan_kernel(KvArgs a, Kind k) {
   const int chunk = chunk_of(a, k, w);
   Counts c{};
   for (int s = s0; s < s1; s++) {
-    const Counts x = counts_of(a, k, lane_of<kCols>(a, k, s), chunk);
+    const Counts x = counts_of(a, k, lane_of<kCols>(a, k, seq_of(a, s, sums[3 * kPlanMost + s])), chunk);
     c = Counts{c.items + x.items, c.cut + x.cut, c.rows + x.rows, 0, 0};
   }
   const Counts in = {scan64(c.items), scan64(c.cut), scan64(c.rows), 0, 0};
@@ -219,9 +229,8 @@ __global__ __launch_bounds__(1024) void kv_plan_kernel(KvArgs a, Kind k) {
   Counts at = {in.items - c.items, in.cut - c.cut, in.rows - c.rows, 0, 0};
   for (int x = 0; x < wave; x++) at = Counts{at.items + tot[x][0], at.cut + tot[x][1], at.rows + tot[x][2], 0, 0};
   if (tid == 0) k.plan[0] = chunk;
-  int* sums = k.plan + 1;
   for (int s = s0; s < s1; s++) {
-    const Counts x = counts_of(a, k, lane_of<kCols>(a, k, s), chunk);
+    const Counts x = counts_of(a, k, lane_of<kCols>(a, k, seq_of(a, s, sums[3 * kPlanMost + s])), chunk);
     at = Counts{at.items + x.items, at.cut + x.cut, at.rows + x.rows, 0, 0};
     sums[s] = at.items;
     sums[kPlanMost + s] = at.cut;
@@ -249,7 +258,7 @@ __device__ __forceinline__ bool find_piece(const KvArgs& a, const Kind& k, int x
     it.kh = blockIdx.y;
     it.cb = it.piece = it.slot = 0;
     it.size = 0x7fffffff;
-    it.sq = seq_of(a, it.b);
+    it.sq = seq_alone(a, it.b);
     return it.sq.n > 0;
   }
   int rel, ns;  // rel: piece of the sequence; ns: pieces of a unit
@@ -257,7 +266,7 @@ __device__ __forceinline__ bool find_piece(const KvArgs& a, const Kind& k, int x
     const int *sums = k.plan + 1, s = search(sums, a.n_seqs, x);
     if (s == a.n_seqs) return false;
     it.b = s;
-    const Lane l = lane_of<kCols>(a, k, s);
+    const Lane l = lane_of<kCols>(a, k, seq_of(a, s, gp<int>(sums)[3 * kPlanMost + s]));
     const Counts c = counts_of(a, k, l, gp<int>(k.plan)[0]);
     it.size = uniform(c.size);
     ns = uniform(c.ns);
@@ -265,11 +274,12 @@ __device__ __forceinline__ bool find_piece(const KvArgs& a, const Kind& k, int x
     it.slot = uniform(gp<int>(sums)[kPlanMost + s] - c.cut + rel);
     it.sq = l.sq;
   } else {
-    Lane l = lane_of<kCols>(a, k, lane);
-    const int chunk = chunk_of(a, k, l, lane);
+    int top = 0;
+    Lane l = lane_of<kCols>(a, k, lane, top);
+    const int chunk = chunk_of(a, k, l, lane, top);
     int base = 0, slots = 0;
     for (int s0 = 0;; s0 += 64) {
-      if (s0) l = lane_of<kCols>(a, k, s0 + lane);
+      if (s0) l = lane_of<kCols>(a, k, s0 + lane, top);
       const Counts c = counts_of(a, k, l, chunk);
       const int sum = scan64(c.items), csum = scan64(c.cut);
       const unsigned long long past = __ballot(base + sum > x);
@@ -304,11 +314,12 @@ __device__ __forceinline__ bool find_block(const KvArgs& a, const Kind& k, int x
     it.b = pair / a.HK;
     it.kh = pair - it.b * a.HK;
     it.cb = k.ncb - 1 - row;
-    it.sq = seq_of(a, it.b);
+    it.sq = seq_alone(a, it.b);
     return it.cb * kBigCols < it.sq.n * a.ratio && (it.sq.ok || it.cb == 0);
   }
+  int top = 0;
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
-    const Lane l = lane_of<kBigCols>(a, k, s0 + lane);
+    const Lane l = lane_of<kBigCols>(a, k, s0 + lane, top);
     const int all = lane_value(scan64(l.ncb), 63) * a.HK;
     if (x >= all) {
       x -= all;
@@ -343,7 +354,7 @@ __device__ __forceinline__ bool find_row(const KvArgs& a, const Kind& k, int x, 
     const int *sums = k.plan + 1, s = search(sums + 2 * kPlanMost, a.n_seqs, x);
     if (s == a.n_seqs) return false;
     it.b = s;
-    const Lane l = lane_of<kCols>(a, k, s);
+    const Lane l = lane_of<kCols>(a, k, seq_of(a, s, gp<int>(sums)[3 * kPlanMost + s]));
     const Counts c = counts_of(a, k, l, gp<int>(k.plan)[0]);
     it.size = uniform(c.size);
     ns = uniform(c.ns);
@@ -351,11 +362,12 @@ __device__ __forceinline__ bool find_row(const KvArgs& a, const Kind& k, int x, 
     slot = uniform(gp<int>(sums)[kPlanMost + s] - c.cut);
     it.sq = l.sq;
   } else {
-    Lane l = lane_of<kCols>(a, k, lane);
-    const int chunk = chunk_of(a, k, l, lane);
+    int top = 0;
+    Lane l = lane_of<kCols>(a, k, lane, top);
+    const int chunk = chunk_of(a, k, l, lane, top);
     int base = 0;
     for (int s0 = 0;; s0 += 64) {
-      if (s0) l = lane_of<kCols>(a, k, s0 + lane);
+      if (s0) l = lane_of<kCols>(a, k, s0 + lane, top);
       const Counts c = counts_of(a, k, l, chunk);
       const int sum = scan64(c.rows), csum = scan64(c.cut);
       const unsigned long long past = __ballot(base + sum > x);
@@ -1304,7 +1316,7 @@ hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
 
 }  // namespace
 
-size_t kv_workspace_bytes() { return kSlots * (kSlotBytes + 2 * sizeof(int)) + sizeof(int) * (1 + 3 * (size_t)kPlanMost); }
+size_t kv_workspace_bytes() { return kSlots * (kSlotBytes + 2 * sizeof(int)) + sizeof(int) * (1 + 4 * (size_t)kPlanMost); }
 
 hipError_t launch_kv_attention(const KvArgs& a, void* ws, hipStream_t s) {
   return a.HD == 256 ? attend<256>(a, static_cast<float*>(ws), s) : attend<128>(a, static_cast<float*>(ws), s);

@@ -14,15 +14,17 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 
 // Sequence b's rows [r0, r0 + n) and its context, positions [len - n, len) of which are the rows'. A sequence whose
 // numbers do not fit the call's (ok false) stores nothing; the rows of it that lie in the call come out as NaN.
+// `top`: the greatest of row_start[0 .. b] (and 0). A sequence that starts below it does not fit, and keeps clear of the rows before
+// it: those of the sequences that fit are then disjoint, whatever row_start holds, and lists of them end within their grids.
 struct Seq {
   int r0, n, len;
   bool ok;
 };
-__device__ __forceinline__ Seq seq_of(const KvArgs& a, int b) {
+__device__ __forceinline__ Seq seq_of(const KvArgs& a, int b, int top) {
   const int r0 = a.row_start[b], r1 = a.row_start[b + 1], len = a.len[b];
   Seq s;
-  s.ok = r0 >= 0 && r1 >= r0 && r1 <= a.n_rows && r1 - r0 <= a.max_rows && len >= r1 - r0 && len <= a.max_len;
-  s.r0 = min(max(r0, 0), a.n_rows);
+  s.ok = r0 >= top && r1 >= r0 && r1 <= a.n_rows && r1 - r0 <= a.max_rows && len >= r1 - r0 && len <= a.max_len;
+  s.r0 = min(top, a.n_rows);
   s.n = min(min(max(r1, s.r0), a.n_rows) - s.r0, a.max_rows);
   s.len = s.ok ? len : 0;
   return s;
@@ -47,9 +49,30 @@ __device__ __forceinline__ F scan64(F v) {
   v = dpp_add<0x142, 0xa>(v);  // row_bcast 15, 31
   return dpp_add<0x143, 0xc>(v);
 }
+// inclusive running maximum over the wave, of values >= 0
+template <int kCtrl, int kRows>
+__device__ __forceinline__ int dpp_max(int v) { return max(v, __builtin_amdgcn_update_dpp(0, v, kCtrl, kRows, 0xf, true)); }
+__device__ __forceinline__ int max64(int v) {
+  v = dpp_max<0x111, 0xf>(v);
+  v = dpp_max<0x112, 0xf>(v);
+  v = dpp_max<0x114, 0xf>(v);
+  v = dpp_max<0x118, 0xf>(v);
+  v = dpp_max<0x142, 0xa>(v);
+  return dpp_max<0x143, 0xc>(v);
+}
 __device__ __forceinline__ int lane_value(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 __device__ __forceinline__ Seq lane_value(const Seq& s, int lane) {
   return Seq{lane_value(s.r0, lane), lane_value(s.n, lane), lane_value(s.len, lane), lane_value((int)s.ok, lane) != 0};
+}
+
+// A sequence that has a place of its own in the grid, whatever those before it hold.
+__device__ __forceinline__ Seq seq_alone(const KvArgs& a, int b) { return seq_of(a, b, max(a.row_start[b], 0)); }
+// A lane's sequence s = s0 + lane, s0 = 0, 64, ... in this order: `top` is 0 at first, and handed on.
+__device__ __forceinline__ Seq seq_in_order(const KvArgs& a, int s, int& top) {
+  const bool in = s < a.n_seqs;
+  const int mine = max(top, max64(in ? max(a.row_start[s], 0) : 0));
+  top = lane_value(mine, 63);
+  return in ? seq_of(a, s, mine) : Seq{};
 }
 
 // f16 index of (token slot, group, 0: scale, 1: zero) among a block's parameters

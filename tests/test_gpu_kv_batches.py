@@ -4,6 +4,7 @@ Tolerances: tests/test_gpu_kv.py."""
 import numpy as np
 import pytest
 
+import hybrid_attention as ha
 import kv_ref as kr
 from test_gpu_kv import Call, check, check_append
 
@@ -195,3 +196,28 @@ def test_sizes_of_values(seqs, heads, size):
     w = np.stack([want[t] for t in sorted(want)])
     # as check(), and f16's steps of 2^-24 in the output and in the products P s, which stand against P of 1 and more and up to 8 codes
     assert np.isfinite(e).all() and np.linalg.norm(e) <= 2 ** -9 * np.linalg.norm(w) + 9 * 2 ** -25 * np.sqrt(e.size)
+
+
+# (the first sequence's rows, sequences, the last one's length, heads): in a list, planned, of many columns
+@pytest.mark.parametrize("rows,n,long,heads", [(64, 59, 1800, MODEL), (40, 201, 2500, MODEL), (3000, 9, 3300, H16)])
+def test_row_start_that_falls_again_and_again(rows, n, long, heads):
+    """Every second sequence claims the first one's rows: those stay the first one's, the others store nothing, and no work is left
+    half done that a later call on the handle would find."""
+    c = Call([(0, rows)] + [(rows, 0)] * (n - 2) + [(long, 0)], heads, 16, seed=15, extra=1)
+    c.max_len = long
+    good = c.dev[0].clone()
+    c.dev[0][::2], c.dev[0][1::2] = 0, rows
+    c.batch = c.make_batch()
+    got = c.attention()
+    check(got[:rows], c.expected(rows=set(range(rows)) if rows < 100 else {0, 1, 500, rows - 1}))
+    assert (got[rows:] == 7).all()
+    check_append(c, *c.append())
+    # the last sequence's rows, in pieces, on this handle and on one that has seen no other call
+    c.dev[0].copy_(good)
+    c.dev[0][:n] = 0
+    one = c.make_batch()
+    first = c.attention(batch=one)
+    c.kv = ha.PagedKV(c.dpool, c.n_pages, page_size=16, max_ctx=long, HQ=c.HQ, HK=c.HK, HD=c.HD, rot_dim=c.rot)
+    want = c.attention(batch=one)
+    assert np.isfinite(want[:rows]).all()
+    np.testing.assert_array_equal(first.view(np.uint16), want.view(np.uint16))
