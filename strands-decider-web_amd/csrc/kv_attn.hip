@@ -13,8 +13,8 @@
 //     afterwards, on its 16 x 16 sums: S = sum_g s_g (q . (c - 8))_g + z_g sum(q_g).
 //   - K's operand is 16 bytes of a token's row a lane, V's 8 bytes of 8 tokens' rows, two tokens' half-words joined by
 //     v_perm; S^T's layout (a column a lane) is that of P^T as an operand, so P goes from registers to registers.
-//   - V's scales go onto P (P s_g, f16), and its zeros and the codes' offset into one more sum for each group:
-//     Z_g = sum P z_g - 24 sum P s_g.
+//   - V's scales go onto P (P s_g, f16), and its zeros into one more sum for each group, sum P z_g; the codes' offset,
+//     -24 sum P s_g, is added after every segment of 1024 keys.
 //   - a column's maximum is the wave's own; it is raised only when a score exceeds it by 2^6 (kRaise).
 // P, at most 2^6, and P s_g are rounded to f16 once each, the roundings that q and the outputs have too; everything that is summed
 // is f32. Pieces leave their O, maximum and sum in the workspace; the last of a unit's pieces joins them, or kv_merge_kernel where
@@ -666,6 +666,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
     locate(seg, seg + kStep * wave);
     fetch_k();
     fetch_v();
+    // The segment's offsets: sums of 16 + c that ran on would lose what remains of c - 8 (131072 values of equal weight whose mean is
+    // zero came out as up to 5.2e-5; now below 2.7e-7).
+#pragma unroll
+    for (int g = 0; g < 4; g++) {
+      const float t = sum_quads(cs[g]);
+      cs[g] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kE; e++) o[g][e] += t;
+    }
   }
   // the four waves' sums: O^T row 4 kg + k of (g, e) is channel G g + 16 kg + 4 k + e (HD 256), G g + 4 (row & 7) + 2 (row >> 3) + e
   // (HD 128)

@@ -221,3 +221,44 @@ def test_row_start_that_falls_again_and_again(rows, n, long, heads):
     want = c.attention(batch=one)
     assert np.isfinite(want[:rows]).all()
     np.testing.assert_array_equal(first.view(np.uint16), want.view(np.uint16))
+
+
+def shared_pages(seqs, heads, n_pages, page=256, seed=0, pool=None, **kw):
+    """A call whose sequences take their full pages from one pool, over and over, in an order of their own (contexts of many pages)."""
+    c = Call([(n_pages * page - n, n) if b == 0 else (0, n) for b, (_, n) in enumerate(seqs)], heads, page, False, seed=seed, max_ctx=max(p + n for p, n in seqs), **kw)
+    ids = c.table[0, :n_pages].copy()
+    c.lens = np.array([p + n for p, n in seqs], np.int32)
+    assert (c.lens % page == 0).all()
+    c.width = int(c.lens.max()) // page
+    c.table = np.stack([c.rng.permutation(np.resize(ids, c.width)) for _ in seqs]).astype(np.int32)
+    c.max_len = int(c.lens.max())
+    c.dev = [c.torch.from_numpy(a).to("cuda:0") for a in (c.start, c.lens, c.table)]
+    c.batch = c.make_batch()
+    if pool is not None:
+        pool(c, ids)
+        c.dpool.copy_(c.torch.from_numpy(c.pool.data))
+    return c
+
+
+@pytest.mark.parametrize("heads", [(8, 8, 128, 8), (8, 8, 256, 8)])
+def test_values_that_cancel_over_a_long_piece(heads):
+    """Equal weights over 131072 values whose mean is zero, by one workgroup (512 units): what the sums of codes and of their offset
+    leave. q is zero, so P is 1 and P s exact; a token's value is s (c - 8) + z, each has a partner with 16 - c and -z."""
+    def pool(c, ids):
+        shape = c.pool.codes()[ids].shape
+        nib = c.rng.integers(1, 16, (len(ids) // 2,) + shape[1:-1] + (c.HD,), dtype=np.uint8)
+        for at, x in ((ids[0::2], nib), (ids[1::2], 16 - nib)):
+            c.pool.codes()[at] = x[..., 0::2] | x[..., 1::2] << 4
+        half = c.pool.data[..., c.page * c.HD // 2:].view(np.float16)
+        par = half.reshape(half.shape[:-1] + (c.page // 4, 4, 2, 4))
+        s, z = (c.rng.uniform(a, b, (len(ids) // 2,) + par.shape[1:-2] + (4,)).astype(np.float16) for a, b in ((0.25, 0.4), (-0.5, 0.5)))
+        for at, sign in ((ids[0::2], 1), (ids[1::2], -1)):
+            par[at, ..., 0, :], par[at, ..., 1, :] = s, sign * z
+
+    c = shared_pages([(131071, 1)] * 64, heads, 16, seed=16, pool=pool)
+    c.dq.zero_()
+    got = c.attention().astype(np.float64)
+    # a wave's 32768 keys are 128 segments of 8 steps. Within one, codes of 16 + c sum up to 24 s 256 < 2^12, so a step's rounding is
+    # 2^-13 at most, 2^-13.8 in the root mean square where it is 2 roundings; 1024 of them of 4 waves are 2^6 times as much: 2^-7.8 on 131072 keys, 2^-24.8.
+    # Seven times that, and the output's own step. (Sums over all of a piece would leave 2^7 times as much.)
+    assert np.abs(got).max() <= 7 * 2 ** -24.8 + 2 ** -25
