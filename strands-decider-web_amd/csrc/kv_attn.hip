@@ -15,8 +15,8 @@
 //     v_perm; S^T's layout (a column a lane) is that of P^T as an operand, so P goes from registers to registers.
 //   - V's scales go onto P (P s_g, f16), and its zeros into one more sum for each group, sum P z_g; the codes' offset,
 //     -24 sum P s_g, is added after every segment of 1024 keys.
-//   - a column's maximum is the wave's own; it is raised only when a score exceeds it by 2^6 (kRaise).
-// P, at most 2^6, and P s_g are rounded to f16 once each, the roundings that q and the outputs have too; everything that is summed
+//   - a column's maximum is the wave's own; it is raised only when a score exceeds what P may be (Range).
+// P and P s_g are rounded to f16 once each, the roundings that q and the outputs have too; everything that is summed
 // is f32. Pieces leave their O, maximum and sum in the workspace; the last of a unit's pieces joins them, or kv_merge_kernel where
 // they are many. Two workgroups a CU (228 registers for HD 256) and codes fetched a step ahead keep memory busy where there are
 // few columns: 8 sequences of 32768 tokens, 2 x 4 heads of 256, 151 MB: 32.5 us, 4.6 TB/s (a copy 4.8). With 16 columns
@@ -32,9 +32,17 @@ namespace {
 
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
-// log2 headroom before a column's maximum is raised; none beside values whose scale is 512 or more, so that P s stays an f16
-constexpr float kRaise = 6.0f;
-__device__ __forceinline__ bool large(unsigned s) { return s & (s << 1) & 0x40004000u; }  // one of two f16 >= 0 is at least 512
+// P = exp2(score - m) and P s are f16, whose steps end at 2^-24, so P is kept high: m is `lift` below a column's maximum when it is
+// set, and set again when a score exceeds m by more than `room`, by the largest scale of the tile's values. P s stays below 2^16, and
+// P is at least 1 for the column's heaviest key.
+struct Range {
+  float room, lift;
+  __device__ __forceinline__ explicit Range(int cls) : room(cls == 0 ? 14.0f : cls == 1 ? 6.0f : 0.0f), lift(cls == 0 ? 8.0f : 0.0f) {}
+};
+// the class of two words of scales: 0 below 2, 1 below 512, 2 (and NaN)
+__device__ __forceinline__ int scale_class(unsigned s, unsigned t) {
+  return ((s & (s << 1)) | (t & (t << 1))) & 0x40004000u ? 2 : (s | t) & 0x40004000u ? 1 : 0;
+}
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kCols = 16, kWaves = 4, kStep = 32;  // few columns: of a workgroup; waves; keys a wave's step
 constexpr int kBigCols = 128, kTile = 32;          // many columns
@@ -499,7 +507,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
         vc[i][k] = *gp<u2>(blk[i] + blk_bytes + (unsigned)((slot[i] + 4 * kg + k) * kRow + 8 * (HD == 256 ? j : j & 7)));
   };
   unsigned char* params = reinterpret_cast<unsigned char*>(ol + wave * (kCols / 2) * kPitch);
-  float room = 0.0f;
+  Range range(0);
   auto put_params = [&](int t0) {
     const bool lost = lane & 16 ? gone[1] : gone[0];
     // beyond the sequence, and in no page: parameters of any bits (a score of no page is NaN)
@@ -514,7 +522,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
         }
     }
     *reinterpret_cast<u4*>(params + 16 * lane) = pr;
-    room = __any(large(pr[0]) || large(pr[1])) ? 0.0f : kRaise;  // (of K too, for simplicity)
+    const int cls = lane & 32 ? scale_class(pr[0], pr[1]) : 0;
+    range = Range(!__any(cls) ? 0 : !__any(cls == 2) ? 1 : 2);
     wave_sync();
   };
   locate(k0, k0 + kStep * wave);  // (a wave without keys: any page)
@@ -591,7 +600,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
 #pragma unroll
       for (int k = 0; k < 4; k++) mx = fmaxf(mx, sc[i][k]);
     mx = max_quads(mx) * scale;
-    const float mn = mx > m + room ? mx : m;
+    const float mn = mx > m + range.room ? mx - range.lift : m;
     if (__any(mn != m)) {
       if (__any(m != -INFINITY)) {  // (else O is zero)
         const float al = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -820,12 +829,12 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 
 // LDS of kv_many_kernel, each part twice: K tile [32][HD] and V^T tile [HD][32] as f16 (rows 16 bytes longer, so that eight rows
 // of an operand lie in different banks), K's scales [4][32] and zeros [32][4] twice each, P f32 in the lanes' order, the columns'
-// factors, the waves' flags and whether scales of V are large; V's scales and zeros [4][32] each of four tiles.
+// factors, the waves' flags and the class of V's scales; V's scales and zeros [4][32] each of four tiles.
 template <int HD>
 struct ManyLds {
   static constexpr int kKPitch = HD * 2 + 16, kVPitch = kTile * 2 + 16;
   static constexpr int kKs = kTile * kKPitch, kKz = kKs + 256, kV = kKz + 512, kP = kV + HD * kVPitch;
-  static constexpr int kAl = kP + kBigCols * kTile * 4, kFlag = kAl + kBigCols * 4, kLarge = kFlag + 16, kBuf = kLarge + 16;
+  static constexpr int kAl = kP + kBigCols * kTile * 4, kFlag = kAl + kBigCols * 4, kClass = kFlag + 16, kBuf = kClass + 16;
   static constexpr int kParam = 2 * kBuf, kAll = kParam + 4 * 512;
 };
 
@@ -909,8 +918,9 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
       unsigned w = pgone ? (pwhich || ppart ? 0u : 0x7E007E00u) : praw;
       if (t0 + pkey >= keys) w = 0;
       else if (t0 + pkey + 1 >= keys) w &= 0xFFFFu;
-      const bool any_large = __any(!ppart && large(w));
-      if (wave >= 2 && lane == 0) *reinterpret_cast<int*>(buf + M::kLarge + 4 * (wave - 2)) = any_large;  // (waves 2, 3: V's)
+      const int cls = ppart ? 0 : scale_class(w, w);
+      const int most = !__any(cls) ? 0 : !__any(cls == 2) ? 1 : 2;
+      if (wave >= 2 && lane == 0) *reinterpret_cast<int*>(buf + M::kClass + 4 * (wave - 2)) = most;  // (waves 2, 3: V's)
       if (pwhich) {
         *reinterpret_cast<unsigned*>(lds + M::kParam + ((t0 / kTile) & 3) * 512 + ppart * 256 + pg * 64 + pkey * 2) = w;
       } else {
@@ -994,8 +1004,9 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
 #pragma unroll
         for (int v = 0; v < 16; v++) mx = fmaxf(mx, st[v]);
         mx = max_halves(mx) * scale;
-        const int* lg = reinterpret_cast<const int*>(buf + M::kLarge);
-        const float mn = mx > m + (lg[0] | lg[1] ? 0.0f : kRaise) ? mx : m;
+        const int* cls = reinterpret_cast<const int*>(buf + M::kClass);
+        const Range range(max(cls[0], cls[1]));
+        const float mn = mx > m + range.room ? mx - range.lift : m;
         const bool raise = __any(mn != m);
         if (lane == 0) *reinterpret_cast<int*>(buf + M::kFlag + 4 * wave) = raise;
         if (raise) {

@@ -262,3 +262,27 @@ def test_values_that_cancel_over_a_long_piece(heads):
     # 2^-13 at most, 2^-13.8 in the root mean square where it is 2 roundings; 1024 of them of 4 waves are 2^6 times as much: 2^-7.8 on 131072 keys, 2^-24.8.
     # Seven times that, and the output's own step. (Sums over all of a piece would leave 2^7 times as much.)
     assert np.abs(got).max() <= 7 * 2 ** -24.8 + 2 ** -25
+
+
+@pytest.mark.parametrize("seqs,heads", [([(4000, 1)], MODEL), ([(4090, 5)], H8), ([(800, 3200)], H16), ([(3000, 700)] * 2, (16, 1, 128, 8))])
+def test_one_heavy_token_of_no_value_and_many_light_ones(seqs, heads):
+    """A first token whose weight is 2^12 times another's and whose value is zero, before thousands of small values: each product P s
+    of the others is 2^-12 of a scale of 2^-9, and the output is their mean."""
+    c = Call(seqs, heads, 64, False, seed=17)
+    u = c.rng.choice([-1.0, 1.0], c.HD)
+    for b in range(len(seqs)):
+        t = np.arange(c.lens[b])
+        for h in range(c.HK):
+            k, v = 0.02 * c.rng.standard_normal((len(t), c.HD)), 0.006 * c.rng.standard_normal((len(t), c.HD))
+            k[0], v[0] = u * (12 * np.log(2) / np.sqrt(c.HD)), 0
+            for w, x in ((0, k), (1, v)):
+                c.pool.put_rows(c.table[b, t // 64], t % 64, h, w, x)
+    c.dpool.copy_(c.torch.from_numpy(c.pool.data))
+    c.q[:] = u  # its score is sqrt(HD) |k| = 12 log 2, the others' 0.3 at most
+    c.dq = c.torch.from_numpy(c.q).to("cuda:0")
+    rows = {int(t) for b in range(len(seqs)) for t in (c.start[b + 1] - 1, c.start[b + 1] - 3) if t >= c.start[b]}
+    got, want = c.attention(), c.expected(rows=rows)
+    e = np.stack([got[t].astype(np.float64) - want[t] for t in sorted(want)])
+    w = np.stack([want[t] for t in sorted(want)])
+    # as check(), and the output's own steps of 2^-24
+    assert np.isfinite(e).all() and np.linalg.norm(e) <= 2 ** -10 * np.linalg.norm(w) + 2 ** -25 * np.sqrt(e.size)
