@@ -13,15 +13,17 @@
 //     afterwards, on its 16 x 16 sums: S = sum_g s_g (q . (c - 8))_g + z_g sum(q_g).
 //   - K's operand is 16 bytes of a token's row a lane, V's 8 bytes of 8 tokens' rows, two tokens' half-words joined by
 //     v_perm; S^T's layout (a column a lane) is that of P^T as an operand, so P goes from registers to registers.
-//   - V's scales go onto P (P s_g, f16), and its zeros into one more sum for each group, sum P z_g; the codes' offset,
-//     -24 sum P s_g, is added after every segment of 1024 keys.
+//   - V's scales go onto P (P s_g), and its zeros into one more sum for each group, sum P z_g; that product's other rows give
+//     sum P s_g, of which the codes' offset, -24 times it, is added after every segment of 1024 keys.
 //   - a column's maximum is the wave's own; it is raised only when a score exceeds what P may be (Range).
-// P and P s_g are rounded to f16 once each, the roundings that q and the outputs have too; everything that is summed
-// is f32. Pieces leave their O, maximum and sum in the workspace; the last of a unit's pieces joins them, or kv_merge_kernel where
-// they are many. Two workgroups a CU (228 registers for HD 256) and codes fetched a step ahead keep memory busy where there are
-// few columns: 8 sequences of 32768 tokens, 2 x 4 heads of 256, 151 MB: 32.5 us, 4.6 TB/s (a copy 4.8). With 16 columns
+// P and P s_g are sums of two f16 each (22 bits), whose products take two matrix instructions: the output's error is its own
+// rounding, 2.07e-4 of its norm, where one f16 each gave 2.5 to 3.1e-4, the more the longer the context, and took up to 4 % less
+// time (us: 61 rows after 1531 16.5 / 16.6, 2 x 1000 rows after 1000 99.5 / 101, 64 sequences of 8192 59.9 / 62.5). Sums are f32.
+// Pieces leave their O, maximum and sum in the workspace; the last of a unit's pieces joins them, or kv_merge_kernel where
+// they are many. Two workgroups a CU (233 registers for HD 256) and codes fetched a step ahead keep memory busy where there are
+// few columns: 8 sequences of 32768 tokens, 2 x 4 heads of 256, 151 MB: 34.8 us, 4.3 TB/s (a copy 4.8). With 16 columns
 // and more it is bound by the vector instructions that unpack codes (2048 rows of 8 sequences: 430 us), which kv_many_kernel shares
-// among 128 columns (284 us, 480 TFLOP/s).
+// among 128 columns (282 us, 485 TFLOP/s).
 #include <algorithm>
 #include <cmath>
 
@@ -91,12 +93,27 @@ __device__ __forceinline__ unsigned code_v(const Magic& k, unsigned x, int e) {
 __device__ __forceinline__ h2 as_h2(unsigned u) { return __builtin_bit_cast(h2, u); }
 __device__ __forceinline__ unsigned as_u(h2 h) { return __builtin_bit_cast(unsigned, h); }
 
-// f16 (a0 s0, a1 s1), one rounding each
-__device__ __forceinline__ unsigned scale2(float a0, float a1, unsigned s) {
-  unsigned r;
-  asm("v_fma_mixlo_f16 %0, %1, %3, 0 op_sel_hi:[0,1,0]\n\t"
-      "v_fma_mixhi_f16 %0, %2, %3, 0 op_sel:[0,1,0] op_sel_hi:[0,1,0]" : "=&v"(r) : "v"(a0), "v"(a1), "v"(s));
-  return r;
+// (Results of inline asm may go straight into a matrix instruction, before which the compiler waits for instructions it knows: they
+// end with the two wait states that it would put there.)
+// (a0, a1) as a sum of two f16 each, 22 bits: the first cut off, so that the rest has its sign
+__device__ __forceinline__ u2 split2(float a0, float a1) {
+  const unsigned hi = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pkrtz(a0, a1));
+  unsigned lo;
+  asm("v_fma_mixlo_f16 %0, %1, 1.0, -%3 op_sel_hi:[0,0,1]\n\t"
+      "v_fma_mixhi_f16 %0, %2, 1.0, -%3 op_sel:[0,0,1] op_sel_hi:[0,0,1]\n\t"
+      "s_nop 1" : "=&v"(lo) : "v"(a0), "v"(a1), "v"(hi));
+  return u2{hi, lo};
+}
+// the products of such a pair of sums and the f16 s, again as two f16: h s rounded, and what that leaves (exact) with l s
+__device__ __forceinline__ u2 scale2(unsigned h, unsigned l, unsigned s) {
+  const h2 w = as_h2(h) * as_h2(s);
+  return u2{as_u(w), as_u(__builtin_elementwise_fma(as_h2(l), as_h2(s), __builtin_elementwise_fma(as_h2(h), as_h2(s), -w)))};
+}
+// the larger of two f16 each, NaN the smaller
+__device__ __forceinline__ u2 max2(u2 x, unsigned y) {
+  unsigned a = x[0], b = x[1];
+  asm("v_pk_max_f16 %0, %0, %2\n\tv_pk_max_f16 %1, %1, %2\n\ts_nop 1" : "+v"(a), "+v"(b) : "v"(y));
+  return u2{a, b};
 }
 
 __device__ __forceinline__ f4 gate4(const KvArgs& a, int t, int h, int ch) {
@@ -550,8 +567,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
     qc[g] = -1032.0f * s0 - 72.0f * s1;
   }
   const float scale = a.scale * kLog2e;
-  f4 o[4][kE], zs = {};  // zs[g]: sum P z_g (row 4 i + g of A is group g's zeros)
-  float m = -INFINITY, sum = 0.0f, cs[4] = {};  // cs[g]: the lane's part of -24 sum P s_g
+  const unsigned least = j & 4 ? 0u : 0xFC00FC00u;  // NaN scales are 0 in zs, where columns share them (O has them where they are seen)
+  f4 o[4][kE], zs = {};  // zs[g]: sum P z_g where kg is even, sum P s_g where it is odd (A's row 4 i + g has group g's zeros or scales)
+  float m = -INFINITY, sum = 0.0f;
 #pragma unroll
   for (int g = 0; g < 4; g++)
 #pragma unroll
@@ -608,7 +626,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
         zs *= al;
 #pragma unroll
         for (int g = 0; g < 4; g++) {
-          cs[g] *= al;
 #pragma unroll
           for (int e = 0; e < kE; e++) o[g][e] *= al;
         }
@@ -616,7 +633,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
       m = mn;
     }
     const float base = m == -INFINITY ? 0.0f : m;
-    u4 p;  // P of tokens (t0 + 4 kg + 0, 1), (2, 3), then those of the second tile: f16
+    u4 p, p2;  // P of tokens (t0 + 4 kg + 0, 1), (2, 3), then those of the second tile
 #pragma unroll
     for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -625,29 +642,38 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
         p0 = __builtin_amdgcn_exp2f(fmaf(p0, scale, -base));
         p1 = __builtin_amdgcn_exp2f(fmaf(p1, scale, -base));
         sum += p0 + p1;
-        p[2 * i + k / 2] = as_u(h2{(_Float16)p0, (_Float16)p1});
+        const u2 x = split2(p0, p1);
+        p[2 * i + k / 2] = x[0];
+        p2[2 * i + k / 2] = x[1];
       }
     {
-      const u2 z0 = reinterpret_cast<const u2*>(par + 32 + (j & 3))[1], z1 = reinterpret_cast<const u2*>(par + 48 + (j & 3))[1];
-      zs = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, u4{z0[0], z0[1], z1[0], z1[1]}), __builtin_bit_cast(h8, p), zs, 0, 0, 0);
+      u2 z[2];
+#pragma unroll
+      for (int i = 0; i < 2; i++) {
+        z[i] = max2(reinterpret_cast<const u2*>(par + 32 + 16 * i + (j & 3))[j & 4 ? 0 : 1], least);
+      }
+      const h8 zh = __builtin_bit_cast(h8, u4{z[0][0], z[0][1], z[1][0], z[1][1]});
+      zs = __builtin_amdgcn_mfma_f32_16x16x32_f16(zh, __builtin_bit_cast(h8, p), zs, 0, 0, 0);
+      zs = __builtin_amdgcn_mfma_f32_16x16x32_f16(zh, __builtin_bit_cast(h8, p2), zs, 0, 0, 0);
     }
-    const h2 off = {(_Float16)-24.0f, (_Float16)-24.0f};
 #pragma unroll
     for (int g = 0; g < 4; g++) {
-      const u2 vs[2] = {*reinterpret_cast<const u2*>(par + 32 + g), *reinterpret_cast<const u2*>(par + 48 + g)};
-      u4 w;  // P s_g
+      u2 vs[2] = {*reinterpret_cast<const u2*>(par + 32 + g), *reinterpret_cast<const u2*>(par + 48 + g)};
+      if (edge) {
 #pragma unroll
-      for (int k = 0; k < 4; k++) w[k] = scale2(sc[k >> 1][2 * (k & 1)], sc[k >> 1][2 * (k & 1) + 1], vs[k >> 1][k & 1]);
-      if (edge) {  // a masked token's scale may be NaN
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < 4; k++) {  // a masked token's scale may be NaN
           const int tok = t0 + 16 * (k >> 1) + 4 * kg + 2 * (k & 1);
-          w[k] = tok + 1 <= last ? w[k] : tok <= last ? w[k] & 0xFFFFu : 0u;
+          vs[k >> 1][k & 1] &= tok + 1 <= last ? 0xFFFFFFFFu : tok <= last ? 0xFFFFu : 0u;
         }
       }
-      const h8 wh = __builtin_bit_cast(h8, w);
+      u4 w, w2;  // P s_g
 #pragma unroll
-      for (int k = 0; k < 4; k++) cs[g] = __builtin_amdgcn_fdot2(as_h2(w[k]), off, cs[g], false);
+      for (int k = 0; k < 4; k++) {
+        const u2 x = scale2(p[k], p2[k], vs[k >> 1][k & 1]);
+        w[k] = x[0];
+        w2[k] = x[1];
+      }
+      const h8 wh = __builtin_bit_cast(h8, w), wh2 = __builtin_bit_cast(h8, w2);
       unsigned x[4];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
@@ -658,6 +684,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
       for (int e = 0; e < kE; e++) {
         const u4 op = {code_v(mg, x[0], e), code_v(mg, x[1], e), code_v(mg, x[2], e), code_v(mg, x[3], e)};
         o[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, op), wh, o[g][e], 0, 0, 0);
+        o[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, op), wh2, o[g][e], 0, 0, 0);
       }
     }
     if constexpr (more) fetch_v();
@@ -665,6 +692,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
   };
   for (int seg = k0;;) {  // segments of 1024 keys, whose pages the lanes hold
     const int end = min(seg + 1024, k1);
+    if (seg > k0) {
+      // The offsets of the segment before: sums of 16 + c that ran on would lose what remains of c - 8 (131072 values of equal weight
+      // whose mean is zero came out as up to 5.2e-5; now below 2.7e-7).
+#pragma unroll
+      for (int g = 0; g < 4; g++) {
+        const float t = sum_quads(kg & 1 ? -12.0f * zs[g] : 0.0f);  // (two of the four lanes have it)
+        if (kg & 1) zs[g] = 0.0f;
+#pragma unroll
+        for (int e = 0; e < kE; e++) o[g][e] += t;
+      }
+    }
     int t0 = seg + kStep * wave;
 #pragma clang loop unroll(disable)
     for (; t0 + kStep * kWaves < end; t0 += kStep * kWaves) step(seg, t0, std::true_type{});
@@ -675,21 +713,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
     locate(seg, seg + kStep * wave);
     fetch_k();
     fetch_v();
-    // The segment's offsets: sums of 16 + c that ran on would lose what remains of c - 8 (131072 values of equal weight whose mean is
-    // zero came out as up to 5.2e-5; now below 2.7e-7).
-#pragma unroll
-    for (int g = 0; g < 4; g++) {
-      const float t = sum_quads(cs[g]);
-      cs[g] = 0.0f;
-#pragma unroll
-      for (int e = 0; e < kE; e++) o[g][e] += t;
-    }
   }
   // the four waves' sums: O^T row 4 kg + k of (g, e) is channel G g + 16 kg + 4 k + e (HD 256), G g + 4 (row & 7) + 2 (row >> 3) + e
   // (HD 128)
   sum = sum_quads(sum);
 #pragma unroll
-  for (int g = 0; g < 4; g++) zs[g] += sum_quads(cs[g]);
+  for (int g = 0; g < 4; g++) zs[g] = sum_quads((kg & 1 ? -12.0f : 0.5f) * zs[g]);
   if (kg == 0) {
     ml[wave][j][0] = m;
     ml[wave][j][1] = sum;
@@ -828,7 +857,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
 typedef float f16v __attribute__((ext_vector_type(16)));
 
 // LDS of kv_many_kernel, each part twice: K tile [32][HD] and V^T tile [HD][32] as f16 (rows 16 bytes longer, so that eight rows
-// of an operand lie in different banks), K's scales [4][32] and zeros [32][4] twice each, P f32 in the lanes' order, the columns'
+// of an operand lie in different banks), K's scales [4][32] and zeros [32][4] twice each, P as two f16 in the lanes' order, the columns'
 // factors, the waves' flags and the class of V's scales; V's scales and zeros [4][32] each of four tiles.
 template <int HD>
 struct ManyLds {
@@ -844,9 +873,12 @@ struct ManyLds {
 // kind, so the matrix products of the one run beside the vector instructions of the other. One barrier a tile, which takes about
 // 3700 cycles (HD 256): matrix products 1060 of them a SIMD, vector instructions about 2150, LDS about 2000 (250 KB read and
 // written), each waiting for the others at times; with 64 columns a wave that compute P, or the values unpacked by both kinds,
-// it took longer (spills; 311 us instead of 296 for 2048 rows of 8 sequences). Scales and zeros
+// it took longer (spills; 311 us where this took 296 for 2048 rows of 8 sequences). Scales and zeros
 // stay apart from the codes, so that both operands are exact: S = sum_g s_g (q . (c - 8))_g + sum_g z_g sum(q_g), the last
-// as one more product (with sum(q_g) / G as two f16), and O takes P s_g, rounded to f16 once, and sum P z_g.
+// as one more product (with sum(q_g) / G as two f16), and O takes P s_g and sum P z_g. P goes through LDS as two f16 each; P s_g is
+// rounded to f16 once here (2.75e-4 of the output's norm, 2.07e-4 of it the output's own rounding; the framework's attention on f16
+// rows rounds its P as well): two f16 each, as above, would be 16 more matrix instructions and as many vector ones a tile in the
+// waves that bound it, 346 us instead of 282.
 template <int HD>
 __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
   constexpr int G = HD / 4, U = HD / 16, kRow = HD / 2, kKs = G / 16, kDt = HD / 64;  // kKs: k-steps of a group; kDt: 32-row blocks of V^T a wave
@@ -1016,7 +1048,7 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
           if (half == 0) *reinterpret_cast<float*>(buf + M::kAl + 4 * (w0 + c32)) = al;
         }
         const float base = m == -INFINITY ? 0.0f : m;
-        f4* pl = reinterpret_cast<f4*>(buf + M::kP) + wave * 256 + lane;
+        u4* pl = reinterpret_cast<u4*>(buf + M::kP) + wave * 256 + lane;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           f4 p;
@@ -1025,7 +1057,8 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
             p[e] = __builtin_amdgcn_exp2f(fmaf(st[4 * k + e], scale, -base));
             sum += p[e];
           }
-          pl[64 * k] = p;
+          const u2 x = split2(p[0], p[1]), y = split2(p[2], p[3]);
+          pl[64 * k] = u4{x[0], y[0], x[1], y[1]};
         }
       }
       if (i + 1 < tiles) {
@@ -1088,15 +1121,14 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
     const int t0 = kTile * (i - 1);
     const unsigned char* buf = lds + ((i & 1) ^ 1) * M::kBuf;
     // what the outputs need first is on its way while the codes are unpacked
-    f4 p[2][4];
-    u4 ps[2][2], pz[2][2];
+    u4 p[2][4], ps[2][2], pz[2][2];  // p: of two pairs of keys, and what their f16 leave
     bool f0 = false, f1 = false;
     const unsigned char* par = lds + M::kParam + ((i - 1) & 3) * 512 + 16 * half;
     if (takes) {
       const int* flag = reinterpret_cast<const int*>(buf + M::kFlag) + 2 * cp;
       f0 = flag[0];
       f1 = flag[1] && 64 * cp + 32 < cols;
-      const f4* pl = reinterpret_cast<const f4*>(buf + M::kP) + 2 * cp * 256 + lane;
+      const u4* pl = reinterpret_cast<const u4*>(buf + M::kP) + 2 * cp * 256 + lane;
 #pragma unroll
       for (int k = 0; k < 4; k++)
 #pragma unroll
@@ -1128,27 +1160,18 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
       const unsigned char* vr = buf + M::kV + (2 * dh * G + c32) * M::kVPitch + 16 * half;
 #pragma unroll
       for (int kb = 0; kb < 2; kb++) {
-        unsigned ph[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; n++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const f4 x = p[n][2 * kb + (k >> 1)];
-            ph[n][k] = as_u(h2{(_Float16)x[2 * (k & 1)], (_Float16)x[2 * (k & 1) + 1]});
-          }
 #pragma unroll
         for (int gg = 0; gg < 2; gg++) {
-          const u4 s = ps[kb][gg];
-#pragma unroll
-          for (int n = 0; n < 2; n++)
-#pragma unroll
-            for (int k = 0; k < 4; k++) zs[n][gg] = __builtin_amdgcn_fdot2(as_h2(ph[n][k]), as_h2(pz[kb][gg][k]), zs[n][gg], false);
           h8 wh[2];
 #pragma unroll
           for (int n = 0; n < 2; n++) {
             u4 w;
 #pragma unroll
-            for (int k = 0; k < 4; k++) w[k] = scale2(p[n][2 * kb + (k >> 1)][2 * (k & 1)], p[n][2 * kb + (k >> 1)][2 * (k & 1) + 1], s[k]);
+            for (int k = 0; k < 4; k++) {
+              const h2 hi = as_h2(p[n][2 * kb + (k >> 1)][k & 1]), lo = as_h2(p[n][2 * kb + (k >> 1)][2 + (k & 1)]), z = as_h2(pz[kb][gg][k]), s = as_h2(ps[kb][gg][k]);
+              zs[n][gg] = __builtin_amdgcn_fdot2(lo, z, __builtin_amdgcn_fdot2(hi, z, zs[n][gg], false), false);
+              w[k] = as_u(__builtin_elementwise_fma(hi, s, lo * s));
+            }
             if (edge) {  // a masked token's scale may be NaN
 #pragma unroll
               for (int k = 0; k < 4; k++) {

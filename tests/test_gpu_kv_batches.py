@@ -286,3 +286,19 @@ def test_one_heavy_token_of_no_value_and_many_light_ones(seqs, heads):
     w = np.stack([want[t] for t in sorted(want)])
     # as check(), and the output's own steps of 2^-24
     assert np.isfinite(e).all() and np.linalg.norm(e) <= 2 ** -10 * np.linalg.norm(w) + 2 ** -25 * np.sqrt(e.size)
+
+
+@pytest.mark.parametrize("seqs,heads", [
+    ([(3000, 1)], MODEL), ([(20000, 1)], (16, 1, 128, 8)), ([(2000, 61)], MODEL), ([(1500, 5), (0, 40), (700, 1)], H8), ([(90, 1)] * 140, H16)])
+def test_outputs_of_few_columns_are_rounded_once(seqs, heads):
+    """P and its products with scales keep 22 bits, so what differs from the rounded exact output is rounding the other way."""
+    c = Call(seqs, heads, 64, seed=18)
+    want = c.expected(rows=some(c, 20))
+    got = c.attention()
+    w = np.stack([want[t] for t in sorted(want)])
+    e = np.stack([got[t].astype(np.float64) for t in sorted(want)]) - w.astype(np.float16)
+    # The largest error is a score's: sums near 2^13 (1032 times the sum of 32 of q) of four groups, rounded some four times to 2^-12 at most,
+    # times a scale of 2^-1.6 and 1 / sqrt(HD) = 2^-4 (2^-3.5): 2^-16 of P, and of the output. Where an output lies within that of the
+    # middle between two f16, it is a step off: in the mean, squared, a step (2^-10.5 of the value) times the error, 2^-26.5, of which the
+    # root is 2^-13.2. (One f16 for P or P s: 2^-12.)
+    assert np.linalg.norm(e) <= 2 ** -12.8 * np.linalg.norm(w)
