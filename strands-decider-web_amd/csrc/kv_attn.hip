@@ -125,7 +125,7 @@ __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf
 // ---- who does what ----
 //
 // The host knows neither how long the sequences are nor which of them have many rows, so the device shares the work out. A
-// sequence has lo < columns <= hi of one of two kinds (few, many); its (column block, KV head)s are units. Units of few columns
+// sequence is of one of two kinds (few or many columns); its (column block, KV head)s are units. Units of few columns
 // are cut into pieces of `chunk` keys, chosen so that all of them make about `want` pieces; those of many columns, which are only
 // used where they fill the chip, are not. A workgroup's index is its place in the list of all pieces of all sequences, which
 // each wave finds by a prefix sum with a sequence a lane. Of more than kScanMost sequences the sums are taken once, by
@@ -134,14 +134,17 @@ __device__ __forceinline__ float sigmoid(float x) { return __builtin_amdgcn_rcpf
 constexpr int kWant = 512;                // pieces: two workgroups a CU
 constexpr size_t kSlots = 2 * kWant;      // (cut units have less than 2 kWant pieces)
 constexpr size_t kSlotBytes = (size_t)kCols * (256 + 4) * sizeof(float);
+constexpr int kFewCols = 256, kManyUnits = 160;  // (see attend())
 struct Kind {
   float* p;  // results of the pieces of cut units: for each piece and column O (unnormalised) [HD], maximum, sum
   int* count;  // of a cut unit's pieces (a group's) that are done, at the first one's slot, then of its groups; zero between calls
-  int* plan;   // or nullptr: keys a piece; then for each sequence the sums up to and with it of its pieces, of those of them that
-               // are cut, and of its (row, head)s to be merged, and the greatest row_start up to its own
+  int* plan;   // or nullptr: keys a piece, limit_of(); then for each sequence the sums up to and with it of its pieces, of those of
+               // them that are cut, and of its (row, head)s to be merged, and the greatest row_start up to its own
   int cols;  // columns a block has, at most
-  int lo, hi, want, direct, ncb;
+  int split;   // both kinds are in use
+  int want, direct, ncb;
 };
+constexpr int kPlanHead = 2;
 struct Item {
   int b, kh, cb, piece, size, slot;  // size: keys a piece; slot: of the piece, where there is more than one
   int row;                            // of the sequence (merge)
@@ -154,15 +157,32 @@ struct Lane {
   Seq sq;
   int ncb;
 };
-template <int BC>
-__device__ __forceinline__ Lane lane_of(const KvArgs& a, const Kind& k, const Seq& sq) {
-  Lane l{sq, 0};
+// A unit of many columns is not cut: one that walks many more keys than the others would end long after them. So a sequence of more
+// than kFewCols columns is only one of many where its context is at most `limit`: the keys of all such sequences' units over
+// kManyUnits, w / kManyUnits: its units then end within 256 / kManyUnits of the time in which those of all would, spread evenly.
+// (6 prompts of 1000 rows and 100 rows after 6000, 20000 and 131000 tokens, us: 126, 166 and 383; 320, 993 and 6320 without a limit.)
+// (No contraction: the kernels of a call have to agree on it.)
+__device__ __forceinline__ float wide_keys(const KvArgs& a, const Seq& sq) {
+#pragma clang fp contract(off)
   const int cols = sq.n * a.ratio;
-  if (cols > k.lo && cols <= k.hi) l.ncb = sq.ok ? (cols + BC - 1) / BC : 1;  // (one unit writes all rows of a sequence that does not fit)
-  return l;
+  return cols > kFewCols ? (float)((cols + kBigCols - 1) / kBigCols) * (float)sq.len : 0.0f;
+}
+__device__ __forceinline__ int limit_of(const KvArgs& a, float w) { return uniform((int)fminf(w * (float)a.HK * (1.0f / kManyUnits), 1e9f)); }
+__device__ __forceinline__ int limit_of(const KvArgs& a, const Kind& k, const Seq& first, int lane, int top) {
+#pragma clang fp contract(off)
+  if (!k.split) return 0;
+  float w = wide_keys(a, first);
+  for (int s0 = 64; s0 < a.n_seqs; s0 += 64) w += wide_keys(a, seq_in_order(a, s0 + lane, top));
+  return limit_of(a, __builtin_bit_cast(float, lane_value(__builtin_bit_cast(int, scan64(w)), 63)));
 }
 template <int BC>
-__device__ __forceinline__ Lane lane_of(const KvArgs& a, const Kind& k, int s, int& top) { return lane_of<BC>(a, k, seq_in_order(a, s, top)); }
+__device__ __forceinline__ Lane lane_of(const KvArgs& a, const Kind& k, const Seq& sq, int limit) {
+  Lane l{sq, 0};
+  const int cols = sq.n * a.ratio;
+  const bool many = k.split && cols > kFewCols && sq.len <= limit;
+  if (cols > 0 && many == (BC == kBigCols)) l.ncb = sq.ok ? (cols + BC - 1) / BC : 1;  // (one unit writes all rows of a sequence that does not fit)
+  return l;
+}
 constexpr int kUnit = kStep * kWaves;  // keys that a piece has at least
 constexpr int kEven = 4;               // times that, from which pieces are made even
 // a / s of 0 <= a < 2^21, s > 0: (a + 1/2) / s is 1 / (2 s) away from the next integer, its error at most a 2^-22 / s
@@ -183,10 +203,10 @@ __device__ __forceinline__ int pieces_of(int len, int size) {
 __device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, float w) {
   return uniform(kUnit * max(1, (int)fminf(ceilf(w * (float)a.HK / (float)(k.want * kUnit)), 1e6f)));
 }
-__device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, const Lane& first, int lane, int top) {
+__device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, const Lane& first, int lane, int top, int limit) {
   float w = (float)first.ncb * (float)first.sq.len;
   for (int s0 = 64; s0 < a.n_seqs; s0 += 64) {
-    const Lane l = lane_of<kCols>(a, k, s0 + lane, top);
+    const Lane l = lane_of<kCols>(a, k, seq_in_order(a, s0 + lane, top), limit);
     w += (float)l.ncb * (float)l.sq.len;
   }
   return chunk_of(a, k, __builtin_bit_cast(float, lane_value(__builtin_bit_cast(int, scan64(w)), 63)));
@@ -217,7 +237,7 @@ __global__ __launch_bounds__(1024) void kv_plan_kernel(KvArgs a, Kind k) {
   __shared__ float ws[16];
   __shared__ int tot[16][3], tops[16];
   const int tid = threadIdx.x, wave = tid >> 6, per = (a.n_seqs + 1023) / 1024, s0 = tid * per, s1 = min(s0 + per, a.n_seqs);
-  int* sums = k.plan + 1;
+  int* sums = k.plan + kPlanHead;
   int top = 0;  // of the thread's sequences, then of those before them
   for (int s = s0; s < s1; s++) top = max(top, a.row_start[s]);
   top = max64(top);
@@ -226,22 +246,33 @@ __global__ __launch_bounds__(1024) void kv_plan_kernel(KvArgs a, Kind k) {
   if ((tid & 63) == 0) top = 0;
   __syncthreads();
   for (int x = 0; x < wave; x++) top = max(top, tops[x]);
+  auto block_sum = [&](float w) {
+    w = scan64(w);
+    __syncthreads();
+    if ((tid & 63) == 63) ws[wave] = w;
+    __syncthreads();
+    w = 0.0f;
+    for (int x = 0; x < 16; x++) w += ws[x];
+    return w;
+  };
   float w = 0.0f;
   for (int s = s0; s < s1; s++) {
     top = max(top, a.row_start[s]);
     sums[3 * kPlanMost + s] = top;
-    const Lane l = lane_of<kCols>(a, k, seq_of(a, s, top));
+    w += wide_keys(a, seq_of(a, s, top));
+  }
+  const int limit = limit_of(a, block_sum(w));
+  auto lane = [&](int s) { return lane_of<kCols>(a, k, seq_of(a, s, sums[3 * kPlanMost + s]), limit); };
+  w = 0.0f;
+  for (int s = s0; s < s1; s++) {
+    const Lane l = lane(s);
     w += (float)l.ncb * (float)l.sq.len;
   }
-  w = scan64(w);
-  if ((tid & 63) == 63) ws[wave] = w;
-  __syncthreads();
-  w = 0.0f;
-  for (int x = 0; x < 16; x++) w += ws[x];
+  w = block_sum(w);
   const int chunk = chunk_of(a, k, w);
   Counts c{};
   for (int s = s0; s < s1; s++) {
-    const Counts x = counts_of(a, k, lane_of<kCols>(a, k, seq_of(a, s, sums[3 * kPlanMost + s])), chunk);
+    const Counts x = counts_of(a, k, lane(s), chunk);
     c = Counts{c.items + x.items, c.cut + x.cut, c.rows + x.rows, 0, 0};
   }
   const Counts in = {scan64(c.items), scan64(c.cut), scan64(c.rows), 0, 0};
@@ -253,9 +284,12 @@ __global__ __launch_bounds__(1024) void kv_plan_kernel(KvArgs a, Kind k) {
   __syncthreads();
   Counts at = {in.items - c.items, in.cut - c.cut, in.rows - c.rows, 0, 0};
   for (int x = 0; x < wave; x++) at = Counts{at.items + tot[x][0], at.cut + tot[x][1], at.rows + tot[x][2], 0, 0};
-  if (tid == 0) k.plan[0] = chunk;
+  if (tid == 0) {
+    k.plan[0] = chunk;
+    k.plan[1] = limit;
+  }
   for (int s = s0; s < s1; s++) {
-    const Counts x = counts_of(a, k, lane_of<kCols>(a, k, seq_of(a, s, sums[3 * kPlanMost + s])), chunk);
+    const Counts x = counts_of(a, k, lane(s), chunk);
     at = Counts{at.items + x.items, at.cut + x.cut, at.rows + x.rows, 0, 0};
     sums[s] = at.items;
     sums[kPlanMost + s] = at.cut;
@@ -288,10 +322,10 @@ __device__ __forceinline__ bool find_piece(const KvArgs& a, const Kind& k, int x
   }
   int rel, ns;  // rel: piece of the sequence; ns: pieces of a unit
   if (k.plan) {
-    const int *sums = k.plan + 1, s = search(sums, a.n_seqs, x);
+    const int *sums = k.plan + kPlanHead, s = search(sums, a.n_seqs, x);
     if (s == a.n_seqs) return false;
     it.b = s;
-    const Lane l = lane_of<kCols>(a, k, seq_of(a, s, gp<int>(sums)[3 * kPlanMost + s]));
+    const Lane l = lane_of<kCols>(a, k, seq_of(a, s, gp<int>(sums)[3 * kPlanMost + s]), gp<int>(k.plan)[1]);
     const Counts c = counts_of(a, k, l, gp<int>(k.plan)[0]);
     it.size = uniform(c.size);
     ns = uniform(c.ns);
@@ -300,11 +334,13 @@ __device__ __forceinline__ bool find_piece(const KvArgs& a, const Kind& k, int x
     it.sq = l.sq;
   } else {
     int top = 0;
-    Lane l = lane_of<kCols>(a, k, lane, top);
-    const int chunk = chunk_of(a, k, l, lane, top);
+    const Seq first = seq_in_order(a, lane, top);
+    const int limit = limit_of(a, k, first, lane, top);
+    Lane l = lane_of<kCols>(a, k, first, limit);
+    const int chunk = chunk_of(a, k, l, lane, top, limit);
     int base = 0, slots = 0;
     for (int s0 = 0;; s0 += 64) {
-      if (s0) l = lane_of<kCols>(a, k, s0 + lane, top);
+      if (s0) l = lane_of<kCols>(a, k, seq_in_order(a, s0 + lane, top), limit);
       const Counts c = counts_of(a, k, l, chunk);
       const int sum = scan64(c.items), csum = scan64(c.cut);
       const unsigned long long past = __ballot(base + sum > x);
@@ -343,8 +379,11 @@ __device__ __forceinline__ bool find_block(const KvArgs& a, const Kind& k, int x
     return it.cb * kBigCols < it.sq.n * a.ratio && (it.sq.ok || it.cb == 0);
   }
   int top = 0;
+  Seq sq = seq_in_order(a, lane, top);
+  const int limit = k.plan ? gp<int>(k.plan)[1] : limit_of(a, k, sq, lane, top);
   for (int s0 = 0; s0 < a.n_seqs; s0 += 64) {
-    const Lane l = lane_of<kBigCols>(a, k, s0 + lane, top);
+    if (s0) sq = seq_in_order(a, s0 + lane, top);
+    const Lane l = lane_of<kBigCols>(a, k, sq, limit);
     const int all = lane_value(scan64(l.ncb), 63) * a.HK;
     if (x >= all) {
       x -= all;
@@ -376,10 +415,10 @@ __device__ __forceinline__ bool find_row(const KvArgs& a, const Kind& k, int x, 
   const int lane = threadIdx.x & 63;
   int rel, ns, slot = 0;
   if (k.plan) {
-    const int *sums = k.plan + 1, s = search(sums + 2 * kPlanMost, a.n_seqs, x);
+    const int *sums = k.plan + kPlanHead, s = search(sums + 2 * kPlanMost, a.n_seqs, x);
     if (s == a.n_seqs) return false;
     it.b = s;
-    const Lane l = lane_of<kCols>(a, k, seq_of(a, s, gp<int>(sums)[3 * kPlanMost + s]));
+    const Lane l = lane_of<kCols>(a, k, seq_of(a, s, gp<int>(sums)[3 * kPlanMost + s]), gp<int>(k.plan)[1]);
     const Counts c = counts_of(a, k, l, gp<int>(k.plan)[0]);
     it.size = uniform(c.size);
     ns = uniform(c.ns);
@@ -388,11 +427,13 @@ __device__ __forceinline__ bool find_row(const KvArgs& a, const Kind& k, int x, 
     it.sq = l.sq;
   } else {
     int top = 0;
-    Lane l = lane_of<kCols>(a, k, lane, top);
-    const int chunk = chunk_of(a, k, l, lane, top);
+    const Seq first = seq_in_order(a, lane, top);
+    const int limit = limit_of(a, k, first, lane, top);
+    Lane l = lane_of<kCols>(a, k, first, limit);
+    const int chunk = chunk_of(a, k, l, lane, top, limit);
     int base = 0;
     for (int s0 = 0;; s0 += 64) {
-      if (s0) l = lane_of<kCols>(a, k, s0 + lane, top);
+      if (s0) l = lane_of<kCols>(a, k, seq_in_order(a, s0 + lane, top), limit);
       const Counts c = counts_of(a, k, l, chunk);
       const int sum = scan64(c.rows), csum = scan64(c.cut);
       const unsigned long long past = __ballot(base + sum > x);
@@ -1304,8 +1345,9 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvArgs a, Kind kind) {
 // 81 / 83, 132 / 94; 3000, 1777, 2000, 1000 rows (243) 218 / 172; 2 or 4 of 1500 rows after 500, 2 of 600, 30 single ones (132,
 // 226) 120 / 133, 205 / 163; 32 heads of 128 on 8: 1000, 1200, 1500 rows of one (125, 150, 187) 50 / 55, 69 / 64, 95 / 78; 777
 // rows, 130 after 2000, 300 after 64, 8 single ones (152) 71 / 118; 100 rows after 500 of 16 (366) 86 / 76. Up to kFewCols columns
-// a sequence stays with the first also beside others that do not.
-constexpr int kFewCols = 256, kManyUnits = 160;
+// a sequence stays with the first also beside others that do not, and so does one whose context is over limit_of(). Only equal
+// numbers of rows on contexts of at most twice as many are laid out in a grid, as other contexts may be of any lengths (8 sequences of
+// 500 rows after 1000, us: 101 in a grid, 105 so; 7 prompts of 800 rows and 800 rows after 60000: 5990 in a grid, 1280 so).
 // Contexts up to which more than kScanMost sequences are neither cut nor planned. Measured, us, in a grid / planned: single rows of
 // 140 sequences of 100, 1000, 3000 tokens 8.2 / 12.2, 25.6 / 31.6, 64.6 / 62.8, of 1000 sequences of 10 tokens 22 / 30, of 200 of
 // 300 and one of 20000 250 / 26.
@@ -1316,37 +1358,38 @@ hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
   const bool equal = (long)a.n_rows == (long)a.n_seqs * a.max_rows;
   const double units_of_many = (double)a.n_rows * a.ratio / kBigCols * a.HK;
   const bool use_many = most > kFewCols && units_of_many * (equal ? 1.0 - 0.5 * a.max_rows / a.max_len : 0.5) >= kManyUnits;
+  const bool direct = use_many && equal && a.max_len <= 2 * a.max_rows;  // (else the contexts may be of any lengths)
   Kind few{}, many{};
   few.p = ws;
   few.count = reinterpret_cast<int*>(ws + kSlots * kSlotBytes / sizeof(float));
-  few.hi = !use_many ? 0x7fffffff : equal ? 0 : kFewCols;
+  few.split = many.split = use_many;
   few.cols = std::min(kCols, most);
   few.want = kWant;
-  many.lo = few.hi;
-  many.hi = 0x7fffffff;
+  few.ncb = (std::min(most, use_many ? kFewCols : most) + kCols - 1) / kCols;
+  const bool rows_in_grid = a.n_seqs > kScanMost && few.ncb == 1 && a.max_len <= kDirectKeys;
   hipError_t e = hipSuccess;
+  if (a.n_seqs > kScanMost && !direct && !rows_in_grid) {
+    few.plan = many.plan = few.count + 2 * kSlots;
+    hipLaunchKernelGGL(kv_plan_kernel, dim3(1), dim3(1024), 0, s, a, few);
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+  }
   if (use_many) {
-    many.direct = equal;
+    many.direct = direct;
     many.ncb = (most + kBigCols - 1) / kBigCols;
-    const long grid = equal ? (long)a.n_seqs * a.HK * many.ncb : ((long)a.n_rows * a.ratio / kBigCols + a.n_seqs) * a.HK;
+    const long grid = direct ? (long)a.n_seqs * a.HK * many.ncb : ((long)a.n_rows * a.ratio / kBigCols + a.n_seqs) * a.HK;
     constexpr int lds = ManyLds<HD>::kAll;
     e = hipFuncSetAttribute(reinterpret_cast<const void*>(kv_many_kernel<HD>), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;
     hipLaunchKernelGGL((kv_many_kernel<HD>), dim3((unsigned)grid), dim3(512), lds, s, a, many);
-    if ((e = hipGetLastError()) != hipSuccess || equal) return e;
+    if ((e = hipGetLastError()) != hipSuccess || direct) return e;
   }
-  few.ncb = (std::min(most, few.hi) + kCols - 1) / kCols;
-  const long units = std::min<long>((long)a.n_seqs * few.ncb, (long)a.n_rows * a.ratio / kCols + a.n_seqs) * a.HK;
+  // units of few columns; those of sequences whose contexts are over the limit are less than kManyUnits of 128 columns
+  const long units = std::min<long>((long)a.n_seqs * few.ncb, (long)a.n_rows * a.ratio / kCols + a.n_seqs) * a.HK +
+                     (use_many ? kManyUnits * (kBigCols / kCols) : 0);
   dim3 grid((unsigned)(units + (a.max_len > kUnit ? kSlots : 0)));
-  if (a.n_seqs > kScanMost) {
-    if (few.ncb == 1 && a.max_len <= kDirectKeys) {
-      few.direct = 1;
-      grid = dim3((unsigned)a.n_seqs, (unsigned)a.HK);
-    } else {
-      few.plan = few.count + 2 * kSlots;
-      hipLaunchKernelGGL(kv_plan_kernel, dim3(1), dim3(1024), 0, s, a, few);
-      if ((e = hipGetLastError()) != hipSuccess) return e;
-    }
+  if (rows_in_grid) {
+    few.direct = 1;
+    grid = dim3((unsigned)a.n_seqs, (unsigned)a.HK);
   }
   hipLaunchKernelGGL((kv_few_kernel<HD>), grid, dim3(64 * kWaves), 0, s, a, few);
   if ((e = hipGetLastError()) != hipSuccess || a.max_len <= kUnit || few.direct) return e;
@@ -1359,7 +1402,7 @@ hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
 
 }  // namespace
 
-size_t kv_workspace_bytes() { return kSlots * (kSlotBytes + 2 * sizeof(int)) + sizeof(int) * (1 + 4 * (size_t)kPlanMost); }
+size_t kv_workspace_bytes() { return kSlots * (kSlotBytes + 2 * sizeof(int)) + sizeof(int) * (kPlanHead + 4 * (size_t)kPlanMost); }
 
 hipError_t launch_kv_attention(const KvArgs& a, void* ws, hipStream_t s) {
   return a.HD == 256 ? attend<256>(a, static_cast<float*>(ws), s) : attend<128>(a, static_cast<float*>(ws), s);

@@ -302,3 +302,26 @@ def test_outputs_of_few_columns_are_rounded_once(seqs, heads):
     # middle between two f16, it is a step off: in the mean, squared, a step (2^-10.5 of the value) times the error, 2^-26.5, of which the
     # root is 2^-13.2. (One f16 for P or P s: 2^-12.)
     assert np.linalg.norm(e) <= 2 ** -12.8 * np.linalg.norm(w)
+
+
+# a sequence of many rows whose context is far longer than the others' (csrc/kv_attn.hip, limit_of) is cut into pieces beside blocks
+# of many columns: in a ragged batch, among rows of equal numbers, by the plan of more than 128 sequences; also where it does not fit
+@pytest.mark.parametrize("seqs,heads", [
+    ([(9000, 40), (0, 900), (5, 1), (0, 900), (0, 900)], H16),
+    ([(0, 800)] * 3 + [(9000, 800)], H16),
+    ([(20, 1)] * 70 + [(0, 1000), (9000, 35), (0, 1000)] + [(3, 2)] * 60 + [(0, 900)], H16),
+    ([(0, 1100), (6000, 50), (0, 1100), (0, 1000)], (16, 2, 128, 128)),
+    ([(0, 3000)] + [(30, 20)] * 130, H16)])
+def test_a_far_longer_context_among_many_rows(seqs, heads):
+    c = Call(seqs, heads, 64, seed=19, extra=3)
+    got = c.attention()
+    check(got[:c.T], c.expected(rows=some(c, 20)))
+    assert np.isfinite(got[:c.T]).all() and (got[c.T:] == 7).all()
+    np.testing.assert_array_equal(c.attention().view(np.uint16), got.view(np.uint16))
+    b = max(range(len(seqs)), key=lambda b: seqs[b][0])
+    c.dev[1][b] = seqs[b][1] - 1
+    bad = c.attention()
+    mine = np.zeros(len(got), bool)
+    mine[c.start[b]:c.start[b + 1]] = True
+    assert np.isnan(bad[mine]).all()
+    check(bad, {t: w for t, w in c.expected(rows=some(c, 20)).items() if not mine[t]})
