@@ -11,6 +11,7 @@ the GPU) or a raw device address as ``int``. There is no CPU path: loading fails
 """
 import ctypes
 import os
+import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libha.so")
@@ -326,6 +327,28 @@ def add_bias(L, N, y, c, device=0, stream=None):
     _check(_lib.ha_add_bias(L, N, _ptr(y), _ptr(c), device, _st(stream)))
 
 
+def _kv_ptr(x, what, dtype, n, device, rows=None):
+    """The address of a tensor (or a plain address). Raises for tensors that the call could not read or write: of another type
+    than `dtype` or GPU than `device`, of fewer than n elements, or not contiguous (``rows`` may lie apart: so many elements)."""
+    if x is None:
+        return x
+    try:  # (about 0.4 us a tensor: a call's launch takes 4)
+        if x.dtype is dtype and x.get_device() == device and x.numel() >= n and x.is_contiguous():
+            return x.data_ptr()
+    except AttributeError:  # an address, or a buffer of the caller's own kind
+        if not hasattr(x, "is_contiguous"):
+            return _ptr(x)
+    ok = x.is_cuda and x.device.index == device and str(x.dtype) == str(dtype)
+    if ok and rows is None:
+        ok = x.numel() >= n and x.is_contiguous()
+    elif ok:
+        have = x.untyped_storage().nbytes() // x.element_size() - x.storage_offset()
+        ok = n <= 0 or x.numel() >= rows and x.stride(-1) == 1 and have >= n
+    if not ok:
+        raise TypeError("%s must be a contiguous %s tensor of %d elements on GPU %d" % (what, dtype, n, device))
+    return x.data_ptr()
+
+
 class KVBatch:
     """A call's sequences on a :class:`PagedKV` (ha_kv_batch): int32 device arrays ``row_start`` [n_seqs + 1], ``lens``
     [n_seqs] and ``pages`` [n_seqs][table_stride], and the host's bounds on them. The arrays are read when a call runs; this
@@ -336,14 +359,20 @@ class KVBatch:
             if hasattr(x, "data_ptr") and not (x.is_cuda and x.is_contiguous() and str(x.dtype) == "torch.int32" and x.numel() >= n):
                 raise TypeError("row_start, lens and pages must be contiguous int32 device tensors of n_seqs + 1, n_seqs and "
                                 "n_seqs * table_stride elements")
+        devices = {x.device.index for x in (row_start, lens, pages) if hasattr(x, "data_ptr")}
+        if len(devices) > 1:
+            raise TypeError("row_start, lens and pages lie on several GPUs")
+        self._device = devices.pop() if devices else None
         self._held = (row_start, lens, pages)
         self.c = HaKvBatch(n_seqs, n_rows, max_rows, max_len, _ptr(row_start), _ptr(lens), _ptr(pages), table_stride)
+        self._ref = ctypes.byref(self.c)
 
 
 class PagedKV:
     """A paged cache of 4-bit keys and values (ha_kv_*): ``pages`` is the device memory of [n_layers][n_pages] pages of
     ``page_bytes`` bytes, which this object keeps a reference to. ``append`` puts a batch's fused rows into the cache and
-    gives the queries, ``attention`` reads it. Calls on one object must be ordered (one stream, or synchronised)."""
+    gives the queries, ``attention`` reads it. Calls on one object must be ordered (one stream, or synchronised). Tensors (not
+    plain addresses) of another type or GPU than the call's, or that end too early, raise."""
 
     def __init__(self, pages, n_pages, page_size=64, n_layers=1, max_ctx=4096, HQ=8, HK=2, HD=256, rot_dim=64, gated=True,
                  dtype=F16, rope_theta=1e7, eps=1e-6, scale=0.0, device=0):
@@ -361,7 +390,20 @@ class PagedKV:
         if tensor and pages.numel() * pages.element_size() < need:
             self.close()
             raise ValueError("pages must be a device tensor of n_layers * n_pages * page_bytes = %d bytes" % need)
+        if tensor and pages.device.index != device:
+            self.close()
+            raise ValueError("pages lie on GPU %d, the cache on GPU %d" % (pages.device.index, device))
         self._borrowed = pages
+        self._sizes(device)
+
+    def _sizes(self, device):
+        """What its calls check their tensors against."""
+        c, torch = self.cfg, sys.modules.get("torch")  # (no tensor comes from elsewhere)
+        self._device = device
+        self._f16, f32 = (torch.float16, torch.float32) if torch else ("torch.float16", "torch.float32")
+        self._row_type = f32 if c.dtype == F32 else self._f16
+        self._q_len, self._kv_len = c.HQ * c.HD, 2 * c.HK * c.HD
+        self._width = self._q_len * (2 if c.gated else 1) + self._kv_len
 
     @staticmethod
     def page_bytes(page_size=64, HK=2, HD=256):
@@ -378,17 +420,29 @@ class PagedKV:
         _check(_lib.ha_kv_set_param(self._h, layer, name.encode(), a.ctypes.data_as(ctypes.POINTER(ctypes.c_float)),
                                     a.size))
 
+    def _rows_ptr(self, batch, rows, row_stride):
+        if batch._device != self._device and batch._device is not None:
+            raise TypeError("the batch's arrays lie on GPU %d, the cache on GPU %d" % (batch._device, self._device))
+        n, c = batch.c.n_rows, self._width
+        if row_stride < c or row_stride % 8:  # (the library refuses it)
+            return _ptr(rows)
+        return _kv_ptr(rows, "rows", self._row_type, (n - 1) * row_stride + c, self._device, n * c)
+
     def append(self, layer, batch, rows, row_stride, q=None, values=None, stream=None):
         """Norm, rotate and store the batch's rows [n_rows][row_stride]; q [n_rows][HQ][HD] and values
         [n_rows][2][HK][HD] (both f16, may be None) take the queries and the rows as the cache holds them."""
-        _check(_lib.ha_kv_append(self._h, layer, ctypes.byref(batch.c), _ptr(rows), row_stride, _ptr(q), _ptr(values),
-                                 _st(stream)))
+        n = batch.c.n_rows
+        _check(_lib.ha_kv_append(self._h, layer, batch._ref, self._rows_ptr(batch, rows, row_stride), row_stride,
+                                 _kv_ptr(q, "q", self._f16, n * self._q_len, self._device),
+                                 _kv_ptr(values, "values", self._f16, n * self._kv_len, self._device), _st(stream)))
 
     def attention(self, layer, batch, q, rows, row_stride, out, stream=None):
         """out [n_rows][HQ][HD] f16 = gated causal attention of q over the cache (rows, row_stride: the fused rows that
         hold the gates; None, 0 without gates)."""
-        _check(_lib.ha_kv_attention(self._h, layer, ctypes.byref(batch.c), _ptr(q), _ptr(rows), row_stride, _ptr(out),
-                                    _st(stream)))
+        n = batch.c.n_rows
+        _check(_lib.ha_kv_attention(self._h, layer, batch._ref, _kv_ptr(q, "q", self._f16, n * self._q_len, self._device),
+                                    self._rows_ptr(batch, rows, row_stride), row_stride,
+                                    _kv_ptr(out, "out", self._f16, n * self._q_len, self._device), _st(stream)))
 
     def close(self):
         if self._h:

@@ -283,8 +283,7 @@ class PagedKV {
     this.engine = engine;
     this.config = kvConfig(config);
     const need = PagedKV.pageBytes(config) * pick(config, 'nPages', 0) * pick(config, 'nLayers', 1);
-    const have = pages instanceof DeviceView ? pages.buf.bytes - pages.offset : pages instanceof DeviceBuffer ? pages.bytes : need;
-    if (have < need) throw new RangeError('pages of ' + have + ' bytes, the cache needs ' + need);
+    checkBytes('pages', pages, need);
     this._h = native.kvCreate(this.config, ptrOf(pages), engine ? engine.device : pick(config, 'device', 0));
     this._borrowed = [pages].map((x) => (x instanceof DeviceView ? x.buf : x)).filter((x) => x instanceof DeviceBuffer);
     this._borrowed.forEach((x) => { x._borrows++; });
@@ -298,11 +297,23 @@ class PagedKV {
   // Puts the batch's fused rows [nRows][rowStride] into the layer's pages; q [nRows][HQ][HD] and values
   // [nRows][2][HK][HD] (f16, may be null) take the queries and the rows as the cache holds them.
   append(layer, batch, rows, rowStride, q, values) {
+    this._checkCall(batch, rows, rowStride, { q: q, values: values });
     native.kvAppend(this._h, layer, kvBatch(batch), ptrOf(rows), rowStride, optPtrOf(q), optPtrOf(values), this._stream());
   }
   // out [nRows][HQ][HD] (f16) = causal attention of q over the cache, gated by the fused rows of a gated cache.
   attention(layer, batch, q, rows, rowStride, out) {
+    this._checkCall(batch, rows, rowStride, { q: q, out: out });
     native.kvAttention(this._h, layer, kvBatch(batch), ptrOf(q), optPtrOf(rows), rowStride, ptrOf(out), this._stream());
+  }
+  // Device buffers that end before what the call reads or writes (addresses pass).
+  _checkCall(batch, rows, rowStride, outputs) {
+    const c = this.config, n = batch.nRows, HQ = pick(c, 'HQ', 8), HK = pick(c, 'HK', 2), HD = pick(c, 'HD', 256);
+    const width = HQ * HD * (c.gated ? 2 : 1) + 2 * HK * HD;
+    checkBytes('rowStart', batch.rowStart, 4 * (batch.nSeqs + 1));
+    checkBytes('lens', batch.lens, 4 * batch.nSeqs);
+    checkBytes('pages', batch.pages, 4 * batch.nSeqs * batch.tableStride);
+    if (n > 0) checkBytes('rows', rows, (c.dtype === F32 ? 4 : 2) * ((n - 1) * rowStride + Math.min(width, rowStride)));
+    Object.keys(outputs).forEach((k) => checkBytes(k, outputs[k], 2 * n * (k === 'values' ? 2 * HK : HQ) * HD));
   }
   _stream() {
     return this.engine ? this.engine._h : null;
@@ -315,6 +326,11 @@ class PagedKV {
       this._borrowed = [];
     }
   }
+}
+
+function checkBytes(what, x, need) {
+  const have = x instanceof DeviceView ? x.buf.bytes - x.offset : x instanceof DeviceBuffer ? x.bytes : need;
+  if (have < need) throw new RangeError(what + ' of ' + have + ' bytes, the cache needs ' + need);
 }
 
 function kvConfig(c) {

@@ -44,3 +44,36 @@ def test_refusals():
     assert out["dtype"] == "TypeError: unsupported dtype bf16" and out["number"] == "TypeError: pages must be a BigInt"
     for k in ("append", "attention", "param", "destroy"):
         assert out[k] == "TypeError: not a PagedKV handle"
+
+
+BUFFERS = r"""
+const path = require('path');
+const ha = require(path.join(%(js)r, 'engine.js'));
+const buffer = (bytes) => Object.assign(Object.create(ha.DeviceBuffer.prototype), {bytes: bytes, ptr: BigInt(4096), _borrows: 0});
+const code = (fn) => { try { return fn(); } catch (e) { return e.name + ': ' + e.message; } };
+const kv = Object.assign(Object.create(ha.PagedKV.prototype), {engine: null, _h: {}, config: {HQ: 4, HK: 2, HD: 128, gated: 1, dtype: %(dtype)d}});
+const width = 4 * 2 * 128 + 2 * 2 * 128, stride = width + 64, e = %(dtype)d ? 2 : 4;
+const need = {rows: e * (2 * stride + width), q: 2 * 3 * 4 * 128, values: 2 * 3 * 2 * 2 * 128, out: 2 * 3 * 4 * 128, rowStart: 12, lens: 8, pages: 32};
+const out = {};
+for (const less of [null].concat(Object.keys(need))) {
+  const at = (k) => k === less ? (k.length & 1 ? buffer(need[k] - 1) : new ha.DeviceView(buffer(need[k] + 4), 8)) : buffer(need[k]);
+  const b = {nSeqs: 2, nRows: 3, maxRows: 2, maxLen: 20, tableStride: 4, rowStart: at('rowStart'), lens: at('lens'), pages: at('pages')};
+  out[less] = [code(() => kv.append(0, b, at('rows'), stride, at('q'), at('values'))), code(() => kv.append(0, b, at('rows'), stride, null, null)),
+               code(() => kv.attention(0, b, at('q'), at('rows'), stride, at('out')))];
+}
+console.log(JSON.stringify(out));
+"""
+
+
+@pytest.mark.parametrize("dtype", [0, 1])
+def test_buffers_that_end_too_early(dtype):
+    """Each buffer of a call one byte (a view: one element) short; a call that gets past that has no handle."""
+    r = subprocess.run([NODE, "-e", BUFFERS % {"js": JS, "dtype": dtype}], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stderr
+    out = json.loads(r.stdout.strip().splitlines()[-1])
+    handle = "TypeError: not a PagedKV handle"
+    reach = {"null": (), "rows": (0, 1, 2), "q": (0, 2), "values": (0,), "out": (2,), "rowStart": (0, 1, 2), "lens": (0, 1, 2), "pages": (0, 1, 2)}
+    for name, calls in reach.items():
+        for i in range(3):
+            want = "RangeError: %s of " % name if i in calls else handle
+            assert out[name][i].startswith(want), (name, i, out[name][i])
