@@ -325,3 +325,60 @@ def test_a_far_longer_context_among_many_rows(seqs, heads):
     mine[c.start[b]:c.start[b + 1]] = True
     assert np.isnan(bad[mine]).all()
     check(bad, {t: w for t, w in c.expected(rows=some(c, 20)).items() if not mine[t]})
+
+
+# append with four passes a wave (csrc/kv.hip: n_rows (HQ + 2 HK) HD / 512 of 32768 and more), in a grid and in a list
+@pytest.mark.parametrize("seqs", [[(0, 1100), (33, 1003), (250, 1100)], [(7, 3000), (0, 0)] + [(30, 1)] * 60 + [(5, 90)]])
+@pytest.mark.parametrize("heads,f32", [((16, 16, 128, 128), False), ((16, 16, 128, 8), True), ((16, 4, 256, 64), True), ((8, 8, 256, 0), False)])
+def test_append_with_four_passes(seqs, heads, f32):
+    c = Call(seqs, heads, 32, not f32, f32, seed=20, extra=1)
+    assert c.n_rows * (c.HQ + 2 * c.HK) * c.HD // 512 >= 32768
+    check_append(c, *c.append())
+
+
+# contexts whose pieces are cut and longer than 1024 keys, so that a wave loads page ids and starts its fetches anew within a piece
+# that does not begin at key 0; the last two by a plan
+@pytest.mark.parametrize("n,len,heads", [
+    (16, 5120, (8, 8, 256, 64)), (16, 5120, (8, 8, 128, 8)), (7, 20480, (4, 4, 256, 64)), (131, 5120, (4, 1, 256, 64)), (131, 5120, (3, 1, 128, 8))])
+def test_cut_pieces_of_more_than_1024_keys(n, len, heads):
+    c = shared_pages([(len - 1, 1)] * n, heads, 8, seed=21)
+    keys = -(-n * heads[1] * len // (512 * 128)) * 128  # of a piece, as the device shares the work out
+    assert 1024 < keys < len - 128
+    check(c.attention(), c.expected(rows={0, n // 2, n - 1}))
+
+
+# equal numbers of rows, laid out in a grid of (sequence, KV head) pairs (contexts of at most twice the rows)
+@pytest.mark.parametrize("seqs,heads", [([(300, 800)] * 4, (16, 2, 128, 128)), ([(100, 1400)] * 4, MODEL), ([(0, 1000)] * 3, (32, 4, 128, 64))])
+def test_equal_numbers_of_rows(seqs, heads):
+    c = Call(seqs, heads, 32, seed=22)
+    assert c.n_rows == len(seqs) * c.max_rows and c.max_len <= 2 * c.max_rows
+    full = c.attention()
+    check(full, c.expected(rows=some(c, 20)))
+    # the same bounds with fewer rows, shorter contexts and a sequence that does not fit
+    n = [c.max_rows, c.max_rows - 77, 5, 130][:len(seqs)]
+    c.start = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+    c.lens = np.array([c.lens[0], c.max_rows, 4, 400][:len(seqs)], np.int32)
+    c.T = int(c.start[-1])
+    c.dev[0].copy_(c.torch.from_numpy(c.start))
+    c.dev[1].copy_(c.torch.from_numpy(c.lens))
+    got = c.attention()
+    bad = set(range(c.start[2], c.start[3]))
+    assert np.isnan(got[sorted(bad)]).all() and (got[c.T:] == 7).all()
+    check(got[:c.T], {t: w for t, w in c.expected(rows=some(c, 20) - bad).items()})
+
+
+@pytest.mark.parametrize("seqs,heads", [([(300, 3), (40, 1)], MODEL), ([(2000, 1)], H8), ([(0, 3000)], H16), ([(0, 800)] * 4, H8)])
+def test_scores_in_the_hundreds(seqs, heads):
+    """Scores of up to 400: one key takes nearly all, and maxima rise by more than P may."""
+    c = Call(seqs, heads, 16, seed=23)
+    c.q[:] = c.q * np.float16(40)
+    c.dq = c.torch.from_numpy(c.q).to("cuda:0")
+    want = c.expected(rows=some(c, 60))
+    got = c.attention()
+    e = np.stack([got[t].astype(np.float64) - want[t] for t in sorted(want)])
+    w = np.stack([want[t] for t in sorted(want)])
+    # q and the codes are exact, so a score's error is that of f32 sums near 1032 times the sum of 32 of q (2^17.8, a rounding 2^-6 at most and
+    # 2^-6.8 in the root mean square), four of them in each of four groups, times a scale of 2^-1.6 (2^-2 for groups of 32 channels) and
+    # 1 / sqrt(HD): 2^-10.4, 2^-10.3 for HD 128. It moves an output between two values, at most once its norm: 2^-9 with P's and the
+    # output's roundings.
+    assert np.isfinite(e).all() and np.linalg.norm(e) <= 2 ** -9 * np.linalg.norm(w)

@@ -222,3 +222,64 @@ def test_captured_calls(seqs, heads, page):
             st.synchronize()
             for x, w in zip((out, q, c.dpool), want[n]):
                 assert t.equal(x, w), "replay %d" % k
+
+
+@pytest.mark.parametrize("new", [[40, 1, 0, 17], [1, 1, 1, 1]])
+def test_projections_around_the_cache(new):
+    """A layer's attention as a host runs it: hidden rows -> qkv projection -> append -> attention -> output projection, eagerly and
+    from a captured graph. Each step is checked against 64 bits on what the one before it left."""
+    import os
+    import sys
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "oracle"))
+    import mnb_oracle as mo
+    s = Server([None] * 4, seed=5)
+    t, K, n = s.t, 512, sum(new)
+    N1, N2 = s.width, s.HQ * s.HD
+    s.stride = N1
+    up = lambda x: t.from_numpy(np.ascontiguousarray(x)).to(DEV)  # noqa: E731
+    weights = []
+    for N, k, size in ((N1, K, 0.01), (K, N2, 0.002)):
+        words = s.rng.integers(0, 2 ** 32, (N, k // 32, 4), dtype=np.uint64).astype(np.uint32)
+        sc = (size * (0.5 + s.rng.random((N, k // 32)))).astype(np.float16)
+        weights.append((ha.MnbWeight(N, k, up(words.view(np.int32)), up(sc)), mo.dequant(words, sc, N, k)))
+    (w1, W1), (w2, W2) = weights
+    start, lens, table = s.batch([30, 200, 5, 0])  # a prompt, so that the cache is not empty
+    rows = s.rows(235)
+    b0 = ha.KVBatch(4, 235, 200, 200, up(start), up(lens), up(table), table.shape[1])
+    s.kv.append(0, b0, up(rows), N1)
+    s.expect(0, start, lens, table, rows)
+    start, lens, table = s.batch(new)
+    x = s.rng.standard_normal((n, K)).astype(np.float16)
+    d, big = up(x), t.empty(n, N1, dtype=t.float16, device=DEV)
+    b = ha.KVBatch(4, n, max(new), int(lens.max()), up(start), up(lens), up(table), table.shape[1])
+    q, mix, y = (t.empty(n, *k, dtype=t.float16, device=DEV) for k in ((s.HQ, s.HD), (s.HQ, s.HD), (K,)))
+    st = t.cuda.Stream()
+    t.cuda.synchronize()
+
+    def layer():
+        w1.forward_noalloc(n, d, big, stream=st.cuda_stream)
+        s.kv.append(0, b, big, N1, q, stream=st.cuda_stream)
+        s.kv.attention(0, b, q, big, N1, mix, stream=st.cuda_stream)
+        w2.forward_noalloc(n, mix, y, stream=st.cuda_stream)
+
+    layer()
+    st.synchronize()
+    big_h, mix_h = big.cpu().numpy(), mix.cpu().numpy()
+    # projections: f16 weights (a code times a scale, rounded) and outputs, f32 sums: 2^-11 each of the largest element at most
+    assert mo.rel_err(big_h.astype(np.float64), mo.matmul(x, W1)) <= 2 ** -10
+    check(mix_h, s.expect(0, start, lens, table, big_h))
+    np.testing.assert_array_equal(s.dpool[0].cpu().numpy().reshape(s.pools[0].data.shape), s.pools[0].data)
+    assert mo.rel_err(y.cpu().numpy().astype(np.float64), mo.matmul(mix_h.reshape(n, N2), W2)) <= 2 ** -10
+    want = y.clone()
+    g = t.cuda.CUDAGraph()
+    with t.cuda.stream(st):
+        with t.cuda.graph(g, stream=st):
+            layer()
+        for k in range(3):
+            if k == 1:
+                layer()
+            for z in (big, q, mix, y):
+                z.fill_(float("nan"))
+            g.replay()
+            st.synchronize()
+            assert t.equal(y, want), "replay %d" % k
