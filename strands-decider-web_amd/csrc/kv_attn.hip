@@ -256,13 +256,16 @@ __global__ __launch_bounds__(1024) void kv_plan_kernel(KvArgs a, Kind k) {
     return w;
   };
   float w = 0.0f;
+  Seq first{};  // of the thread's sequences (there is one where n_seqs <= 1024)
   for (int s = s0; s < s1; s++) {
     top = max(top, a.row_start[s]);
     sums[3 * kPlanMost + s] = top;
-    w += wide_keys(a, seq_of(a, s, top));
+    const Seq sq = seq_of(a, s, top);
+    if (s == s0) first = sq;
+    w += wide_keys(a, sq);
   }
-  const int limit = limit_of(a, block_sum(w));
-  auto lane = [&](int s) { return lane_of<kCols>(a, k, seq_of(a, s, sums[3 * kPlanMost + s]), limit); };
+  const int limit = k.split ? limit_of(a, block_sum(w)) : 0;
+  auto lane = [&](int s) { return lane_of<kCols>(a, k, s == s0 ? first : seq_of(a, s, sums[3 * kPlanMost + s]), limit); };
   w = 0.0f;
   for (int s = s0; s < s1; s++) {
     const Lane l = lane(s);
