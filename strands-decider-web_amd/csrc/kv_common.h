@@ -20,8 +20,7 @@ struct Seq {
   int r0, n, len;
   bool ok;
 };
-__device__ __forceinline__ Seq seq_of(const KvArgs& a, int b, int top) {
-  const int r0 = a.row_start[b], r1 = a.row_start[b + 1], len = a.len[b];
+__device__ __forceinline__ Seq seq_of(const KvArgs& a, int r0, int r1, int len, int top) {
   Seq s;
   s.ok = r0 >= top && r1 >= r0 && r1 <= a.n_rows && r1 - r0 <= a.max_rows && len >= r1 - r0 && len <= a.max_len;
   s.r0 = min(top, a.n_rows);
@@ -29,6 +28,7 @@ __device__ __forceinline__ Seq seq_of(const KvArgs& a, int b, int top) {
   s.len = s.ok ? len : 0;
   return s;
 }
+__device__ __forceinline__ Seq seq_of(const KvArgs& a, int b, int top) { return seq_of(a, a.row_start[b], a.row_start[b + 1], a.len[b], top); }
 
 // ---- over a wave, with a sequence a lane ----
 
@@ -70,9 +70,12 @@ __device__ __forceinline__ Seq seq_alone(const KvArgs& a, int b) { return seq_of
 // A lane's sequence s = s0 + lane, s0 = 0, 64, ... in this order: `top` is 0 at first, and handed on.
 __device__ __forceinline__ Seq seq_in_order(const KvArgs& a, int s, int& top) {
   const bool in = s < a.n_seqs;
-  const int mine = max(top, max64(in ? max(a.row_start[s], 0) : 0));
+  const int at = min(s, a.n_seqs - 1), r0 = a.row_start[at], r1 = a.row_start[at + 1], len = a.len[at];  // (all loads at once)
+  const int mine = max(top, max64(max(r0, 0)));
   top = lane_value(mine, 63);
-  return in ? seq_of(a, s, mine) : Seq{};
+  Seq q = seq_of(a, r0, r1, len, mine);
+  if (!in) q = Seq{};
+  return q;
 }
 
 // f16 index of (token slot, group, 0: scale, 1: zero) among a block's parameters
