@@ -319,8 +319,10 @@ int ha_kv_append(ha_kv* k, int layer, const ha_kv_batch* batch, const void* rows
 /* out[n_rows][HQ][HD] (f16) = causal attention of the queries q (as append gives them) over their sequences' contexts, times
    sigmoid(gate) with the gates of the fused rows where the cache is gated (rows may be NULL otherwise). A row that sees a token
    whose table entry is no page of the pool is NaN, and so are the (first max_rows) rows of a sequence that does not fit the
-   batch; rows of no sequence are left as they were. q and out must not overlap. Uses a workspace of the handle: calls on one handle must be ordered. Neither call
-   allocates or synchronises, and both can be captured into a HIP graph. */
+   batch; rows of no sequence are left as they were. q and out must not overlap. Uses a workspace of the handle: calls on one
+   handle must be ordered. Neither call allocates or synchronises, and both can be captured into a HIP graph. Probabilities and
+   their products with scales keep 22 bits, with more than 256 (row, head)s of a sequence on a KV head in large calls 11; sums
+   are f32. */
 int ha_kv_attention(ha_kv* k, int layer, const ha_kv_batch* batch, const void* q, const void* rows, long row_stride, void* out,
                     void* stream);
 int ha_kv_destroy(ha_kv* k);

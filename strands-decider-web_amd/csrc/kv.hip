@@ -28,8 +28,8 @@ __global__ void kv_rope_kernel(float* rope, const double* theta_pow, int n, int 
 // A lane has 8 consecutive channels of a row, HD / 8 lanes a row, a wave 64 / (HD / 8) rows of one head at a time; a group's
 // channels are in HD / 32 neighbouring lanes. All sums and extremes are DPP steps, and a rotated channel's partner is loaded
 // once more instead of exchanged, so that only the norms' factors go through LDS. It is bound by memory where there are many rows
-// (16384 of the model's heads, 211 MB: 53.8 us, 3.9 TB/s, on new buffers, 46.6 on the same ones again, where a copy reaches 4.8) and by a chain of loads where there are few (one
-// row each of 8 sequences: 4.4 us).
+// (16384 of the model's heads, 211 MB: 53.8 us, 3.9 TB/s, on new buffers, 46.6 on the same ones again, where a copy reaches 4.8)
+// and by a chain of loads where there are few (one row each of 8 sequences: 3.3 us, in a graph of such calls).
 
 typedef unsigned u2v __attribute__((ext_vector_type(2)));
 template <int kCtrl>
@@ -232,7 +232,8 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvArgs a, int listed) {
     return;
   }
   const int per = a.gated ? 2 * HD : HD, which = slot >= a.HQ + a.HK, kh = slot - a.HQ - which * a.HK;
-  const T* base = static_cast<const T*>(a.rows) + (slot < a.HQ ? (size_t)slot * per : (size_t)a.HQ * per + (size_t)(slot - a.HQ) * HD) + (size_t)sq.r0 * a.stride;
+  const size_t col = slot < a.HQ ? (size_t)slot * per : (size_t)a.HQ * per + (size_t)(slot - a.HQ) * HD;
+  const T* base = static_cast<const T*>(a.rows) + col + (size_t)sq.r0 * a.stride;
   const int first_pos = sq.len - sq.n;
   auto row_of = [&](int n) { return min(b0 + lr + n * kRows, sq.n - 1); };
   Eight<T> x[NR];
@@ -353,17 +354,17 @@ hipError_t launch_kv_rope(float* rope, const double* theta_pow, int max_ctx, int
 }
 
 // A workgroup's place is in a grid of (rows, sequences), or, where most of that would be empty, in a list that the wave goes through.
-// Measured, us, grid / list, the model's heads: one new row each of 8 sequences 4.7 / 4.0, 2048 rows each 48.8 / 51.4; 2048 rows and 47
-// single ones 46.4 / 11.1, 400 rows and 200 single ones 58.8 / 7.7; 20 rows and 500 single ones 14.0 / 11.5, 8 rows and 1000 single
-// ones (the list is 16 loads deep, the grid a quarter full) 21.2 / 27.3.
+// Measured, us, grid / list, the model's heads, in a graph of 40 calls: one new row each of 8 sequences 3.3 / 3.6, 2048 rows each
+// 46.5 / 48.0; 2048 rows and 47 single ones 46.2 / 11.4, 400 rows and 200 single ones 58.5 / 7.9; 20 rows and 500 single ones
+// 13.8 / 12.0, 8 rows and 1000 single ones (the list is 16 loads deep, the grid a quarter full) 20.9 / 29.1.
 constexpr int kListFrom = 2;
 template <int HD, typename T, int NR>
 hipError_t append_rows(const KvArgs& a, hipStream_t s) {
   constexpr int kBlock = NR * 64 / (HD / 8);
   const long grid = (long)a.n_seqs * ((a.max_rows + kBlock - 1) / kBlock), list = a.n_rows / kBlock + a.n_seqs;
   const bool listed = grid > kListFrom * list;
-  hipLaunchKernelGGL((kv_append_kernel<HD, T, NR>), dim3((unsigned)(listed ? list : (a.max_rows + kBlock - 1) / kBlock), (a.HQ + 2 * a.HK + 3) / 4, listed ? 1 : a.n_seqs),
-                     dim3(256), 0, s, a, (int)listed);
+  const dim3 blocks((unsigned)(listed ? list : (a.max_rows + kBlock - 1) / kBlock), (a.HQ + 2 * a.HK + 3) / 4, listed ? 1 : a.n_seqs);
+  hipLaunchKernelGGL((kv_append_kernel<HD, T, NR>), blocks, dim3(256), 0, s, a, (int)listed);
   return hipGetLastError();
 }
 // More rows a wave where there are enough waves. Measured, us, 1 / 2 / 4 times 64 / (HD / 8) rows a wave, the model's heads: 256 rows

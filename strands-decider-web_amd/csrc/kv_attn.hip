@@ -7,23 +7,24 @@
 //
 // kv_few_kernel: a workgroup has 16 columns and a piece of the keys, its four waves 32 keys each in turn, with nothing shared
 // until the end. It computes S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16, straight from the codes:
-//   - a code c in the low bits of an f16 whose exponent is 2^10 (2^6, 2^4) is the number 1024 + c (64 + c, 16 + c): with a v_perm
-//     and an and-or for two codes, the operands need no arithmetic. K's products start at -1032 sum(q) (-72 sum(q) for the
-//     others), as the C operand, which leaves sum(q (c - 8)) with f32 roundings only; the scale and zero of a group come in
-//     afterwards, on its 16 x 16 sums: S = sum_g s_g (q . (c - 8))_g + z_g sum(q_g).
+//   - a code c in the low bits of an f16 whose exponent is 2^10 (2^6, 2^4) is the number 1024 + c (64 + c, 16 + c), as published for
+//     4-bit weights (Kim et al. 2022, arXiv 2211.10017): with a v_perm and an and-or for two codes, the operands need no
+//     arithmetic. K's products start at -1032 sum(q) (-72 sum(q) for the others), as the C operand, which leaves
+//     sum(q (c - 8)) with f32 roundings only; the scale and zero of a group come in afterwards, on its 16 x 16 sums:
+//     S = sum_g s_g (q . (c - 8))_g + z_g sum(q_g).
 //   - K's operand is 16 bytes of a token's row a lane, V's 8 bytes of 8 tokens' rows, two tokens' half-words joined by
 //     v_perm; S^T's layout (a column a lane) is that of P^T as an operand, so P goes from registers to registers.
 //   - V's scales go onto P (P s_g), and its zeros into one more sum for each group, sum P z_g; that product's other rows give
 //     sum P s_g, of which the codes' offset, -24 times it, is added after every segment of 1024 keys.
 //   - a column's maximum is the wave's own; it is raised only when a score exceeds what P may be (Range).
 // P and P s_g are sums of two f16 each (22 bits), whose products take two matrix instructions: the output's error is its own
-// rounding, 2.07e-4 of its norm, where one f16 each gave 2.5 to 3.1e-4, the more the longer the context, and took up to 4 % less
-// time (us: 61 rows after 1531 16.5 / 16.6, 2 x 1000 rows after 1000 99.5 / 101, 64 sequences of 8192 59.9 / 62.5). Sums are f32.
+// rounding, 2.07e-4 of its norm, where one f16 each gave 2.5 to 3.1e-4, the more the longer the context, and took 1 to 5 % less
+// time (us: 61 rows after 1531 16.4 / 16.7, 2 x 1000 rows after 1000 97 / 101, 64 sequences of 8192 59.4 / 62.2). Sums are f32.
 // Pieces leave their O, maximum and sum in the workspace; the last of a unit's pieces joins them, or kv_merge_kernel where
-// they are many. Two workgroups a CU (233 registers for HD 256) and codes fetched a step ahead keep memory busy where there are
-// few columns: 8 sequences of 32768 tokens, 2 x 4 heads of 256, 151 MB: 34.8 us, 4.3 TB/s (a copy 4.8). With 16 columns
-// and more it is bound by the vector instructions that unpack codes (2048 rows of 8 sequences: 430 us), which kv_many_kernel shares
-// among 128 columns (282 us, 485 TFLOP/s).
+// they are many. Two workgroups a CU (242 registers for HD 256) and codes fetched a step ahead keep memory busy where there are
+// few columns: 8 sequences of 32768 tokens, 2 x 4 heads of 256, 151 MB: 34.7 us, 4.4 TB/s (a copy 4.8). With 16 columns
+// and more it is bound by the vector instructions that unpack codes (2048 rows of 8 sequences: 455 us), which kv_many_kernel shares
+// among 128 columns (284 us, 485 TFLOP/s).
 #include <algorithm>
 #include <cmath>
 
@@ -160,7 +161,7 @@ struct Lane {
 // A unit of many columns is not cut: one that walks many more keys than the others would end long after them. So a sequence of more
 // than kFewCols columns is only one of many where its context is at most `limit`: the keys of all such sequences' units over
 // kManyUnits, w / kManyUnits: its units then end within 256 / kManyUnits of the time in which those of all would, spread evenly.
-// (6 prompts of 1000 rows and 100 rows after 6000, 20000 and 131000 tokens, us: 126, 166 and 383; 320, 993 and 6320 without a limit.)
+// (6 prompts of 1000 rows and 100 rows after 6000, 20000 and 131000 tokens, us: 124, 167 and 384; 326, 1010 and 6470 without a limit.)
 // (No contraction: the kernels of a call have to agree on it.)
 __device__ __forceinline__ float wide_keys(const KvArgs& a, const Seq& sq) {
 #pragma clang fp contract(off)
@@ -213,9 +214,10 @@ __device__ __forceinline__ int chunk_of(const KvArgs& a, const Kind& k, const La
 }
 // A unit's ns pieces are joined by the last of them, or by the last of each group of neighbours and then the last of the groups, or
 // by kv_merge_kernel. The pieces of a group (ns: one group), or 0 for the merge: joining costs what a thread loads one after the other.
-// Measured, us, joined / merged: 61 rows after 500 (5 pieces of 16 columns) 14.5 / 19.2, after 1531 (13) 23.0 / 16.7; 2 after 8000
-// (63 of 8 columns, groups of 16) 16.0 / 12.9; one row (4 columns) after 8000 (63) 10.7 / 12.9, after 20000 (157) 15.3 / 16.5, after
-// 131071 (512) 24.8 / 26.8; 4 sequences of 8000 (63) 13.7 / 15.5; after 4000 (32) 10.3 in groups, 11.6 at once.
+// Measured, us, joined / merged: one row (4 columns) after 8000 (63 pieces) 11.1 / 12.9, after 20000 (157) 15.9 / 16.7, after 131071
+// (512) 25.1 / 27.2; 4 sequences of 8000 (63) 14.4 / 15.7; after 4000 (32) 11.0 in groups, 12.0 at once; 2 rows (8 columns) after
+// 1000 (8) 10.6 / 11.6, after 8000 (63) 23.6 / 13.3; 61 rows (16 columns) after 1531 (13) 24.4 / 17.3, of heads of 128 after 1000 (9)
+// 14.7 / 16.6. (61 rows after 500 (5), 14.9 / 13.6, are on the wrong side of this rule by 1.3 us: it does not tell heads of 256 apart.)
 constexpr int kJoinMost = 32;
 __host__ __device__ inline int group_of(const KvArgs& a, const Kind& k, int ns) {
   const int per = (k.cols * (a.HD / 4) + 64 * kWaves - 1) / (64 * kWaves);  // columns' channels a thread
@@ -369,7 +371,7 @@ __device__ __forceinline__ bool find_piece(const KvArgs& a, const Kind& k, int x
   return true;
 }
 // Column block x of many columns, or false where there is none: those with the most keys first (each of 64 sequences, in
-// kOrder steps of the longest; 3000, 1777, 2000 and 1000 rows of 4 sequences, us: 172 so, 246 by the blocks' numbers).
+// kOrder steps of the longest; 3000, 1777, 2000 and 1000 rows of 4 sequences, us: 171 so, 246 by the blocks' numbers).
 constexpr int kOrder = 16;
 __device__ __forceinline__ bool find_block(const KvArgs& a, const Kind& k, int x, Item& it) {
   const int lane = threadIdx.x & 63;
@@ -724,12 +726,15 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv_few_kernel(KvArgs a, Kind k
         x[k] = halves(vc[k >> 1][2 * (k & 1)][g >> 1], vc[k >> 1][2 * (k & 1) + 1][g >> 1], g & 1);
         if constexpr (HD == 128) x[k] >>= 8 * (j >> 3);
       }
+      h8 op[kE];
 #pragma unroll
-      for (int e = 0; e < kE; e++) {
-        const u4 op = {code_v(mg, x[0], e), code_v(mg, x[1], e), code_v(mg, x[2], e), code_v(mg, x[3], e)};
-        o[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, op), wh, o[g][e], 0, 0, 0);
-        o[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, op), wh2, o[g][e], 0, 0, 0);
-      }
+      for (int e = 0; e < kE; e++)
+        op[e] = __builtin_bit_cast(h8, u4{code_v(mg, x[0], e), code_v(mg, x[1], e), code_v(mg, x[2], e), code_v(mg, x[3], e)});
+      // (not one sum's two products in succession: the second waits for the first)
+#pragma unroll
+      for (int e = 0; e < kE; e++) o[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op[e], wh, o[g][e], 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < kE; e++) o[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(op[e], wh2, o[g][e], 0, 0, 0);
     }
     if constexpr (more) fetch_v();
     wave_sync();  // (the parameters' place is used again)
@@ -922,7 +927,7 @@ struct ManyLds {
 // as one more product (with sum(q_g) / G as two f16), and O takes P s_g and sum P z_g. P goes through LDS as two f16 each; P s_g is
 // rounded to f16 once here (2.75e-4 of the output's norm, 2.07e-4 of it the output's own rounding; the framework's attention on f16
 // rows rounds its P as well): two f16 each, as above, would be 16 more matrix instructions and as many vector ones a tile in the
-// waves that bound it, 346 us instead of 282.
+// waves that bound it, 346 us instead of 284.
 template <int HD>
 __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
   constexpr int G = HD / 4, U = HD / 16, kRow = HD / 2, kKs = G / 16, kDt = HD / 64;  // kKs: k-steps of a group; kDt: 32-row blocks of V^T a wave
@@ -1212,7 +1217,8 @@ __global__ __launch_bounds__(512, 2) void kv_many_kernel(KvArgs a, Kind kind) {
             u4 w;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-              const h2 hi = as_h2(p[n][2 * kb + (k >> 1)][k & 1]), lo = as_h2(p[n][2 * kb + (k >> 1)][2 + (k & 1)]), z = as_h2(pz[kb][gg][k]), s = as_h2(ps[kb][gg][k]);
+              const u4& pk = p[n][2 * kb + (k >> 1)];
+              const h2 hi = as_h2(pk[k & 1]), lo = as_h2(pk[2 + (k & 1)]), z = as_h2(pz[kb][gg][k]), s = as_h2(ps[kb][gg][k]);
               zs[n][gg] = __builtin_amdgcn_fdot2(lo, z, __builtin_amdgcn_fdot2(hi, z, zs[n][gg], false), false);
               w[k] = as_u(__builtin_elementwise_fma(hi, s, lo * s));
             }
@@ -1344,16 +1350,16 @@ __global__ __launch_bounds__(1024) void kv_merge_kernel(KvArgs a, Kind kind) {
 // enough units for the longest of them, about 1.5 us for 32 keys, to end with the others: units x (mean keys / most keys) is at
 // least kManyUnits, with the mean as in a batch of equal sequences, or half of the most where they are not. Measured, us, few
 // columns' kernel / many columns', with that product: the model's heads, rows of n sequences without a prefix, 4096 of 1 (128)
-// 197 / 219, 2048 of 2 (128) 126 / 121, of 3 (192) 175 / 120, of 8 (512) 430 / 281; 300, 500 rows after 1000 of 8 (133, 208)
-// 81 / 83, 132 / 94; 3000, 1777, 2000, 1000 rows (243) 218 / 172; 2 or 4 of 1500 rows after 500, 2 of 600, 30 single ones (132,
-// 226) 120 / 133, 205 / 163; 32 heads of 128 on 8: 1000, 1200, 1500 rows of one (125, 150, 187) 50 / 55, 69 / 64, 95 / 78; 777
-// rows, 130 after 2000, 300 after 64, 8 single ones (152) 71 / 118; 100 rows after 500 of 16 (366) 86 / 76. Up to kFewCols columns
+// 215 / 218, 2048 of 2 (128) 132 / 117, of 3 (192) 184 / 120, of 8 (512) 455 / 277; 300, 500 rows after 1000 of 8 (133, 208)
+// 89 / 91, 141 / 105; 3000, 1777, 2000, 1000 rows (243) 232 / 171; 2 or 4 of 1500 rows after 500, 2 of 600, 30 single ones (132,
+// 226) 124 / 130, 213 / 162; 32 heads of 128 on 8: 1000, 1200, 1500 rows of one (125, 150, 187) 55 / 55, 74 / 65, 102 / 79; 777
+// rows, 130 after 2000, 300 after 64, 8 single ones (152) 81 / 123; 100 rows after 500 of 16 (366) 90 / 86. Up to kFewCols columns
 // a sequence stays with the first also beside others that do not, and so does one whose context is over limit_of(). Only equal
 // numbers of rows on contexts of at most twice as many are laid out in a grid, as other contexts may be of any lengths (8 sequences of
-// 500 rows after 1000, us: 101 in a grid, 105 so; 7 prompts of 800 rows and 800 rows after 60000: 5990 in a grid, 1280 so).
+// 500 rows after 1000, us: 100 in a grid, 106 so; 7 prompts of 800 rows and 800 rows after 60000: 5970 in a grid, 1280 so).
 // Contexts up to which more than kScanMost sequences are neither cut nor planned. Measured, us, in a grid / planned: single rows of
-// 140 sequences of 100, 1000, 3000 tokens 8.2 / 12.2, 25.6 / 31.6, 64.6 / 62.8, of 1000 sequences of 10 tokens 22 / 30, of 200 of
-// 300 and one of 20000 250 / 26.
+// 140 sequences of 100, 1000, 3000 tokens 9.1 / 13.9, 27.4 / 34.0, 71.3 / 68.7, of 1000 sequences of 10 tokens 24 / 34, of 200 of
+// 300 and one of 20000 269 / 23.
 constexpr int kDirectKeys = 1024;
 template <int HD>
 hipError_t attend(const KvArgs& a, float* ws, hipStream_t s) {
