@@ -382,3 +382,35 @@ def test_scores_in_the_hundreds(seqs, heads):
     # 1 / sqrt(HD): 2^-10.4, 2^-10.3 for HD 128. It moves an output between two values, at most once its norm: 2^-9 with P's and the
     # output's roundings.
     assert np.isfinite(e).all() and np.linalg.norm(e) <= 2 ** -9 * np.linalg.norm(w)
+
+
+@pytest.mark.parametrize("seqs,heads,f32", [([(700, 1), (40, 6), (0, 30)], MODEL, False), ([(0, 700), (9, 1)], H16, False), ([(20, 7), (300, 5)], H8, True)])
+def test_offsets_beyond_32_bits(seqs, heads, f32):
+    """Pages behind the first 4 GiB of a pool, and fused rows 512 MiB apart: the bits of the same calls nearby."""
+    c = Call(seqs, heads, 64, True, f32, seed=24)
+    t = c.torch
+    q, v, pool = c.append()
+    want = c.attention(q=t.from_numpy(q).to("cuda:0"))
+    far = (1 << 32) // c.dpool[0].numel() + 5
+    big = t.empty((far + c.n_pages,) + tuple(c.dpool.shape[1:]), dtype=t.uint8, device="cuda:0")
+    big[far:].copy_(t.from_numpy(c.pool.data))
+    kv = ha.PagedKV(big, far + c.n_pages, page_size=64, max_ctx=c.max_len, HQ=c.HQ, HK=c.HK, HD=c.HD, rot_dim=c.rot, dtype=ha.F32 if f32 else ha.F16)
+    kv.set_param(0, "q_norm", c.qw)
+    kv.set_param(0, "k_norm", c.kw)
+    table = t.where(c.dev[2] >= 0, c.dev[2] + far, c.dev[2])
+    b = c.make_batch(pages=table)
+    n = min(c.n_rows, 12)
+    rows, stride = c.drows, c.stride
+    if n == c.n_rows:  # (few rows: far apart as well)
+        stride = (1 << 29) // c.drows.element_size()
+        rows = t.empty(n * stride, dtype=c.drows.dtype, device="cuda:0").view(n, stride)
+        rows[:, :c.stride].copy_(c.drows)
+    dq, dv = t.full_like(c.dq, 7.0), t.full((c.n_rows, 2, c.HK, c.HD), 7.0, dtype=t.float16, device="cuda:0")
+    out = t.full_like(c.dq, 7.0)
+    kv.append(0, b, rows, stride, dq, dv)
+    kv.attention(0, b, dq, rows, stride, out)
+    t.cuda.synchronize()
+    for got, x in ((dq, q), (dv, v), (out, want)):
+        np.testing.assert_array_equal(got.cpu().numpy().view(np.uint16), x.view(np.uint16))
+    np.testing.assert_array_equal(big[far:].cpu().numpy(), pool)
+    kv.close()
