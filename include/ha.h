@@ -234,6 +234,48 @@ int ha_mnb_forward(ha_mnb* w, int M, const void* a, void* y, void* stream);
 #define HA_MNB_SCRATCH_BYTES (40u << 20)
 int ha_mnb_forward_noalloc(ha_mnb* w, int M, const void* a, void* y, void* stream);
 int ha_mnb_destroy(ha_mnb* w);
+/* ---- Products whose results go straight into what follows. No counterpart in the reference, which stores the product in f16
+   and runs SILU_MUL, ADD_BIAS and ADD_NORM on it (wgsl.js:55-121).
+   Both take any weight of ha_mnb_create, with any N (gated: an even one), its codes 4-byte aligned. a is [M][K] f16, 16-byte
+   aligned, M up to 2^20. Weights are what the format says, without a rounding of their own (ha_mnb_forward rounds each to f16);
+   sums are f32. Operands that ha_mnb_forward's fast kernels take (K a multiple of 64, with groups of 64 of 128; codes 16-byte
+   aligned with 4 bits, scales and biases 4-byte aligned) are served by fast kernels here too. Neither call allocates, synchronises or keeps anything in the handle: calls on
+   one handle may overlap, and both can be captured into a HIP graph. */
+typedef enum ha_act { HA_ACT_NONE = 0, HA_ACT_SILU = 1, HA_ACT_GELU = 2 /* the tanh form */ } ha_act;
+typedef struct ha_epilogue {
+  int act;               /* ha_act */
+  int gated;             /* 1: the weight's first N / 2 rows are the gate's, the others the up projection's */
+  const float* bias;     /* device [N] or NULL, added before the activation */
+  const void* residual;  /* device [M][residual_stride] or NULL, added last */
+  int residual_dtype;    /* ha_dtype */
+  int out_dtype;         /* ha_dtype */
+  long residual_stride;  /* elements between rows; 0: as many as there are columns */
+  long out_stride;
+} ha_epilogue;
+/* With z = a W^T + bias: out[m][j] = residual[m][j] + act(z[m][j]), j < N, or gated out[m][j] = residual[m][j] + act(z[m][j])
+   z[m][N / 2 + j], j < N / 2, in f32 and rounded once. Values between the rows of out stay as they are. out may be the residual
+   itself (same address, type and stride: x += ...) and else overlaps neither it nor a nor bias. */
+int ha_mnb_fused(ha_mnb* w, int M, const void* a, const ha_epilogue* e, void* out, void* stream);
+
+/* Log probabilities over a vocabulary, from the final norm's rows and the table (an embedding table, where model and vocabulary
+   share one): z[m][n] = scale a[m] . W[n] for n < n_vocab, p[m] = softmax(z[m]). The logits are not stored. */
+typedef struct ha_logprobs {
+  int n_vocab;         /* the table's first n_vocab rows are tokens, up to 2^20 (0: all N; rows behind them are padding) */
+  float scale;         /* of the logits, one over the temperature (0: 1) */
+  int n_targets;       /* tokens asked for in each row, up to 1024 */
+  const int* targets;  /* device [M][n_targets]; a number outside [0, n_vocab) gives NaN */
+  int top_k;           /* largest tokens of each row, up to 64 and n_vocab */
+  float* logp;         /* device [M][n_targets]: log p of the targets */
+  float* entropy;      /* device [M] or NULL: -sum p log p, in nats */
+  float* lse;          /* device [M] or NULL: log sum e^z */
+  int* top_ids;        /* device [M][top_k]: the largest first, equal ones by their number. In the order of the logits in 64 bits */
+  float* top_logp;     /* device [M][top_k]: log p of those */
+} ha_logprobs;
+/* A row with a logit that is not finite gives NaN and top_ids of -1. The workspace (16-byte aligned device memory, as many bytes
+   as ha_mnb_logprobs_bytes says) is the caller's: calls that may overlap need one each. */
+int ha_mnb_logprobs_bytes(const ha_mnb* w, int M, const ha_logprobs* p, size_t* bytes);
+int ha_mnb_logprobs(ha_mnb* w, int M, const void* a, const ha_logprobs* p, void* workspace, size_t bytes, void* stream);
+
 /* In-place orthonormal Walsh-Hadamard transform of every contiguous n-block of the f16 array x (elems values, a
    multiple of n; n a power of two up to 8192): the online input rotation of a tensor exported with `had: n`
    (FWHT, web/public/engine/wgsl.js:94-110; applied before the matmul at engine.js:240). */

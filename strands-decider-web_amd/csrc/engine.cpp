@@ -367,6 +367,15 @@ bool mnb_ok(const ha_mnb* w) {
 }
 }  // namespace
 
+namespace ha {
+bool mnb_weight(const ha_mnb* w, MnbArgs* args, int* device) {
+  if (!mnb_ok(w)) return false;
+  *args = w->args;
+  *device = w->device;
+  return true;
+}
+}  // namespace ha
+
 extern "C" {
 
 const char* ha_last_error(void) { return g_err.c_str(); }

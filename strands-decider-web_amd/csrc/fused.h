@@ -1,0 +1,63 @@
+// Products with quantised weights whose results go straight into what follows (fused_*.h, fused.hip, logprobs.hip): argument
+// blocks shared with their host side (fused_host.cpp).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <string>
+
+#include "ha_kernels.h"
+
+namespace ha {
+
+constexpr int kLpBlock = 64;     // columns of a block of logits (a record of its own)
+constexpr int kLpMargin = 8;     // blocks looked at beyond the top_k largest
+constexpr int kLpMaxTop = 64;    // top_k, at most
+constexpr int kLpMaxVocab = 1 << 20;
+
+// What a 64-column block of a row's scaled logits comes to: its largest value, over the other columns the sums of e^(z - max)
+// and e^(z - max) (z - max), and a word whose upper 26 bits are a bound from above of the second largest value (as an unsigned
+// number in the same order) and whose lower 6 say which column is the largest (the first of equals).
+struct LpRecord {
+  float max, rest, rest_z;
+  unsigned second;
+};
+
+struct FusedArgs {
+  int M, N, K, group;  // N: rows of the weight that count
+  const void* a;       // [M][K] f16, 16-byte aligned
+  const void* q;       // [N][K/32][bits] u32
+  const void* s;       // [N][K/group] f16
+  const void* b;       // the same, asymmetric only
+  int bits, asym;
+  // products
+  int half;            // gated: N / 2, the columns of the result; 0: not gated
+  int act, out_f32, res_f32;
+  const float* bias;   // [N] or nullptr
+  const void* res;     // or nullptr
+  long res_stride;
+  void* out;
+  long out_stride;
+  // logits
+  float scale;
+  LpRecord* rec;       // [M][ceil(N / 64)]
+};
+
+struct LpArgs {
+  FusedArgs p;         // the product that the records are of
+  int n_targets, top_k;
+  const int* targets;  // [M][n_targets]
+  float* logp;         // [M][n_targets]
+  float* entropy;      // [M] or nullptr
+  float* lse;          // [M] or nullptr
+  int* top_ids;        // [M][top_k]
+  float* top_logp;     // [M][top_k]
+};
+
+hipError_t launch_fused(const FusedArgs& a, hipStream_t s);         // product with its activation, bias and residual
+hipError_t launch_logit_records(const FusedArgs& a, hipStream_t s);  // records of the scaled logits
+hipError_t launch_logprobs(const LpArgs& a, hipStream_t s);          // what the records come to
+
+int set_error(int code, const std::string& msg);  // the calling thread's ha_last_error(); returns the code
+
+}  // namespace ha

@@ -1,0 +1,139 @@
+// Shared by the kernels of fused.hip: decoding without rounding, and what is done with a finished tile.
+//
+// Weights stay exact. A code less 2^(bits-1) is a small integer, which f16 holds; the matrix unit sums its products with the 32
+// f16 values of a in f32, and the group's f16 scale multiplies that sum in f32 (one fma a sum). Against weights rounded to f16
+// before the product (mnb_common.h: 2^-12 of each weight) the sums are some 500 times nearer to 64 bits (3e-7 against 1.4e-4 of
+// their size at K = 2048), which results in f32 show, and the decoding has no multiplications. Asymmetric weights s c + b are
+// s (c - 2^(bits-1)) + b', b' = b + 2^(bits-1) s: b' times the group's sum of a, which a product with ones gives.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include "fused.h"
+#include "mnb_common.h"
+
+namespace ha {
+namespace {
+
+template <typename T>
+using gptr = const __attribute__((address_space(1))) T*;
+template <typename T>
+__device__ __forceinline__ gptr<T> gp(const void* p) { return (gptr<T>)(p); }
+
+constexpr int kEpiAct = 0, kEpiLogits = 1;
+
+// Eight consecutive codes less 2^(BITS-1), in element order. 4 bits: lo is their word; else lo holds their low two bits
+// (element e at bits 2 e) and, for 3, hi their third (element e at bit e).
+template <int BITS>
+__device__ __forceinline__ h8 codes8(unsigned lo, unsigned hi) {
+  h8 r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    h2 q;
+    if constexpr (BITS == 4) {
+      // a byte (two codes) in both halves; bit 0 of 1024.0's mantissa is worth 1, bit 4 of 64.0's likewise
+      const unsigned p = __builtin_amdgcn_perm(lo, lo, 0x01010101u * i);
+      q = __builtin_bit_cast(h2, (p & 0x00F0000Fu) | 0x54006400u) - h2{(_Float16)1032.0f, (_Float16)72.0f};
+    } else {
+      const unsigned x = lo >> (4 * i);
+      unsigned p = (x & 3u) | ((x & 12u) << 14);
+      if constexpr (BITS == 3) {
+        const unsigned t = hi >> (2 * i);
+        p |= ((t & 1u) << 2) | ((t & 2u) << 17);
+      }
+      constexpr float kOff = 1024 + (1 << (BITS - 1));
+      q = __builtin_bit_cast(h2, p | 0x64006400u) - h2{(_Float16)kOff, (_Float16)kOff};
+    }
+    r[2 * i] = q[0];
+    r[2 * i + 1] = q[1];
+  }
+  return r;
+}
+
+__device__ __forceinline__ float f16_bits(unsigned u) { return (float)__builtin_bit_cast(_Float16, (unsigned short)u); }
+// b + 2^(BITS-1) s
+template <int BITS>
+__device__ __forceinline__ float centred(float s, float b) { return fmaf((float)(1 << (BITS - 1)), s, b); }
+
+__device__ __forceinline__ h8 ones8() {
+  const _Float16 o = (_Float16)1.0f;
+  return h8{o, o, o, o, o, o, o, o};
+}
+
+// ---- results ----
+
+// silu(z) = z / (1 + e^-z), gelu(z) = z / (1 + e^(-2 sqrt(2/pi) (z + 0.044715 z^3))) (the tanh form). Where e^.. is infinite
+// the result is -0.
+__device__ __forceinline__ float activate(int act, float z) {
+  if (act == 0) return z;
+  const float t = act == 1 ? z : 1.5957691216057308f * fmaf(0.044715f * z * z, z, z);
+  return z * __builtin_amdgcn_rcpf(1.0f + __expf(-t));
+}
+
+// One value of the result: row m, column j (z with bias and activation done).
+__device__ __forceinline__ void store_result(const FusedArgs& p, int m, int j, float v) {
+  if (p.res) {
+    const size_t i = (size_t)m * p.res_stride + j;
+    v += p.res_f32 ? ((const float*)p.res)[i] : (float)((const _Float16*)p.res)[i];
+  }
+  const size_t o = (size_t)m * p.out_stride + j;
+  if (p.out_f32) ((float*)p.out)[o] = v;
+  else ((_Float16*)p.out)[o] = (_Float16)v;
+}
+__device__ __forceinline__ float with_bias(const FusedArgs& p, int n, float z) { return p.bias ? z + p.bias[n] : z; }
+// A value of the result from its sums: of column j, or gated of columns j and half + j.
+__device__ __forceinline__ float result_of(const FusedArgs& p, int j, float z) { return activate(p.act, with_bias(p, j, z)); }
+__device__ __forceinline__ float result_of(const FusedArgs& p, int j, float z, float up) {
+  return result_of(p, j, z) * with_bias(p, p.half + j, up);
+}
+
+// ---- records of logits ----
+
+__device__ __forceinline__ unsigned ordered(float f) {
+  const unsigned u = __builtin_bit_cast(unsigned, f);
+  return u >> 31 ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(unsigned o) {
+  return __builtin_bit_cast(float, o >> 31 ? o & 0x7FFFFFFFu : ~o);
+}
+__device__ __forceinline__ unsigned pack_second(float second, int arg) {
+  return (min(ordered(second) >> 6, (1u << 26) - 2) + 1) << 6 | (unsigned)arg;
+}
+
+// The largest of a set of columns, which one it is (the first of equals), and the second largest.
+struct Largest {
+  float max, second;
+  int arg;
+  __device__ __forceinline__ void take(float v, int at) {  // columns in ascending order
+    if (v > max) second = max, max = v, arg = at;
+    else second = fmaxf(second, v);
+  }
+  __device__ __forceinline__ void join(float m, float s, int at) {  // another set's
+    const bool theirs = m > max || (m == max && at < arg);
+    second = fmaxf(fmaxf(second, s), theirs ? max : m);
+    if (theirs) max = m, arg = at;
+  }
+};
+constexpr float kNone = -__builtin_huge_valf();
+
+// The record of a row's block where lane c of 16 has columns 16 t + c, t < 4, of it (z: scaled; valid: columns of the block).
+// All 16 lanes get it.
+__device__ __forceinline__ LpRecord record16(const float* z, int c, int valid) {
+  Largest l{kNone, kNone, 0};
+#pragma unroll
+  for (int t = 0; t < 4; t++)
+    if (16 * t + c < valid) l.take(z[t], 16 * t + c);
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) l.join(__shfl_xor(l.max, d), __shfl_xor(l.second, d), __shfl_xor(l.arg, d));
+  float rest = 0.0f, rest_z = 0.0f;
+#pragma unroll
+  for (int t = 0; t < 4; t++) {
+    const float x = z[t] - l.max, e = __expf(x);
+    if (16 * t + c < valid && 16 * t + c != l.arg) rest += e, rest_z = fmaf(e, x, rest_z);
+  }
+#pragma unroll
+  for (int d = 1; d < 16; d *= 2) rest += __shfl_xor(rest, d), rest_z += __shfl_xor(rest_z, d);
+  return LpRecord{l.max, rest, rest_z, pack_second(l.second, l.arg)};
+}
+
+}  // namespace
+}  // namespace ha

@@ -6,6 +6,8 @@
 
 #include "mnb_plan.h"
 
+struct ha_mnb;
+
 namespace ha {
 
 // Cross-workgroup waits of one launch (the paired form's tile-set wait, the split form's packed-state wait, the split
@@ -132,6 +134,7 @@ struct MnbArgs {
   float* ws = nullptr;  // [split][M][N] fp32 partial products when split > 1
 };
 hipError_t mnb_check(const MnbArgs& a);
+bool mnb_weight(const ha_mnb* w, MnbArgs* args, int* device);  // a live handle's weight and device; false where it is none
 bool mnb_strip_takes(const MnbArgs& a);     // whether launch_mnb_strip can run these operands (K, alignment)
 hipError_t launch_mnb_strip(const MnbArgs& a, hipStream_t s);
 bool mnb_tiles_takes(const MnbArgs& a);     // likewise launch_mnb_tiles (4-bit weights)

@@ -10,28 +10,16 @@
 
 #include "ha.h"
 #include "kv.h"
+#include "on_device.h"
 
 namespace {
 
+using ha::OnDevice;
 using ha::set_error;
 
 constexpr uint32_t kKvMagic = 0x48414b56u;
 std::mutex g_kv_mu;
 std::unordered_set<const ha_kv*> g_live_kvs;  // handles that exist: a destroyed or forged one is refused before it is read
-
-// The calling thread's current device is the caller's again after a call.
-struct OnDevice {
-  int before = -1;
-  hipError_t rc;
-  explicit OnDevice(int device) {
-    rc = hipGetDevice(&before);
-    if (rc == hipSuccess && before != device) rc = hipSetDevice(device);
-    else before = -1;
-  }
-  ~OnDevice() {
-    if (before >= 0) (void)hipSetDevice(before);
-  }
-};
 
 int hip_error(const char* what, hipError_t e) { return set_error(HA_ERR_DEVICE, std::string(what) + ": " + hipGetErrorString(e)); }
 

@@ -20,6 +20,7 @@ HA_OK, HA_ERR_ARG, HA_ERR_CONTEXT, HA_ERR_HANDLE, HA_ERR_DEVICE, HA_ERR_NOMEM, H
 LINEAR, FULL, ADAPTER = 0, 1, 2  # ADAPTER: no token mixer (engine.js:256-261); its forward buffers may be None
 F32, F16 = 0, 1
 CHUNKED, SEQUENTIAL, CHUNKED_FUSED, CHUNKED_SPLIT, CHUNKED_PAIRED = 0, 1, 2, 3, 4
+ACTS = {None: 0, "none": 0, "silu": 1, "gelu": 2}
 KIND_NAMES = {"linear_attention": LINEAR, "full_attention": FULL, "adapter": ADAPTER}
 
 
@@ -53,6 +54,18 @@ class HaKvBatch(ctypes.Structure):
     _fields_ = [("n_seqs", ctypes.c_int), ("n_rows", ctypes.c_int), ("max_rows", ctypes.c_int), ("max_len", ctypes.c_int),
                 ("row_start", ctypes.c_void_p), ("len", ctypes.c_void_p), ("pages", ctypes.c_void_p),
                 ("table_stride", ctypes.c_int)]
+
+
+class HaEpilogue(ctypes.Structure):
+    _fields_ = [("act", ctypes.c_int), ("gated", ctypes.c_int), ("bias", ctypes.c_void_p), ("residual", ctypes.c_void_p),
+                ("residual_dtype", ctypes.c_int), ("out_dtype", ctypes.c_int), ("residual_stride", ctypes.c_long),
+                ("out_stride", ctypes.c_long)]
+
+
+class HaLogprobs(ctypes.Structure):
+    _fields_ = [("n_vocab", ctypes.c_int), ("scale", ctypes.c_float), ("n_targets", ctypes.c_int), ("targets", ctypes.c_void_p),
+                ("top_k", ctypes.c_int), ("logp", ctypes.c_void_p), ("entropy", ctypes.c_void_p), ("lse", ctypes.c_void_p),
+                ("top_ids", ctypes.c_void_p), ("top_logp", ctypes.c_void_p)]
 
 
 class HaForwardOpts(ctypes.Structure):
@@ -97,6 +110,9 @@ def load_library(path=LIB_PATH):
         "ha_mnb_forward": ([vp, i, vp, vp, vp], i),
         "ha_mnb_forward_noalloc": ([vp, i, vp, vp, vp], i),
         "ha_mnb_destroy": ([vp], i),
+        "ha_mnb_fused": ([vp, i, vp, ctypes.POINTER(HaEpilogue), vp, vp], i),
+        "ha_mnb_logprobs_bytes": ([vp, i, ctypes.POINTER(HaLogprobs), ctypes.POINTER(sz)], i),
+        "ha_mnb_logprobs": ([vp, i, vp, ctypes.POINTER(HaLogprobs), vp, sz, vp], i),
         "ha_fwht": ([vp, ctypes.c_long, i, i, vp], i),
         "ha_embed": ([vp, i, vp, vp, vp], i),
         "ha_add_norm": ([i, i, i, vp, vp, vp, vp, i, vp, ctypes.c_float, i, vp], i),
@@ -267,6 +283,7 @@ class MnbWeight:
         h = ctypes.c_void_p()
         _check(_lib.ha_mnb_create(N, K, ctypes.byref(fmt), _ptr(q), _ptr(s), _ptr(b), device, ctypes.byref(h)))
         self._h = h
+        self._device = device
         self._borrowed = (q, s, b)
 
     def forward(self, M, a, y, stream=None):
@@ -276,6 +293,37 @@ class MnbWeight:
         """forward() without any device allocation: split-K partials go to the library's fixed per-GPU scratch
         (ha_mnb_forward_noalloc; calls that overlap on one GPU race)."""
         _check(_lib.ha_mnb_forward_noalloc(self._h, M, _ptr(a), _ptr(y), _ptr(stream) if stream is not None else None))
+
+    def fused(self, M, a, out, epilogue, stream=None):
+        """out = residual + act(a x W^T + bias), or gated (ha_mnb_fused), as the :class:`Epilogue` says. Weights are exact here
+        and the result is rounded once, to out's type. Tensors (not plain addresses) of another type or GPU than the call's, or
+        that end too early, raise."""
+        e = epilogue
+        cols = self.N // 2 if e.c.gated else self.N
+        if M > 0:
+            e._check(self, M, cols)
+            a = _kv_ptr(a, "a", _torch_type(F16), M * self.K, self._device)
+            out = _rows_ptr(out, "out", _torch_type(e.c.out_dtype), M, cols, e.c.out_stride or cols, self._device)
+        _check(_lib.ha_mnb_fused(self._h, M, _ptr(a), e._ref, _ptr(out), _st(stream)))
+
+    def logprobs_bytes(self, M, logprobs):
+        """Bytes of the workspace of a call of M rows."""
+        n = ctypes.c_size_t()
+        _check(_lib.ha_mnb_logprobs_bytes(self._h, M, logprobs._ref, ctypes.byref(n)))
+        return n.value
+
+    def logprobs(self, M, a, logprobs, workspace, workspace_bytes=None, stream=None):
+        """Log probabilities over this table of M rows a (ha_mnb_logprobs), into the buffers of the :class:`LogProbs`.
+        workspace: a device tensor, or an address with workspace_bytes; calls that may overlap need one each."""
+        p = logprobs
+        if M > 0:
+            p._check(M, self._device)
+            a = _kv_ptr(a, "a", _torch_type(F16), M * self.K, self._device)
+            if workspace_bytes is None and hasattr(workspace, "is_contiguous"):
+                if not (workspace.is_cuda and workspace.device.index == self._device and workspace.is_contiguous()):
+                    raise TypeError("workspace must be a contiguous tensor on GPU %d" % self._device)
+                workspace_bytes = workspace.numel() * workspace.element_size()
+        _check(_lib.ha_mnb_logprobs(self._h, M, _ptr(a), p._ref, _ptr(workspace), workspace_bytes or 0, _st(stream)))
 
     def close(self):
         if self._h:
@@ -347,6 +395,74 @@ def _kv_ptr(x, what, dtype, n, device, rows=None):
     if not ok:
         raise TypeError("%s must be a contiguous %s tensor of %d elements on GPU %d" % (what, dtype, n, device))
     return x.data_ptr()
+
+
+def _torch_type(dtype):
+    """F32 or F16 as torch names it (as a text where torch is not loaded: no tensor comes from elsewhere)."""
+    torch = sys.modules.get("torch")
+    if dtype == F32:
+        return torch.float32 if torch else "torch.float32"
+    return torch.float16 if torch else "torch.float16"
+
+
+def _rows_ptr(x, what, dtype, M, cols, stride, device):
+    """The address of M rows of cols values, stride apart."""
+    if hasattr(x, "dim") and x.dim() == 2 and M > 1 and x.stride(0) != stride:
+        raise TypeError("%s has rows %d apart, not %d" % (what, x.stride(0), stride))
+    if stride < cols:  # (the library refuses it)
+        return _ptr(x)
+    return _kv_ptr(x, what, dtype, (M - 1) * stride + cols, device, M * cols)
+
+
+class Epilogue:
+    """What becomes of a product's sums (ha_epilogue): ``act`` None, "silu" or "gelu" (the tanh form); ``gated``: act(first half
+    of the columns) times the second half; ``bias`` f32 [N] before it; ``residual`` (f32 or f16 rows) added last; the result's
+    type. Strides are elements between rows, 0: dense. May be kept and used for many calls; it holds references to its tensors."""
+
+    def __init__(self, act=None, gated=False, bias=None, residual=None, residual_dtype=F32, residual_stride=0, out_dtype=F16,
+                 out_stride=0):
+        if act not in ACTS:
+            raise ValueError("act must be None, 'silu' or 'gelu'")
+        self._held, self._checked = (bias, residual), None
+        self.c = HaEpilogue(ACTS[act], int(bool(gated)), _ptr(bias), _ptr(residual), residual_dtype, out_dtype, residual_stride,
+                            out_stride)
+        self._ref = ctypes.byref(self.c)
+
+    def _check(self, w, M, cols):
+        if self._checked == (w.N, M, w._device):
+            return
+        bias, residual = self._held
+        _kv_ptr(bias, "bias", _torch_type(F32), w.N, w._device)
+        if residual is not None:
+            _rows_ptr(residual, "residual", _torch_type(self.c.residual_dtype), M, cols, self.c.residual_stride or cols, w._device)
+        self._checked = (w.N, M, w._device)
+
+
+class LogProbs:
+    """What is asked of the rows' distributions over a vocabulary (ha_logprobs) and the device buffers that take it: ``targets``
+    int32 [M][n_targets] with ``logp`` f32, ``top_k`` with ``top_ids`` int32 and ``top_logp`` f32 [M][top_k], ``entropy`` and
+    ``lse`` f32 [M] (or None). n_vocab: the table's rows that are tokens (0: all); scale: one over the temperature (0: 1). It
+    holds references to its tensors."""
+
+    def __init__(self, n_vocab=0, scale=0.0, targets=None, n_targets=0, top_k=0, logp=None, entropy=None, lse=None, top_ids=None,
+                 top_logp=None):
+        self._held = (targets, logp, entropy, lse, top_ids, top_logp)
+        self._checked = None
+        self.c = HaLogprobs(n_vocab, scale, n_targets, _ptr(targets), top_k, _ptr(logp), _ptr(entropy), _ptr(lse), _ptr(top_ids),
+                            _ptr(top_logp))
+        self._ref = ctypes.byref(self.c)
+
+    def _check(self, M, device):
+        if self._checked == (M, device):
+            return
+        torch = sys.modules.get("torch")
+        i32, f32 = (torch.int32, torch.float32) if torch else ("torch.int32", "torch.float32")
+        T, k = self.c.n_targets, self.c.top_k
+        for x, what, dtype, n in zip(self._held, ("targets", "logp", "entropy", "lse", "top_ids", "top_logp"),
+                                     (i32, f32, f32, f32, i32, f32), (M * T, M * T, M, M, M * k, M * k)):
+            if n:
+                _kv_ptr(x, what, dtype, n, device)
+        self._checked = (M, device)
 
 
 class KVBatch:
