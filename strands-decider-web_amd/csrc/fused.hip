@@ -7,6 +7,7 @@
 
 #include "fused.h"
 #include "fused_common.h"
+#include "fused_tiles.h"
 
 namespace ha {
 namespace {
@@ -88,9 +89,18 @@ hipError_t launch_any(const FusedArgs& p, hipStream_t s) {
   return hipGetLastError();
 }
 
+// Whether the kernels that move whole 64-k tiles can run the operands: codes in whole words of a block's half, two scales at once.
+bool aligned(const FusedArgs& p) {
+  const uintptr_t sb = (uintptr_t)p.s | (p.asym ? (uintptr_t)p.b : 0);
+  return p.K % 64 == 0 && (p.group == 32 || p.K % 128 == 0) && (uintptr_t)p.q % (p.bits == 4 ? 16 : 4) == 0 && sb % 4 == 0;
+}
+
 template <int BITS, bool ASYM, int EPI>
 hipError_t launch(const FusedArgs& p, hipStream_t s) {
-  return launch_any<BITS, ASYM, EPI>(p, s);
+  if (!aligned(p) || p.M <= 16) return launch_any<BITS, ASYM, EPI>(p, s);
+  if (p.M <= 32) return launch_tiles<BITS, ASYM, EPI, 1>(p, s);
+  if (ASYM || p.M <= 64) return launch_tiles<BITS, ASYM, EPI, 2>(p, s);
+  return launch_tiles<BITS, ASYM, EPI, ASYM ? 2 : 4>(p, s);
 }
 
 template <int EPI>

@@ -26,13 +26,15 @@ constexpr int kEpiAct = 0, kEpiLogits = 1;
 template <int BITS>
 __device__ __forceinline__ h8 codes8(unsigned lo, unsigned hi) {
   h8 r;
+  unsigned mask = 0x00F0000Fu, one = 0x54006400u;
+  if constexpr (BITS == 4) asm("" : "+s"(mask), "+v"(one));  // (in registers: one v_and_or_b32 takes one literal at most)
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     h2 q;
     if constexpr (BITS == 4) {
       // a byte (two codes) in both halves; bit 0 of 1024.0's mantissa is worth 1, bit 4 of 64.0's likewise
       const unsigned p = __builtin_amdgcn_perm(lo, lo, 0x01010101u * i);
-      q = __builtin_bit_cast(h2, (p & 0x00F0000Fu) | 0x54006400u) - h2{(_Float16)1032.0f, (_Float16)72.0f};
+      q = __builtin_bit_cast(h2, (p & mask) | one) - h2{(_Float16)1032.0f, (_Float16)72.0f};
     } else {
       const unsigned x = lo >> (4 * i);
       unsigned p = (x & 3u) | ((x & 12u) << 14);
@@ -49,7 +51,13 @@ __device__ __forceinline__ h8 codes8(unsigned lo, unsigned hi) {
   return r;
 }
 
-__device__ __forceinline__ float f16_bits(unsigned u) { return (float)__builtin_bit_cast(_Float16, (unsigned short)u); }
+// The f16 of u's low half as an f32 in a register of its own: the compiler would otherwise put the conversion into each fma that
+// takes it (v_fma_mix_f32, twice as long and not bound to its accumulator's register, which made the tile kernel spill).
+__device__ __forceinline__ float f16_bits(unsigned u) {
+  float v = (float)__builtin_bit_cast(_Float16, (unsigned short)u);
+  asm("" : "+v"(v));
+  return v;
+}
 // b + 2^(BITS-1) s
 template <int BITS>
 __device__ __forceinline__ float centred(float s, float b) { return fmaf((float)(1 << (BITS - 1)), s, b); }
@@ -132,6 +140,24 @@ __device__ __forceinline__ LpRecord record16(const float* z, int c, int valid) {
   }
 #pragma unroll
   for (int d = 1; d < 16; d *= 2) rest += __shfl_xor(rest, d), rest_z += __shfl_xor(rest_z, d);
+  return LpRecord{l.max, rest, rest_z, pack_second(l.second, l.arg)};
+}
+
+// The same where lane half h has columns 32 h .. + 31 of a row's block. Both halves get it.
+__device__ __forceinline__ LpRecord record32(const float* z, int h, int valid) {
+  Largest l{kNone, kNone, 32 * h};
+#pragma unroll
+  for (int t = 0; t < 32; t++)
+    if (32 * h + t < valid) l.take(z[t], 32 * h + t);
+  l.join(__shfl_xor(l.max, 32), __shfl_xor(l.second, 32), __shfl_xor(l.arg, 32));
+  float rest = 0.0f, rest_z = 0.0f;
+#pragma unroll
+  for (int t = 0; t < 32; t++) {
+    const float x = z[t] - l.max, e = __expf(x);
+    if (32 * h + t < valid && 32 * h + t != l.arg) rest += e, rest_z = fmaf(e, x, rest_z);
+  }
+  rest += __shfl_xor(rest, 32);
+  rest_z += __shfl_xor(rest_z, 32);
   return LpRecord{l.max, rest, rest_z, pack_second(l.second, l.arg)};
 }
 
