@@ -58,24 +58,20 @@ __global__ __launch_bounds__(256) void fused_any_kernel(FusedArgs p) {
       }
     }
   }
+  const int m = m0 + 4 * g;
+  if constexpr (EPI == kEpiLogits) {
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const int m = m0 + 4 * g + e;
-    if constexpr (EPI == kEpiLogits) {
+    for (int e = 0; e < 4; e++) {
       const float z[4] = {p.scale * acc[0][e], p.scale * acc[1][e], p.scale * acc[2][e], p.scale * acc[3][e]};
       const LpRecord r = record16(z, c, cols - n0);
-      if (c == 0 && m < p.M) p.rec[(size_t)m * ntn + tn] = r;
-    } else {
-      if (m >= p.M) continue;
+      if (c == 0 && m + e < p.M) p.rec[(size_t)(m + e) * ntn + tn] = r;
+    }
+  } else {
+    if (m >= p.M) return;
 #pragma unroll
-      for (int t = 0; t < 4; t++) {
-        const int j = n0 + 16 * t + c;
-        if (wide == 32) {
-          if (t < 2 && j < cols) store_result(p, m, j, result_of(p, j, acc[t][e], acc[t + 2 < 4 ? t + 2 : 3][e]));
-        } else if (j < cols) {
-          store_result(p, m, j, result_of(p, j, acc[t][e]));
-        }
-      }
+    for (int t = 0; t < 4; t++) {
+      if (wide == 32 && t >= 2) break;
+      results<4>(p, m, n0 + 16 * t + c, cols, [](int v) { return v; }, (const float*)&acc[t], wide == 32 ? (const float*)&acc[t ^ 2] : nullptr);
     }
   }
 }

@@ -17,6 +17,13 @@ __device__ __forceinline__ void dma4(unsigned lds, unsigned voff, const void* ba
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                "v"(voff), "s"(base) : "memory", "m0");
 }
+// the same from a lane's own 64-bit address
+__device__ __forceinline__ void dma16_at(unsigned lds, const void* from) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ void dma4_at(unsigned lds, const void* from) {
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dword %1, off" ::"s"(__builtin_amdgcn_readfirstlane(lds)), "v"(from) : "memory", "m0");
+}
 __device__ __forceinline__ unsigned lds_addr(const void* p) {
   return (unsigned)(size_t)(const __attribute__((address_space(3))) char*)p;
 }
