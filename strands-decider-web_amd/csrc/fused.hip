@@ -7,7 +7,7 @@
 
 #include "fused.h"
 #include "fused_common.h"
-#include "fused_tiles.h"
+#include "fused_plan.h"
 
 namespace ha {
 namespace {
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256) void fused_any_kernel(FusedArgs p) {
 }
 
 template <int BITS, bool ASYM, int EPI>
-hipError_t launch_any(const FusedArgs& p, hipStream_t s) {
+hipError_t launch_any_as(const FusedArgs& p, hipStream_t s) {
   const int cols = EPI == kEpiAct && p.half ? p.half : p.N, wide = EPI == kEpiAct && p.half ? 32 : 64;
   const long groups = ((cols + wide - 1) / wide + 3) / 4, rows = (p.M + 15) / 16;
   if (groups * rows > 0x7FFFFFFFl) return hipErrorInvalidValue;
@@ -85,36 +85,36 @@ hipError_t launch_any(const FusedArgs& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-// Whether the kernels that move whole 64-k tiles can run the operands: codes in whole words of a block's half, two scales at once.
-bool aligned(const FusedArgs& p) {
-  const uintptr_t sb = (uintptr_t)p.s | (p.asym ? (uintptr_t)p.b : 0);
-  return p.K % 64 == 0 && (p.group == 32 || p.K % 128 == 0) && (uintptr_t)p.q % (p.bits == 4 ? 16 : 4) == 0 && sb % 4 == 0;
-}
-
-template <int BITS, bool ASYM, int EPI>
-hipError_t launch(const FusedArgs& p, hipStream_t s) {
-  if (!aligned(p) || p.M <= 16) return launch_any<BITS, ASYM, EPI>(p, s);
-  if (p.M <= 32) return launch_tiles<BITS, ASYM, EPI, 1>(p, s);
-  if (ASYM || p.M <= 64) return launch_tiles<BITS, ASYM, EPI, 2>(p, s);
-  return launch_tiles<BITS, ASYM, EPI, ASYM ? 2 : 4>(p, s);
-}
-
 template <int EPI>
-hipError_t dispatch(const FusedArgs& p, hipStream_t s) {
+hipError_t launch_any(const FusedArgs& p, hipStream_t s) {
   switch (2 * p.bits + (p.asym ? 1 : 0)) {
-    case 4: return launch<2, false, EPI>(p, s);
-    case 5: return launch<2, true, EPI>(p, s);
-    case 6: return launch<3, false, EPI>(p, s);
-    case 7: return launch<3, true, EPI>(p, s);
-    case 8: return launch<4, false, EPI>(p, s);
-    case 9: return launch<4, true, EPI>(p, s);
+    case 4: return launch_any_as<2, false, EPI>(p, s);
+    case 5: return launch_any_as<2, true, EPI>(p, s);
+    case 6: return launch_any_as<3, false, EPI>(p, s);
+    case 7: return launch_any_as<3, true, EPI>(p, s);
+    case 8: return launch_any_as<4, false, EPI>(p, s);
+    case 9: return launch_any_as<4, true, EPI>(p, s);
   }
   return hipErrorInvalidValue;
 }
 
+// Whether the kernels that move whole 64-k tiles can run the operands: codes in whole words of a block's half, two scales at once.
+bool whole(const FusedArgs& p) {
+  const uintptr_t sb = (uintptr_t)p.s | (p.asym ? (uintptr_t)p.b : 0);
+  return p.K % 64 == 0 && (p.group == 32 || p.K % 128 == 0) && (uintptr_t)p.q % (p.bits == 4 ? 16 : 4) == 0 && sb % 4 == 0;
+}
+
 }  // namespace
 
-hipError_t launch_fused(const FusedArgs& p, hipStream_t s) { return dispatch<kEpiAct>(p, s); }
-hipError_t launch_logit_records(const FusedArgs& p, hipStream_t s) { return dispatch<kEpiLogits>(p, s); }
+hipError_t launch_fused(const FusedArgs& p, hipStream_t s) {
+  const fused::Plan plan = fused::plan({p.M, p.half ? p.half : p.N, p.K, p.half != 0, p.asym != 0, whole(p)});
+  if (plan.path == fused::kRows) return launch_fused_rows(p, plan.a, plan.b, s);
+  if (plan.path == fused::kTiles) return launch_fused_tiles(p, plan.a, plan.b, s);
+  return launch_any<kEpiAct>(p, s);
+}
+
+hipError_t launch_logit_records(const FusedArgs& p, hipStream_t s) {
+  return whole(p) && p.M > 16 ? launch_logit_tiles(p, s) : launch_any<kEpiLogits>(p, s);
+}
 
 }  // namespace ha

@@ -1,0 +1,28 @@
+// Records of logits (launch_logit_records of fused.hip) by the tile kernels of every format.
+#include "fused_tiles.h"
+
+namespace ha {
+namespace {
+
+template <int BITS, bool ASYM>
+hipError_t launch(const FusedArgs& p, hipStream_t s) {
+  if (p.M <= 32) return launch_tiles<BITS, ASYM, kEpiLogits, 1, 2>(p, s);
+  if (ASYM || p.M <= 64) return launch_tiles<BITS, ASYM, kEpiLogits, 2, 2>(p, s);
+  return launch_tiles<BITS, ASYM, kEpiLogits, ASYM ? 2 : 4, 2>(p, s);
+}
+
+}  // namespace
+
+hipError_t launch_logit_tiles(const FusedArgs& p, hipStream_t s) {
+  switch (2 * p.bits + (p.asym ? 1 : 0)) {
+    case 4: return launch<2, false>(p, s);
+    case 5: return launch<2, true>(p, s);
+    case 6: return launch<3, false>(p, s);
+    case 7: return launch<3, true>(p, s);
+    case 8: return launch<4, false>(p, s);
+    case 9: return launch<4, true>(p, s);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace ha

@@ -19,11 +19,11 @@ namespace ha {
 namespace {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
-constexpr int kTileCols = 256, kTileWaves = 4, kTileStages = 3;
+constexpr int kTileWaves = 4, kTileStages = 3;
 
-template <int BITS, bool ASYM, int EPI, int RT>
-__global__ __launch_bounds__(64 * kTileWaves, RT <= 2 && !ASYM ? 3 : 2) void fused_tiles_kernel(FusedArgs p) {
-  constexpr int CT = 2, kRows = 32 * RT, kA = kRows * 128;
+template <int BITS, bool ASYM, int EPI, int RT, int CT>
+__global__ __launch_bounds__(64 * kTileWaves, RT * CT <= 2 ? 4 : RT * CT <= 4 && !ASYM ? 3 : 2) void fused_tiles_kernel(FusedArgs p) {
+  constexpr int kRows = 32 * RT, kA = kRows * 128, kCols = 32 * CT;  // kCols: of a wave
   constexpr int kW = CT * 64 * 4 * BITS, kS = ASYM ? 512 : 256;    // a wave's packed words and scales (, biases) of a stage
   constexpr int kStage = kA + kTileWaves * (kW + kS);
   constexpr int kCopiesA = kRows / 8 / kTileWaves, kCopiesW = (BITS == 4 ? CT : CT * BITS) + (ASYM ? 2 : 1);  // DMA instructions of a wave
@@ -33,7 +33,7 @@ __global__ __launch_bounds__(64 * kTileWaves, RT <= 2 && !ASYM ? 3 : 2) void fus
   const int tid = threadIdx.x, lane = tid & 63, f = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool gated = EPI == kEpiAct && p.half;
-  const int cols = gated ? p.half : p.N, wide = gated ? kTileCols / 2 : kTileCols;
+  const int cols = gated ? p.half : p.N, wide = kTileWaves * (gated ? 32 : kCols);
   const int ntn = (cols + wide - 1) / wide, ntm = (p.M + kRows - 1) / kRows, ntiles = ntn * ntm;
   // workgroups go to the 8 XCDs in turn: XCD x takes a contiguous range of tiles, in bands of 8 tile rows, rows fastest, so that
   // neighbours share rows of a and columns of W in its L2
@@ -45,7 +45,7 @@ __global__ __launch_bounds__(64 * kTileWaves, RT <= 2 && !ASYM ? 3 : 2) void fus
   constexpr int kBand = 8;
   const int band = id / (kBand * ntn), in_band = id - band * kBand * ntn, rows = min(kBand, ntm - band * kBand);
   const int tm = band * kBand + in_band % rows, tn = in_band / rows;
-  const int m0 = tm * kRows, j0 = tn * wide + (gated ? 32 : 64) * w;  // the wave's first column (of the result)
+  const int m0 = tm * kRows, j0 = tn * wide + (gated ? 32 : kCols) * w;  // the wave's first column (of the result)
   const int nblk = p.K / 32, nkt = p.K / 64, ng = p.K / p.group;
   // rows past M repeat the last one, columns past the last likewise; neither is stored
   const unsigned last = (unsigned)(p.M - 1 - m0), k2 = 2u * (unsigned)p.K;
@@ -64,7 +64,7 @@ __global__ __launch_bounds__(64 * kTileWaves, RT <= 2 && !ASYM ? 3 : 2) void fus
     wo[c] = ((unsigned)min(f, left) * (unsigned)nblk + h) * (4u * BITS);
     if (c == h) so = (unsigned)min(f, left) * (unsigned)ng * 2u;
   }
-  const char *sl = h ? sp[1] + so : sp[0] + so, *bl = h ? bp[1] + so : bp[0] + so;
+  const char *sl = (h ? sp[CT - 1] : sp[0]) + so, *bl = (h ? bp[CT - 1] : bp[0]) + so;
   const bool g64 = p.group == 64;
   const unsigned lds_a = __builtin_amdgcn_readfirstlane(lds_addr(sm) + 1024u * kCopiesA * w);
   const unsigned lds_w = __builtin_amdgcn_readfirstlane(lds_addr(sm) + kA + (kW + kS) * w);
@@ -175,14 +175,14 @@ __global__ __launch_bounds__(64 * kTileWaves, RT <= 2 && !ASYM ? 3 : 2) void fus
         af[u ^ 1][0] = operand((t + CT) / kPairs, (t + CT) / CT % RT, 0);
         af[u ^ 1][1] = operand((t + CT) / kPairs, (t + CT) / CT % RT, 1);
       }
-      if (t == 1) x1 = words(stage, 1);
+      if (t == CT - 1) x1 = words(stage, 1);
       add(t == 0 ? 2 * kPairs - 1 : t - 1, 0);
       __builtin_amdgcn_sched_barrier(0);
       d[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[u][1], bf[c][1], d[t & 1], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
       add(t == 0 ? 2 * kPairs - 1 : t - 1, 8);
       if (t == 0) {  // (the last tile's scales are done with)
-        decode(x0, 1);
+        if constexpr (CT == 2) decode(x0, 1);
 #pragma unroll
         for (int n = 0; n < CT; n++) {
           const unsigned sv = g64 ? sw[n] >> (16 * (kt & 1)) : sw[n], bv = g64 ? bw[n] >> (16 * (kt & 1)) : bw[n];
@@ -194,7 +194,9 @@ __global__ __launch_bounds__(64 * kTileWaves, RT <= 2 && !ASYM ? 3 : 2) void fus
         }
       }
       if (t == kPairs - 1) decode(x1, 0);
-      if (t == kPairs) decode(x1, 1);
+      if constexpr (CT == 2) {
+        if (t == kPairs) decode(x1, 1);
+      }
       if (t == 2 * kPairs - CT - 1) {  // the next tile's first words (its copies into this wave's part have landed)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kCopiesA + kCopiesW) : "memory");
         x0 = words(next_stage, 0);
@@ -241,7 +243,7 @@ __global__ __launch_bounds__(64 * kTileWaves, RT <= 2 && !ASYM ? 3 : 2) void fus
       if (m0 + 32 * i >= p.M) break;
       auto row_of = [](int v) { return 8 * (v >> 2) + (v & 3); };
       if (gated) {
-        results<16>(p, m, j0 + f, cols, row_of, (const float*)&acc[i][0], (const float*)&acc[i][1]);
+        if constexpr (CT == 2) results<16>(p, m, j0 + f, cols, row_of, (const float*)&acc[i][0], (const float*)&acc[i][1]);
       } else {
 #pragma unroll
         for (int c = 0; c < CT; c++) results<16>(p, m, j0 + 32 * c + f, cols, row_of, (const float*)&acc[i][c], nullptr);
@@ -250,13 +252,14 @@ __global__ __launch_bounds__(64 * kTileWaves, RT <= 2 && !ASYM ? 3 : 2) void fus
   }
 }
 
-template <int BITS, bool ASYM, int EPI, int RT>
+template <int BITS, bool ASYM, int EPI, int RT, int CT>
 hipError_t launch_tiles(const FusedArgs& p, hipStream_t s) {
   const bool gated = EPI == kEpiAct && p.half;
-  const int cols = gated ? p.half : p.N, wide = gated ? kTileCols / 2 : kTileCols;
+  const int cols = gated ? p.half : p.N, wide = kTileWaves * (gated ? 32 : 32 * CT);
+  if (CT == 1 && (gated || EPI == kEpiLogits)) return hipErrorInvalidValue;  // (a pair of column tiles a wave)
   const long tiles = (long)((cols + wide - 1) / wide) * ((p.M + 32 * RT - 1) / (32 * RT));
   if (tiles > 0x7FFFFFFFl) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((fused_tiles_kernel<BITS, ASYM, EPI, RT>), dim3((unsigned)tiles), dim3(64 * kTileWaves), 0, s, p);
+  hipLaunchKernelGGL((fused_tiles_kernel<BITS, ASYM, EPI, RT, CT>), dim3((unsigned)tiles), dim3(64 * kTileWaves), 0, s, p);
   return hipGetLastError();
 }
 
