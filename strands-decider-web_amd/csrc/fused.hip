@@ -114,7 +114,7 @@ hipError_t launch_fused(const FusedArgs& p, hipStream_t s) {
 }
 
 hipError_t launch_logit_records(const FusedArgs& p, hipStream_t s) {
-  return whole(p) && p.M > 16 ? launch_logit_tiles(p, s) : launch_any<kEpiLogits>(p, s);
+  return whole(p) ? launch_logit_tiles(p, s) : launch_any<kEpiLogits>(p, s);
 }
 
 }  // namespace ha

@@ -1,4 +1,6 @@
-// Records of logits (launch_logit_records of fused.hip) by the tile kernels of every format.
+// Records of logits (launch_logit_records of fused.hip) of every format: up to 16 rows by the stream kernel
+// (fused_stream.h), more by tiles (fused_tiles.h).
+#include "fused_stream.h"
 #include "fused_tiles.h"
 
 namespace ha {
@@ -6,6 +8,7 @@ namespace {
 
 template <int BITS, bool ASYM>
 hipError_t launch(const FusedArgs& p, hipStream_t s) {
+  if (stream_takes(p)) return launch_stream<BITS, ASYM>(p, s);
   if (p.M <= 32) return launch_tiles<BITS, ASYM, kEpiLogits, 1, 2>(p, s);
   if (ASYM || p.M <= 64) return launch_tiles<BITS, ASYM, kEpiLogits, 2, 2>(p, s);
   return launch_tiles<BITS, ASYM, kEpiLogits, ASYM ? 2 : 4, 2>(p, s);
