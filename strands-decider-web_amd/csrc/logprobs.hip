@@ -20,7 +20,9 @@
 namespace ha {
 namespace {
 
-constexpr int kT = 512, kWaves = kT / 64;
+constexpr int kLpSets = 256;  // sets of threads whose largest keys the cut is looked for in
+static_assert(kLpSets >= kLpMaxTop + kLpMargin, "as many sets as blocks that are chosen");
+
 typedef unsigned long long u64;
 
 __device__ __forceinline__ double wave_sum(double v) {
@@ -29,44 +31,61 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
-// a[m] . W[n] in 64 bits, by one wave: lanes over the packed blocks.
+// a[m] . W[n] of two rows n in 64 bits, by one wave: lanes over the packed blocks.
 template <int BITS, bool ASYM>
-__device__ double dot64(const FusedArgs& p, int m, int n, int lane) {
+__device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double* out) {
   const int nblk = p.K / 32, ng = p.K / p.group, gl = p.group == 64 ? 1 : 0;
-  gptr<unsigned> wp = gp<unsigned>(p.q) + (size_t)n * nblk * BITS;
   gptr<h8> ap = (gptr<h8>)(gp<_Float16>(p.a) + (size_t)m * p.K);
-  double acc = 0.0;
+  out[0] = out[1] = 0.0;
   for (int k = lane; k < nblk; k += 64) {
-    unsigned wd[BITS];
+    unsigned wd[2][BITS];
+    float s[2], b[2] = {0.0f, 0.0f};
+    h8 av[4];
 #pragma unroll
-    for (int i = 0; i < BITS; i++) wd[i] = wp[(size_t)k * BITS + i];
-    const double s = f16_bits(gp<unsigned short>(p.s)[(size_t)n * ng + (k >> gl)]);
-    double d = 0.0, sum = 0.0;
+    for (int x = 0; x < 2; x++) {
+      gptr<unsigned> wp = gp<unsigned>(p.q) + ((size_t)n[x] * nblk + k) * BITS;
+#pragma unroll
+      for (int i = 0; i < BITS; i++) wd[x][i] = wp[i];
+      s[x] = f16_bits(gp<unsigned short>(p.s)[(size_t)n[x] * ng + (k >> gl)]);
+      if constexpr (ASYM) b[x] = f16_bits(gp<unsigned short>(p.b)[(size_t)n[x] * ng + (k >> gl)]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) av[j] = ap[4 * k + j];
+    double d[2] = {0.0, 0.0}, sum = 0.0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const h8 av = ap[4 * k + j];
-      unsigned lo, hi = 0;
-      if constexpr (BITS == 4) lo = wd[j];
-      else lo = wd[j >> 1] >> (16 * (j & 1)) & 0xFFFFu;
-      if constexpr (BITS == 3) hi = wd[BITS - 1] >> (8 * j) & 0xFFu;
-      const h8 c = codes8<BITS>(lo, hi);
+      h8 c[2];
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        unsigned lo, hi = 0;
+        if constexpr (BITS == 4) lo = wd[x][j];
+        else lo = wd[x][j >> 1] >> (16 * (j & 1)) & 0xFFFFu;
+        if constexpr (BITS == 3) hi = wd[x][BITS - 1] >> (8 * j) & 0xFFu;
+        c[x] = codes8<BITS>(lo, hi);
+      }
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        d += (double)((float)av[e] * (float)c[e]);  // (15 bits: exact)
-        if constexpr (ASYM) sum += (double)(float)av[e];
+#pragma unroll
+        for (int x = 0; x < 2; x++) d[x] += (double)((float)av[j][e] * (float)c[x][e]);  // (15 bits: exact)
+        if constexpr (ASYM) sum += (double)(float)av[j][e];
       }
     }
-    acc += s * d;
-    if constexpr (ASYM) acc += ((double)f16_bits(gp<unsigned short>(p.b)[(size_t)n * ng + (k >> gl)]) + (1 << (BITS - 1)) * s) * sum;
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      out[x] += (double)s[x] * d[x];
+      if constexpr (ASYM) out[x] += ((double)b[x] + (1 << (BITS - 1)) * (double)s[x]) * sum;
+    }
   }
-  return wave_sum(acc);
+#pragma unroll
+  for (int x = 0; x < 2; x++) out[x] = wave_sum(out[x]);
 }
 
-// A workgroup for a row. Dynamic LDS: list_cap keys, then cand_cap values and their columns.
-template <int BITS, bool ASYM>
-__global__ __launch_bounds__(kT) void logprobs_kernel(LpArgs a, int nb, int list_cap, int cand_cap) {
+// A workgroup of T threads for a row. Dynamic LDS: list_cap keys, then cand_cap values and their columns.
+template <int BITS, bool ASYM, int T>
+__global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_cap, int cand_cap) {
+  constexpr int kWaves = T / 64, kKeep = 4096 / T, kSets = kLpSets / 64;
   extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
-  __shared__ u64 best[kT];
+  __shared__ u64 best[kLpSets];
   __shared__ u64 threshold;
   __shared__ double red[2][kWaves];
   __shared__ int chosen[kLpMaxTop + kLpMargin];
@@ -75,33 +94,45 @@ __global__ __launch_bounds__(kT) void logprobs_kernel(LpArgs a, int nb, int list
   double* val = (double*)(list + list_cap);
   int* ids = (int*)(val + cand_cap);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), m = blockIdx.x;
-  const int n_vocab = a.p.N, k = a.top_k, kk = min(k + kLpMargin, nb);
+  const int n_vocab = a.p.N, k = a.top_k, kk = min(k + kLpMargin, nb), nt = a.n_targets;
   const LpRecord* rec = a.p.rec + (size_t)m * nb;
   auto key_of = [](float max, int i) { return (u64)ordered(max) << 32 | (0xFFFFFFFFu - (unsigned)i); };
-  // the thread's largest key (0: no block)
+  // records tid, tid + T, ...: the first kKeep stay in registers
+  LpRecord keep[kKeep];
+#pragma unroll
+  for (int i = 0; i < kKeep; i++)
+    if (tid + i * T < nb) keep[i] = rec[tid + i * T];
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int i = 0; i < kKeep; i++)
+      if (tid + i * T < nb) f(keep[i], tid + i * T);
+    for (int i = tid + kKeep * T; i < nb; i += T) f(rec[i], i);
+  };
   u64 mine = 0;
   bool bad = false;
-  for (int i = tid; i < nb; i += kT) {
-    const LpRecord r = rec[i];
+  each([&](const LpRecord& r, int i) {
     bad |= !(fabsf(r.max) <= 3.4e38f && fabsf(r.rest) <= 3.4e38f && fabsf(r.rest_z) <= 3.4e38f);
     mine = max(mine, key_of(r.max, i));
-  }
-  best[tid] = mine;
+  });
+  // the largest key of every T / kLpSets threads (0: no block)
+#pragma unroll
+  for (int d = 1; d < T / kLpSets; d *= 2) mine = max(mine, (u64)__shfl_xor((long long)mine, d));
+  if (tid % (T / kLpSets) == 0) best[tid / (T / kLpSets)] = mine;
   if (tid == 0) n_list = 0, n_cand = 0;
   if (__syncthreads_or(bad)) {  // a logit that is not finite
     const float nan = __builtin_nanf("");
-    for (int t = tid; t < a.n_targets; t += kT) a.logp[(size_t)m * a.n_targets + t] = nan;
-    for (int t = tid; t < k; t += kT) a.top_ids[(size_t)m * k + t] = -1, a.top_logp[(size_t)m * k + t] = nan;
+    for (int t = tid; t < nt; t += T) a.logp[(size_t)m * nt + t] = nan;
+    for (int t = tid; t < k; t += T) a.top_ids[(size_t)m * k + t] = -1, a.top_logp[(size_t)m * k + t] = nan;
     if (tid == 0 && a.entropy) a.entropy[m] = nan;
     if (tid == 0 && a.lse) a.lse[m] = nan;
     return;
   }
-  // a key that at least kk blocks reach and few others: the kk-th largest of the threads' largest, found bit by bit
+  // a key that at least kk blocks reach and few others: the kk-th largest of those, found bit by bit (where there are fewer, 0)
   if (w == 0) {
-    u64 v[kWaves];
+    u64 v[kSets];
     u64 top = 0;
 #pragma unroll
-    for (int i = 0; i < kWaves; i++) v[i] = best[lane + 64 * i], top = max(top, v[i]);
+    for (int i = 0; i < kSets; i++) v[i] = best[lane + 64 * i], top = max(top, v[i]);
 #pragma unroll
     for (int d = 32; d >= 1; d /= 2) top = max(top, (u64)__shfl_xor((long long)top, d));
     u64 t = 0;
@@ -109,7 +140,7 @@ __global__ __launch_bounds__(kT) void logprobs_kernel(LpArgs a, int nb, int list
       const u64 next = t | 1ull << bit;
       int n = 0;
 #pragma unroll
-      for (int i = 0; i < kWaves; i++) n += __popcll(__ballot(v[i] >= next));
+      for (int i = 0; i < kSets; i++) n += __popcll(__ballot(v[i] >= next));
       if (n >= kk) t = next;
       if (n == kk) break;
     }
@@ -120,8 +151,7 @@ __global__ __launch_bounds__(kT) void logprobs_kernel(LpArgs a, int nb, int list
   const float M = unordered((unsigned)(top_key >> 32));
   // sums over the blocks; the largest columns of those from the cut on wait
   double z = 0.0, zx = 0.0;
-  for (int i = tid; i < nb; i += kT) {
-    const LpRecord r = rec[i];
+  each([&](const LpRecord& r, int i) {
     const u64 key = key_of(r.max, i);
     const double x = (double)r.max - (double)M, e = (double)__expf((float)x);
     double rest = r.rest;
@@ -129,10 +159,10 @@ __global__ __launch_bounds__(kT) void logprobs_kernel(LpArgs a, int nb, int list
     else rest += 1.0;
     z += e * rest;
     zx += e * ((double)r.rest_z + rest * x);
-  }
+  });
   __syncthreads();
   const int nl = n_list;
-  for (int i = tid; i < nl; i += kT) {
+  for (int i = tid; i < nl; i += T) {
     const u64 key = list[i];
     int rank = 0;
     for (int j = 0; j < nl; j++) rank += list[j] > key;
@@ -166,31 +196,40 @@ __global__ __launch_bounds__(kT) void logprobs_kernel(LpArgs a, int nb, int list
     }
   }
   __syncthreads();
-  const int nc = kk + n_cand, nt = a.n_targets;
-  for (int i = w; i < nc + nt; i += kWaves) {
-    int n = i < nc ? ids[i] : a.targets[(size_t)m * nt + i - nc];
-    if ((unsigned)n >= (unsigned)n_vocab) {  // no token: its log probability is NaN
-      if (lane == 0) val[i] = __builtin_nan("");
-      continue;
+  const int nc = kk + n_cand;
+  for (int i = 2 * w; i < nc + nt; i += 2 * kWaves) {
+    int n[2];
+    bool token[2];
+#pragma unroll
+    for (int x = 0; x < 2; x++) {
+      const int at = min(i + x, nc + nt - 1), id = at < nc ? ids[at] : a.targets[(size_t)m * nt + at - nc];
+      token[x] = (unsigned)id < (unsigned)n_vocab;  // (no token: its log probability is NaN)
+      n[x] = token[x] ? id : 0;
     }
-    const double d = (double)a.p.scale * dot64<BITS, ASYM>(a.p, m, n, lane);
-    if (lane == 0) val[i] = d;
+    double d[2];
+    dot64<BITS, ASYM>(a.p, m, n, lane, d);
+#pragma unroll
+    for (int x = 0; x < 2; x++)
+      if (lane == 0 && i + x < nc + nt) val[i + x] = token[x] ? (double)a.p.scale * d[x] : __builtin_nan("");
   }
   __syncthreads();
-  z = zx = 0.0;
-  for (int i = 0; i < kWaves; i++) z += red[0][i], zx += red[1][i];
-  for (int i = 0; i < kk; i++) {
+  // every wave: the sums, with the chosen blocks' largest columns from 64 bits
+  z = lane < kWaves ? red[0][lane] : 0.0;
+  zx = lane < kWaves ? red[1][lane] : 0.0;
+  for (int i = lane; i < kk; i += 64) {
     const double x = val[i] - (double)M, e = exp(x);
     z += e;
     zx += e * x;
   }
+  z = wave_sum(z);
+  zx = wave_sum(zx);
   const double log_z = log(z);
   auto logp = [&](double v) { return (float)((v - (double)M) - log_z); };
   if (tid == 0 && a.entropy) a.entropy[m] = (float)(log_z - zx / z);
   if (tid == 0 && a.lse) a.lse[m] = (float)((double)M + log_z);
-  for (int t = tid; t < nt; t += kT) a.logp[(size_t)m * nt + t] = logp(val[nc + t]);
+  for (int t = tid; t < nt; t += T) a.logp[(size_t)m * nt + t] = logp(val[nc + t]);
   if (k > 0) {
-    for (int i = tid; i < nc; i += kT) {
+    for (int i = tid; i < nc; i += T) {
       const double v = val[i];
       const int id = ids[i];
       int rank = 0;
@@ -200,18 +239,24 @@ __global__ __launch_bounds__(kT) void logprobs_kernel(LpArgs a, int nb, int list
   }
 }
 
-template <int BITS, bool ASYM>
-hipError_t launch(const LpArgs& a, hipStream_t s) {
+template <int BITS, bool ASYM, int T>
+hipError_t launch_as(const LpArgs& a, hipStream_t s) {
   const int nb = (a.p.N + kLpBlock - 1) / kLpBlock, kk = std::min(a.top_k + kLpMargin, nb);
-  const int list_cap = kk * ((nb + kT - 1) / kT), cand_cap = (a.top_k > 0 ? kk * kLpBlock : kk) + a.n_targets;
+  // the kk sets of T / kLpSets threads that hold a key from the cut on (where there are fewer sets, all of them)
+  const int list_cap = std::min(nb, kk * (T / kLpSets) * ((nb + T - 1) / T)), cand_cap = (a.top_k > 0 ? kk * kLpBlock : kk) + a.n_targets;
   const size_t lds = 8 * (size_t)list_cap + 12 * (size_t)cand_cap;
-  auto k = logprobs_kernel<BITS, ASYM>;
+  auto k = logprobs_kernel<BITS, ASYM, T>;
   if (lds > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(k, dim3(a.p.M), dim3(kT), lds, s, a, nb, list_cap, cand_cap);
+  hipLaunchKernelGGL(k, dim3(a.p.M), dim3(T), lds, s, a, nb, list_cap, cand_cap);
   return hipGetLastError();
+}
+// Few rows: 16 waves for each, more of its loads and products at once (one row over 248320 tokens, top 8: us).
+template <int BITS, bool ASYM>
+hipError_t launch(const LpArgs& a, hipStream_t s) {
+  return a.p.M <= 256 ? launch_as<BITS, ASYM, 1024>(a, s) : launch_as<BITS, ASYM, 512>(a, s);
 }
 
 }  // namespace
