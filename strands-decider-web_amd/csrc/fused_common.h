@@ -139,58 +139,50 @@ __device__ __forceinline__ unsigned pack_second(float second, int arg) {
   return (min(ordered(second) >> 6, (1u << 26) - 2) + 1) << 6 | (unsigned)arg;
 }
 
-// The largest of a set of columns, which one it is (the first of equals), and the second largest.
-struct Largest {
-  float max, second;
-  int arg;
-  __device__ __forceinline__ void take(float v, int at) {  // columns in ascending order
-    if (v > max) second = max, max = v, arg = at;
-    else second = fmaxf(second, v);
-  }
-  __device__ __forceinline__ void join(float m, float s, int at) {  // another set's
-    const bool theirs = m > max || (m == max && at < arg);
-    second = fmaxf(fmaxf(second, s), theirs ? max : m);
-    if (theirs) max = m, arg = at;
-  }
-};
-constexpr float kNone = -__builtin_huge_valf();
+// What stands for a column that is none: below every logit (|z| < 10^23: f16 rows and scales, fused_host.cpp bounds the factor).
+constexpr float kNoLogit = -3e38f;
 
-// The record of a row's block where lane c of 16 has columns 16 t + c, t < 4, of it (z: scaled; valid: columns of the block).
-// All 16 lanes get it.
-__device__ __forceinline__ LpRecord record16(const float* z, int c, int valid) {
-  Largest l{kNone, kNone, 0};
+// The record of a row's block of which this lane has the N columns col(0) < col(1) < ..., and the lanes at distance D, 2 D, ...
+// < L of it the others (z: scaled, kNoLogit where there is no column). All of them get it. About ten instructions a value and an
+// exponential: columns that equal the largest are taken out of the sums, counted, and put back but for one.
+template <int N, int D, int L, class Col>
+__device__ __forceinline__ LpRecord record_of(const float* z, Col col) {
+  float top = z[0];
 #pragma unroll
-  for (int t = 0; t < 4; t++)
-    if (16 * t + c < valid) l.take(z[t], 16 * t + c);
+  for (int i = 1; i < N; i++) top = fmaxf(top, z[i]);
 #pragma unroll
-  for (int d = 1; d < 16; d *= 2) l.join(__shfl_xor(l.max, d), __shfl_xor(l.second, d), __shfl_xor(l.arg, d));
-  float rest = 0.0f, rest_z = 0.0f;
+  for (int d = D; d < L; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+  float second = kNoLogit, rest = 0.0f, rest_z = 0.0f;
+  int arg = kLpBlock - 1, equal = 0;
 #pragma unroll
-  for (int t = 0; t < 4; t++) {
-    const float x = z[t] - l.max, e = __expf(x);
-    if (16 * t + c < valid && 16 * t + c != l.arg) rest += e, rest_z = fmaf(e, x, rest_z);
+  for (int i = N - 1; i >= 0; i--) {
+    const bool is = z[i] == top;
+    const float other = is ? kNoLogit : z[i];
+    equal += is;
+    arg = is ? col(i) : arg;
+    second = fmaxf(second, other);
+    const float x = other - top, e = __expf(x);  // (0 of kNoLogit)
+    rest += e;
+    rest_z = fmaf(e, x, rest_z);
   }
+  if (!equal) arg = kLpBlock - 1;
 #pragma unroll
-  for (int d = 1; d < 16; d *= 2) rest += __shfl_xor(rest, d), rest_z += __shfl_xor(rest_z, d);
-  return LpRecord{l.max, rest, rest_z, pack_second(l.second, l.arg)};
+  for (int d = D; d < L; d *= 2) {
+    second = fmaxf(second, __shfl_xor(second, d));
+    rest += __shfl_xor(rest, d);
+    rest_z += __shfl_xor(rest_z, d);
+    arg = min(arg, __shfl_xor(arg, d));
+    equal += __shfl_xor(equal, d);
+  }
+  if (equal > 1) second = top, rest += (float)(equal - 1);
+  return LpRecord{top, rest, rest_z, pack_second(second, arg)};
 }
-
-// The same where lane half h has columns 32 h .. + 31 of a row's block. Both halves get it.
-__device__ __forceinline__ LpRecord record32(const float* z, int h, int valid) {
-  Largest l{kNone, kNone, 32 * h};
+// Lane c of 16 has columns 16 t + c, t < 4, `valid` of the block's columns exist.
+__device__ __forceinline__ LpRecord record16(const float* z, int c, int valid) {
+  float y[4];
 #pragma unroll
-  for (int t = 0; t < 32; t++)
-    if (32 * h + t < valid) l.take(z[t], 32 * h + t);
-  l.join(__shfl_xor(l.max, 32), __shfl_xor(l.second, 32), __shfl_xor(l.arg, 32));
-  float rest = 0.0f, rest_z = 0.0f;
-#pragma unroll
-  for (int t = 0; t < 32; t++) {
-    const float x = z[t] - l.max, e = __expf(x);
-    if (32 * h + t < valid && 32 * h + t != l.arg) rest += e, rest_z = fmaf(e, x, rest_z);
-  }
-  rest += __shfl_xor(rest, 32);
-  rest_z += __shfl_xor(rest_z, 32);
-  return LpRecord{l.max, rest, rest_z, pack_second(l.second, l.arg)};
+  for (int t = 0; t < 4; t++) y[t] = 16 * t + c < valid ? z[t] : kNoLogit;
+  return record_of<4, 1, 16>(y, [c](int t) { return 16 * t + c; });
 }
 
 }  // namespace

@@ -1,6 +1,5 @@
 // Host side of the products whose results are not stored as they are (ha_mnb_fused, ha_mnb_logprobs, include/ha.h): checks of
 // arguments, launches of fused.hip and logprobs.hip. No counterpart in the reference.
-#include <cmath>
 #include <cstdint>
 #include <string>
 
@@ -44,7 +43,7 @@ int check_logprobs(const ha_logprobs* p, int N, int* n_vocab) {
   if (*n_vocab > ha::kLpMaxVocab) return bad("n_vocab must be at most 2^20");
   if (p->n_targets < 0 || p->n_targets > 1024) return bad("n_targets must be in [0, 1024]");
   if (p->top_k < 0 || p->top_k > ha::kLpMaxTop || p->top_k > *n_vocab) return bad("top_k must be in [0, 64] and at most n_vocab");
-  if (!(p->scale >= 0.0f) || !std::isfinite(p->scale)) return bad("scale must be finite and >= 0 (0: 1)");
+  if (!(p->scale >= 0.0f && p->scale <= 1e6f)) return bad("scale must be in [0, 1e6] (0: 1)");
   return HA_OK;
 }
 

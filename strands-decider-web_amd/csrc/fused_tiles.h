@@ -231,7 +231,11 @@ __global__ __launch_bounds__(64 * kTileWaves, RT * CT <= 2 ? 4 : RT * CT <= 4 &&
       }
       __builtin_amdgcn_wave_barrier();
       if (valid > 0) {
-        const LpRecord r = record32(z, h, valid);
+        if (valid < 64) {
+#pragma unroll
+          for (int t = 0; t < 32; t++) z[t] = 32 * h + t < valid ? z[t] : kNoLogit;
+        }
+        const LpRecord r = record_of<32, 32, 64>(z, [h](int t) { return 32 * h + t; });
         const int m = m0 + 32 * i + f;
         if (h == 0 && m < p.M) p.rec[(size_t)m * nb + (j0 >> 6)] = r;
       }

@@ -127,7 +127,7 @@ int main() {
   WITH(n_vocab, 101, "n_vocab"); WITH(n_vocab, -1, "n_vocab");
   WITH(n_targets, -1, "n_targets"); WITH(n_targets, 1025, "n_targets");
   WITH(top_k, -1, "top_k"); WITH(top_k, 65, "top_k");
-  WITH(scale, -1.0f, "scale"); WITH(scale, INFINITY, "scale"); WITH(scale, NAN, "scale");
+  WITH(scale, -1.0f, "scale"); WITH(scale, 1.1e6f, "scale"); WITH(scale, INFINITY, "scale"); WITH(scale, NAN, "scale");
   WITH(targets, nullptr, "targets"); WITH(logp, nullptr, "targets"); WITH(top_ids, nullptr, "top_ids"); WITH(top_logp, nullptr, "top_ids");
   WITH(targets, (int*)(base + 2), "aligned"); WITH(entropy, (float*)(base + 1), "aligned"); WITH(lse, (float*)(base + 3), "aligned");
   { ha_logprobs b = p; b.n_vocab = 3; b.top_k = 4; BAD(ha_mnb_logprobs(&good, 7, a, &b, res, 1 << 20, nullptr), "top_k"); }
