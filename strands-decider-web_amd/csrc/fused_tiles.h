@@ -5,11 +5,16 @@
 // and one fma a value adds s times their sum: 16 fma beside 64 cycles of the matrix unit, so the vector unit (fma, decoding:
 // some 46 instructions a tile and group with RT = 4) is the busier of the two and what bounds the loop.
 //
-// A workgroup makes 32 RT rows x 256 columns, a wave all of the rows and 64 columns (gated: 32 of the gate and the 32 of the up
-// projection that they multiply). Rows of a and packed weights come through LDS by DMA, three stages of 64 k; a wave copies and
-// reads weights and scales of its own columns, so only a needs the barrier. Two workgroups a CU.
+// A workgroup makes 32 RT rows x 128 CT columns, a wave all of the rows and 32 CT columns (gated: 32 of the gate and the 32 of the
+// up projection that they multiply). Everything comes through LDS by DMA: rows of a by 64 k, two stages, shared; packed words by
+// 128 k and scales by 128 U k, two stages each, of a wave's own columns, so only a needs the barrier. The L2 hands out whole lines
+// of 128 bytes, and a line of a column that is asked for in four parts, 64 k at a time, has left the L1 in between: four times
+// the words' bytes and, scales 4 bytes at a time, 32 times theirs were most of what a CU fetched (2048 x 248320 x 2048: 80 KB a
+// tile and workgroup, 1480 us without any arithmetic, 2415 with it).
 #pragma once
 #include <hip/hip_runtime.h>
+
+#include <type_traits>
 
 #include "fused.h"
 #include "fused_common.h"
@@ -19,17 +24,27 @@ namespace ha {
 namespace {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
-constexpr int kTileWaves = 4, kTileStages = 3;
+constexpr int kTileWaves = 4;
+
+// A workgroup's LDS and waves a SIMD. U: 128-k pieces whose scales come together.
+template <int BITS, bool ASYM, int RT, int CT>
+struct TileShape {
+  static constexpr int U = 4;
+  static constexpr int kRows = 32 * RT, kCols = 32 * CT;
+  static constexpr int kA = kRows * 128, kW = kCols * 16 * BITS, kS = kCols * 8 * U;  // stages: rows of a; a wave's words, scales
+  static constexpr int kOwn = 2 * (kW + kS * (ASYM ? 2 : 1));
+  static constexpr int kPitch = 68;  // of a wave's 32 x 64 results
+  static constexpr int kStaged = 2 * kA + kTileWaves * kOwn, kResults = kTileWaves * 32 * kPitch * 4;
+  static constexpr int kLds = kStaged > kResults ? kStaged : kResults;
+  static constexpr int kWaves = RT * CT <= 2 ? 4 : RT * CT <= 4 && !ASYM && 3 * kLds <= 160 * 1024 ? 3 : 2;
+};
 
 template <int BITS, bool ASYM, int EPI, int RT, int CT>
-__global__ __launch_bounds__(64 * kTileWaves, RT * CT <= 2 ? 4 : RT * CT <= 4 && !ASYM ? 3 : 2) void fused_tiles_kernel(FusedArgs p) {
-  constexpr int kRows = 32 * RT, kA = kRows * 128, kCols = 32 * CT;  // kCols: of a wave
-  constexpr int kW = CT * 64 * 4 * BITS, kS = ASYM ? 512 : 256;    // a wave's packed words and scales (, biases) of a stage
-  constexpr int kStage = kA + kTileWaves * (kW + kS);
-  constexpr int kCopiesA = kRows / 8 / kTileWaves, kCopiesW = (BITS == 4 ? CT : CT * BITS) + (ASYM ? 2 : 1);  // DMA instructions of a wave
-  constexpr int kPitch = 68;                                       // of a wave's 32 x 64 results in LDS
-  constexpr int kLds = kTileStages * kStage > kTileWaves * 32 * kPitch * 4 ? kTileStages * kStage : kTileWaves * 32 * kPitch * 4;
-  __shared__ __attribute__((aligned(16))) unsigned char sm[kLds];
+__global__ __launch_bounds__(64 * kTileWaves, (TileShape<BITS, ASYM, RT, CT>::kWaves)) void fused_tiles_kernel(FusedArgs p) {
+  using L = TileShape<BITS, ASYM, RT, CT>;
+  constexpr int kRows = L::kRows, kCols = L::kCols, kA = L::kA, kW = L::kW, kS = L::kS, U = L::U, kPitch = L::kPitch;
+  constexpr int kCopiesA = kRows / 8 / kTileWaves, kCopiesW = BITS == 4 ? kCols / 16 : kCols * 4 * BITS / 64, kCopiesS = ASYM ? 4 : 2;
+  __shared__ __attribute__((aligned(16))) unsigned char sm[L::kLds];
   const int tid = threadIdx.x, lane = tid & 63, f = lane & 31, h = lane >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const bool gated = EPI == kEpiAct && p.half;
@@ -51,58 +66,76 @@ __global__ __launch_bounds__(64 * kTileWaves, RT * CT <= 2 ? 4 : RT * CT <= 4 &&
   const unsigned last = (unsigned)(p.M - 1 - m0), k2 = 2u * (unsigned)p.K;
   const unsigned chunk = 16u * ((lane & 7) ^ (lane >> 3));  // chunk j of row r in slot j ^ (r & 7)
   const char* ap = (const char*)p.a + (size_t)m0 * p.K * 2;
-  // a wave's columns: from a scalar address for each column tile, 32 bits of lane offset on. Copies of packed words: lane (h, f)
-  // takes block h of column f, 16 bytes or a word at a time; of scales: lane l the pair of column l
+  // a wave's columns: from a scalar address for each column tile, 32 bits of lane offset on
   const char *wp[CT], *sp[CT], *bp[CT];
-  unsigned wo[CT], so = 0;
+  int left[CT];  // the last of the wave's columns of a tile
 #pragma unroll
   for (int c = 0; c < CT; c++) {
-    const int first = gated ? min(j0, cols - 1) + c * p.half : min(j0 + 32 * c, cols - 1), left = (gated ? c * p.half : 0) + cols - 1 - first;
+    const int first = gated ? min(j0, cols - 1) + c * p.half : min(j0 + 32 * c, cols - 1);
+    left[c] = (gated ? c * p.half : 0) + cols - 1 - first;
     wp[c] = (const char*)p.q + (size_t)first * nblk * (4 * BITS);
     sp[c] = (const char*)p.s + (size_t)first * ng * 2;
     bp[c] = ASYM ? (const char*)p.b + (size_t)first * ng * 2 : sp[c];
-    wo[c] = ((unsigned)min(f, left) * (unsigned)nblk + h) * (4u * BITS);
-    if (c == h) so = (unsigned)min(f, left) * (unsigned)ng * 2u;
   }
-  const char *sl = (h ? sp[CT - 1] : sp[0]) + so, *bl = (h ? bp[CT - 1] : bp[0]) + so;
   const bool g64 = p.group == 64;
   const unsigned lds_a = __builtin_amdgcn_readfirstlane(lds_addr(sm) + 1024u * kCopiesA * w);
-  const unsigned lds_w = __builtin_amdgcn_readfirstlane(lds_addr(sm) + kA + (kW + kS) * w);
-  auto copy = [&](int kt, int stage) {
+  const unsigned lds_w = __builtin_amdgcn_readfirstlane(lds_addr(sm) + 2 * kA + L::kOwn * w), lds_s = lds_w + 2 * kW;
+  auto copy_a = [&](int kt, int stage) {
     kt = min(kt, nkt - 1);  // (past the last tile: that one again, not read)
-    const unsigned to = lds_w + (unsigned)(stage * kStage);
-#pragma unroll
-    for (int c = 0; c < CT; c++) {
-      if constexpr (BITS == 4) {
-        dma16(to + 1024 * c, wo[c], wp[c] + (size_t)kt * (8 * BITS));
-      } else {
-#pragma unroll
-        for (int i = 0; i < BITS; i++) dma4(to + 256 * (c * BITS + i), wo[c] + 4 * i, wp[c] + (size_t)kt * (8 * BITS));
-      }
-    }
-    const size_t st = g64 ? 2 * (size_t)(kt & ~1) : 4 * (size_t)kt;  // the tile's two scales, or two tiles'
-    dma4_at(to + kW, sl + st);
-    if constexpr (ASYM) dma4_at(to + kW + 256, bl + st);
 #pragma unroll
     for (int i = 0; i < kCopiesA; i++)
-      dma16(lds_a + (unsigned)(stage * kStage + 1024 * i), min(8u * (kCopiesA * w + i) + (lane >> 3), last) * k2 + chunk, ap + (size_t)kt * 128);
+      dma16(lds_a + (unsigned)(stage * kA + 1024 * i), min(8u * (kCopiesA * w + i) + (lane >> 3), last) * k2 + chunk, ap + (size_t)kt * 128);
   };
-  // the words of group g of the tile in a stage as codes8 takes them, and the scales
+  // Packed words of piece u (blocks 4 u .. + 3). 4 bits: four lanes a column, block b of column f in slot b ^ (f / 4 % 4) of the
+  // column's four, so that reads of 32 columns fall in distinct banks; else word by word
+  auto copy_w = [&](int u, int stage) {
+    u = min(u, (nkt - 1) / 2);
+    const unsigned to = lds_w + (unsigned)(stage * kW);
+    const int blocks = min(4, nblk - 4 * u);  // (the last piece may have two)
+#pragma unroll
+    for (int i = 0; i < kCopiesW; i++) {
+      if constexpr (BITS == 4) {
+        const int f0 = 16 * (i & 1) + (lane >> 2), c = i >> 1;
+        const unsigned blk = min((lane & 3) ^ ((f0 >> 2) & 3), blocks - 1);
+        dma16(to + 1024 * i, (unsigned)min(f0, left[c]) * (unsigned)nblk * 16u + 16u * blk, wp[c] + (size_t)u * 64);
+      } else {
+        constexpr int kWords = 4 * BITS, kEach = 32 * kWords / 64;  // a column's words; instructions of a column tile
+        const int x = 64 * (i % kEach) + lane, f0 = x / kWords, c = i / kEach;
+        dma4(to + 256 * i, ((unsigned)min(f0, left[c]) * (unsigned)nblk * BITS + min(x % kWords, blocks * BITS - 1)) * 4u, wp[c] + (size_t)u * (16 * BITS));
+      }
+    }
+  };
+  // Two of the 2 U instructions that bring U pieces' scales (groups of 64: 2 U pieces'), pairs of f16, column by column
+  auto copy_s = [&](int part, int piece, int stage) {
+    constexpr int kPairs = 2 * U;
+    part = min(part, (ng / 2 - 1) / kPairs);
+    const unsigned to = lds_s + (unsigned)(stage * kS * (ASYM ? 2 : 1)) + 256u * piece;
+    const int x = 64 * piece + lane, f0 = x / kPairs % 32;
+    const unsigned pair = min(x % kPairs, ng / 2 - 1 - part * kPairs);
+    const bool second = CT == 2 && x >= 32 * kPairs;
+    const unsigned at = (unsigned)min(f0, second ? left[CT - 1] : left[0]) * (unsigned)ng * 2u + 4u * pair;
+    const char* from = (second ? sp[CT - 1] : sp[0]) + (size_t)part * (4 * kPairs);
+    dma4_at(to, from + at);
+    if constexpr (ASYM) dma4_at(to + kS, (second ? bp[CT - 1] : bp[0]) + (size_t)part * (4 * kPairs) + at);
+  };
+  constexpr int kPieces = kCols * 2 * U / 64;  // instructions for U pieces' scales
+  const int per_part = g64 ? 2 * U : U;        // pieces u of a part
+  // the words of group g of tile kt = 2 u + q as codes8 takes them
   struct Words {
     unsigned lo[CT][2], hi[CT][2];
   };
-  const unsigned char* const own = sm + kA + (kW + kS) * w;
-  auto words = [&](int stage, int g) {
-    const unsigned char* from = own + stage * kStage;
+  const unsigned char* const own = sm + 2 * kA + L::kOwn * w;
+  auto words = [&](int stage, int block) {
+    const unsigned char* from = own + stage * kW;
     Words x;
 #pragma unroll
     for (int c = 0; c < CT; c++) {
       if constexpr (BITS == 4) {
-        const uint2 v = *(const uint2*)(from + 1024 * c + 16 * (32 * g + f) + 8 * h);  // k 16 h .. + 15 of the group
+        const uint2 v = *(const uint2*)(from + 64 * (32 * c + f) + 16 * (block ^ ((f >> 2) & 3)) + 8 * h);  // k 16 h .. + 15 of the group
         x.lo[c][0] = v.x, x.lo[c][1] = v.y, x.hi[c][0] = x.hi[c][1] = 0;
       } else {
-        const unsigned v = *(const unsigned*)(from + 256 * (c * BITS + h) + 4 * (32 * g + f));
-        const unsigned t = BITS == 3 ? *(const unsigned*)(from + 256 * (c * BITS + 2) + 4 * (32 * g + f)) >> (16 * h) : 0u;
+        const unsigned char* at = from + 4 * (4 * BITS * (32 * c + f) + BITS * block);
+        const unsigned v = *(const unsigned*)(at + 4 * h), t = BITS == 3 ? *(const unsigned*)(at + 8) >> (16 * h) : 0u;
 #pragma unroll
         for (int j = 0; j < 2; j++) x.lo[c][j] = v >> (16 * j) & 0xFFFFu, x.hi[c][j] = t >> (8 * j) & 0xFFu;
       }
@@ -131,65 +164,73 @@ __global__ __launch_bounds__(64 * kTileWaves, RT * CT <= 2 ? 4 : RT * CT <= 4 &&
 #pragma unroll
     for (int j = 0; j < 2; j++) bf[c][j] = codes8<BITS>(x.lo[c][j], x.hi[c][j]);
   };
-  // Copies complete in order. At the top of tile kt this wave's copies of tile kt + 1 may still be in flight, those of tile kt have
-  // landed; behind the barrier everybody's have, and everybody has read tile kt - 1, whose stage takes tile kt + 2.
-  copy(0, 0);
-  copy(1, 1);
-  int stage = 0;
+  // Copies complete in order. At the top of tile 2 u those of a(2 u), words and scales of piece u have landed (nothing newer is in
+  // flight); at the top of 2 u + 1 those of a(2 u + 1), issued at the top of 2 u before the next piece's words and scales. Behind
+  // the barrier everybody's have, and everybody has read the tile before, whose stage takes the next one.
   Words x0;
-  for (int kt = 0; kt < nkt; kt++) {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kCopiesA + kCopiesW) : "memory");
+  auto tile = [&](auto parity, int kt, int ws, int ss) {
+    constexpr int q = decltype(parity)::value;
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(q ? kCopiesW + kCopiesS : 0) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    copy(kt + 2, stage == 0 ? 2 : stage - 1);
-    const int next_stage = stage == kTileStages - 1 ? 0 : stage + 1;
-    const unsigned char* as = sm + stage * kStage + arow;
+    copy_a(kt + 1, q ^ 1);
+    if (q == 0) {
+      const int u = kt >> 1, in_part = u % per_part, part = u / per_part + 1;
+      copy_w(u + 1, ws ^ 1);
+      // (groups of 64 have twice the time: a piece of them twice; one column tile has half the pieces: each twice)
+      const int piece = g64 ? in_part : 2 * in_part;
+      copy_s(part, piece % kPieces, ss ^ 1);
+      copy_s(part, (g64 ? piece : piece + 1) % kPieces, ss ^ 1);
+    }
+    const unsigned char* as = sm + q * kA + arow;
     auto operand = [&](int g, int i, int j) { return *(const h8*)(as + 32 * 128 * i + 16 * ((4 * g + 2 * h + j) ^ (f & 7))); };
     af[0][0] = operand(0, 0, 0);
     af[0][1] = operand(0, 0, 1);
-    if (kt == 0) {
+    if (q == 0 && kt == 0) {
       x0 = words(0, 0);
       decode(x0, 0);
     }
     unsigned sw[CT], bw[CT];
+    const int pair = g64 ? (kt >> 1) % (2 * U) : kt % (2 * U);
 #pragma unroll
     for (int c = 0; c < CT; c++) {
-      sw[c] = *(const unsigned*)(own + stage * kStage + kW + 4 * (32 * c + f));
-      bw[c] = ASYM ? *(const unsigned*)(own + stage * kStage + kW + 256 + 4 * (32 * c + f)) : 0u;
+      const unsigned char* at = own + 2 * kW + ss * kS * (ASYM ? 2 : 1) + 8 * U * (32 * c + f) + 4 * pair;
+      sw[c] = *(const unsigned*)at;
+      bw[c] = ASYM ? *(const unsigned*)(at + kS) : 0u;
     }
     Words x1;
     // The pairs of both groups in turn: a pair's two products go with the fma of the pair before (of a tile's first, with those of
     // the last tile's last), with the next row tile's reads and the next group's decoding
 #pragma unroll
     for (int t = 0; t < 2 * kPairs; t++) {
-      const int g = t / kPairs, i = t / CT % RT, c = t % CT, u = (t / CT) & 1;
+      const int c = t % CT, v = (t / CT) & 1;
       if constexpr (ASYM) {
         if (c == 0) {
-          sum[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[u][0], ones8(), f16v{}, 0, 0, 0);
-          sum[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[u][1], ones8(), sum[u], 0, 0, 0);
+          sum[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[v][0], ones8(), f16v{}, 0, 0, 0);
+          sum[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[v][1], ones8(), sum[v], 0, 0, 0);
         }
       }
-      d[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[u][0], bf[c][0], f16v{}, 0, 0, 0);
+      d[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[v][0], bf[c][0], f16v{}, 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
       if (c == 0 && t + CT < 2 * kPairs) {
-        af[u ^ 1][0] = operand((t + CT) / kPairs, (t + CT) / CT % RT, 0);
-        af[u ^ 1][1] = operand((t + CT) / kPairs, (t + CT) / CT % RT, 1);
+        af[v ^ 1][0] = operand((t + CT) / kPairs, (t + CT) / CT % RT, 0);
+        af[v ^ 1][1] = operand((t + CT) / kPairs, (t + CT) / CT % RT, 1);
       }
-      if (t == CT - 1) x1 = words(stage, 1);
+      if (t == CT - 1) x1 = words(ws, 2 * q + 1);
       add(t == 0 ? 2 * kPairs - 1 : t - 1, 0);
       __builtin_amdgcn_sched_barrier(0);
-      d[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[u][1], bf[c][1], d[t & 1], 0, 0, 0);
+      d[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[v][1], bf[c][1], d[t & 1], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
       add(t == 0 ? 2 * kPairs - 1 : t - 1, 8);
       if (t == 0) {  // (the last tile's scales are done with)
         if constexpr (CT == 2) decode(x0, 1);
 #pragma unroll
         for (int n = 0; n < CT; n++) {
-          const unsigned sv = g64 ? sw[n] >> (16 * (kt & 1)) : sw[n], bv = g64 ? bw[n] >> (16 * (kt & 1)) : bw[n];
+          const unsigned sv = g64 ? sw[n] >> (16 * q) : sw[n], bv = g64 ? bw[n] >> (16 * q) : bw[n];
 #pragma unroll
-          for (int q = 0; q < 2; q++) {
-            s[q][n] = f16_bits(g64 ? sv : sv >> (16 * q));
-            if constexpr (ASYM) b[q][n] = centred<BITS>(s[q][n], f16_bits(g64 ? bv : bv >> (16 * q)));
+          for (int e = 0; e < 2; e++) {
+            s[e][n] = f16_bits(g64 ? sv : sv >> (16 * e));
+            if constexpr (ASYM) b[e][n] = centred<BITS>(s[e][n], f16_bits(g64 ? bv : bv >> (16 * e)));
           }
         }
       }
@@ -197,15 +238,26 @@ __global__ __launch_bounds__(64 * kTileWaves, RT * CT <= 2 ? 4 : RT * CT <= 4 &&
       if constexpr (CT == 2) {
         if (t == kPairs) decode(x1, 1);
       }
-      if (t == 2 * kPairs - CT - 1) {  // the next tile's first words (its copies into this wave's part have landed)
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * kCopiesA + kCopiesW) : "memory");
-        x0 = words(next_stage, 0);
+      if (t == 2 * kPairs - CT - 1) {  // the next tile's first words: of this piece, or of the next, whose copies have landed
+        if (q) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kCopiesA) : "memory");
+        x0 = words(q ? ws ^ 1 : ws, q ? 0 : 2);
       }
       if (t == 2 * kPairs - 1) decode(x0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
-    stage = next_stage;
+  };
+  for (int i = 0; i < kPieces; i++) copy_s(0, i, 0);
+  copy_w(0, 0);
+  copy_a(0, 0);
+  int ws = 0, ss = 0;
+  int kt = 0;
+  for (; kt + 2 <= nkt; kt += 2) {
+    tile(std::integral_constant<int, 0>{}, kt, ws, ss);
+    tile(std::integral_constant<int, 1>{}, kt + 1, ws, ss);
+    ws ^= 1;
+    if ((kt / 2 + 1) % per_part == 0) ss ^= 1;
   }
+  if (kt < nkt) tile(std::integral_constant<int, 0>{}, kt, ws, ss);
   add(2 * kPairs - 1, 0);
   add(2 * kPairs - 1, 8);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies past the end land before the LDS is given up
