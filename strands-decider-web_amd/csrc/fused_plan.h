@@ -25,18 +25,22 @@ inline long groups(const Shape& p, int rows, int weights) {
   return (long)((p.cols + wide - 1) / wide) * ((p.M + rows - 1) / rows);
 }
 
-// The rows kernel: rounds of 256 workgroups, each of which takes as long as the rows of a and columns of W that it reads. Measured,
-// us, 4 bits, K = 2048 unless said (cost: rounds x (a + b + 2)): 61 x 5120 4 x 2 7.6 (8), 512 x 5120 4 x 2 27 (40), 2048 x 2048
-// 4 x 2 41 (64), 512 x 2048 x 6144 4 x 4 27 (10), 2048 x 2048 x 6144 4 x 4 97 (40), 61 x 2048 x 6144 1 x 2 9.0 (5).
+// Both fitted to 1 to 2048 rows of 2048 to 12288 columns at K = 2048 and 6144 (4 bits, groups of 32; r.m.s. error 9 and 6 %); what
+// they choose is 2 % slower than the best of all shapes on the mean of those, 16 % at most. n: workgroups on the busiest of 256 CUs.
+// The rows kernel: a workgroup's time grows with the rows of a and columns of W that it reads. Shapes of 12 tiles and more run one
+// to a CU. us, a x b: 1 row, gated 12288 x 2048 1 x 3 6.9, 1 x 4 7.5; 61 rows 4 x 3 10.6, 4 x 4 11.1, 2 x 4 12.6; 256 rows, 2048
+// x 2048 4 x 2 7.8, 2 x 4 8.6; 512 rows, 2048 x 6144 4 x 4 26, 4 x 2 29.
 inline float rows_us(const Shape& p, int a, int b) {
-  const float x = p.K / 2048.0f;
-  return 2.0f + (float)((groups(p, 16 * a, 16 * b) + 255) / 256) * (a + b + 2) * (0.1f + 0.5f * x + 0.08f * x * x);
+  const float x = p.K / 2048.0f, n = (float)((groups(p, 16 * a, 16 * b) + 255) / 256);
+  const float each = x * (0.19f + 0.48f * a + 0.60f * b + 0.15f * a * b) - 0.25f;
+  return std::max(2.0f, 3.9f - 0.4f * x + (1.0f + (n - 1.0f) * (a * b >= 12 ? 1.5f : 1.0f)) * each);
 }
-// The tile kernel: a workgroup takes b_us of a CU's time, and one alone a_us more. Measured, us, 4 bits, K = 2048, for n workgroups
-// on the busiest CU: 4 x 2 n = 1 50, 2 71, 3 106; 2 x 2 31, 45, 70, n = 6 128; 4 x 1 30, 45, 67; 2 x 1 19, 33, 43, n = 5 67.
+// The tile kernel. us: 512 rows, gated 12288 x 2048 2 x 2 43.5, 4 x 2 43.7 (rows kernel 54); 2048 rows 119, 100; 1024 rows, 2048 x
+// 2048 2 x 1 21, 4 x 1 31, 2 x 2 32 (rows kernel 22); 2048 rows, 2048 x 6144 2 x 1 76, 4 x 1 76, 2 x 2 82, 4 x 2 121.
 inline float tiles_us(const Shape& p, int a, int b) {
-  const float alone = a * b == 8 ? 15.0f : a * b == 2 ? 6.0f : 9.0f, each = a * b == 8 ? 32.0f : a * b == 2 ? 12.5f : 20.5f;
-  return p.K / 2048.0f * (alone + each * (float)((groups(p, 32 * a, 128 * b) + 255) / 256)) * (p.asym ? 1.5f : 1.0f);
+  const float n = (float)((groups(p, 32 * a, 128 * b) + 255) / 256), x = p.K / 2048.0f * (p.asym ? 1.5f : 1.0f);
+  if (a == 4) return 7.9f + x * (b == 2 ? 14.3f + 25.2f * n : 4.8f + 17.1f * n);
+  return 7.9f + x * (b == 2 ? 6.8f + 16.8f * n : 3.7f + 9.3f * n);
 }
 
 inline Plan plan(const Shape& p) {
@@ -46,8 +50,7 @@ inline Plan plan(const Shape& p) {
     if (us < best.us) best = {path, a, b, us};
   };
   for (int a : {1, 2, 4})
-    for (int b : {1, 2, 4})
-      if (!p.gated || b > 1) look(kRows, a, b, rows_us(p, a, b));  // (gated: tiles of both halves)
+    for (int b : {1, 2, 3, 4}) look(kRows, a, b, rows_us(p, a, b));
   for (int a : {2, 4})
     for (int b : {1, 2})
       if ((!p.gated || b == 2) && !(p.asym && a * b == 8)) look(kTiles, a, b, tiles_us(p, a, b));  // (asymmetric 4 x 2: too many registers)

@@ -1,7 +1,6 @@
 // Products of few rows for fused.hip, gfx950: a workgroup's waves split K and meet once, at the end.
 //
-// A workgroup makes 16 MT rows x 16 NT columns (gated: NT / 2 tiles of the gate and the NT / 2 of the up projection that they
-// multiply). Its waves take the 128-k pieces w, w + SW, ... of K in 64-k halves: each copies rows of a, codes and scales of a half
+// A workgroup makes 16 MT rows x 16 NT columns (gated: 8 NT of the gate and the 8 NT of the up projection that they multiply). Its waves take the 128-k pieces w, w + SW, ... of K in 64-k halves: each copies rows of a, codes and scales of a half
 // into LDS of its own by DMA and waits for its own copies only, so there is no barrier in the loop; it reads a half into registers,
 // starts the next half's copies into the same place and multiplies. Rows of a go through LDS because lanes hold different rows: a
 // 16-byte load straight into the operands is a cache line a lane. The order of a row's sums depends on K and SW alone.
@@ -69,7 +68,8 @@ __global__ __launch_bounds__(64 * SW) void fused_rows_kernel(FusedArgs p) {
   auto issue = [&](int t) {
     const int h = half_of(t);
 #pragma unroll
-    for (int i = 0; i < 2 * MT; i++) dma16(lds + 1024 * i, ao[i], ap + (size_t)h * 128);
+    for (int i = 0; i < 2 * MT; i++)
+      if (m0 + 8 * i < p.M) dma16(lds + 1024 * i, ao[i], ap + (size_t)h * 128);  // (rows that are not there may be anything)
 #pragma unroll
     for (int i = 0; i < kUnits; i++) {
       if (64 * i + lane < kLanes) {
@@ -154,18 +154,20 @@ __global__ __launch_bounds__(64 * SW) void fused_rows_kernel(FusedArgs p) {
     for (int q = 0; q < MT * NT; q++) red[(w * MT * NT + q) * 64 + lane] += acc[q / NT][q % NT];
   }
   __syncthreads();
-  auto total = [&](int q) {
-    f4 s = red[q * 64 + lane];
+  // a row tile's sums of the workgroup's column `col`, rows 4 g ..
+  auto total = [&](int i, int col) {
+    const f4* from = red + (i * NT + col / 16) * 64 + 16 * g + col % 16;
+    f4 s = from[0];
 #pragma unroll
-    for (int v = 1; v < SW / 2; v++) s += red[(v * MT * NT + q) * 64 + lane];
+    for (int v = 1; v < SW / 2; v++) s += from[v * MT * NT * 64];
     return s;
   };
-  const int per = gated ? NT / 2 : NT;  // column tiles of the result
+  const int per = (wide + 15) / 16;  // 16-column pieces of the result
   for (int q = w; q < MT * per; q += SW) {
-    const int i = q / per, n = q % per, j = j0 + 16 * n + c;
-    const f4 z = total(i * NT + n), up = gated ? total(i * NT + n + per) : f4{};
-    const int m = m0 + 16 * i + 4 * g;
-    if (m < p.M) results<4>(p, m, j, cols, [](int v) { return v; }, (const float*)&z, gated ? (const float*)&up : nullptr);
+    const int i = q / per, col = 16 * (q % per) + c, m = m0 + 16 * i + 4 * g;
+    if (col >= wide || m >= p.M) continue;
+    const f4 z = total(i, col), up = gated ? total(i, wide + col) : f4{};
+    results<4>(p, m, j0 + col, cols, [](int v) { return v; }, (const float*)&z, gated ? (const float*)&up : nullptr);
   }
 }
 

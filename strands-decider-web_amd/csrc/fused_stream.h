@@ -1,13 +1,16 @@
-// Records of the logits of up to 16 rows for fused.hip, gfx950: the table passes once through the registers of waves that share
-// nothing but the rows of a.
+// Records of the logits of up to 16 rows for fused.hip, gfx950: the table passes once, straight into the registers of waves that
+// share nothing but the rows of a.
 //
-// A wave makes a 64-column block of all rows. It loads 256 k of each column straight into registers: lane (g = l / 16, c = l % 16)
-// the packed blocks 2 g and 2 g + 1 of column 16 t + c, so that four lanes read a 128-byte line of a column, and turns them by swaps
-// of lane groups into the operands of v_mfma_f32_16x16x32_f16, of which lane (g, c) holds k 8 g .. + 7 of one 32-k group of column
-// c: a 4 x 4 transposition of (lane group, word). a stands in LDS, 16-byte chunk j of row r in slot j ^ (r & 15) of its 16.
+// A wave makes a 64-column block, all of K, 256 k of 16 columns at a time: lane (g = l / 16, c = l % 16) loads the packed blocks 2 g and 2 g + 1 of column c, so
+// that four lanes read whole 128-byte lines, and swaps of lane groups turn them into the operands of v_mfma_f32_16x16x32_f16, of
+// which lane (g, c) holds k 8 g .. + 7 of one 32-k group of column c: a 4 x 4 transposition of (lane group, word).
 //
-// Bound: the table's bytes. The vector unit's share (12 instructions for 8 codes, a swap a word, four fma a group) is about half of
-// the time that they take.
+// a stands in LDS, 16-byte chunk j of row r in slot j ^ (r & 15) of its 16.
+//
+// Bound: the table's bytes: 74 us for one row over 248320 tokens of 2048, 3.9 TB/s (with cur and next parts in registers of their
+// own, two waves a SIMD in place of four: 99). The vector unit's share (12 instructions for 8 codes, a swap a word, four fma a
+// group) is about half of that. Products of up to 16 rows, with K split over the waves of a workgroup, gained nothing on the rows
+// kernel this way (1 x 12288 x 2048 7.5 : 7.4 us, 8 rows 8.3 : 7.2).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -31,6 +34,83 @@ __device__ __forceinline__ void transpose4(unsigned* r) {
   r[3] = (unsigned)y[1];
 }
 
+// A lane's share of 256 k of a column.
+template <int BITS, bool ASYM>
+struct Part {
+  unsigned wd[2 * BITS];           // two packed blocks
+  unsigned s[4], b[ASYM ? 4 : 1];  // eight groups' f16, with groups of 64 four
+};
+
+// q, s and b: where 256-k piece 0 of the lane's column starts (q: at the lane's blocks)
+template <int BITS, bool ASYM, bool G64>
+__device__ __forceinline__ void load_part(const char* q, unsigned qo, const char* s, const char* b, unsigned so, int u, Part<BITS, ASYM>& x) {
+  typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef unsigned u2 __attribute__((ext_vector_type(2), aligned(4)));
+  const gptr<char> from = gp<char>(q + (size_t)u * (32 * BITS)) + qo;
+#pragma unroll
+  for (int i = 0; i < 2 * BITS; i += 4) {
+    if (2 * BITS - i >= 4) {
+      const u4 v = *(gptr<u4>)(from + 4 * i);
+      x.wd[i] = v[0], x.wd[i + 1] = v[1], x.wd[i + 2] = v[2], x.wd[i + 3] = v[3];
+    } else {
+      const u2 v = *(gptr<u2>)(from + 4 * i);
+      x.wd[i] = v[0], x.wd[i + 1] = v[1];
+    }
+  }
+  auto eight = [&](const char* table, unsigned* to) {
+    if constexpr (G64) {
+      const u2 v = *(gptr<u2>)(gp<char>(table + (size_t)u * 8) + so);
+      to[0] = v[0], to[1] = v[1], to[2] = to[3] = 0;
+    } else {
+      const u4 v = *(gptr<u4>)(gp<char>(table + (size_t)u * 16) + so);
+      to[0] = v[0], to[1] = v[1], to[2] = v[2], to[3] = v[3];
+    }
+  };
+  eight(s, x.s);
+  if constexpr (ASYM) eight(b, x.b);
+}
+
+// acc += the part's products. operand(b): the lane's k of group b of the 256 k; sum[b]: their sums over k (asymmetric).
+template <int BITS, bool ASYM, bool G64, class Operand>
+__device__ __forceinline__ void add_part(const Part<BITS, ASYM>& y, int g, Operand operand, const f4* sum, f4& acc) {
+#pragma unroll
+  for (int e = 0; e < 2; e++) {  // groups 2 b + e
+    // (operands of a are read again for each column tile: kept, they would cost a wave of four on a SIMD)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    unsigned r[4], hi[4] = {0, 0, 0, 0};
+    const unsigned* wd = y.wd + e * BITS;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = BITS == 4 ? wd[i] : wd[i >> 1];
+    transpose4(r);
+    if constexpr (BITS == 3) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) hi[i] = wd[2];
+      transpose4(hi);
+    }
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+      const unsigned lo = BITS == 4 ? r[b] : r[b] >> (16 * (g & 1)) & 0xFFFFu;
+      const f4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(2 * b + e), codes8<BITS>(lo, hi[b] >> (8 * g) & 0xFFu), f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+      const float s = f16_bits(G64 ? y.s[b >> 1] >> (16 * (b & 1)) : y.s[b] >> (16 * e));
+#pragma unroll
+      for (int i = 0; i < 4; i++) acc[i] = fmaf(s, d[i], acc[i]);
+      if constexpr (ASYM) {
+        const float bias = centred<BITS>(s, f16_bits(G64 ? y.b[b >> 1] >> (16 * (b & 1)) : y.b[b] >> (16 * e)));
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[i] = fmaf(bias, sum[2 * b + e][i], acc[i]);
+      }
+    }
+  }
+}
+template <bool ASYM, class Operand>
+__device__ __forceinline__ void part_sums(Operand operand, f4* sum) {
+  if constexpr (ASYM) {
+#pragma unroll
+    for (int b = 0; b < 8; b++) sum[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(b), ones8(), f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+  }
+}
+
 template <int BITS, bool ASYM, bool G64>
 __global__ __launch_bounds__(64 * kStreamWaves, ASYM ? 2 : 4) void fused_stream_kernel(FusedArgs p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
@@ -38,10 +118,6 @@ __global__ __launch_bounds__(64 * kStreamWaves, ASYM ? 2 : 4) void fused_stream_
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), nb = (p.N + kLpBlock - 1) / kLpBlock;
   const int block = blockIdx.x * kStreamWaves + w, n0 = kLpBlock * min(block, nb - 1);
   const int nblk = p.K / 32, ng = p.K / p.group, chunks = p.K / kStreamK;
-  struct Part {
-    unsigned wd[2 * BITS];  // two packed blocks of a column
-    unsigned s[4], b[ASYM ? 4 : 1];  // eight groups' f16, with groups of 64 four
-  };
   // a wave's columns: 32 bits of lane offset from a scalar address on (columns past the last repeat it and do not count)
   unsigned wo[4], so[4];
 #pragma unroll
@@ -53,36 +129,10 @@ __global__ __launch_bounds__(64 * kStreamWaves, ASYM ? 2 : 4) void fused_stream_
   const char* wp = (const char*)p.q + (size_t)n0 * nblk * (4 * BITS);
   const char* sp = (const char*)p.s + (size_t)n0 * ng * 2;
   const char* bp = ASYM ? (const char*)p.b + (size_t)n0 * ng * 2 : sp;
-  typedef unsigned u4 __attribute__((ext_vector_type(4), aligned(4)));
-  typedef unsigned u2 __attribute__((ext_vector_type(2), aligned(4)));
-  auto load = [&](int u, int t, Part& x) {
-    u = min(u, chunks - 1);
-    const gptr<char> from = gp<char>(wp + (size_t)u * (32 * BITS)) + wo[t];
+  Part<BITS, ASYM> x[4];
+  auto load = [&](int u, int t) { load_part<BITS, ASYM, G64>(wp, wo[t], sp, bp, so[t], min(u, chunks - 1), x[t]); };
 #pragma unroll
-    for (int i = 0; i < 2 * BITS; i += 4) {
-      if (2 * BITS - i >= 4) {
-        const u4 v = *(gptr<u4>)(from + 4 * i);
-        x.wd[i] = v[0], x.wd[i + 1] = v[1], x.wd[i + 2] = v[2], x.wd[i + 3] = v[3];
-      } else {
-        const u2 v = *(gptr<u2>)(from + 4 * i);
-        x.wd[i] = v[0], x.wd[i + 1] = v[1];
-      }
-    }
-    auto eight = [&](const char* table, unsigned* to) {
-      if constexpr (G64) {
-        const u2 v = *(gptr<u2>)(gp<char>(table + (size_t)u * 8) + so[t]);
-        to[0] = v[0], to[1] = v[1], to[2] = to[3] = 0;
-      } else {
-        const u4 v = *(gptr<u4>)(gp<char>(table + (size_t)u * 16) + so[t]);
-        to[0] = v[0], to[1] = v[1], to[2] = v[2], to[3] = v[3];
-      }
-    };
-    eight(sp, x.s);
-    if constexpr (ASYM) eight(bp, x.b);
-  };
-  Part x[4];
-#pragma unroll
-  for (int t = 0; t < 4; t++) load(0, t, x[t]);
+  for (int t = 0; t < 4; t++) load(0, t);
   const int per = p.K / 8;  // 16-byte chunks of a row
   for (int i = tid; i < p.M * per; i += 64 * kStreamWaves) {
     const int r = i / per, j = i - r * per;
@@ -97,48 +147,17 @@ __global__ __launch_bounds__(64 * kStreamWaves, ASYM ? 2 : 4) void fused_stream_
   for (int t = 0; t < 4; t++) acc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
   for (int u = 0; u < chunks; u++) {
-    auto operand = [&](int b) {  // group b of the 256 k
+    auto operand = [&](int b) {
       const int j = 32 * u + 4 * b + g;
       return *(const h8*)(ar + 16 * ((j & ~15) | ((j ^ row) & 15)));
     };
     f4 sum[ASYM ? 8 : 1];
-    if constexpr (ASYM) {
-#pragma unroll
-      for (int b = 0; b < 8; b++) sum[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(b), ones8(), f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-    }
+    part_sums<ASYM>(operand, sum);
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      Part y = x[t];  // (and the next 256 k on their way into its place)
-      load(u + 1, t, x[t]);
-#pragma unroll
-      for (int e = 0; e < 2; e++) {  // groups 2 b + e
-        // (operands of a are read again for each column tile: kept, they would cost a wave of four on a SIMD)
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_sched_barrier(0);
-        unsigned r[4], hi[4] = {0, 0, 0, 0};
-        const unsigned* wd = y.wd + e * BITS;
-#pragma unroll
-        for (int i = 0; i < 4; i++) r[i] = BITS == 4 ? wd[i] : wd[i >> 1];
-        transpose4(r);
-        if constexpr (BITS == 3) {
-#pragma unroll
-          for (int i = 0; i < 4; i++) hi[i] = wd[2];
-          transpose4(hi);
-        }
-#pragma unroll
-        for (int b = 0; b < 4; b++) {
-          const unsigned lo = BITS == 4 ? r[b] : r[b] >> (16 * (g & 1)) & 0xFFFFu;
-          const f4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(2 * b + e), codes8<BITS>(lo, hi[b] >> (8 * g) & 0xFFu), f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-          const float s = f16_bits(G64 ? y.s[b >> 1] >> (16 * (b & 1)) : y.s[b] >> (16 * e));
-#pragma unroll
-          for (int i = 0; i < 4; i++) acc[t][i] = fmaf(s, d[i], acc[t][i]);
-          if constexpr (ASYM) {
-            const float bias = centred<BITS>(s, f16_bits(G64 ? y.b[b >> 1] >> (16 * (b & 1)) : y.b[b] >> (16 * e)));
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[t][i] = fmaf(bias, sum[2 * b + e][i], acc[t][i]);
-          }
-        }
-      }
+      const Part<BITS, ASYM> y = x[t];  // (and the next 256 k on their way into its place)
+      load(u + 1, t);
+      add_part<BITS, ASYM, G64>(y, g, operand, sum, acc[t]);
     }
   }
 #pragma unroll
@@ -151,7 +170,7 @@ __global__ __launch_bounds__(64 * kStreamWaves, ASYM ? 2 : 4) void fused_stream_
   }
 }
 
-// Whether the kernel can run a call: whole 256 k, rows that fit LDS.
+// Whether it can run a call: whole 256 k, rows that fit LDS.
 inline bool stream_takes(const FusedArgs& p) {
   return p.M <= kStreamRows && p.K % kStreamK == 0 && (size_t)p.M * p.K * 2 <= kStreamLds;
 }

@@ -1,0 +1,74 @@
+"""Which kernel and tiles a product with its bias, activation and residual gets (csrc/fused_plan.h, compiled by itself): only
+combinations that exist, for every size, and near the best of those measured."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+CSRC = os.path.join(ROOT, "strands-decider-web_amd", "csrc")
+
+CODE = r"""
+#include <cstdio>
+#include "fused_plan.h"
+using namespace ha::fused;
+int main() {
+  int M, cols, K, gated, asym, whole;
+  while (scanf("%d %d %d %d %d %d", &M, &cols, &K, &gated, &asym, &whole) == 6) {
+    const Plan p = plan({M, cols, K, gated != 0, asym != 0, whole != 0});
+    printf("%d %d %d %g\n", (int)p.path, p.a, p.b, p.us);
+  }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def plans(tmp_path_factory):
+    if not shutil.which("g++"):
+        pytest.skip("g++ is missing")
+    d = tmp_path_factory.mktemp("plan")
+    (d / "p.cpp").write_text(CODE)
+    r = subprocess.run(["g++", "-O1", "-std=c++17", "-I" + CSRC, str(d / "p.cpp"), "-o", str(d / "p")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+
+    def ask(shapes):
+        r = subprocess.run([str(d / "p")], input="\n".join(" ".join(map(str, s)) for s in shapes), capture_output=True, text=True)
+        return [tuple(float(x) if "." in x or "e" in x else int(x) for x in l.split()) for l in r.stdout.splitlines()]
+    return ask
+
+
+def test_only_kernels_that_exist(plans):
+    sizes = [(M, cols, K, g, a, 1) for M in (1, 2, 15, 16, 17, 31, 64, 65, 200, 513, 2048, 5000, 1 << 20)
+             for cols in (1, 7, 16, 100, 1000, 2048, 6144, 8256, 100000) for K in (64, 128, 2048, 6144, 16384) for g in (0, 1) for a in (0, 1)]
+    for s, (path, a, b, us) in zip(sizes, plans(sizes)):
+        assert path in (1, 2) and us > 0, s
+        if path == 1:
+            assert a in (1, 2, 4) and b in (1, 2, 3, 4), s
+        else:
+            assert (a, b) in ((2, 1), (2, 2), (4, 1), (4, 2)), s
+            assert not (s[3] and b == 1) and not (s[4] and (a, b) == (4, 2)), s
+    assert [p[0] for p in plans([(3, 100, 96, 0, 0, 0), (3000, 100, 2048, 1, 0, 0)])] == [0, 0]
+
+
+# us of some measured shapes: (M, columns of the result, K, gated): {(path, a, b): us}
+MEASURED = {
+    (1, 6144, 2048, 1): {(1, 1, 1): 6.9, (1, 1, 2): 7.0, (1, 1, 3): 6.9, (1, 1, 4): 7.5},
+    (61, 6144, 2048, 1): {(1, 4, 3): 10.6, (1, 4, 4): 11.1, (1, 2, 3): 11.5, (1, 2, 4): 12.6, (1, 4, 2): 12.3},
+    (512, 6144, 2048, 1): {(2, 2, 2): 43.5, (2, 4, 2): 43.7, (1, 2, 4): 53.9, (1, 4, 2): 54.8},
+    (2048, 6144, 2048, 1): {(2, 2, 2): 119.0, (2, 4, 2): 100.5},
+    (1, 2048, 6144, 0): {(1, 1, 1): 6.1, (1, 1, 2): 8.3, (1, 1, 3): 10.6},
+    (61, 2048, 6144, 0): {(1, 1, 2): 8.9, (1, 2, 1): 9.0, (1, 2, 2): 10.2, (1, 1, 1): 11.0},
+    (256, 2048, 2048, 0): {(1, 4, 2): 7.8, (1, 2, 4): 8.6, (1, 2, 2): 9.0, (1, 4, 1): 10.5},
+    (512, 2048, 6144, 0): {(1, 4, 4): 26.4, (1, 4, 2): 28.9, (1, 2, 4): 32.4, (2, 2, 1): 49.6},
+    (2048, 2048, 6144, 0): {(2, 2, 1): 75.7, (2, 4, 1): 76.3, (2, 2, 2): 82.1, (2, 4, 2): 121.4},
+    (2048, 5120, 2048, 0): {(2, 2, 1): 58.3, (2, 4, 1): 66.8, (2, 2, 2): 71.0, (2, 4, 2): 78.0},
+}
+
+
+def test_near_the_best_measured(plans):
+    got = plans([(M, c, K, g, 0, 1) for M, c, K, g in MEASURED])
+    for (shape, times), (path, a, b, us) in zip(MEASURED.items(), got):
+        t = times.get((path, a, b))
+        assert t is not None and t <= 1.12 * min(times.values()), (shape, path, a, b)
+        assert 0.7 < us / t < 1.4, (shape, us, t)
