@@ -45,6 +45,7 @@ struct FusedArgs {
 
 struct LpArgs {
   FusedArgs p;         // the product that the records are of
+  const float* logits; // [M][N] in the records' place, or nullptr
   int n_targets, top_k;
   const int* targets;  // [M][n_targets]
   float* logp;         // [M][n_targets]

@@ -12,16 +12,19 @@
 namespace ha {
 namespace {
 
-// Any operands (K a multiple of 32, a 16-byte and codes 4-byte aligned). A wave makes 16 rows x 4 tiles of 16 columns (gated:
-// two of the gate and the two of the up projection 32 columns on): v_mfma_f32_16x16x32_f16, lane (g = l / 16, c = l % 16) row c
-// of a and column c of a tile, k 8 g .. + 7 of a 32-k block; D: rows 4 g + e, column c. Operands come straight from memory.
+// Any operands (K a multiple of 32, a 16-byte and codes 4-byte aligned). A workgroup makes 16 rows x 4 tiles of 16 columns (gated:
+// two of the gate and the two of the up projection 32 columns on), its waves taking every kAnyWaves-th 32-k group:
+// v_mfma_f32_16x16x32_f16, lane (g = l / 16, c = l % 16) row c of a and column c of a tile, k 8 g .. + 7 of the group; D: rows
+// 4 g + e, column c. Operands come straight from memory, four groups a wave at a time (7 x 36 x 4000, 3 bits: 115 us with one
+// wave for all of K).
+constexpr int kAnyWaves = 8;
 template <int BITS, bool ASYM, int EPI>
-__global__ __launch_bounds__(256) void fused_any_kernel(FusedArgs p) {
+__global__ __launch_bounds__(64 * kAnyWaves) void fused_any_kernel(FusedArgs p) {
+  __shared__ f4 red[kAnyWaves][4][64];
   const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int cols = EPI == kEpiAct && p.half ? p.half : p.N, wide = EPI == kEpiAct && p.half ? 32 : 64;
-  const int ntn = (cols + wide - 1) / wide, groups = (ntn + 3) / 4;
-  const int tn = 4 * (blockIdx.x % groups) + (threadIdx.x >> 6), m0 = 16 * (blockIdx.x / groups), n0 = wide * tn;
-  if (tn >= ntn) return;
+  const int ntn = (cols + wide - 1) / wide, tn = blockIdx.x % ntn, m0 = 16 * (blockIdx.x / ntn), n0 = wide * tn;
   const int nblk = p.K / 32, ng = p.K / p.group, gl = p.group == 64 ? 1 : 0;
   gptr<h8> ap = (gptr<h8>)(gp<_Float16>(p.a) + (size_t)min(m0 + c, p.M - 1) * p.K + 8 * g);
   gptr<unsigned> wp[4];
@@ -36,8 +39,8 @@ __global__ __launch_bounds__(256) void fused_any_kernel(FusedArgs p) {
   f4 acc[4];
 #pragma unroll
   for (int t = 0; t < 4; t++) acc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 2
-  for (int k = 0; k < nblk; k++) {
+#pragma unroll 4
+  for (int k = w; k < nblk; k += kAnyWaves) {
     const h8 av = ap[4 * k];
     f4 sum{0.0f, 0.0f, 0.0f, 0.0f};
     if constexpr (ASYM) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, ones8(), sum, 0, 0, 0);
@@ -58,8 +61,20 @@ __global__ __launch_bounds__(256) void fused_any_kernel(FusedArgs p) {
       }
     }
   }
+#pragma unroll
+  for (int t = 0; t < 4; t++) red[w][t][lane] = acc[t];
+  __syncthreads();
+  auto total = [&](int t) {
+    f4 s = red[0][t][lane];
+#pragma unroll
+    for (int v = 1; v < kAnyWaves; v++) s += red[v][t][lane];
+    return s;
+  };
   const int m = m0 + 4 * g;
   if constexpr (EPI == kEpiLogits) {
+    if (w) return;
+#pragma unroll
+    for (int t = 0; t < 4; t++) acc[t] = total(t);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const float z[4] = {p.scale * acc[0][e], p.scale * acc[1][e], p.scale * acc[2][e], p.scale * acc[3][e]};
@@ -67,21 +82,18 @@ __global__ __launch_bounds__(256) void fused_any_kernel(FusedArgs p) {
       if (c == 0 && m + e < p.M) p.rec[(size_t)(m + e) * ntn + tn] = r;
     }
   } else {
-    if (m >= p.M) return;
-#pragma unroll
-    for (int t = 0; t < 4; t++) {
-      if (wide == 32 && t >= 2) break;
-      results<4>(p, m, n0 + 16 * t + c, cols, [](int v) { return v; }, (const float*)&acc[t], wide == 32 ? (const float*)&acc[t ^ 2] : nullptr);
-    }
+    if (m >= p.M || w >= wide / 16) return;
+    const f4 z = total(w), up = wide == 32 ? total(w ^ 2) : f4{};
+    results<4>(p, m, n0 + 16 * w + c, cols, [](int v) { return v; }, (const float*)&z, wide == 32 ? (const float*)&up : nullptr);
   }
 }
 
 template <int BITS, bool ASYM, int EPI>
 hipError_t launch_any_as(const FusedArgs& p, hipStream_t s) {
   const int cols = EPI == kEpiAct && p.half ? p.half : p.N, wide = EPI == kEpiAct && p.half ? 32 : 64;
-  const long groups = ((cols + wide - 1) / wide + 3) / 4, rows = (p.M + 15) / 16;
-  if (groups * rows > 0x7FFFFFFFl) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((fused_any_kernel<BITS, ASYM, EPI>), dim3((unsigned)(groups * rows)), dim3(256), 0, s, p);
+  const long tiles = (long)((cols + wide - 1) / wide) * ((p.M + 15) / 16);
+  if (tiles > 0x7FFFFFFFl) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((fused_any_kernel<BITS, ASYM, EPI>), dim3((unsigned)tiles), dim3(64 * kAnyWaves), 0, s, p);
   return hipGetLastError();
 }
 

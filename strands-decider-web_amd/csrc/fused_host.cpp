@@ -4,6 +4,7 @@
 #include <string>
 
 #include "fused.h"
+#include "fused_plan.h"
 #include "ha.h"
 #include "on_device.h"
 
@@ -47,7 +48,10 @@ int check_logprobs(const ha_logprobs* p, int N, int* n_vocab) {
   return HA_OK;
 }
 
-size_t record_bytes(int M, int n_vocab) { return (size_t)M * ((n_vocab + ha::kLpBlock - 1) / ha::kLpBlock) * sizeof(ha::LpRecord); }
+size_t workspace_bytes(int M, int n_vocab, int top_k) {
+  if (ha::fused::store_logits(M, n_vocab, top_k)) return (size_t)M * n_vocab * sizeof(float);
+  return (size_t)M * ((n_vocab + ha::kLpBlock - 1) / ha::kLpBlock) * sizeof(ha::LpRecord);
+}
 
 }  // namespace
 
@@ -93,7 +97,7 @@ int ha_mnb_logprobs_bytes(const ha_mnb* w, int M, const ha_logprobs* p, size_t* 
   if (!ha::mnb_weight(w, &g, &device)) return set_error(HA_ERR_HANDLE, "invalid MatMulNBits handle");
   if (M < 1 || M > 1 << 20) return bad("M must be in [1, 2^20]");
   if (int rc = check_logprobs(p, g.N, &n_vocab)) return rc;
-  *bytes = record_bytes(M, n_vocab);
+  *bytes = workspace_bytes(M, n_vocab, p->top_k);
   return HA_OK;
 }
 
@@ -108,17 +112,23 @@ int ha_mnb_logprobs(ha_mnb* w, int M, const void* a, const ha_logprobs* p, void*
   for (const void* q : {(const void*)p->targets, (const void*)p->logp, (const void*)p->entropy, (const void*)p->lse, (const void*)p->top_ids,
                         (const void*)p->top_logp})
     if (off(q, 4)) return bad("targets and outputs must be 4-byte aligned");
-  const size_t need = record_bytes(M, n_vocab);
+  const size_t need = workspace_bytes(M, n_vocab, p->top_k);
   if (!workspace || off(workspace, 16) || bytes < need) return bad("the workspace must be 16-byte aligned and have " + std::to_string(need) + " bytes");
   l.p.N = n_vocab;
   l.p.scale = p->scale > 0.0f ? p->scale : 1.0f;
-  l.p.rec = (ha::LpRecord*)workspace;
+  const bool stored = ha::fused::store_logits(M, n_vocab, p->top_k);
+  if (stored) {  // a product in f32
+    l.logits = (const float*)workspace;
+    l.p.out = workspace; l.p.out_f32 = 1; l.p.out_stride = n_vocab;
+  } else {
+    l.p.rec = (ha::LpRecord*)workspace;
+  }
   l.n_targets = p->n_targets; l.targets = p->targets; l.logp = p->logp;
   l.entropy = p->entropy; l.lse = p->lse;
   l.top_k = p->top_k; l.top_ids = p->top_ids; l.top_logp = p->top_logp;
   ha::OnDevice on(device);
   if (on.rc != hipSuccess) return hip_error("hipSetDevice", on.rc);
-  hipError_t he = ha::launch_logit_records(l.p, (hipStream_t)stream);
+  hipError_t he = stored ? ha::launch_fused(l.p, (hipStream_t)stream) : ha::launch_logit_records(l.p, (hipStream_t)stream);
   if (he == hipSuccess) he = ha::launch_logprobs(l, (hipStream_t)stream);
   return he == hipSuccess ? HA_OK : hip_error("log probabilities", he);
 }

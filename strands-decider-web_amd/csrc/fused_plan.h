@@ -25,22 +25,23 @@ inline long groups(const Shape& p, int rows, int weights) {
   return (long)((p.cols + wide - 1) / wide) * ((p.M + rows - 1) / rows);
 }
 
-// Both fitted to 1 to 2048 rows of 2048 to 12288 columns at K = 2048 and 6144 (4 bits, groups of 32; r.m.s. error 9 and 6 %); what
-// they choose is 2 % slower than the best of all shapes on the mean of those, 16 % at most. n: workgroups on the busiest of 256 CUs.
-// The rows kernel: a workgroup's time grows with the rows of a and columns of W that it reads. Shapes of 12 tiles and more run one
-// to a CU. us, a x b: 1 row, gated 12288 x 2048 1 x 3 6.9, 1 x 4 7.5; 61 rows 4 x 3 10.6, 4 x 4 11.1, 2 x 4 12.6; 256 rows, 2048
-// x 2048 4 x 2 7.8, 2 x 4 8.6; 512 rows, 2048 x 6144 4 x 4 26, 4 x 2 29.
+// Both fitted to 1 to 2048 rows of 2048 to 12288 columns at K = 192 to 6144 (4 bits, groups of 32; r.m.s. error 12 and 9 %); what
+// they choose is 3 % slower than the best of all shapes in the mean. n: workgroups on the busiest of 256 CUs.
+// The rows kernel: a workgroup's time grows with the rows of a and columns of W that it reads and the results that it writes. Shapes
+// of 12 tiles and more run one to a CU. us, a x b: 1 row, gated 12288 x 2048 1 x 3 6.9, 1 x 4 7.5; 61 rows 4 x 3 10.6, 4 x 4 11.1,
+// 2 x 4 12.6; 256 rows, 2048 x 2048 4 x 2 7.8, 2 x 4 8.6; 512 rows, 2048 x 6144 4 x 4 26, 4 x 2 29.
 inline float rows_us(const Shape& p, int a, int b) {
   const float x = p.K / 2048.0f, n = (float)((groups(p, 16 * a, 16 * b) + 255) / 256);
-  const float each = x * (0.19f + 0.48f * a + 0.60f * b + 0.15f * a * b) - 0.25f;
-  return std::max(2.0f, 3.9f - 0.4f * x + (1.0f + (n - 1.0f) * (a * b >= 12 ? 1.5f : 1.0f)) * each);
+  const float each = x * (0.51f * a + 0.73f * b - 0.2f) + 0.26f + 0.09f * a + 0.145f * a * b;
+  return 2.85f + 0.18f * x + (1.0f + (n - 1.0f) * (a * b >= 12 ? 1.34f : 0.87f)) * each;
 }
 // The tile kernel. us: 512 rows, gated 12288 x 2048 2 x 2 43.5, 4 x 2 43.7 (rows kernel 54); 2048 rows 119, 100; 1024 rows, 2048 x
-// 2048 2 x 1 21, 4 x 1 31, 2 x 2 32 (rows kernel 22); 2048 rows, 2048 x 6144 2 x 1 76, 4 x 1 76, 2 x 2 82, 4 x 2 121.
+// 2048 2 x 1 21, 4 x 1 31, 2 x 2 32 (rows kernel 22); 2048 rows, 2048 x 6144 2 x 1 76, 4 x 1 76, 2 x 2 82, 4 x 2 121; 512 rows,
+// 12288 x 192 2 x 1 12, 4 x 1 16 (rows kernel 26).
 inline float tiles_us(const Shape& p, int a, int b) {
   const float n = (float)((groups(p, 32 * a, 128 * b) + 255) / 256), x = p.K / 2048.0f * (p.asym ? 1.5f : 1.0f);
-  if (a == 4) return 7.9f + x * (b == 2 ? 14.3f + 25.2f * n : 4.8f + 17.1f * n);
-  return 7.9f + x * (b == 2 ? 6.8f + 16.8f * n : 3.7f + 9.3f * n);
+  const float k = a == 4 ? (b == 2 ? 21.8f + 12.5f * n : 10.3f + 11.4f * n) : (b == 2 ? 11.5f + 11.3f * n : 8.2f + 6.35f * n);
+  return 2.6f + x * k + 1.46f * a * b * n;
 }
 
 inline Plan plan(const Shape& p) {
@@ -55,6 +56,16 @@ inline Plan plan(const Shape& p) {
     for (int b : {1, 2})
       if ((!p.gated || b == 2) && !(p.asym && a * b == 8)) look(kTiles, a, b, tiles_us(p, a, b));  // (asymmetric 4 x 2: too many registers)
   return best;
+}
+
+// Whether log probabilities store the logits (f32) and read them back rather than leave records of 64 columns: in vocabularies up
+// to 32768 for few rows, where the records' kernels are few workgroups, and where more than one block in two rows would hold two
+// of the top_k largest, which costs 62 products in 64 bits each. Measured, us, records : stored: 1431 x 1383 x 256 top 20 1125 :
+// 51, 1 x 4284 x 640 (3 bits) top 32 178 : 25, 187 x 2507 x 4096 (3 bits) 114 : 35, 605 x 20658 x 192 top 20 108 : 106; the other
+// way, 2048 x 32768 x 2048 top 5 372, stored (top 30) 616; 1024 x 8192 x 2048 top 5 98, stored (top 12) 97.
+inline bool store_logits(int M, int n_vocab, int top_k) {
+  const int nb = (n_vocab + 63) / 64;
+  return nb <= 512 && (M <= 64 || top_k * top_k > nb || (long)((n_vocab + 255) / 256) * ((M + 127) / 128) < 256);
 }
 
 }  // namespace fused

@@ -3,13 +3,16 @@
 //
 // With M the row's largest logit and Z = sum e^(z - M): lse = M + log Z, log p(t) = z_t - lse, entropy = log Z - sum e^(z - M)
 // (z - M) / Z. Each block's record has its largest value apart from the sums over the others, so that a row with one near
-// certain token keeps the digits of what is left. Sums over blocks are in 64 bits.
+// certain token keeps the digits of what is left. Sums over threads are in 64 bits.
 //
 // The top_k largest logits stand in the top_k blocks of the largest maxima: a block further down has nothing that top_k others
 // do not exceed (with fewer blocks than that, all are looked at). Their largest columns, and every column of such a block whose second largest comes near the last of them, are
 // multiplied out again in 64 bits, and so are the given tokens: sums in f32 differ by 1e-6 of the logits, which is enough to
 // change the order of two tokens. kLpMargin more blocks are looked at, and blocks are taken by (largest value, first block), so
 // that equal logits come in order too. The 64-bit values of the blocks' largest columns also replace their f32 ones in Z.
+//
+// Smaller vocabularies, where two of the top_k often share a block, or whose blocks are too few workgroups, have their logits
+// stored in f32 by a product (fused.hip) and read here in the records' place (fused_plan.h says when).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -80,10 +83,11 @@ __device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double*
   for (int x = 0; x < 2; x++) out[x] = wave_sum(out[x]);
 }
 
-// A workgroup of T threads for a row. Dynamic LDS: list_cap keys, then cand_cap values and their columns.
-template <int BITS, bool ASYM, int T>
+// A workgroup of T threads for a row. Dynamic LDS: list_cap keys, then cand_cap values and their columns. STORED: the row's
+// logits themselves (unscaled, f32), each a block of its own.
+template <int BITS, bool ASYM, int T, bool STORED>
 __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_cap, int cand_cap) {
-  constexpr int kWaves = T / 64, kKeep = 4096 / T, kSets = kLpSets / 64;
+  constexpr int kWaves = T / 64, kKeep = STORED || T < 512 ? 0 : 4096 / T, kSets = kLpSets / 64;
   extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
   __shared__ u64 best[kLpSets];
   __shared__ u64 threshold;
@@ -95,10 +99,11 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
   int* ids = (int*)(val + cand_cap);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), m = blockIdx.x;
   const int n_vocab = a.p.N, k = a.top_k, kk = min(k + kLpMargin, nb), nt = a.n_targets;
-  const LpRecord* rec = a.p.rec + (size_t)m * nb;
+  const LpRecord* rec = STORED ? nullptr : a.p.rec + (size_t)m * nb;
+  const float* logits = STORED ? a.logits + (size_t)m * nb : nullptr;
   auto key_of = [](float max, int i) { return (u64)ordered(max) << 32 | (0xFFFFFFFFu - (unsigned)i); };
   // records tid, tid + T, ...: the first kKeep stay in registers
-  LpRecord keep[kKeep];
+  LpRecord keep[kKeep + 1];
 #pragma unroll
   for (int i = 0; i < kKeep; i++)
     if (tid + i * T < nb) keep[i] = rec[tid + i * T];
@@ -106,14 +111,19 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
 #pragma unroll
     for (int i = 0; i < kKeep; i++)
       if (tid + i * T < nb) f(keep[i], tid + i * T);
-    for (int i = tid + kKeep * T; i < nb; i += T) f(rec[i], i);
+    for (int i = tid + kKeep * T; i < nb; i += T) {
+      if constexpr (STORED) f(LpRecord{a.p.scale * logits[i], 0.0f, 0.0f, 0u}, i);
+      else f(rec[i], i);
+    }
   };
-  u64 mine = 0;
+  float most = kNoLogit;
+  int at = -1;
   bool bad = false;
   each([&](const LpRecord& r, int i) {
     bad |= !(fabsf(r.max) <= 3.4e38f && fabsf(r.rest) <= 3.4e38f && fabsf(r.rest_z) <= 3.4e38f);
-    mine = max(mine, key_of(r.max, i));
+    if (r.max > most) most = r.max, at = i;
   });
+  u64 mine = at < 0 ? 0 : key_of(most, at);
   // the largest key of every T / kLpSets threads (0: no block)
 #pragma unroll
   for (int d = 1; d < T / kLpSets; d *= 2) mine = max(mine, (u64)__shfl_xor((long long)mine, d));
@@ -149,17 +159,17 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
   __syncthreads();
   const u64 cut = threshold, top_key = best[0];
   const float M = unordered((unsigned)(top_key >> 32));
-  // sums over the blocks; the largest columns of those from the cut on wait
-  double z = 0.0, zx = 0.0;
+  // sums over the blocks, a thread's in f32; the largest columns of those from the cut on wait
+  const float cut_max = cut ? unordered((unsigned)(cut >> 32)) : kNoLogit;
+  float z32 = 0.0f, zx32 = 0.0f;
   each([&](const LpRecord& r, int i) {
-    const u64 key = key_of(r.max, i);
-    const double x = (double)r.max - (double)M, e = (double)__expf((float)x);
-    double rest = r.rest;
-    if (key >= cut) list[atomicAdd(&n_list, 1)] = key;
-    else rest += 1.0;
-    z += e * rest;
-    zx += e * ((double)r.rest_z + rest * x);
+    const float x = r.max - M, e = __expf(x);
+    float rest = r.rest + 1.0f;
+    if (r.max >= cut_max && key_of(r.max, i) >= cut) list[atomicAdd(&n_list, 1)] = key_of(r.max, i), rest = r.rest;
+    z32 = fmaf(e, rest, z32);
+    zx32 = fmaf(e, fmaf(rest, x, r.rest_z), zx32);
   });
+  double z = z32, zx = zx32;
   __syncthreads();
   const int nl = n_list;
   for (int i = tid; i < nl; i += T) {
@@ -179,7 +189,8 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
   if (lane == 0) red[0][w] = z, red[1][w] = zx;
   __syncthreads();
   // candidates: the chosen blocks' largest columns, and blocks whose second largest may be among the top_k
-  if (tid < kk) {
+  if (STORED && tid < kk) ids[tid] = chosen[tid];
+  if (!STORED && tid < kk) {
     const int i = chosen[tid];
     const LpRecord r = rec[i];
     const int arg = (int)(r.second & 63u);
@@ -239,13 +250,14 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
   }
 }
 
-template <int BITS, bool ASYM, int T>
+template <int BITS, bool ASYM, int T, bool STORED>
 hipError_t launch_as(const LpArgs& a, hipStream_t s) {
-  const int nb = (a.p.N + kLpBlock - 1) / kLpBlock, kk = std::min(a.top_k + kLpMargin, nb);
+  const int nb = STORED ? a.p.N : (a.p.N + kLpBlock - 1) / kLpBlock, kk = std::min(a.top_k + kLpMargin, nb);
   // the kk sets of T / kLpSets threads that hold a key from the cut on (where there are fewer sets, all of them)
-  const int list_cap = std::min(nb, kk * (T / kLpSets) * ((nb + T - 1) / T)), cand_cap = (a.top_k > 0 ? kk * kLpBlock : kk) + a.n_targets;
+  const int list_cap = std::min(nb, kk * (T / kLpSets) * ((nb + T - 1) / T));
+  const int cand_cap = (a.top_k > 0 && !STORED ? kk * kLpBlock : kk) + a.n_targets;
   const size_t lds = 8 * (size_t)list_cap + 12 * (size_t)cand_cap;
-  auto k = logprobs_kernel<BITS, ASYM, T>;
+  auto k = logprobs_kernel<BITS, ASYM, T, STORED>;
   if (lds > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
@@ -253,10 +265,17 @@ hipError_t launch_as(const LpArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(k, dim3(a.p.M), dim3(T), lds, s, a, nb, list_cap, cand_cap);
   return hipGetLastError();
 }
-// Few rows: 16 waves for each, more of its loads and products at once (one row over 248320 tokens, top 8: us).
+// Few rows: 16 waves for each, more of its loads and products at once (one row over 248320 tokens, top 8: 19 -> 12 us). Many: as
+// many rows on a CU as their blocks leave work for (2048 x 248320, 3880 blocks: 8 waves 75 us, 4 waves 92; 1431 rows of 1383 logits
+// 53 and 41).
+template <int BITS, bool ASYM, bool STORED>
+hipError_t launch_for(const LpArgs& a, hipStream_t s) {
+  if (a.p.M <= 256) return launch_as<BITS, ASYM, 1024, STORED>(a, s);
+  return a.p.N > (STORED ? 4096 : 4096 * kLpBlock / 2) ? launch_as<BITS, ASYM, 512, STORED>(a, s) : launch_as<BITS, ASYM, 256, STORED>(a, s);
+}
 template <int BITS, bool ASYM>
 hipError_t launch(const LpArgs& a, hipStream_t s) {
-  return a.p.M <= 256 ? launch_as<BITS, ASYM, 1024>(a, s) : launch_as<BITS, ASYM, 512>(a, s);
+  return a.logits ? launch_for<BITS, ASYM, true>(a, s) : launch_for<BITS, ASYM, false>(a, s);
 }
 
 }  // namespace

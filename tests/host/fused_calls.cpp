@@ -109,20 +109,20 @@ int main() {
   p.n_vocab = 90; p.n_targets = 2; p.targets = (int*)base; p.logp = (float*)out; p.entropy = (float*)(out + 64);
   p.top_k = 5; p.top_ids = (int*)(out + 128); p.top_logp = (float*)(out + 256);
   size_t bytes = 1;
-  CHECK(ha_mnb_logprobs_bytes(&good, 7, &p, &bytes) == HA_OK && bytes == 7 * 2 * 16);
+  CHECK(ha_mnb_logprobs_bytes(&good, 7, &p, &bytes) == HA_OK && bytes == 7 * 90 * 4);
   CHECK(ha_mnb_logprobs_bytes(nullptr, 7, &p, &bytes) == HA_ERR_HANDLE && bytes == 0);
   BAD(ha_mnb_logprobs_bytes(&good, 7, &p, nullptr), "bytes");
   BAD(ha_mnb_logprobs_bytes(&good, 0, &p, &bytes), "M must");
   BAD(ha_mnb_logprobs_bytes(&good, 7, nullptr, &bytes), "NULL");
   launches = 0;
-  CHECK(ha_mnb_logprobs(&good, 7, a, &p, res, 224, nullptr) == HA_OK && launches == 2 && launched_on == 1 && current == 0);
-  CHECK(got.N == 90 && got.scale == 1.0f && (char*)got.rec == res && got_lp.n_targets == 2 && got_lp.top_k == 5 && got_lp.p.N == 90 && !got_lp.lse);
-  CHECK(ha_mnb_logprobs(nullptr, 7, a, &p, res, 224, nullptr) == HA_ERR_HANDLE);
-  BAD(ha_mnb_logprobs(&good, 7, a, &p, res, 223, nullptr), "224 bytes");
-  BAD(ha_mnb_logprobs(&good, 7, a, &p, res + 8, 300, nullptr), "workspace");
-  BAD(ha_mnb_logprobs(&good, 7, a, &p, nullptr, 300, nullptr), "workspace");
-  BAD(ha_mnb_logprobs(&good, 7, a, nullptr, res, 300, nullptr), "NULL");
-  BAD(ha_mnb_logprobs(&good, 7, a + 2, &p, res, 300, nullptr), "a must");
+  CHECK(ha_mnb_logprobs(&good, 7, a, &p, res, 2520, nullptr) == HA_OK && launches == 2 && launched_on == 1 && current == 0);
+  CHECK(got.N == 90 && got.scale == 1.0f && got.out == res && got.out_f32 && got.out_stride == 90 && (char*)got_lp.logits == res && got_lp.n_targets == 2 && got_lp.top_k == 5 && got_lp.p.N == 90 && !got_lp.lse);
+  CHECK(ha_mnb_logprobs(nullptr, 7, a, &p, res, 2520, nullptr) == HA_ERR_HANDLE);
+  BAD(ha_mnb_logprobs(&good, 7, a, &p, res, 2519, nullptr), "2520 bytes");
+  BAD(ha_mnb_logprobs(&good, 7, a, &p, res + 8, 3000, nullptr), "workspace");
+  BAD(ha_mnb_logprobs(&good, 7, a, &p, nullptr, 3000, nullptr), "workspace");
+  BAD(ha_mnb_logprobs(&good, 7, a, nullptr, res, 3000, nullptr), "NULL");
+  BAD(ha_mnb_logprobs(&good, 7, a + 2, &p, res, 3000, nullptr), "a must");
 #define WITH(field, value, text) do { ha_logprobs b = p; b.field = value; BAD(ha_mnb_logprobs(&good, 7, a, &b, res, 1 << 20, nullptr), text); } while (0)
   WITH(n_vocab, 101, "n_vocab"); WITH(n_vocab, -1, "n_vocab");
   WITH(n_targets, -1, "n_targets"); WITH(n_targets, 1025, "n_targets");
@@ -134,10 +134,14 @@ int main() {
   { ha_logprobs b = {}; BAD(ha_mnb_logprobs(&good, 7, a, &b, res, 1 << 20, nullptr), "nothing"); }
   { ha_logprobs b = {}; b.lse = (float*)out; b.scale = 2.5f;
     CHECK(ha_mnb_logprobs(&good, 7, a, &b, res, 1 << 20, nullptr) == HA_OK && got.scale == 2.5f && got.N == 100); }
+  good.args.N = 40000;  // (a larger vocabulary: records)
+  { ha_logprobs b = p; b.n_vocab = 0;
+    CHECK(ha_mnb_logprobs_bytes(&good, 7, &b, &bytes) == HA_OK && bytes == 7 * 625 * 16);
+    CHECK(ha_mnb_logprobs(&good, 7, a, &b, res, bytes, nullptr) == HA_OK && (char*)got.rec == res && !got.out && !got_lp.logits); }
   good.args.N = (1 << 20) + 64;
   { ha_logprobs b = p; b.n_vocab = 0; BAD(ha_mnb_logprobs(&good, 7, a, &b, res, 1 << 30, nullptr), "2^20");
     b.n_vocab = 1 << 20; CHECK(ha_mnb_logprobs(&good, 7, a, &b, res, 1 << 30, nullptr) == HA_OK); }
   launch_result = hipErrorInvalidValue;
-  CHECK(ha_mnb_logprobs(&good, 7, a, &p, res, 224, nullptr) == HA_ERR_DEVICE && current == 0);
+  CHECK(ha_mnb_logprobs(&good, 7, a, &p, res, 2520, nullptr) == HA_ERR_DEVICE && current == 0);
   return 0;
 }
