@@ -258,7 +258,8 @@ typedef struct ha_epilogue {
 int ha_mnb_fused(ha_mnb* w, int M, const void* a, const ha_epilogue* e, void* out, void* stream);
 
 /* Log probabilities over a vocabulary, from the final norm's rows and the table (an embedding table, where model and vocabulary
-   share one): z[m][n] = scale a[m] . W[n] for n < n_vocab, p[m] = softmax(z[m]). The logits are not stored. */
+   share one): z[m][n] = scale a[m] . W[n] for n < n_vocab, p[m] = softmax(z[m]). Of larger vocabularies no logit is stored: the workspace
+   holds a few numbers for each 64 of them; where that is less work it holds the f32 logits of a smaller one. */
 typedef struct ha_logprobs {
   int n_vocab;         /* the table's first n_vocab rows are tokens, up to 2^20 (0: all N; rows behind them are padding) */
   float scale;         /* of the logits, one over the temperature, up to 1e6 (0: 1) */

@@ -610,14 +610,19 @@ class Torso:
 
     set_weight(name, MnbWeight) for the quantised tensors ("embed", "layers.<i>.in_proj" | "qkv" | "out_proj" |
     "o_proj" | "gate_up" | "down" | "proj"); set_param(name, f32 array) for "final_norm", "layers.<i>.in_norm" |
-    "post_norm" | "bias" and the mixers' "conv" | "neg_exp_A" | "dt_bias" | "gnorm" | "q_norm" | "k_norm"."""
+    "post_norm" | "bias" and the mixers' "conv" | "neg_exp_A" | "dt_bias" | "gnorm" | "q_norm" | "k_norm".
+
+    fused: out_proj, o_proj, down and an adapter's proj add onto the f32 residual stream themselves, and gate_up gives
+    SILU_MUL's rows (ha_mnb_fused): fewer launches, and the sums between are not rounded to f16. Its results differ from the
+    default's within those roundings."""
 
     _MIXER = ("conv", "neg_exp_A", "dt_bias", "gnorm", "q_norm", "k_norm")
 
-    def __init__(self, layer_types, D=2048, I=6144, max_ctx=4096, device=0):
+    def __init__(self, layer_types, D=2048, I=6144, max_ctx=4096, device=0, fused=False):
         import torch
         self.torch = torch
         self.types, self.D, self.I, self.device = list(layer_types), D, I, device
+        self.fused = bool(fused)
         self.dev = "cuda:%d" % device
         self.stream = torch.cuda.Stream(device=self.dev)
         self.st = self.stream.cuda_stream
@@ -657,10 +662,47 @@ class Torso:
         (engine.js:313-376) go to self.diag: "gpu_ms" (timestamps: GPU time from the embedding to the final norm) and
         "layers" (debug_layers: the residual stream x entering each layer i >= 1, f32 [L][D], read back between the
         layers)."""
+        out, snaps = self._run(ids, list(range(len(ids))) if rows is None else list(rows), cache, keep, timestamps, debug_layers)
+        return out.cpu().numpy(), snaps
+
+    def score(self, ids, rows=None, targets=None, top_k=0, n_vocab=0, scale=0.0, table="embed", cache=None, keep=False,
+              timestamps=False):
+        """The distributions of the tokens that follow the rows (indices into ids; default all) over a vocabulary table: the
+        weight ``table``, the embedding's where the model ties them. ids, cache, keep and timestamps as forward; n_vocab and
+        scale as :class:`LogProbs`. ``targets``: integers [len(rows)][T], whose log probabilities are asked for. Returns ({"logp"
+        [rows][T], "entropy" [rows], "lse" [rows], "top_ids" [rows][top_k], "top_logp"} on the host, snapshots when keep)."""
+        import numpy as np
+        rows = list(range(len(ids))) if rows is None else list(rows)
+        M, w = len(rows), self.w[table]
+        if w.K != self.D:
+            raise ValueError("%s has rows of %d values, the hidden state %d" % (table, w.K, self.D))
+        if targets is not None:
+            t = np.asarray(targets)
+            if t.ndim != 2 or t.shape[0] != M or t.size and t.dtype.kind not in "iu":
+                raise ValueError("targets must be integers [rows][T]")
+            if t.size and (t.min() < -2 ** 31 or t.max() >= 2 ** 31):
+                raise ValueError("targets must fit 32 bits")
+            targets = np.ascontiguousarray(t, np.int32)
+        return self._run(ids, rows, cache, keep, timestamps, False, (w, targets, top_k, n_vocab, scale))
+
+    def _score(self, M, h, ask):
+        """Log probabilities of M rows h (f16) on this torso's stream; nothing is read back yet."""
+        torch, (w, targets, top_k, n_vocab, scale) = self.torch, ask
+        T = 0 if targets is None else targets.shape[1]
+        new = lambda n, dtype=torch.float32: torch.empty(M, n, dtype=dtype, device=self.dev)  # noqa: E731
+        out = {"logp": new(T), "entropy": new(1)[:, 0], "lse": new(1)[:, 0], "top_ids": new(top_k, torch.int32),
+               "top_logp": new(top_k)}
+        if M:
+            t = torch.from_numpy(targets).to(self.dev) if T else None
+            p = LogProbs(n_vocab, scale, t, T, top_k, **{k: x if x.numel() else None for k, x in out.items()})
+            work = torch.empty(w.logprobs_bytes(M, p), dtype=torch.uint8, device=self.dev)
+            self._step("logprobs", lambda: w.logprobs(M, h, p, work, stream=self.st))
+        return out
+
+    def _run(self, ids, rows, cache, keep, timestamps, debug_layers, ask=None):
         import numpy as np
         torch, D, I, st = self.torch, self.D, self.I, self.st
         L = len(ids)
-        rows = list(range(L)) if rows is None else list(rows)
         f16, f32 = torch.float16, torch.float32
         maxN = max([2 * I] + [w.N for w in self.w.values()])
         step = self._step
@@ -676,38 +718,50 @@ class Torso:
             y = torch.empty(L, D, dtype=f16, device=self.dev)
             mid = torch.empty(L, I, dtype=f16, device=self.dev)
             rd = torch.as_tensor(np.asarray(rows or [0], np.uint32).view(np.int32)).to(self.dev)
-            out = torch.empty(len(rows), D, dtype=f32, device=self.dev)
+            out = torch.empty(len(rows), D, dtype=f16 if ask else f32, device=self.dev)
+            add = Epilogue(residual=x, out_dtype=F32) if self.fused else None  # x += the product
+            gate = Epilogue("silu", gated=True)
+            mm = lambda name, a, to: self.w[name].forward(L, a, to, st)  # noqa: E731
+            onto = lambda name, a: self.w[name].fused(L, a, x, add, st) if add else mm(name, a, y)  # noqa: E731
+            left = None  # rows that the next norm adds to x
             if timer:
                 timer.mark(0, st)
             step("embed", lambda: embed(self.w["embed"], L, idd, x, stream=st))
             snaps = {}
             for i, t in enumerate(self.types):
                 p, S = "layers.%d." % i, "L%d/" % i
-                step(S + "in_norm", lambda: add_norm(L, D, L, x, y if i > 0 else None, self.v[p + "in_norm"], h,
-                                                     device=self.device, stream=st))
+                step(S + "in_norm", lambda: add_norm(L, D, L, x, left, self.v[p + "in_norm"], h, device=self.device, stream=st))
                 if debug_layers and i > 0:
                     self.stream.synchronize()
                     layers.append(x.cpu().numpy())
+                left = None if add else y
                 if t == "adapter":
-                    step(S + "proj", lambda: self.w[p + "proj"].forward(L, h, y, st))
+                    if add:
+                        plus = Epilogue(bias=self.v[p + "bias"], residual=x, out_dtype=F32)
+                        step(S + "proj", lambda: self.w[p + "proj"].fused(L, h, x, plus, st))
+                        continue
+                    step(S + "proj", lambda: mm(p + "proj", h, y))
                     step(S + "bias", lambda: add_bias(L, D, y, self.v[p + "bias"], device=self.device, stream=st))
                     continue
                 lin = t == "linear_attention"
-                step(S + ("in_proj" if lin else "qkv"),
-                     lambda: self.w[p + ("in_proj" if lin else "qkv")].forward(L, h, big, st))
+                step(S + ("in_proj" if lin else "qkv"), lambda: mm(p + ("in_proj" if lin else "qkv"), h, big))
                 r = step(S + ("gdn" if lin else "attn"),
                          lambda: self.mix[i].forward(L, [big], [o], cache=cache[i] if cache else None, keep_cache=keep))
                 snaps[i] = r["cache"]
-                step(S + ("out_proj" if lin else "o_proj"),
-                     lambda: self.w[p + ("out_proj" if lin else "o_proj")].forward(L, o, y, st))
-                step(S + "post_norm", lambda: add_norm(L, D, L, x, y, self.v[p + "post_norm"], h, device=self.device,
+                step(S + ("out_proj" if lin else "o_proj"), lambda: onto(p + ("out_proj" if lin else "o_proj"), o))
+                step(S + "post_norm", lambda: add_norm(L, D, L, x, left, self.v[p + "post_norm"], h, device=self.device,
                                                        stream=st))
-                step(S + "gate_up", lambda: self.w[p + "gate_up"].forward(L, h, big, st))
-                step(S + "silu", lambda: silu_mul(L, I, big, mid, device=self.device, stream=st))
-                step(S + "down", lambda: self.w[p + "down"].forward(L, mid, y, st))
+                if add:
+                    step(S + "gate_up", lambda: self.w[p + "gate_up"].fused(L, h, mid, gate, st))
+                else:
+                    step(S + "gate_up", lambda: mm(p + "gate_up", h, big))
+                    step(S + "silu", lambda: silu_mul(L, I, big, mid, device=self.device, stream=st))
+                step(S + "down", lambda: onto(p + "down", mid))
             if rows:
-                step("final_norm", lambda: add_norm(len(rows), D, L, x, y, self.v["final_norm"], out, out_f32=True,
+                step("final_norm", lambda: add_norm(len(rows), D, L, x, left, self.v["final_norm"], out, out_f32=not ask,
                                                     rows=rd, device=self.device, stream=st))
+            if ask:
+                out = self._score(len(rows), out, ask)
             if timer:
                 timer.mark(1, st)
         self.stream.synchronize()
@@ -716,7 +770,9 @@ class Torso:
             timer.close()
         if debug_layers:
             self.diag["layers"] = layers
-        return out.cpu().numpy(), (snaps if keep else None)
+        if ask:
+            out = {k: v.cpu().numpy() for k, v in out.items()}
+        return out, (snaps if keep else None)
 
     def profile(self, ids, cache=None):
         """GPU time of every step of a forward over ids, summed over the layers by the step's name without its layer

@@ -261,6 +261,50 @@ class MatMulNBits {
   forward(M, a, y) {
     native.mnbForward(this._h, M, ptrOf(a), ptrOf(y), this.engine ? this.engine._h : null);
   }
+  /*
+   * out = residual + act(a W^T + bias), or gated residual + act(first half of the columns) * second half (ha_mnb_fused,
+   * include/ha.h). epilogue: {act: null | 'silu' | 'gelu', gated, bias, residual, residualDtype, residualStride, outDtype,
+   * outStride}, device buffers bias (f32 [N]) and residual; types F32 (residual) and F16 (out) where they are not given,
+   * strides in elements between rows (0: dense). out may be the residual itself.
+   */
+  fused(M, a, out, epilogue) {
+    const e = epilogue || {}, act = pick(e, 'act', null);
+    if (act !== null && !(Object.prototype.hasOwnProperty.call(ACTS, act))) throw new RangeError("act must be null, 'silu' or 'gelu'");
+    const c = Object.assign({}, e, { act: act === null ? 0 : ACTS[act], gated: pick(e, 'gated', false) ? 1 : 0,
+      bias: optPtrOf(e.bias), residual: optPtrOf(e.residual), residualDtype: dtypeCode(pick(e, 'residualDtype', null), F32),
+      outDtype: dtypeCode(pick(e, 'outDtype', null), F16) });
+    const cols = c.gated ? this.N / 2 : this.N;
+    const rows = (type, stride) => (type === F32 ? 4 : 2) * ((M - 1) * (stride || cols) + cols);
+    if (M > 0) {
+      checkBytes('a', a, 2 * M * this.K, 'the product');
+      checkBytes('bias', e.bias, 4 * this.N, 'the product');
+      checkBytes('residual', e.residual, rows(c.residualDtype, pick(e, 'residualStride', 0)), 'the product');
+      checkBytes('out', out, rows(c.outDtype, pick(e, 'outStride', 0)), 'the product');
+    }
+    native.mnbFused(this._h, M, ptrOf(a), c, ptrOf(out), this.engine ? this.engine._h : null);
+  }
+  // Bytes of the workspace of a logprobs call of M rows (p needs no buffers here, only its numbers and which are asked for).
+  logprobsBytes(M, p) {
+    return native.mnbLogprobsBytes(this._h, M, logprobsOf(p));
+  }
+  /*
+   * Log probabilities over this vocabulary table of M rows a (ha_mnb_logprobs, include/ha.h). p: {nVocab, scale, nTargets,
+   * topK} and device buffers {targets (i32 [M][nTargets]), logp, entropy, lse, topIds (i32 [M][topK]), topLogp}.
+   * workspace: device memory of logprobsBytes(M, p) bytes (an address: with workspaceBytes).
+   */
+  logprobs(M, a, p, workspace, workspaceBytes) {
+    const T = pick(p, 'nTargets', 0), k = pick(p, 'topK', 0);
+    if (M > 0) {
+      checkBytes('a', a, 2 * M * this.K, 'the call');
+      [['targets', T], ['logp', T], ['entropy', 1], ['lse', 1], ['topIds', k], ['topLogp', k]].forEach((x) => {
+        checkBytes(x[0], p[x[0]], 4 * M * x[1], 'the call');
+      });
+    }
+    const have = bytesOf(workspace);
+    const bytes = pick({ bytes: workspaceBytes }, 'bytes', have === null ? 0 : have);
+    checkBytes('workspace', workspace, bytes, 'the call');
+    native.mnbLogprobs(this._h, M, ptrOf(a), logprobsOf(p), ptrOf(workspace), bytes, this.engine ? this.engine._h : null);
+  }
   destroy() {
     if (this._h) {
       native.mnbDestroy(this._h);
@@ -328,9 +372,22 @@ class PagedKV {
   }
 }
 
-function checkBytes(what, x, need) {
-  const have = x instanceof DeviceView ? x.buf.bytes - x.offset : x instanceof DeviceBuffer ? x.bytes : need;
-  if (have < need) throw new RangeError(what + ' of ' + have + ' bytes, the cache needs ' + need);
+// Bytes of a device buffer or view, null of an address.
+function bytesOf(x) {
+  return x instanceof DeviceView ? x.buf.bytes - x.offset : x instanceof DeviceBuffer ? x.bytes : null;
+}
+
+function checkBytes(what, x, need, who) {
+  const have = bytesOf(x);
+  if (have !== null && have < need) throw new RangeError(what + ' of ' + have + ' bytes, ' + (who || 'the cache') + ' needs ' + need);
+}
+
+const ACTS = { silu: 1, gelu: 2 };
+
+function logprobsOf(p) {
+  const c = Object.assign({}, p);
+  ['targets', 'logp', 'entropy', 'lse', 'topIds', 'topLogp'].forEach((k) => { c[k] = optPtrOf(c[k]); });
+  return c;
 }
 
 function kvConfig(c) {
@@ -378,6 +435,9 @@ function fwhtHost(a, off, n) {
  * setParam(name, Float32Array) for "final_norm", "layers.<i>.in_norm" | "post_norm" | "bias" (uploaded here) and the
  * token mixers' "conv" | "neg_exp_A" | "dt_bias" | "gnorm" | "q_norm" | "k_norm" (forwarded to the layer's mixer).
  * A quantised tensor's device buffers are the caller's and must stay alive.
+ * opts.fused: out_proj, o_proj, down and an adapter's proj add onto the f32 residual stream themselves, and gate_up gives
+ * SILU_MUL's rows (MatMulNBits.fused): fewer launches, and the sums between are not rounded to f16. Its results differ from
+ * the default's within those roundings.
  */
 class Torso {
   constructor(manifest, opts) {
@@ -387,6 +447,7 @@ class Torso {
     this.I = pick(manifest, 'intermediate_size', 6144);
     this.device = pick(o, 'device', 0);
     this.types = manifest.layer_types.slice();
+    this.fused = !!pick(o, 'fused', false);
     this.unrotate = pick(o, 'unrotate', pick(manifest, 'unrotate', null));
     this.mixers = this.types.map((t) => {
       if (t === 'adapter') return null;
@@ -444,12 +505,13 @@ class Torso {
     pr.labels.push(label);
     return r;
   }
-  _matmul(L, a, name, y, label) {
+  // y = a W^T, or with an epilogue the fused product.
+  _matmul(L, a, name, y, label, epilogue) {
     const w = this._w(name);
     if (w.had) {  // a is not read again
       this._step(label + '/had', () => native.fwht(a.ptr, L * w.K, w.had, this.device, this.lead._h));
     }
-    this._step(label, () => w.h.forward(L, a, y));
+    this._step(label, () => (epilogue ? w.h.fused(L, a, y, epilogue) : w.h.forward(L, a, y)));
     return w.N;
   }
   _norm(R, nx, x, y, wname, h, outF32, rows) {
@@ -467,6 +529,48 @@ class Torso {
    * fetch_ms (host time of embedRows)[, gpu_ms][, layers]}.
    */
   forward(ids, rows, options) {
+    return this._run(ids, rows, options, null);
+  }
+  /*
+   * The distributions of the tokens that follow the rows (indices into ids; default all) over a vocabulary table, as
+   * Torso.score of the Python host. ask: {table: the weight's name ('embed', where the model ties them), targets: one array
+   * of T integers for each row, topK, nVocab, scale}; options {cache, keepCache, timestamps} as forward. Returns {logp:
+   * Float32Array(rows * T), entropy, lse, topIds: Int32Array(rows * topK), topLogp, cache, kernel, fetch_ms[, gpu_ms]}; gpu_ms
+   * ends with the log probabilities.
+   */
+  score(ids, rows, ask, options) {
+    const a = Object.assign({ table: 'embed', targets: null, topK: 0, nVocab: 0, scale: 0 }, ask);
+    const R = rows ? rows.length : ids.length, w = this._w(a.table);
+    if (w.K !== this.D) throw new RangeError(a.table + ' has rows of ' + w.K + ' values, the hidden state ' + this.D);
+    if (this.unrotate) throw new Error('score: this torso leaves its hidden rows in a rotated basis');
+    if (w.had) throw new Error('score: ' + a.table + ' reads rotated rows');
+    if (a.table === 'embed' && this.embedRows) throw new Error('score: the embedding table is filled row by row');
+    const T = a.targets && R ? a.targets[0].length : 0;
+    if (a.targets && (a.targets.length !== R || a.targets.some((t) => t.length !== T ||
+      Array.from(t).some((x) => (x | 0) !== x)))) throw new RangeError('targets must be integers, as many for each row');
+    return this._run(ids, rows, Object.assign({}, options, { debugLayers: false }),
+      { w: w, T: T, k: a.topK, targets: a.targets, nVocab: a.nVocab, scale: a.scale });
+  }
+  // Log probabilities of R rows h (f16) of a forward; done() when they are queued, then they are read back.
+  _score(R, h, ask, done) {
+    const T = ask.T, k = ask.k;
+    const size = { targets: R * T, logp: R * T, entropy: R, lse: R, topIds: R * k, topLogp: R * k };
+    const p = { nVocab: ask.nVocab, scale: ask.scale, nTargets: T, topK: k };
+    if (R) {
+      Object.keys(size).forEach((x) => { p[x] = size[x] > 0 ? this._buf('score_' + x, 4 * size[x]) : null; });
+      if (T) p.targets.upload(Int32Array.from([].concat.apply([], ask.targets.map((t) => Array.from(t)))));
+      const work = this._buf('score_work', ask.w.h.logprobsBytes(R, p));
+      this._step('logprobs', () => ask.w.h.logprobs(R, h, p, work));
+    }
+    done();
+    const out = {};
+    ['logp', 'entropy', 'lse', 'topIds', 'topLogp'].forEach((x) => {
+      out[x] = new (x === 'topIds' ? Int32Array : Float32Array)(size[x]);
+      if (p[x]) p[x].download(out[x]);  // synchronous on the shared stream
+    });
+    return out;
+  }
+  _run(ids, rows, options, ask) {
     const o = options || {};
     const L = ids.length, D = this.D, I = this.I;
     const cache = pick(o, 'cache', null), keep = !!pick(o, 'keepCache', false);
@@ -480,19 +584,25 @@ class Torso {
     const bufs = this._work(L, Math.max(R.length, 1), maxN);
     bufs.ids.upload(Uint32Array.from(tableRows));
     const snaps = [], layers = [];
+    const add = this.fused ? { residual: bufs.x, outDtype: F32 } : null;  // x += the product
+    let left = null;  // rows that the next norm adds to x
     const timer = stamps ? native.timerCreate(this.device, 2) : null;
     try {
       if (timer) native.timerMark(timer, 0, this.lead._h);
       this._step('embed', () => native.embed(this._w('embed').h._h, L, bufs.ids.ptr, bufs.x.ptr, this.lead._h));
       this.types.forEach((t, i) => {
         const P = 'layers.' + i + '.', S = 'L' + i + '/';
-        this._step(S + 'in_norm', () => this._norm(L, L, bufs.x, i > 0 ? bufs.y : null, P + 'in_norm', bufs.h, false,
-          null));
+        this._step(S + 'in_norm', () => this._norm(L, L, bufs.x, left, P + 'in_norm', bufs.h, false, null));
         if (debug && i > 0) layers.push(bufs.x.download(new Float32Array(L * D)));
-        if (t === 'adapter') {  // x += proj(rms_norm(x)) + bias, the add in the next norm (engine.js:256-261)
-          this._matmul(L, bufs.h, P + 'proj', bufs.y, S + 'proj');
-          this._step(S + 'bias', () => native.addBias(L, D, bufs.y.ptr, this._v(P + 'bias').ptr, this.device,
-            this.lead._h));
+        left = add ? null : bufs.y;
+        if (t === 'adapter') {  // x += proj(rms_norm(x)) + bias (engine.js:256-261)
+          if (add) {
+            this._matmul(L, bufs.h, P + 'proj', bufs.x, S + 'proj', Object.assign({ bias: this._v(P + 'bias') }, add));
+          } else {  // the add in the next norm
+            this._matmul(L, bufs.h, P + 'proj', bufs.y, S + 'proj');
+            this._step(S + 'bias', () => native.addBias(L, D, bufs.y.ptr, this._v(P + 'bias').ptr, this.device,
+              this.lead._h));
+          }
           snaps.push(null);
           return;
         }
@@ -506,28 +616,34 @@ class Torso {
         const r = this._step(S + (lin ? 'gdn' : 'attn'), () => this.mixers[i].forward(L, [bufs.big], [bufs.o],
           { cache: cache ? cache.layers[i] : null, keepCache: keep }));
         snaps.push(r.cache);
-        this._matmul(L, bufs.o, P + (lin ? 'out_proj' : 'o_proj'), bufs.y, S + (lin ? 'out_proj' : 'o_proj'));
-        this._step(S + 'post_norm', () => this._norm(L, L, bufs.x, bufs.y, P + 'post_norm', bufs.h, false, null));
-        this._matmul(L, bufs.h, P + 'gate_up', bufs.big, S + 'gate_up');
-        this._step(S + 'silu', () => native.siluMul(L, I, bufs.big.ptr, bufs.mid.ptr, this.device, this.lead._h));
-        this._matmul(L, bufs.mid, P + 'down', bufs.y, S + 'down');
+        this._matmul(L, bufs.o, P + (lin ? 'out_proj' : 'o_proj'), add ? bufs.x : bufs.y,
+          S + (lin ? 'out_proj' : 'o_proj'), add);
+        this._step(S + 'post_norm', () => this._norm(L, L, bufs.x, left, P + 'post_norm', bufs.h, false, null));
+        if (add) {
+          this._matmul(L, bufs.h, P + 'gate_up', bufs.mid, S + 'gate_up', { act: 'silu', gated: true });
+        } else {
+          this._matmul(L, bufs.h, P + 'gate_up', bufs.big, S + 'gate_up');
+          this._step(S + 'silu', () => native.siluMul(L, I, bufs.big.ptr, bufs.mid.ptr, this.device, this.lead._h));
+        }
+        this._matmul(L, bufs.mid, P + 'down', add ? bufs.x : bufs.y, S + 'down', add);
       });
-      const out = new Float32Array(R.length * D);
+      const out = new Float32Array(ask ? 0 : R.length * D);
       if (R.length) {
         bufs.rows.upload(Uint32Array.from(R));
-        this._step('final_norm', () => this._norm(R.length, L, bufs.x, bufs.y, 'final_norm', bufs.out, true,
-          bufs.rows));
+        this._step('final_norm', () => this._norm(R.length, L, bufs.x, left, 'final_norm', bufs.out, !ask, bufs.rows));
       }
-      if (timer) native.timerMark(timer, 1, this.lead._h);
-      if (R.length) bufs.out.download(out);  // synchronous on the shared stream
+      const done = () => { if (timer) native.timerMark(timer, 1, this.lead._h); };
+      const scores = ask ? this._score(R.length, bufs.out, ask, done) : done();
+      if (R.length && !ask) bufs.out.download(out);  // synchronous on the shared stream
       const c = this.unrotate;  // rotated torso: the original basis is c * FWHT(row) (engine.js:365-366)
-      if (c) for (let r = 0; r < R.length; r++) { fwhtHost(out, r * D, D); for (let j = 0; j < D; j++) out[r * D + j] *= c[j]; }
+      if (c && !ask) for (let r = 0; r < R.length; r++) { fwhtHost(out, r * D, D); for (let j = 0; j < D; j++) out[r * D + j] *= c[j]; }
       let snap = null;
       if (keep) {
         snap = { P: (cache ? cache.P : 0) + L, ids: (cache ? cache.ids : []).concat(Array.from(ids)), layers: snaps,
           release: function () { snaps.forEach((s) => { if (s) s.release(); }); } };
       }
-      const res = { hidden: out, d: D, kernel: projectionKernel(L), cache: snap, fetch_ms: fetchMs };
+      const res = Object.assign(ask ? scores : { hidden: out, d: D },
+        { kernel: projectionKernel(L), cache: snap, fetch_ms: fetchMs });
       if (timer) res.gpu_ms = native.timerElapsed(timer, 0, 1);
       if (debug) res.layers = layers;
       return res;
@@ -567,18 +683,21 @@ class Torso {
     const D = this.D, I = this.I;
     const need = { ids: L * 4, x: L * D * 4, h: L * D * 2, big: L * maxN * 2, o: L * D * 2, y: L * D * 2,
       mid: L * I * 2, rows: R * 4, out: R * D * 4 };
-    if (!this._bufs) this._bufs = {};
-    Object.keys(need).forEach((k) => {
-      const b = this._bufs[k];
-      if (!b || b.bytes < need[k]) {
-        if (b) b.free();
-        this._bufs[k] = this.lead.alloc(need[k]);
-      }
-    });
+    Object.keys(need).forEach((k) => this._buf(k, need[k]));
     return this._bufs;
   }
+  _buf(k, bytes) {
+    if (!this._bufs) this._bufs = {};
+    const b = this._bufs[k];
+    if (!b || b.bytes < bytes) {
+      if (b) b.free();
+      this._bufs[k] = null;
+      this._bufs[k] = this.lead.alloc(bytes);
+    }
+    return this._bufs[k];
+  }
   destroy() {
-    if (this._bufs) Object.keys(this._bufs).forEach((k) => this._bufs[k].free());
+    if (this._bufs) Object.keys(this._bufs).forEach((k) => { if (this._bufs[k]) this._bufs[k].free(); });
     this._bufs = null;
     Object.keys(this.weights).forEach((k) => this.weights[k].h.destroy());
     Object.keys(this.vectors).forEach((k) => this.vectors[k].free());

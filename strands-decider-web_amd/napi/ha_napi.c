@@ -661,6 +661,119 @@ static napi_value js_mnb_forward(napi_env env, napi_callback_info info) {
   return NULL;
 }
 
+/* obj[key] as a device pointer, NULL where it is missing, null or undefined */
+static int get_opt_ptr(napi_env env, napi_value obj, const char* key, void** out) {
+  napi_value v;
+  bool has = false;
+  *out = NULL;
+  if (napi_has_named_property(env, obj, key, &has) != napi_ok) return 0;
+  if (!has) return 1;
+  if (napi_get_named_property(env, obj, key, &v) != napi_ok) return 0;
+  return is_nullish(env, v) || get_ptr(env, v, out);
+}
+
+static int get_long(napi_env env, napi_value obj, const char* key, long* out) {
+  napi_value v;
+  bool has = false;
+  int64_t x = 0;
+  *out = 0;
+  if (napi_has_named_property(env, obj, key, &has) != napi_ok) return 0;
+  if (!has) return 1;
+  if (napi_get_named_property(env, obj, key, &v) != napi_ok) return 0;
+  if (is_nullish(env, v)) return 1;
+  if (napi_get_value_int64(env, v, &x) != napi_ok) return 0;
+  *out = (long)x;
+  return 1;
+}
+
+/* the live weight of argv[0], or NULL with an exception set */
+static ha_mnb* get_weight(napi_env env, napi_value v) {
+  mnb_box* mb = get_mnb(env, v);
+  if (!mb) type_error(env, "not a MatMulNBits handle");
+  else if (!mb->w) type_error(env, "MatMulNBits handle was destroyed");
+  return mb ? mb->w : NULL;
+}
+
+/* mnbFused(handle, M, a: BigInt, {act, gated, bias, residual, residualDtype, outDtype, residualStride, outStride}, out: BigInt,
+   engine|null) */
+static napi_value js_mnb_fused(napi_env env, napi_callback_info info) {
+  napi_value argv[6];
+  if (!get_args(env, info, 6, argv)) return NULL;
+  ha_mnb* w = get_weight(env, argv[0]);
+  if (!w) return NULL;
+  int32_t M;
+  ha_epilogue e;
+  void *a, *out, *st, *bias, *residual;
+  memset(&e, 0, sizeof(e));
+  if (napi_get_value_int32(env, argv[1], &M) != napi_ok) return type_error(env, "M must be an integer");
+  if (!get_ptr(env, argv[2], &a) || !get_ptr(env, argv[4], &out)) return type_error(env, "a and out must be BigInt");
+  if (is_nullish(env, argv[3]) || !get_int(env, argv[3], "act", HA_ACT_NONE, &e.act) ||
+      !get_int(env, argv[3], "gated", 0, &e.gated) || !get_opt_ptr(env, argv[3], "bias", &bias) ||
+      !get_opt_ptr(env, argv[3], "residual", &residual) || !get_int(env, argv[3], "residualDtype", HA_F32, &e.residual_dtype) ||
+      !get_int(env, argv[3], "outDtype", HA_F16, &e.out_dtype) || !get_long(env, argv[3], "residualStride", &e.residual_stride) ||
+      !get_long(env, argv[3], "outStride", &e.out_stride))
+    return type_error(env, "invalid epilogue field");
+  e.bias = (const float*)bias;
+  e.residual = residual;
+  if (!stream_of(env, argv[5], &st)) return type_error(env, "the last argument must be an engine handle or null");
+  CHECK_HA(ha_mnb_fused(w, M, a, &e, out, st));
+  return NULL;
+}
+
+/* {nVocab, scale, nTargets, targets, topK, logp, entropy, lse, topIds, topLogp} */
+static int logprobs_args(napi_env env, napi_value v, ha_logprobs* p) {
+  void *targets, *logp, *entropy, *lse, *ids, *top;
+  memset(p, 0, sizeof(*p));
+  if (is_nullish(env, v) || !get_int(env, v, "nVocab", 0, &p->n_vocab) || !get_float(env, v, "scale", 0.0f, &p->scale) ||
+      !get_int(env, v, "nTargets", 0, &p->n_targets) || !get_opt_ptr(env, v, "targets", &targets) ||
+      !get_int(env, v, "topK", 0, &p->top_k) || !get_opt_ptr(env, v, "logp", &logp) ||
+      !get_opt_ptr(env, v, "entropy", &entropy) || !get_opt_ptr(env, v, "lse", &lse) ||
+      !get_opt_ptr(env, v, "topIds", &ids) || !get_opt_ptr(env, v, "topLogp", &top))
+    return 0;
+  p->targets = (const int*)targets;
+  p->logp = (float*)logp;
+  p->entropy = (float*)entropy;
+  p->lse = (float*)lse;
+  p->top_ids = (int*)ids;
+  p->top_logp = (float*)top;
+  return 1;
+}
+
+/* mnbLogprobsBytes(handle, M, p) -> bytes of the workspace */
+static napi_value js_mnb_logprobs_bytes(napi_env env, napi_callback_info info) {
+  napi_value argv[3], r;
+  if (!get_args(env, info, 3, argv)) return NULL;
+  ha_mnb* w = get_weight(env, argv[0]);
+  if (!w) return NULL;
+  int32_t M;
+  ha_logprobs p;
+  size_t bytes = 0;
+  if (napi_get_value_int32(env, argv[1], &M) != napi_ok) return type_error(env, "M must be an integer");
+  if (!logprobs_args(env, argv[2], &p)) return type_error(env, "invalid logprobs field");
+  CHECK_HA(ha_mnb_logprobs_bytes(w, M, &p, &bytes));
+  CHECK_NAPI(napi_create_double(env, (double)bytes, &r));
+  return r;
+}
+
+/* mnbLogprobs(handle, M, a: BigInt, p, workspace: BigInt, bytes, engine|null) */
+static napi_value js_mnb_logprobs(napi_env env, napi_callback_info info) {
+  napi_value argv[7];
+  if (!get_args(env, info, 7, argv)) return NULL;
+  ha_mnb* w = get_weight(env, argv[0]);
+  if (!w) return NULL;
+  int32_t M;
+  int64_t bytes;
+  ha_logprobs p;
+  void *a, *work, *st;
+  if (napi_get_value_int32(env, argv[1], &M) != napi_ok || napi_get_value_int64(env, argv[5], &bytes) != napi_ok || bytes < 0)
+    return type_error(env, "M and bytes must be integers");
+  if (!get_ptr(env, argv[2], &a) || !get_ptr(env, argv[4], &work)) return type_error(env, "a and workspace must be BigInt");
+  if (!logprobs_args(env, argv[3], &p)) return type_error(env, "invalid logprobs field");
+  if (!stream_of(env, argv[6], &st)) return type_error(env, "the last argument must be an engine handle or null");
+  CHECK_HA(ha_mnb_logprobs(w, M, a, &p, work, (size_t)bytes, st));
+  return NULL;
+}
+
 static napi_value js_mnb_destroy(napi_env env, napi_callback_info info) {
   napi_value argv[1];
   if (!get_args(env, info, 1, argv)) return NULL;
@@ -1041,6 +1154,8 @@ static napi_value init(napi_env env, napi_value exports) {
       {"synchronize", js_synchronize},
       {"mnbCreate", js_mnb_create},         {"mnbForward", js_mnb_forward},
       {"mnbDestroy", js_mnb_destroy},       {"fwht", js_fwht},
+      {"mnbFused", js_mnb_fused},           {"mnbLogprobs", js_mnb_logprobs},
+      {"mnbLogprobsBytes", js_mnb_logprobs_bytes},
       {"kvPageBytes", js_kv_page_bytes},    {"kvCreate", js_kv_create},
       {"kvSetParam", js_kv_set_param},      {"kvAppend", js_kv_append},
       {"kvAttention", js_kv_attention},     {"kvDestroy", js_kv_destroy},
