@@ -18,13 +18,14 @@ NAPI_OUT = os.path.join(HERE, "js", "ha_napi.node")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 
 SOURCES = ["engine.cpp", "gdn_seq.hip", "gdn_chunk.hip", "gdn_duo.hip", "gdn_split.hip", "gqa.hip", "tail.hip", "mnb.hip", "torso.hip",
-           "kv_host.cpp", "kv.hip", "kv_attn.hip", "fused_host.cpp", "fused.hip", "fused_rows.hip", "fused_tiles.hip", "fused_logits.hip",
-           "logprobs.hip"]
+           "kv_host.cpp", "kv.hip", "kv_attn.hip", "fused_host.cpp", "fused.hip", "fused_lanes.hip", "fused_rows.hip", "fused_tiles.hip",
+           "fused_logits.hip", "logprobs.hip"]
 HIP_FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
              "-I" + os.path.join(ROOT, "include"), "-I" + CSRC]
 # Per-source additions. -amdgpu-mfma-vgpr-form keeps MFMA accumulators in VGPRs: the state passes scale their fp32
-# accumulators on the VALU every chunk (products with exact weights: every group of 32), which with AGPR accumulators costs a read and a write-back per element.
+# accumulators on the VALU every chunk (products with exact weights: every group of 32), which with AGPR accumulators costs a
+# read and a write-back per element.
 FILE_FLAGS = {"gdn_split.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "fused_tiles.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
               "fused_rows.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "fused_logits.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 

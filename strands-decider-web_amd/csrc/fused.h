@@ -57,6 +57,7 @@ struct LpArgs {
 
 hipError_t launch_fused(const FusedArgs& a, hipStream_t s);         // product with its activation, bias and residual
 hipError_t launch_logit_records(const FusedArgs& a, hipStream_t s);  // records of the scaled logits
+hipError_t launch_fused_lanes(const FusedArgs& a, hipStream_t s);  // one or two rows, up to 64 KiB of them
 hipError_t launch_fused_rows(const FusedArgs& a, int mt, int nt, hipStream_t s);   // with the tiles that fused_plan.h gives
 hipError_t launch_fused_tiles(const FusedArgs& a, int rt, int ct, hipStream_t s);
 hipError_t launch_logit_tiles(const FusedArgs& a, hipStream_t s);

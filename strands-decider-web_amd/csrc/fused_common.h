@@ -72,30 +72,42 @@ __device__ __forceinline__ h8 ones8() {
 // 1 / (1 + e^-t), 0 where e^-t is infinite. silu(z) = z sigmoid(z), gelu(z) = z sigmoid(2 sqrt(2/pi) (z + 0.044715 z^3)) (the
 // tanh form).
 __device__ __forceinline__ float sigmoid(float t) { return __builtin_amdgcn_rcpf(1.0f + __expf(-t)); }
-// N values of a column of the result, rows m + row_of(v), from their sums z (gated: of the gate, with the up projection's; column j
-// and half + j). Bias, activation, residual and type are asked for once for all N, and the residual's values are loaded
-// together: asked for one by one, a tile's results took longer than its products (2048 x 2048 x 6144: 172 us).
+// What goes into N values of a column of the result besides their sums, rows m + row_of(v): residual and biases. Loaded together:
+// asked for one by one, a tile's results took longer than its products (2048 x 2048 x 6144: 172 us).
+template <int N>
+struct Given {
+  float res[N], bias, up_bias;
+};
 template <int N, class Row>
-__device__ __forceinline__ void results(const FusedArgs& p, int m, int j, int cols, Row row_of, const float* z, const float* up) {
-  if (j >= cols) return;
-  float r[N], x[N];
+__device__ __forceinline__ Given<N> given(const FusedArgs& p, int m, int j, Row row_of) {
+  Given<N> x;
 #pragma unroll
-  for (int v = 0; v < N; v++) r[v] = z[v];
+  for (int v = 0; v < N; v++) x.res[v] = 0.0f;
   if (p.res) {
     const size_t from = (size_t)m * p.res_stride + j;
     const int last = p.M - 1 - m;
     if (p.res_f32) {
 #pragma unroll
-      for (int v = 0; v < N; v++) x[v] = row_of(v) <= last ? gp<float>(p.res)[from + (size_t)row_of(v) * p.res_stride] : 0.0f;
+      for (int v = 0; v < N; v++) x.res[v] = row_of(v) <= last ? gp<float>(p.res)[from + (size_t)row_of(v) * p.res_stride] : 0.0f;
     } else {
 #pragma unroll
-      for (int v = 0; v < N; v++) x[v] = row_of(v) <= last ? (float)gp<_Float16>(p.res)[from + (size_t)row_of(v) * p.res_stride] : 0.0f;
+      for (int v = 0; v < N; v++) x.res[v] = row_of(v) <= last ? (float)gp<_Float16>(p.res)[from + (size_t)row_of(v) * p.res_stride] : 0.0f;
     }
   }
-  if (p.bias) {
-    const float b = p.bias[j];
+  x.bias = p.bias ? p.bias[j] : 0.0f;
+  x.up_bias = p.bias && p.half ? p.bias[p.half + j] : 0.0f;
+  return x;
+}
+// The N values from their sums z (gated: of the gate, with the up projection's) and what is given; type and activation are asked for
+// once for all N.
+template <int N, class Row>
+__device__ __forceinline__ void finish(const FusedArgs& p, int m, int j, Row row_of, const float* z, const float* up, const Given<N>& x) {
+  float r[N];
 #pragma unroll
-    for (int v = 0; v < N; v++) r[v] += b;
+  for (int v = 0; v < N; v++) r[v] = z[v];
+  if (p.bias) {
+#pragma unroll
+    for (int v = 0; v < N; v++) r[v] += x.bias;
   }
   if (p.act == 1) {
 #pragma unroll
@@ -105,13 +117,12 @@ __device__ __forceinline__ void results(const FusedArgs& p, int m, int j, int co
     for (int v = 0; v < N; v++) r[v] = r[v] * sigmoid(1.5957691216057308f * fmaf(0.044715f * r[v] * r[v], r[v], r[v]));
   }
   if (up) {
-    const float b = p.bias ? p.bias[p.half + j] : 0.0f;
 #pragma unroll
-    for (int v = 0; v < N; v++) r[v] *= up[v] + b;
+    for (int v = 0; v < N; v++) r[v] *= up[v] + x.up_bias;
   }
   if (p.res) {
 #pragma unroll
-    for (int v = 0; v < N; v++) r[v] += x[v];
+    for (int v = 0; v < N; v++) r[v] += x.res[v];
   }
   const size_t to = (size_t)m * p.out_stride + j;
   const int last = p.M - 1 - m;
@@ -124,6 +135,11 @@ __device__ __forceinline__ void results(const FusedArgs& p, int m, int j, int co
     for (int v = 0; v < N; v++)
       if (row_of(v) <= last) ((_Float16*)p.out)[to + (size_t)row_of(v) * p.out_stride] = (_Float16)r[v];
   }
+}
+template <int N, class Row>
+__device__ __forceinline__ void results(const FusedArgs& p, int m, int j, int cols, Row row_of, const float* z, const float* up) {
+  if (j >= cols) return;
+  finish<N>(p, m, j, row_of, z, up, given<N>(p, m, j, row_of));
 }
 
 // ---- records of logits ----

@@ -6,7 +6,7 @@
 namespace ha {
 namespace fused {
 
-enum Path { kAny, kRows, kTiles };
+enum Path { kAny, kRows, kTiles, kLanes };
 struct Shape {
   int M, cols, K;  // cols: of the result
   bool gated, asym;
@@ -44,12 +44,22 @@ inline float tiles_us(const Shape& p, int a, int b) {
   return 2.6f + x * k + 1.46f * a * b * n;
 }
 
+// The lanes kernel (one or two rows that fit 64 KiB of LDS; any alignment). Times in fused_lanes.h; each 2048 k are a step, each 2048
+// columns a wave on every SIMD.
+constexpr int kLanesRows = 2, kLanesValues = 32768;
+inline float lanes_us(const Shape& p) {
+  const float x = std::max(1.0f, p.K / 2048.0f), n = std::max(1.0f, p.cols * (p.gated ? 2.0f : 1.0f) / 2048.0f);
+  return p.M == 1 ? 2.1f + 0.75f * x + 0.6f * (n - 1.0f) * x : 2.2f + x + 0.85f * (n - 1.0f) * x;
+}
+
 inline Plan plan(const Shape& p) {
-  if (!p.whole) return {kAny, 0, 0, 0.0f};
+  const bool lanes = p.M <= kLanesRows && p.M * p.K <= kLanesValues;
+  if (!p.whole) return {lanes ? kLanes : kAny, 0, 0, 0.0f};
   Plan best{kAny, 0, 0, 1e30f};
   auto look = [&](Path path, int a, int b, float us) {
     if (us < best.us) best = {path, a, b, us};
   };
+  if (lanes) look(kLanes, 0, 0, lanes_us(p));
   for (int a : {1, 2, 4})
     for (int b : {1, 2, 3, 4}) look(kRows, a, b, rows_us(p, a, b));
   for (int a : {2, 4})

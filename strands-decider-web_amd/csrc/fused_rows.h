@@ -90,6 +90,16 @@ __global__ __launch_bounds__(64 * SW) void fused_rows_kernel(FusedArgs p) {
 #pragma unroll
     for (int n = 0; n < NT; n++) acc[i][n] = f4{0.0f, 0.0f, 0.0f, 0.0f};
   if (T > 0) issue(0);
+  // Where a wave finishes one 16-column piece at most, what goes into it besides the sums is on its way from here on (at the end it is
+  // a round trip of its own)
+  const int per = (wide + 15) / 16;  // 16-column pieces of the result
+  auto next = [](int v) { return v; };
+  constexpr bool kEarly = MT * NT <= SW;
+  Given<4> early{};
+  if constexpr (kEarly) {
+    const int col = 16 * (w % per) + c, m = m0 + 16 * (w / per) + 4 * g;
+    if (w < MT * per && col < wide && m < p.M && j0 + col < cols) early = given<4>(p, m, j0 + col, next);
+  }
   for (int t = 0; t < T; t++) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     h8 af[MT][2];
@@ -142,6 +152,7 @@ __global__ __launch_bounds__(64 * SW) void fused_rows_kernel(FusedArgs p) {
     }
   }
   // the waves' sums: w + (w + SW / 2), then those SW / 2 in order
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (none is in flight: the last half issues none)
   __syncthreads();  // every wave has drained and read its stage
   f4* red = (f4*)sm;
   if (w >= SW / 2) {
@@ -162,12 +173,12 @@ __global__ __launch_bounds__(64 * SW) void fused_rows_kernel(FusedArgs p) {
     for (int v = 1; v < SW / 2; v++) s += from[v * MT * NT * 64];
     return s;
   };
-  const int per = (wide + 15) / 16;  // 16-column pieces of the result
   for (int q = w; q < MT * per; q += SW) {
     const int i = q / per, col = 16 * (q % per) + c, m = m0 + 16 * i + 4 * g;
-    if (col >= wide || m >= p.M) continue;
+    if (col >= wide || m >= p.M || j0 + col >= cols) continue;
     const f4 z = total(i, col), up = gated ? total(i, wide + col) : f4{};
-    results<4>(p, m, j0 + col, cols, [](int v) { return v; }, (const float*)&z, gated ? (const float*)&up : nullptr);
+    if constexpr (kEarly) finish<4>(p, m, j0 + col, next, (const float*)&z, gated ? (const float*)&up : nullptr, early);
+    else results<4>(p, m, j0 + col, cols, next, (const float*)&z, gated ? (const float*)&up : nullptr);
   }
 }
 

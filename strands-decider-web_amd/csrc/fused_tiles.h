@@ -36,7 +36,7 @@ struct TileShape {
   static constexpr int kPitch = 68;  // of a wave's 32 x 64 results
   static constexpr int kStaged = 2 * kA + kTileWaves * kOwn, kResults = kTileWaves * 32 * kPitch * 4;
   static constexpr int kLds = kStaged > kResults ? kStaged : kResults;
-  static constexpr int kWaves = RT * CT <= 2 ? 4 : RT * CT <= 4 && !ASYM && 3 * kLds <= 160 * 1024 ? 3 : 2;
+  static constexpr int kWaves = RT * CT > 2 || ASYM ? 2 : BITS == 4 ? 4 : 3;  // that the registers fit
 };
 
 template <int BITS, bool ASYM, int EPI, int RT, int CT>

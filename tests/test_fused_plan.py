@@ -42,22 +42,29 @@ def test_only_kernels_that_exist(plans):
     sizes = [(M, cols, K, g, a, 1) for M in (1, 2, 15, 16, 17, 31, 64, 65, 200, 513, 2048, 5000, 1 << 20)
              for cols in (1, 7, 16, 100, 1000, 2048, 6144, 8256, 100000) for K in (64, 128, 2048, 6144, 16384) for g in (0, 1) for a in (0, 1)]
     for s, (path, a, b, us) in zip(sizes, plans(sizes)):
-        assert path in (1, 2) and us > 0, s
-        if path == 1:
+        assert path in (1, 2, 3) and us > 0, s
+        if path == 3:
+            assert s[0] <= 2 and s[0] * s[2] <= 32768, s
+        elif path == 1:
             assert a in (1, 2, 4) and b in (1, 2, 3, 4), s
         else:
             assert (a, b) in ((2, 1), (2, 2), (4, 1), (4, 2)), s
             assert not (s[3] and b == 1) and not (s[4] and (a, b) == (4, 2)), s
     assert [p[0] for p in plans([(3, 100, 96, 0, 0, 0), (3000, 100, 2048, 1, 0, 0)])] == [0, 0]
+    assert [p[0] for p in plans([(2, 100, 96, 0, 0, 0), (2, 100, 16416, 1, 0, 0), (1, 100, 32800, 0, 1, 0)])] == [3, 0, 0]
 
 
 # us of some measured shapes: (M, columns of the result, K, gated): {(path, a, b): us}
 MEASURED = {
-    (1, 6144, 2048, 1): {(1, 1, 1): 6.9, (1, 1, 2): 7.0, (1, 1, 3): 6.9, (1, 1, 4): 7.5},
+    (1, 2048, 2048, 0): {(3, 0, 0): 2.9, (1, 1, 1): 4.1, (1, 1, 2): 4.5},
+    (2, 2048, 6144, 0): {(3, 0, 0): 5.3, (1, 1, 1): 6.3, (1, 1, 2): 8.3},
+    (2, 6144, 2048, 1): {(3, 0, 0): 7.5, (1, 1, 1): 6.8, (1, 1, 2): 7.0, (1, 1, 3): 6.7, (1, 1, 4): 7.2},
+    (1, 6144, 512, 1): {(3, 0, 0): 5.1, (1, 1, 1): 4.8, (1, 1, 2): 4.4, (1, 1, 3): 4.4, (1, 1, 4): 4.6},
+    (1, 6144, 2048, 1): {(3, 0, 0): 5.7, (1, 1, 1): 6.9, (1, 1, 2): 7.0, (1, 1, 3): 6.9, (1, 1, 4): 7.5},
     (61, 6144, 2048, 1): {(1, 4, 3): 10.6, (1, 4, 4): 11.1, (1, 2, 3): 11.5, (1, 2, 4): 12.6, (1, 4, 2): 12.3},
     (512, 6144, 2048, 1): {(2, 2, 2): 43.5, (2, 4, 2): 43.7, (1, 2, 4): 53.9, (1, 4, 2): 54.8},
     (2048, 6144, 2048, 1): {(2, 2, 2): 119.0, (2, 4, 2): 100.5},
-    (1, 2048, 6144, 0): {(1, 1, 1): 6.1, (1, 1, 2): 8.3, (1, 1, 3): 10.6},
+    (1, 2048, 6144, 0): {(3, 0, 0): 4.4, (1, 1, 1): 6.1, (1, 1, 2): 8.3, (1, 1, 3): 10.6},
     (61, 2048, 6144, 0): {(1, 1, 2): 8.9, (1, 2, 1): 9.0, (1, 2, 2): 10.2, (1, 1, 1): 11.0},
     (256, 2048, 2048, 0): {(1, 4, 2): 7.8, (1, 2, 4): 8.6, (1, 2, 2): 9.0, (1, 4, 1): 10.5},
     (512, 2048, 6144, 0): {(1, 4, 4): 26.4, (1, 4, 2): 28.9, (1, 2, 4): 32.4, (2, 2, 1): 49.6},

@@ -226,3 +226,37 @@ def test_a_run_of_calls():
         check(mid.cpu().numpy().astype(np.float64), want, off, D, ha.F16)
         want, off = fr.fused(mid.cpu().numpy(), down[3], residual=before)
         check(x.cpu().numpy().astype(np.float64), want, off, I, ha.F32)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M", [1, 2])
+@pytest.mark.parametrize("N,K", [(6, 64), (130, 1984), (34, 2112), (1022, 4160), (16, 16384), (16, 32768)])
+def test_one_and_two_rows(M, fmt, N, K):
+    """Lanes without a block, blocks in one to eight steps, columns past the last; rows longer than go through LDS."""
+    if fmt[1] == 64 and K % 64:
+        pytest.skip("K is not whole groups")
+    run(M, N, K, fmt, out=ha.F32, bias=True, residual=ha.F16, pad=3)
+    run(M, N, K, fmt, act="gelu", gated=True, bias=True, residual=ha.F32, out=ha.F32, pad=1, inplace=True)
+
+
+@pytest.mark.parametrize("fmt", [(4, 32, True), (3, 32, False), (2, 32, True)])
+@pytest.mark.parametrize("M", [1, 2, 3])
+def test_operands_at_odd_places(M, fmt):
+    """Codes 4 bytes and scales 2 bytes past an aligned address, one to three rows of an odd number of blocks."""
+    import torch
+    N, K = 50, 32 * 67
+    words, s, b, W = fr.weight(N, K, *fmt, seed=4)
+    a = np.random.default_rng(M).standard_normal((M, K)).astype(np.float16)
+
+    def late(x, by):
+        raw = torch.from_numpy(np.concatenate([np.zeros(by, np.uint8), np.ascontiguousarray(x).view(np.uint8).ravel()])).to(DEV)
+        assert raw.data_ptr() % 16 == 0
+        return raw, raw.data_ptr() + by
+    q, sd, bd = late(words, 4), late(s, 2), None if b is None else late(b, 2)
+    w = ha.MnbWeight(N, K, q[1], sd[1], bd and bd[1], bits=fmt[0], group=fmt[1], asym=fmt[2])
+    out = torch.empty(M, N, device=DEV)
+    w.fused(M, dev(a), out, ha.Epilogue(out_dtype=ha.F32))
+    torch.cuda.synchronize()
+    want, off = fr.fused(a, W)
+    check(out.cpu().numpy().astype(np.float64), want, off, K, ha.F32)
+    w.close()
