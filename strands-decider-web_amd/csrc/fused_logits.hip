@@ -1,5 +1,6 @@
 // Records of logits (launch_logit_records of fused.hip) of every format: up to 16 rows by the stream kernel
 // (fused_stream.h), more by tiles (fused_tiles.h).
+#include "fused_plan.h"
 #include "fused_stream.h"
 #include "fused_tiles.h"
 
@@ -9,9 +10,15 @@ namespace {
 template <int BITS, bool ASYM>
 hipError_t launch(const FusedArgs& p, hipStream_t s) {
   if (stream_takes(p)) return launch_stream<BITS, ASYM>(p, s);
-  if (p.M <= 32) return launch_tiles<BITS, ASYM, kEpiLogits, 1, 2>(p, s);
-  if (ASYM || p.M <= 64) return launch_tiles<BITS, ASYM, kEpiLogits, 2, 2>(p, s);
-  return launch_tiles<BITS, ASYM, kEpiLogits, ASYM ? 2 : 4, 2>(p, s);
+  const fused::Plan plan = fused::logit_tiles(p.M, ASYM);
+  switch (4 * plan.a + plan.b) {
+    case 5: return launch_tiles<BITS, ASYM, kEpiLogits, 1, 1>(p, s);
+    case 9: return launch_tiles<BITS, ASYM, kEpiLogits, 2, 1>(p, s);
+    case 13: return launch_tiles<BITS, ASYM, kEpiLogits, 3, 1>(p, s);
+    case 17: return launch_tiles<BITS, ASYM, kEpiLogits, 4, 1>(p, s);
+  }
+  if constexpr (!ASYM) return launch_tiles<BITS, ASYM, kEpiLogits, 4, 2>(p, s);
+  return hipErrorInvalidValue;
 }
 
 }  // namespace

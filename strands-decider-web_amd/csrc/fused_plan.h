@@ -40,7 +40,8 @@ inline float rows_us(const Shape& p, int a, int b) {
 // 12288 x 192 2 x 1 12, 4 x 1 16 (rows kernel 26).
 inline float tiles_us(const Shape& p, int a, int b) {
   const float n = (float)((groups(p, 32 * a, 128 * b) + 255) / 256), x = p.K / 2048.0f * (p.asym ? 1.5f : 1.0f);
-  const float k = a == 4 ? (b == 2 ? 21.8f + 12.5f * n : 10.3f + 11.4f * n) : (b == 2 ? 11.5f + 11.3f * n : 8.2f + 6.35f * n);
+  const float k = a == 4 ? (b == 2 ? 21.8f + 12.5f * n : 10.3f + 11.4f * n) : a == 3 ? (b == 2 ? 5.4f + 17.5f * n : 8.0f + 8.7f * n)
+                         : (b == 2 ? 11.5f + 11.3f * n : 8.2f + 6.35f * n);
   return 2.6f + x * k + 1.46f * a * b * n;
 }
 
@@ -62,9 +63,23 @@ inline Plan plan(const Shape& p) {
   if (lanes) look(kLanes, 0, 0, lanes_us(p));
   for (int a : {1, 2, 4})
     for (int b : {1, 2, 3, 4}) look(kRows, a, b, rows_us(p, a, b));
-  for (int a : {2, 4})
+  for (int a : {2, 3, 4})
     for (int b : {1, 2})
-      if ((!p.gated || b == 2) && !(p.asym && a * b == 8)) look(kTiles, a, b, tiles_us(p, a, b));  // (asymmetric 4 x 2: too many registers)
+      if ((!p.gated || b == 2) && !(p.asym && a * b > 4)) look(kTiles, a, b, tiles_us(p, a, b));  // (asymmetric 3 x 2, 4 x 2: too many registers)
+  return best;
+}
+
+// The tile kernel's shape for logits, of so many columns that rounds of workgroups count for little: base + each for every 32 a rows.
+// Fitted to 98304 x 2048, us (4 bits; symmetric, then asymmetric), 61 rows 2 x 1 38, 2 x 2 46, 1 x 1 50; 58, 63, 66; 128 rows 4 x 1
+// 60, 2 x 1 65, 4 x 2 70; 92, 103, -; 192 rows 3 x 1 89, 2 x 1 91, 4 x 2 101; 138, 149, -; 512 rows 4 x 2 188, 4 x 1 213, 2 x 1 226;
+// -, 333, 391. One column tile leaves room for twice the waves.
+inline Plan logit_tiles(int M, bool asym) {
+  const struct { int a, b; float base, each; } shapes[] = {{1, 1, 10.0f, 20.3f}, {2, 1, 11.5f, 26.8f}, {3, 1, 10.0f, 39.4f}, {4, 1, 10.0f, 51.0f}, {4, 2, 25.0f, 42.0f}};
+  Plan best{kTiles, 0, 0, 1e30f};
+  for (const auto& x : shapes) {
+    const float us = x.base + x.each * (float)((M + 32 * x.a - 1) / (32 * x.a));
+    if (us < best.us && !(asym && x.b == 2)) best = {kTiles, x.a, x.b, us};
+  }
   return best;
 }
 

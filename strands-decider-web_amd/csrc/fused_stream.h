@@ -1,16 +1,17 @@
 // Records of the logits of up to 16 rows for fused.hip, gfx950: the table passes once, straight into the registers of waves that
 // share nothing but the rows of a.
 //
-// A wave makes a 64-column block, all of K, 256 k of 16 columns at a time: lane (g = l / 16, c = l % 16) loads the packed blocks 2 g and 2 g + 1 of column c, so
-// that four lanes read whole 128-byte lines, and swaps of lane groups turn them into the operands of v_mfma_f32_16x16x32_f16, of
-// which lane (g, c) holds k 8 g .. + 7 of one 32-k group of column c: a 4 x 4 transposition of (lane group, word).
+// A wave makes a 64-column block, 16 columns at a time, all of K in parts of 256 k: lane (g = l / 16, c = l % 16) loads the packed
+// blocks 2 g and 2 g + 1 of column c, so that four lanes read whole 128-byte lines, and swaps of lane groups turn them into the operands
+// of v_mfma_f32_16x16x32_f16, of which lane (g, c) holds k 8 g .. + 7 of one 32-k group of column c: a 4 x 4 transposition of (lane
+// group, word). Four parts are on their way at any time. Along K first: the eight parts that share a column's line of scales follow
+// each other (16 columns after another for each 256 k, which shares the operands of a, fetched those lines again: 74 us for 63).
 //
 // a stands in LDS, 16-byte chunk j of row r in slot j ^ (r & 15) of its 16.
 //
-// Bound: the table's bytes: 74 us for one row over 248320 tokens of 2048, 3.9 TB/s (with cur and next parts in registers of their
-// own, two waves a SIMD in place of four: 99). The vector unit's share (12 instructions for 8 codes, a swap a word, four fma a
-// group) is about half of that. Products of up to 16 rows, with K split over the waves of a workgroup, gained nothing on the rows
-// kernel this way (1 x 12288 x 2048 7.5 : 7.4 us, 8 rows 8.3 : 7.2).
+// Bound: the table's bytes: 63 us for one row over 248320 tokens of 2048 (4 bits, groups of 32), 4.5 TB/s, 57 with groups of 64; with 3
+// and 2 bits (82 and 53) the vector unit: decoding, a swap a word, four fma a group. Products of up to 16 rows, with K split over the
+// waves of a workgroup, gained nothing on the rows kernel this way (1 x 12288 x 2048 7.5 : 7.4 us, 8 rows 8.3 : 7.2).
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -70,9 +71,11 @@ __device__ __forceinline__ void load_part(const char* q, unsigned qo, const char
   if constexpr (ASYM) eight(b, x.b);
 }
 
-// acc += the part's products. operand(b): the lane's k of group b of the 256 k; sum[b]: their sums over k (asymmetric).
+// acc += the part's products. operand(b): the lane's k of group b of the 256 k.
 template <int BITS, bool ASYM, bool G64, class Operand>
-__device__ __forceinline__ void add_part(const Part<BITS, ASYM>& y, int g, Operand operand, const f4* sum, f4& acc) {
+__device__ __forceinline__ void add_part(const Part<BITS, ASYM>& y, int g, Operand operand, f4& acc) {
+  const f4 zero = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  f4 d[4], sum[ASYM ? 4 : 1];  // of groups of 64 both halves together
 #pragma unroll
   for (int e = 0; e < 2; e++) {  // groups 2 b + e
     // (operands of a are read again for each column tile: kept, they would cost a wave of four on a SIMD)
@@ -91,48 +94,44 @@ __device__ __forceinline__ void add_part(const Part<BITS, ASYM>& y, int g, Opera
 #pragma unroll
     for (int b = 0; b < 4; b++) {
       const unsigned lo = BITS == 4 ? r[b] : r[b] >> (16 * (g & 1)) & 0xFFFFu;
-      const f4 d = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(2 * b + e), codes8<BITS>(lo, hi[b] >> (8 * g) & 0xFFu), f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+      const h8 av = operand(2 * b + e);
+      const bool fresh = !G64 || e == 0;
+      d[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, codes8<BITS>(lo, hi[b] >> (8 * g) & 0xFFu), fresh ? zero : d[b], 0, 0, 0);
+      if constexpr (ASYM) sum[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, ones8(), fresh ? zero : sum[b], 0, 0, 0);
+      if (G64 && e == 0) continue;
       const float s = f16_bits(G64 ? y.s[b >> 1] >> (16 * (b & 1)) : y.s[b] >> (16 * e));
 #pragma unroll
-      for (int i = 0; i < 4; i++) acc[i] = fmaf(s, d[i], acc[i]);
+      for (int i = 0; i < 4; i++) acc[i] = fmaf(s, d[b][i], acc[i]);
       if constexpr (ASYM) {
         const float bias = centred<BITS>(s, f16_bits(G64 ? y.b[b >> 1] >> (16 * (b & 1)) : y.b[b] >> (16 * e)));
 #pragma unroll
-        for (int i = 0; i < 4; i++) acc[i] = fmaf(bias, sum[2 * b + e][i], acc[i]);
+        for (int i = 0; i < 4; i++) acc[i] = fmaf(bias, sum[b][i], acc[i]);
       }
     }
   }
 }
-template <bool ASYM, class Operand>
-__device__ __forceinline__ void part_sums(Operand operand, f4* sum) {
-  if constexpr (ASYM) {
-#pragma unroll
-    for (int b = 0; b < 8; b++) sum[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(operand(b), ones8(), f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-  }
-}
 
 template <int BITS, bool ASYM, bool G64>
-__global__ __launch_bounds__(64 * kStreamWaves, ASYM ? 2 : 4) void fused_stream_kernel(FusedArgs p) {
+__global__ __launch_bounds__(64 * kStreamWaves, 4) void fused_stream_kernel(FusedArgs p) {
   extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
   const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), nb = (p.N + kLpBlock - 1) / kLpBlock;
   const int block = blockIdx.x * kStreamWaves + w, n0 = kLpBlock * min(block, nb - 1);
   const int nblk = p.K / 32, ng = p.K / p.group, chunks = p.K / kStreamK;
-  // a wave's columns: 32 bits of lane offset from a scalar address on (columns past the last repeat it and do not count)
-  unsigned wo[4], so[4];
-#pragma unroll
-  for (int t = 0; t < 4; t++) {
-    const unsigned n = min(16 * t + c, p.N - 1 - n0);
-    wo[t] = (n * nblk + 2 * g) * (4 * BITS);
-    so[t] = n * ng * 2;
-  }
   const char* wp = (const char*)p.q + (size_t)n0 * nblk * (4 * BITS);
   const char* sp = (const char*)p.s + (size_t)n0 * ng * 2;
   const char* bp = ASYM ? (const char*)p.b + (size_t)n0 * ng * 2 : sp;
+  const int left = p.N - 1 - n0;  // (columns past the last repeat it and do not count)
+  // part i is 256-k piece i % chunks of column tile i / chunks: 32 bits of lane offset from a scalar address on
   Part<BITS, ASYM> x[4];
-  auto load = [&](int u, int t) { load_part<BITS, ASYM, G64>(wp, wo[t], sp, bp, so[t], min(u, chunks - 1), x[t]); };
+  int lt = 0, lu = 0;  // of the next part to load
+  auto load = [&](int slot) {
+    const unsigned n = min(16 * min(lt, 3) + c, left);
+    load_part<BITS, ASYM, G64>(wp, (n * nblk + 2 * g) * (4 * BITS), sp, bp, n * ng * 2, lu, x[slot]);
+    if (++lu == chunks) lu = 0, lt++;
+  };
 #pragma unroll
-  for (int t = 0; t < 4; t++) load(0, t);
+  for (int t = 0; t < 4; t++) load(t);
   const int per = p.K / 8;  // 16-byte chunks of a row
   for (int i = tid; i < p.M * per; i += 64 * kStreamWaves) {
     const int r = i / per, j = i - r * per;
@@ -142,28 +141,34 @@ __global__ __launch_bounds__(64 * kStreamWaves, ASYM ? 2 : 4) void fused_stream_
   if (block >= nb) return;
   const int row = min(c, p.M - 1);
   const unsigned char* ar = sm + (size_t)row * per * 16;
-  f4 acc[4];
+  f4 acc = f4{0.0f, 0.0f, 0.0f, 0.0f}, done[4];
 #pragma unroll
-  for (int t = 0; t < 4; t++) acc[t] = f4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t = 0; t < 4; t++) done[t] = acc;
+  int t = 0, u = 0;
 #pragma unroll 1
-  for (int u = 0; u < chunks; u++) {
-    auto operand = [&](int b) {
-      const int j = 32 * u + 4 * b + g;
-      return *(const h8*)(ar + 16 * ((j & ~15) | ((j ^ row) & 15)));
-    };
-    f4 sum[ASYM ? 8 : 1];
-    part_sums<ASYM>(operand, sum);
+  for (int i = 0; i < chunks; i++) {
 #pragma unroll
-    for (int t = 0; t < 4; t++) {
-      const Part<BITS, ASYM> y = x[t];  // (and the next 256 k on their way into its place)
-      load(u + 1, t);
-      add_part<BITS, ASYM, G64>(y, g, operand, sum, acc[t]);
+    for (int k = 0; k < 4; k++) {
+      auto operand = [&](int b) {
+        const int j = 32 * u + 4 * b + g;
+        return *(const h8*)(ar + 16 * ((j & ~15) | ((j ^ row) & 15)));
+      };
+      const Part<BITS, ASYM> y = x[k];  // (and the part after the next three on its way into its place)
+      load(k);
+      add_part<BITS, ASYM, G64>(y, g, operand, acc);
+      if (++u == chunks) {
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+          if (n == t) done[n] = acc;
+        acc = f4{0.0f, 0.0f, 0.0f, 0.0f};
+        u = 0, t++;
+      }
     }
   }
 #pragma unroll
   for (int e = 0; e < 4; e++) {
     if (e >= p.M) break;
-    const float z[4] = {p.scale * acc[0][e], p.scale * acc[1][e], p.scale * acc[2][e], p.scale * acc[3][e]};
+    const float z[4] = {p.scale * done[0][e], p.scale * done[1][e], p.scale * done[2][e], p.scale * done[3][e]};
     const LpRecord r = record16(z, c, p.N - n0);
     const int m = 4 * g + e;
     if (c == 0 && m < p.M) p.rec[(size_t)m * nb + block] = r;

@@ -262,34 +262,50 @@ __global__ __launch_bounds__(64 * kTileWaves, (TileShape<BITS, ASYM, RT, CT>::kW
   add(2 * kPairs - 1, 8);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // copies past the end land before the LDS is given up
   if constexpr (EPI == kEpiLogits) {
-    __syncthreads();  // the stages become the waves' own
-    float* mine = (float*)sm + w * 32 * kPitch;
-    const int nb = (p.N + kLpBlock - 1) / kLpBlock, valid = min(p.N - j0, 64);
+    __syncthreads();  // the stages become the waves' own, or those of two waves that share blocks of 64 columns
+    const int nb = (p.N + kLpBlock - 1) / kLpBlock, part = CT == 2 ? 0 : w & 1, first = j0 - 32 * part, valid = min(p.N - first, 64);
+    float* mine = (float*)sm + (CT == 2 ? w : w & ~1) * 32 * kPitch;
+    // row tile i, columns 32 n + f of the block
+    auto put = [&](float* to, int i, int c, int n) {
 #pragma unroll
-    for (int i = 0; i < RT; i++) {
-#pragma unroll
-      for (int c = 0; c < CT; c++)
-#pragma unroll
-        for (int v = 0; v < 16; v++) mine[(8 * (v >> 2) + 4 * h + (v & 3)) * kPitch + 32 * c + f] = p.scale * acc[i][c][v];
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_wave_barrier();
-      // lane (h, f): columns 32 h .. + 31 of row f
+      for (int v = 0; v < 16; v++) to[(8 * (v >> 2) + 4 * h + (v & 3)) * kPitch + 32 * n + f] = p.scale * acc[i][c][v];
+    };
+    auto record = [&](const float* from, int i) {  // lane (h, f): columns 32 h .. + 31 of row f
       float z[32];
 #pragma unroll
       for (int t = 0; t < 8; t++) {
-        const f4 v = *(const f4*)(mine + f * kPitch + 32 * h + 4 * t);
+        const f4 v = *(const f4*)(from + f * kPitch + 32 * h + 4 * t);
 #pragma unroll
         for (int e = 0; e < 4; e++) z[4 * t + e] = v[e];
       }
-      __builtin_amdgcn_wave_barrier();
-      if (valid > 0) {
-        if (valid < 64) {
+      if (valid < 64) {
 #pragma unroll
-          for (int t = 0; t < 32; t++) z[t] = 32 * h + t < valid ? z[t] : kNoLogit;
+        for (int t = 0; t < 32; t++) z[t] = 32 * h + t < valid ? z[t] : kNoLogit;
+      }
+      const LpRecord r = record_of<32, 32, 64>(z, [h](int t) { return 32 * h + t; });
+      const int m = m0 + 32 * i + f;
+      if (h == 0 && m < p.M) p.rec[(size_t)m * nb + (first >> 6)] = r;
+    };
+    if constexpr (CT == 2) {
+#pragma unroll
+      for (int i = 0; i < RT; i++) {
+        put(mine, i, 0, 0);
+        put(mine, i, 1, 1);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        if (valid > 0) record(mine, i);
+        __builtin_amdgcn_wave_barrier();
+      }
+    } else {  // two row tiles at a time, one for each wave of a pair
+#pragma unroll
+      for (int i = 0; i < RT; i += 2) {
+        put(mine, i, 0, part);
+        if constexpr (RT > 1) {
+          if (i + 1 < RT) put(mine + 32 * kPitch, i + 1 < RT ? i + 1 : i, 0, part);
         }
-        const LpRecord r = record_of<32, 32, 64>(z, [h](int t) { return 32 * h + t; });
-        const int m = m0 + 32 * i + f;
-        if (h == 0 && m < p.M) p.rec[(size_t)m * nb + (j0 >> 6)] = r;
+        __syncthreads();
+        if (valid > 0 && i + part < RT) record(mine + 32 * kPitch * part, i + part);
+        if (i + 2 < RT) __syncthreads();
       }
     }
   } else {
@@ -312,7 +328,7 @@ template <int BITS, bool ASYM, int EPI, int RT, int CT>
 hipError_t launch_tiles(const FusedArgs& p, hipStream_t s) {
   const bool gated = EPI == kEpiAct && p.half;
   const int cols = gated ? p.half : p.N, wide = kTileWaves * (gated ? 32 : 32 * CT);
-  if (CT == 1 && (gated || EPI == kEpiLogits)) return hipErrorInvalidValue;  // (a pair of column tiles a wave)
+  if (CT == 1 && gated) return hipErrorInvalidValue;  // (a pair of column tiles a wave)
   const long tiles = (long)((cols + wide - 1) / wide) * ((p.M + 32 * RT - 1) / (32 * RT));
   if (tiles > 0x7FFFFFFFl) return hipErrorInvalidValue;
   hipLaunchKernelGGL((fused_tiles_kernel<BITS, ASYM, EPI, RT, CT>), dim3((unsigned)tiles), dim3(64 * kTileWaves), 0, s, p);

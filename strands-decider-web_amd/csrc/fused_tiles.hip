@@ -9,9 +9,11 @@ hipError_t launch(const FusedArgs& p, int rt, int ct, hipStream_t s) {
   switch (4 * rt + ct) {
     case 9: return launch_tiles<BITS, ASYM, kEpiAct, 2, 1>(p, s);
     case 10: return launch_tiles<BITS, ASYM, kEpiAct, 2, 2>(p, s);
+    case 13: return launch_tiles<BITS, ASYM, kEpiAct, 3, 1>(p, s);
     case 17: return launch_tiles<BITS, ASYM, kEpiAct, 4, 1>(p, s);
   }
   if constexpr (!ASYM) {
+    if (rt == 3 && ct == 2) return launch_tiles<BITS, ASYM, kEpiAct, 3, 2>(p, s);
     if (rt == 4 && ct == 2) return launch_tiles<BITS, ASYM, kEpiAct, 4, 2>(p, s);
   }
   return hipErrorInvalidValue;

@@ -48,8 +48,8 @@ def test_only_kernels_that_exist(plans):
         elif path == 1:
             assert a in (1, 2, 4) and b in (1, 2, 3, 4), s
         else:
-            assert (a, b) in ((2, 1), (2, 2), (4, 1), (4, 2)), s
-            assert not (s[3] and b == 1) and not (s[4] and (a, b) == (4, 2)), s
+            assert (a, b) in ((2, 1), (2, 2), (3, 1), (3, 2), (4, 1), (4, 2)), s
+            assert not (s[3] and b == 1) and not (s[4] and (a, b) in ((3, 2), (4, 2))), s
     assert [p[0] for p in plans([(3, 100, 96, 0, 0, 0), (3000, 100, 2048, 1, 0, 0)])] == [0, 0]
     assert [p[0] for p in plans([(2, 100, 96, 0, 0, 0), (2, 100, 16416, 1, 0, 0), (1, 100, 32800, 0, 1, 0)])] == [3, 0, 0]
 
@@ -62,6 +62,9 @@ MEASURED = {
     (1, 6144, 512, 1): {(3, 0, 0): 5.1, (1, 1, 1): 4.8, (1, 1, 2): 4.4, (1, 1, 3): 4.4, (1, 1, 4): 4.6},
     (1, 6144, 2048, 1): {(3, 0, 0): 5.7, (1, 1, 1): 6.9, (1, 1, 2): 7.0, (1, 1, 3): 6.9, (1, 1, 4): 7.5},
     (61, 6144, 2048, 1): {(1, 4, 3): 10.6, (1, 4, 4): 11.1, (1, 2, 3): 11.5, (1, 2, 4): 12.6, (1, 4, 2): 12.3},
+    (333, 6144, 2048, 1): {(2, 3, 2): 35.6, (2, 2, 2): 42.7, (2, 4, 2): 42.4, (1, 4, 2): 41.4, (1, 2, 4): 41.9},
+    (288, 98304, 2048, 0): {(2, 2, 2): 162.8, (2, 3, 2): 139.2, (2, 4, 2): 165.7, (2, 2, 1): 155.0, (2, 3, 1): 129.8, (2, 4, 1): 166.0},
+    (384, 98304, 2048, 0): {(2, 2, 2): 186.4, (2, 3, 2): 167.0, (2, 4, 2): 170.5, (2, 2, 1): 181.9, (2, 3, 1): 167.9, (2, 4, 1): 170.6},
     (512, 6144, 2048, 1): {(2, 2, 2): 43.5, (2, 4, 2): 43.7, (1, 2, 4): 53.9, (1, 4, 2): 54.8},
     (2048, 6144, 2048, 1): {(2, 2, 2): 119.0, (2, 4, 2): 100.5},
     (1, 2048, 6144, 0): {(3, 0, 0): 4.4, (1, 1, 1): 6.1, (1, 1, 2): 8.3, (1, 1, 3): 10.6},
