@@ -59,7 +59,7 @@ hipError_t launch_fused(const FusedArgs& a, hipStream_t s);         // product w
 hipError_t launch_logit_records(const FusedArgs& a, hipStream_t s);  // records of the scaled logits
 hipError_t launch_fused_lanes(const FusedArgs& a, hipStream_t s);  // one or two rows, up to 64 KiB of them
 hipError_t launch_fused_rows(const FusedArgs& a, int mt, int nt, hipStream_t s);   // with the tiles that fused_plan.h gives
-hipError_t launch_fused_tiles(const FusedArgs& a, int rt, int ct, hipStream_t s);
+hipError_t launch_fused_tiles(const FusedArgs& a, int rt, int ct, int halves, hipStream_t s);
 hipError_t launch_logit_tiles(const FusedArgs& a, hipStream_t s);
 hipError_t launch_logprobs(const LpArgs& a, hipStream_t s);          // what the records come to
 

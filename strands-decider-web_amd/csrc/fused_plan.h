@@ -11,12 +11,15 @@ struct Shape {
   int M, cols, K;  // cols: of the result
   bool gated, asym;
   bool whole;      // K and alignment as the kernels that move whole 64-k tiles need them
+  bool halves;     // K / 2 is whole pieces of the tile kernel's scales
 };
-// Rows: 16 a x 16 b columns of weights a workgroup. Tiles: 32 a rows, 128 b columns of weights. us: the time this is expected to take.
+// Rows: 16 a x 16 b columns of weights a workgroup. Tiles: 32 a rows, 128 b columns of weights, `halves` of K. us: the time this is
+// expected to take.
 struct Plan {
   Path path;
   int a, b;
   float us;
+  int halves = 1;
 };
 
 // Workgroups of a product with tiles of `rows` x `weights` columns of weights.
@@ -45,6 +48,13 @@ inline float tiles_us(const Shape& p, int a, int b) {
   return 2.6f + x * k + 1.46f * a * b * n;
 }
 
+// Tiles of 64 x 128 by twice the waves, half of them for each half of K: for products of few workgroups, which leave the vector unit
+// waiting. us, against whole K: 1024 rows, 2048 x 2048 17.8 (22.1), 2048 x 6144 43.4 (51.9); 2048 rows 28.8 (32.5), 65 (75); 512 rows,
+// 4096 x 4096 31 (36); 2048 rows, 12288 x 1024 86 (77). 128 x 128 by halves has 29.2, 64 and 43 where this has 28.8, 65 and 31.
+inline float halves_us(const Shape& p) {
+  const float n = (float)((groups(p, 64, 128) + 255) / 256), x = p.K / 2048.0f * (p.asym ? 1.5f : 1.0f);
+  return 2.6f + x * (3.1f + 8.0f * n) + 2.4f * n;
+}
 // The lanes kernel (one or two rows that fit 64 KiB of LDS; any alignment). Times in fused_lanes.h; each 2048 k are a step, each 2048
 // columns a wave on every SIMD.
 constexpr int kLanesRows = 2, kLanesValues = 32768;
@@ -66,6 +76,11 @@ inline Plan plan(const Shape& p) {
   for (int a : {2, 3, 4})
     for (int b : {1, 2})
       if ((!p.gated || b == 2) && !(p.asym && a * b > 4)) look(kTiles, a, b, tiles_us(p, a, b));  // (asymmetric 3 x 2, 4 x 2: too many registers)
+  // (asymmetric: one such workgroup fits a CU)
+  if (p.halves && !p.gated && (!p.asym || groups(p, 64, 128) <= 256)) {
+    const float us = halves_us(p);
+    if (us < best.us) best = {kTiles, 2, 1, us, 2};
+  }
   return best;
 }
 

@@ -27,7 +27,7 @@ typedef float f16v __attribute__((ext_vector_type(16)));
 constexpr int kTileWaves = 4;
 
 // A workgroup's LDS and waves a SIMD. U: 128-k pieces whose scales come together.
-template <int BITS, bool ASYM, int RT, int CT>
+template <int BITS, bool ASYM, int RT, int CT, int KS>
 struct TileShape {
   static constexpr int U = 4;
   static constexpr int kRows = 32 * RT, kCols = 32 * CT;
@@ -35,18 +35,19 @@ struct TileShape {
   static constexpr int kOwn = 2 * (kW + kS * (ASYM ? 2 : 1));
   static constexpr int kPitch = 68;  // of a wave's 32 x 64 results
   static constexpr int kStaged = 2 * kA + kTileWaves * kOwn, kResults = kTileWaves * 32 * kPitch * 4;
-  static constexpr int kLds = kStaged > kResults ? kStaged : kResults;
+  static constexpr int kSums = KS == 1 ? 0 : kTileWaves * RT * CT * 4096;  // what two halves of K give each other
+  static constexpr int kMost = kSums > kResults ? kSums : kResults, kLds = KS * kStaged > kMost ? KS * kStaged : kMost;
   static constexpr int kWaves = RT * CT > 2 || ASYM ? 2 : BITS == 4 ? 4 : 3;  // that the registers fit
 };
 
-template <int BITS, bool ASYM, int EPI, int RT, int CT>
-__global__ __launch_bounds__(64 * kTileWaves, (TileShape<BITS, ASYM, RT, CT>::kWaves)) void fused_tiles_kernel(FusedArgs p) {
-  using L = TileShape<BITS, ASYM, RT, CT>;
+template <int BITS, bool ASYM, int EPI, int RT, int CT, int KS>
+__global__ __launch_bounds__(64 * kTileWaves * KS, (TileShape<BITS, ASYM, RT, CT, KS>::kWaves)) void fused_tiles_kernel(FusedArgs p) {
+  using L = TileShape<BITS, ASYM, RT, CT, KS>;
   constexpr int kRows = L::kRows, kCols = L::kCols, kA = L::kA, kW = L::kW, kS = L::kS, U = L::U, kPitch = L::kPitch;
   constexpr int kCopiesA = kRows / 8 / kTileWaves, kCopiesW = BITS == 4 ? kCols / 16 : kCols * 4 * BITS / 64, kCopiesS = ASYM ? 4 : 2;
   __shared__ __attribute__((aligned(16))) unsigned char sm[L::kLds];
   const int tid = threadIdx.x, lane = tid & 63, f = lane & 31, h = lane >> 5;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int w = __builtin_amdgcn_readfirstlane((tid >> 6) % kTileWaves), ks = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(tid / (64 * kTileWaves));
   const bool gated = EPI == kEpiAct && p.half;
   const int cols = gated ? p.half : p.N, wide = kTileWaves * (gated ? 32 : kCols);
   const int ntn = (cols + wide - 1) / wide, ntm = (p.M + kRows - 1) / kRows, ntiles = ntn * ntm;
@@ -61,11 +62,12 @@ __global__ __launch_bounds__(64 * kTileWaves, (TileShape<BITS, ASYM, RT, CT>::kW
   const int band = id / (kBand * ntn), in_band = id - band * kBand * ntn, rows = min(kBand, ntm - band * kBand);
   const int tm = band * kBand + in_band % rows, tn = in_band / rows;
   const int m0 = tm * kRows, j0 = tn * wide + (gated ? 32 : kCols) * w;  // the wave's first column (of the result)
-  const int nblk = p.K / 32, nkt = p.K / 64, ng = p.K / p.group;
+  // a column's blocks and scales; those of this wave's part of K
+  const int nblk = p.K / 32, ng = p.K / p.group, kblk = nblk / KS, kg = ng / KS, nkt = kblk / 2;
   // rows past M repeat the last one, columns past the last likewise; neither is stored
   const unsigned last = (unsigned)(p.M - 1 - m0), k2 = 2u * (unsigned)p.K;
   const unsigned chunk = 16u * ((lane & 7) ^ (lane >> 3));  // chunk j of row r in slot j ^ (r & 7)
-  const char* ap = (const char*)p.a + (size_t)m0 * p.K * 2;
+  const char* ap = (const char*)p.a + (size_t)m0 * p.K * 2 + (size_t)ks * kblk * 64;
   // a wave's columns: from a scalar address for each column tile, 32 bits of lane offset on
   const char *wp[CT], *sp[CT], *bp[CT];
   int left[CT];  // the last of the wave's columns of a tile
@@ -73,13 +75,14 @@ __global__ __launch_bounds__(64 * kTileWaves, (TileShape<BITS, ASYM, RT, CT>::kW
   for (int c = 0; c < CT; c++) {
     const int first = gated ? min(j0, cols - 1) + c * p.half : min(j0 + 32 * c, cols - 1);
     left[c] = (gated ? c * p.half : 0) + cols - 1 - first;
-    wp[c] = (const char*)p.q + (size_t)first * nblk * (4 * BITS);
-    sp[c] = (const char*)p.s + (size_t)first * ng * 2;
-    bp[c] = ASYM ? (const char*)p.b + (size_t)first * ng * 2 : sp[c];
+    wp[c] = (const char*)p.q + ((size_t)first * nblk + ks * kblk) * (4 * BITS);
+    sp[c] = (const char*)p.s + ((size_t)first * ng + ks * kg) * 2;
+    bp[c] = ASYM ? (const char*)p.b + ((size_t)first * ng + ks * kg) * 2 : sp[c];
   }
   const bool g64 = p.group == 64;
-  const unsigned lds_a = __builtin_amdgcn_readfirstlane(lds_addr(sm) + 1024u * kCopiesA * w);
-  const unsigned lds_w = __builtin_amdgcn_readfirstlane(lds_addr(sm) + 2 * kA + L::kOwn * w), lds_s = lds_w + 2 * kW;
+  unsigned char* const stage0 = sm + ks * L::kStaged;
+  const unsigned lds_a = __builtin_amdgcn_readfirstlane(lds_addr(stage0) + 1024u * kCopiesA * w);
+  const unsigned lds_w = __builtin_amdgcn_readfirstlane(lds_addr(stage0) + 2 * kA + L::kOwn * w), lds_s = lds_w + 2 * kW;
   auto copy_a = [&](int kt, int stage) {
     kt = min(kt, nkt - 1);  // (past the last tile: that one again, not read)
 #pragma unroll
@@ -91,7 +94,7 @@ __global__ __launch_bounds__(64 * kTileWaves, (TileShape<BITS, ASYM, RT, CT>::kW
   auto copy_w = [&](int u, int stage) {
     u = min(u, (nkt - 1) / 2);
     const unsigned to = lds_w + (unsigned)(stage * kW);
-    const int blocks = min(4, nblk - 4 * u);  // (the last piece may have two)
+    const int blocks = min(4, kblk - 4 * u);  // (the last piece may have two)
 #pragma unroll
     for (int i = 0; i < kCopiesW; i++) {
       if constexpr (BITS == 4) {
@@ -108,10 +111,10 @@ __global__ __launch_bounds__(64 * kTileWaves, (TileShape<BITS, ASYM, RT, CT>::kW
   // Two of the 2 U instructions that bring U pieces' scales (groups of 64: 2 U pieces'), pairs of f16, column by column
   auto copy_s = [&](int part, int piece, int stage) {
     constexpr int kPairs = 2 * U;
-    part = min(part, (ng / 2 - 1) / kPairs);
+    part = min(part, (kg / 2 - 1) / kPairs);
     const unsigned to = lds_s + (unsigned)(stage * kS * (ASYM ? 2 : 1)) + 256u * piece;
     const int x = 64 * piece + lane, f0 = x / kPairs % 32;
-    const unsigned pair = min(x % kPairs, ng / 2 - 1 - part * kPairs);
+    const unsigned pair = min(x % kPairs, kg / 2 - 1 - part * kPairs);
     const bool second = CT == 2 && x >= 32 * kPairs;
     const unsigned at = (unsigned)min(f0, second ? left[CT - 1] : left[0]) * (unsigned)ng * 2u + 4u * pair;
     const char* from = (second ? sp[CT - 1] : sp[0]) + (size_t)part * (4 * kPairs);
@@ -124,7 +127,7 @@ __global__ __launch_bounds__(64 * kTileWaves, (TileShape<BITS, ASYM, RT, CT>::kW
   struct Words {
     unsigned lo[CT][2], hi[CT][2];
   };
-  const unsigned char* const own = sm + 2 * kA + L::kOwn * w;
+  const unsigned char* const own = stage0 + 2 * kA + L::kOwn * w;
   auto words = [&](int stage, int block) {
     const unsigned char* from = own + stage * kW;
     Words x;
@@ -182,7 +185,7 @@ __global__ __launch_bounds__(64 * kTileWaves, (TileShape<BITS, ASYM, RT, CT>::kW
       copy_s(part, piece % kPieces, ss ^ 1);
       copy_s(part, (g64 ? piece : piece + 1) % kPieces, ss ^ 1);
     }
-    const unsigned char* as = sm + q * kA + arow;
+    const unsigned char* as = stage0 + q * kA + arow;
     auto operand = [&](int g, int i, int j) { return *(const h8*)(as + 32 * 128 * i + 16 * ((4 * g + 2 * h + j) ^ (f & 7))); };
     af[0][0] = operand(0, 0, 0);
     af[0][1] = operand(0, 0, 1);
@@ -309,29 +312,53 @@ __global__ __launch_bounds__(64 * kTileWaves, (TileShape<BITS, ASYM, RT, CT>::kW
       }
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < RT; i++) {
+    auto row_of = [](int v) { return 8 * (v >> 2) + (v & 3); };
+    auto store = [&](int i) __attribute__((always_inline)) {
       const int m = m0 + 32 * i + 4 * h;  // the lane's first row; its 16 are m + 8 (v / 4) + v % 4
-      if (m0 + 32 * i >= p.M) break;
-      auto row_of = [](int v) { return 8 * (v >> 2) + (v & 3); };
+      if (m0 + 32 * i >= p.M) return;
       if (gated) {
         if constexpr (CT == 2) results<16>(p, m, j0 + f, cols, row_of, (const float*)&acc[i][0], (const float*)&acc[i][1]);
       } else {
 #pragma unroll
         for (int c = 0; c < CT; c++) results<16>(p, m, j0 + 32 * c + f, cols, row_of, (const float*)&acc[i][c], nullptr);
       }
+    };
+    if constexpr (KS == 1) {
+#pragma unroll
+      for (int i = 0; i < RT; i++) store(i);
+    } else {  // each half of K finishes half of the row tiles: it takes the other's sums of those and gives its own of the rest
+      f16v* const give = (f16v*)sm + (size_t)w * RT * CT * 64 + lane;
+      __syncthreads();  // the stages have been read
+      auto meet = [&](auto half) __attribute__((always_inline)) {
+        constexpr int H = decltype(half)::value, R = RT / 2;
+#pragma unroll
+        for (int i = 0; i < R; i++)
+#pragma unroll
+          for (int c = 0; c < CT; c++) give[((R * (1 - H) + i) * CT + c) * 64] = acc[R * (1 - H) + i][c];
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+#pragma unroll
+          for (int c = 0; c < CT; c++) acc[R * H + i][c] += give[((R * H + i) * CT + c) * 64];
+          store(R * H + i);
+        }
+      };
+      if (ks == 0) meet(std::integral_constant<int, 0>{});
+      else meet(std::integral_constant<int, 1>{});
     }
   }
 }
 
-template <int BITS, bool ASYM, int EPI, int RT, int CT>
+// KS = 2 takes K of whole parts of scales for each half (512 k, with groups of 64 1024).
+template <int BITS, bool ASYM, int EPI, int RT, int CT, int KS = 1>
 hipError_t launch_tiles(const FusedArgs& p, hipStream_t s) {
+  if (KS == 2 && p.K % (32 * p.group) != 0) return hipErrorInvalidValue;
   const bool gated = EPI == kEpiAct && p.half;
   const int cols = gated ? p.half : p.N, wide = kTileWaves * (gated ? 32 : 32 * CT);
   if (CT == 1 && gated) return hipErrorInvalidValue;  // (a pair of column tiles a wave)
   const long tiles = (long)((cols + wide - 1) / wide) * ((p.M + 32 * RT - 1) / (32 * RT));
   if (tiles > 0x7FFFFFFFl) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((fused_tiles_kernel<BITS, ASYM, EPI, RT, CT>), dim3((unsigned)tiles), dim3(64 * kTileWaves), 0, s, p);
+  hipLaunchKernelGGL((fused_tiles_kernel<BITS, ASYM, EPI, RT, CT, KS>), dim3((unsigned)tiles), dim3(64 * kTileWaves * KS), 0, s, p);
   return hipGetLastError();
 }
 

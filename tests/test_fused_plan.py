@@ -16,8 +16,8 @@ using namespace ha::fused;
 int main() {
   int M, cols, K, gated, asym, whole;
   while (scanf("%d %d %d %d %d %d", &M, &cols, &K, &gated, &asym, &whole) == 6) {
-    const Plan p = plan({M, cols, K, gated != 0, asym != 0, whole != 0});
-    printf("%d %d %d %g\n", (int)p.path, p.a, p.b, p.us);
+    const Plan p = plan({M, cols, K, gated != 0, asym != 0, whole != 0, K % 1024 == 0});
+    printf("%d %d %d %g\n", (int)p.path + (p.halves == 2 ? 2 : 0), p.a, p.b, p.us);  // 4: tiles by halves of K
   }
 }
 """
@@ -42,7 +42,10 @@ def test_only_kernels_that_exist(plans):
     sizes = [(M, cols, K, g, a, 1) for M in (1, 2, 15, 16, 17, 31, 64, 65, 200, 513, 2048, 5000, 1 << 20)
              for cols in (1, 7, 16, 100, 1000, 2048, 6144, 8256, 100000) for K in (64, 128, 2048, 6144, 16384) for g in (0, 1) for a in (0, 1)]
     for s, (path, a, b, us) in zip(sizes, plans(sizes)):
-        assert path in (1, 2, 3) and us > 0, s
+        assert path in (1, 2, 3, 4) and us > 0, s
+        if path == 4:
+            assert (a, b) == (2, 1) and not s[3] and s[2] % 1024 == 0, s
+            continue
         if path == 3:
             assert s[0] <= 2 and s[0] * s[2] <= 32768, s
         elif path == 1:
@@ -69,10 +72,13 @@ MEASURED = {
     (2048, 6144, 2048, 1): {(2, 2, 2): 119.0, (2, 4, 2): 100.5},
     (1, 2048, 6144, 0): {(3, 0, 0): 4.4, (1, 1, 1): 6.1, (1, 1, 2): 8.3, (1, 1, 3): 10.6},
     (61, 2048, 6144, 0): {(1, 1, 2): 8.9, (1, 2, 1): 9.0, (1, 2, 2): 10.2, (1, 1, 1): 11.0},
-    (256, 2048, 2048, 0): {(1, 4, 2): 7.8, (1, 2, 4): 8.6, (1, 2, 2): 9.0, (1, 4, 1): 10.5},
-    (512, 2048, 6144, 0): {(1, 4, 4): 26.4, (1, 4, 2): 28.9, (1, 2, 4): 32.4, (2, 2, 1): 49.6},
-    (2048, 2048, 6144, 0): {(2, 2, 1): 75.7, (2, 4, 1): 76.3, (2, 2, 2): 82.1, (2, 4, 2): 121.4},
-    (2048, 5120, 2048, 0): {(2, 2, 1): 58.3, (2, 4, 1): 66.8, (2, 2, 2): 71.0, (2, 4, 2): 78.0},
+    (256, 2048, 2048, 0): {(4, 2, 1): 15.9, (1, 4, 2): 7.8, (1, 2, 4): 8.6, (1, 2, 2): 9.0, (1, 4, 1): 10.5},
+    (512, 2048, 6144, 0): {(4, 2, 1): 41.5, (1, 4, 4): 26.4, (1, 4, 2): 28.9, (1, 2, 4): 32.4, (2, 2, 1): 49.6},
+    (1024, 2048, 2048, 0): {(4, 2, 1): 17.8, (2, 2, 1): 22.1, (2, 3, 1): 27.2, (2, 4, 1): 31.3},
+    (512, 4096, 4096, 0): {(4, 2, 1): 30.8, (2, 2, 1): 36.4, (1, 4, 4): 35.9, (1, 4, 2): 37.5},
+    (2048, 12288, 1024, 0): {(4, 2, 1): 86.2, (2, 2, 1): 77.0, (2, 4, 1): 77.4, (2, 4, 2): 84.9, (2, 3, 2): 90.2},
+    (2048, 2048, 6144, 0): {(4, 2, 1): 65.1, (2, 2, 1): 75.7, (2, 4, 1): 76.3, (2, 2, 2): 82.1, (2, 4, 2): 121.4},
+    (2048, 5120, 2048, 0): {(4, 2, 1): 60.6, (2, 2, 1): 58.3, (2, 4, 1): 66.8, (2, 2, 2): 71.0, (2, 4, 2): 78.0},
 }
 
 

@@ -260,3 +260,18 @@ def test_operands_at_odd_places(M, fmt):
     want, off = fr.fused(a, W)
     check(out.cpu().numpy().astype(np.float64), want, off, K, ha.F32)
     w.close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("M,N,K", [(1000, 2048, 2048), (1024, 1999, 4096)])
+def test_halves_of_k(M, fmt, N, K):
+    """Many rows of few columns: waves that take half of K each and finish half of the row tiles each."""
+    run(M, N, K, fmt, out=ha.F32, bias=True, residual=ha.F32, inplace=True, pad=5)
+    run(M, N, K, fmt, act="gelu", residual=ha.F16)
+
+
+@pytest.mark.parametrize("M", [65, 96, 97, 192, 270, 333, 380])
+def test_tiles_of_96_rows(M):
+    run(M, 12288, 256, act="silu", gated=True, out=ha.F32)
+    run(M, 5120, 512, (4, 32, True), out=ha.F32, bias=True)
+    run(M, 5120, 512, (3, 64, False), residual=ha.F16)
