@@ -119,7 +119,7 @@ bool whole(const FusedArgs& p) {
 }  // namespace
 
 hipError_t launch_fused(const FusedArgs& p, hipStream_t s) {
-  const fused::Plan plan = fused::plan({p.M, p.half ? p.half : p.N, p.K, p.half != 0, p.asym != 0, whole(p), p.K % (32 * p.group) == 0});
+  const fused::Plan plan = fused::plan({p.M, p.half ? p.half : p.N, p.K, p.half != 0, p.asym != 0, whole(p), p.K % (32 * p.group) == 0, p.bits});
   if (plan.path == fused::kLanes) return launch_fused_lanes(p, s);
   if (plan.path == fused::kRows) return launch_fused_rows(p, plan.a, plan.b, s);
   if (plan.path == fused::kTiles) return launch_fused_tiles(p, plan.a, plan.b, plan.halves, s);

@@ -12,6 +12,7 @@ struct Shape {
   bool gated, asym;
   bool whole;      // K and alignment as the kernels that move whole 64-k tiles need them
   bool halves;     // K / 2 is whole pieces of the tile kernel's scales
+  int bits = 4;
 };
 // Rows: 16 a x 16 b columns of weights a workgroup. Tiles: 32 a rows, 128 b columns of weights, `halves` of K. us: the time this is
 // expected to take.
@@ -28,6 +29,11 @@ inline long groups(const Shape& p, int rows, int weights) {
   return (long)((p.cols + wide - 1) / wide) * ((p.M + rows - 1) / rows);
 }
 
+// What asymmetric weights and 3 bits cost where arithmetic counts: 1744 x 2560 x 2560, us, rows 4 x 2 and tiles 2 x 1, 4 bits 56 and 49,
+// asymmetric 75 and 74, 3 bits 74 and 58, both 84 and 88 (2 bits as 4).
+inline float rows_cost(const Shape& p) { return 1.0f + (p.asym ? 0.35f : 0.0f) + (p.bits == 3 ? 0.3f : 0.0f); }
+inline float tiles_cost(const Shape& p) { return 1.0f + (p.asym ? 0.45f : 0.0f) + (p.bits == 3 ? 0.25f : 0.0f); }
+
 // Both fitted to 1 to 2048 rows of 2048 to 12288 columns at K = 192 to 6144 (4 bits, groups of 32; r.m.s. error 12 and 9 %); what
 // they choose is 3 % slower than the best of all shapes in the mean. n: workgroups on the busiest of 256 CUs.
 // The rows kernel: a workgroup's time grows with the rows of a and columns of W that it reads and the results that it writes. Shapes
@@ -36,13 +42,13 @@ inline long groups(const Shape& p, int rows, int weights) {
 inline float rows_us(const Shape& p, int a, int b) {
   const float x = p.K / 2048.0f, n = (float)((groups(p, 16 * a, 16 * b) + 255) / 256);
   const float each = x * (0.51f * a + 0.73f * b - 0.2f) + 0.26f + 0.09f * a + 0.145f * a * b;
-  return 2.85f + 0.18f * x + (1.0f + (n - 1.0f) * (a * b >= 12 ? 1.34f : 0.87f)) * each;
+  return 2.85f + 0.18f * x + (1.0f + (n - 1.0f) * (a * b >= 12 ? 1.34f : 0.87f)) * each * rows_cost(p);
 }
 // The tile kernel. us: 512 rows, gated 12288 x 2048 2 x 2 43.5, 4 x 2 43.7 (rows kernel 54); 2048 rows 119, 100; 1024 rows, 2048 x
 // 2048 2 x 1 21, 4 x 1 31, 2 x 2 32 (rows kernel 22); 2048 rows, 2048 x 6144 2 x 1 76, 4 x 1 76, 2 x 2 82, 4 x 2 121; 512 rows,
 // 12288 x 192 2 x 1 12, 4 x 1 16 (rows kernel 26).
 inline float tiles_us(const Shape& p, int a, int b) {
-  const float n = (float)((groups(p, 32 * a, 128 * b) + 255) / 256), x = p.K / 2048.0f * (p.asym ? 1.5f : 1.0f);
+  const float n = (float)((groups(p, 32 * a, 128 * b) + 255) / 256), x = p.K / 2048.0f * tiles_cost(p);
   const float k = a == 4 ? (b == 2 ? 21.8f + 12.5f * n : 10.3f + 11.4f * n) : a == 3 ? (b == 2 ? 5.4f + 17.5f * n : 8.0f + 8.7f * n)
                          : (b == 2 ? 11.5f + 11.3f * n : 8.2f + 6.35f * n);
   return 2.6f + x * k + 1.46f * a * b * n;
@@ -52,7 +58,7 @@ inline float tiles_us(const Shape& p, int a, int b) {
 // waiting. us, against whole K: 1024 rows, 2048 x 2048 17.8 (22.1), 2048 x 6144 43.4 (51.9); 2048 rows 28.8 (32.5), 65 (75); 512 rows,
 // 4096 x 4096 31 (36); 2048 rows, 12288 x 1024 86 (77). 128 x 128 by halves has 29.2, 64 and 43 where this has 28.8, 65 and 31.
 inline float halves_us(const Shape& p) {
-  const float n = (float)((groups(p, 64, 128) + 255) / 256), x = p.K / 2048.0f * (p.asym ? 1.5f : 1.0f);
+  const float n = (float)((groups(p, 64, 128) + 255) / 256), x = p.K / 2048.0f * tiles_cost(p);
   return 2.6f + x * (3.1f + 8.0f * n) + 2.4f * n;
 }
 // The lanes kernel (one or two rows that fit 64 KiB of LDS; any alignment). Times in fused_lanes.h; each 2048 k are a step, each 2048

@@ -83,11 +83,11 @@ __device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double*
   for (int x = 0; x < 2; x++) out[x] = wave_sum(out[x]);
 }
 
-// A workgroup of T threads for a row. Dynamic LDS: list_cap keys, then cand_cap values and their columns. STORED: the row's
+// A workgroup of T threads for a row. Dynamic LDS: list_cap keys, cand_cap values, their columns, the targets, list_cap maxima. STORED: the row's
 // logits themselves (unscaled, f32), each a block of its own.
 template <int BITS, bool ASYM, int T, bool STORED>
 __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_cap, int cand_cap) {
-  constexpr int kWaves = T / 64, kKeep = STORED || T < 512 ? 0 : 4096 / T, kSets = kLpSets / 64;
+  constexpr int kWaves = T / 64, kKeep = STORED ? (T < 512 ? 16 : 32) : T < 512 ? 0 : 4096 / T, kSets = kLpSets / 64;
   extern __shared__ __attribute__((aligned(16))) unsigned char sm[];
   __shared__ u64 best[kLpSets];
   __shared__ u64 threshold;
@@ -97,24 +97,29 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
   u64* list = (u64*)sm;
   double* val = (double*)(list + list_cap);
   int* ids = (int*)(val + cand_cap);
+  int* wanted = ids + cand_cap;
+  unsigned* others = (unsigned*)(wanted + a.n_targets);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), m = blockIdx.x;
   const int n_vocab = a.p.N, k = a.top_k, kk = min(k + kLpMargin, nb), nt = a.n_targets;
   const LpRecord* rec = STORED ? nullptr : a.p.rec + (size_t)m * nb;
   const float* logits = STORED ? a.logits + (size_t)m * nb : nullptr;
   auto key_of = [](float max, int i) { return (u64)ordered(max) << 32 | (0xFFFFFFFFu - (unsigned)i); };
-  // records tid, tid + T, ...: the first kKeep stay in registers
+  // records tid, tid + T, ...: the first kKeep stay in registers, loaded at once
+  auto record = [&](int i) __attribute__((always_inline)) {
+    if constexpr (STORED) return LpRecord{a.p.scale * logits[i], 0.0f, 0.0f, 0u};
+    else return rec[i];
+  };
+  for (int t = tid; t < nt; t += T) wanted[t] = a.targets[(size_t)m * nt + t];
   LpRecord keep[kKeep + 1];
 #pragma unroll
   for (int i = 0; i < kKeep; i++)
-    if (tid + i * T < nb) keep[i] = rec[tid + i * T];
+    if (i * T < nb) keep[i] = record(min(tid + i * T, nb - 1));
   auto each = [&](auto f) {
 #pragma unroll
     for (int i = 0; i < kKeep; i++)
       if (tid + i * T < nb) f(keep[i], tid + i * T);
-    for (int i = tid + kKeep * T; i < nb; i += T) {
-      if constexpr (STORED) f(LpRecord{a.p.scale * logits[i], 0.0f, 0.0f, 0u}, i);
-      else f(rec[i], i);
-    }
+#pragma unroll 4
+    for (int i = tid + kKeep * T; i < nb; i += T) f(record(i), i);
   };
   float most = kNoLogit;
   int at = -1;
@@ -171,18 +176,20 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
   });
   double z = z32, zx = zx32;
   __syncthreads();
+  // those in order, a wave for each (in the list they come in any order): the kk largest are chosen, the others go into the sums
   const int nl = n_list;
-  for (int i = tid; i < nl; i += T) {
+  for (int i = w; i < nl; i += kWaves) {
     const u64 key = list[i];
     int rank = 0;
-    for (int j = 0; j < nl; j++) rank += list[j] > key;
-    if (rank < kk) {
-      chosen[rank] = (int)(0xFFFFFFFFu - (unsigned)key);
-    } else {
-      const double x = (double)unordered((unsigned)(key >> 32)) - (double)M, e = (double)__expf((float)x);
-      z += e;
-      zx += e * x;
-    }
+    for (int j = 0; j < nl; j += 64) rank += __popcll(__ballot(j + lane < nl && list[min(j + lane, nl - 1)] > key));
+    if (lane == 0 && rank < kk) chosen[rank] = (int)(0xFFFFFFFFu - (unsigned)key);
+    if (lane == 0 && rank >= kk) others[rank - kk] = (unsigned)(key >> 32);
+  }
+  __syncthreads();
+  for (int i = tid; i < nl - kk; i += T) {
+    const double x = (double)unordered(others[i]) - (double)M, e = (double)__expf((float)x);
+    z += e;
+    zx += e * x;
   }
   z = wave_sum(z);
   zx = wave_sum(zx);
@@ -213,7 +220,7 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
     bool token[2];
 #pragma unroll
     for (int x = 0; x < 2; x++) {
-      const int at = min(i + x, nc + nt - 1), id = at < nc ? ids[at] : a.targets[(size_t)m * nt + at - nc];
+      const int at = min(i + x, nc + nt - 1), id = at < nc ? ids[at] : wanted[at - nc];
       token[x] = (unsigned)id < (unsigned)n_vocab;  // (no token: its log probability is NaN)
       n[x] = token[x] ? id : 0;
     }
@@ -240,12 +247,15 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
   if (tid == 0 && a.lse) a.lse[m] = (float)((double)M + log_z);
   for (int t = tid; t < nt; t += T) a.logp[(size_t)m * nt + t] = logp(val[nc + t]);
   if (k > 0) {
-    for (int i = tid; i < nc; i += T) {
+    for (int i = w; i < nc; i += kWaves) {
       const double v = val[i];
       const int id = ids[i];
       int rank = 0;
-      for (int j = 0; j < nc; j++) rank += val[j] > v || (val[j] == v && ids[j] < id);
-      if (rank < k) a.top_ids[(size_t)m * k + rank] = id, a.top_logp[(size_t)m * k + rank] = logp(v);
+      for (int j = 0; j < nc; j += 64) {
+        const int at = min(j + lane, nc - 1);
+        rank += __popcll(__ballot(j + lane < nc && (val[at] > v || (val[at] == v && ids[at] < id))));
+      }
+      if (lane == 0 && rank < k) a.top_ids[(size_t)m * k + rank] = id, a.top_logp[(size_t)m * k + rank] = logp(v);
     }
   }
 }
@@ -256,7 +266,7 @@ hipError_t launch_as(const LpArgs& a, hipStream_t s) {
   // the kk sets of T / kLpSets threads that hold a key from the cut on (where there are fewer sets, all of them)
   const int list_cap = std::min(nb, kk * (T / kLpSets) * ((nb + T - 1) / T));
   const int cand_cap = (a.top_k > 0 && !STORED ? kk * kLpBlock : kk) + a.n_targets;
-  const size_t lds = 8 * (size_t)list_cap + 12 * (size_t)cand_cap;
+  const size_t lds = 12 * (size_t)list_cap + 12 * (size_t)cand_cap + 4 * (size_t)a.n_targets;
   auto k = logprobs_kernel<BITS, ASYM, T, STORED>;
   if (lds > 48 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
