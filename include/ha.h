@@ -236,7 +236,7 @@ int ha_mnb_forward_noalloc(ha_mnb* w, int M, const void* a, void* y, void* strea
 int ha_mnb_destroy(ha_mnb* w);
 /* ---- Products whose results go straight into what follows. No counterpart in the reference, which stores the product in f16
    and runs SILU_MUL, ADD_BIAS and ADD_NORM on it (wgsl.js:55-121).
-   Both take any weight of ha_mnb_create, with any N (gated: an even one), its codes 4-byte aligned. a is [M][K] f16, 16-byte
+   Both take any weight of ha_mnb_create, N up to 2^30 (gated: an even one) and K up to 2^24, its codes 4-byte aligned. a is [M][K] f16, 16-byte
    aligned, M up to 2^20. Weights are what the format says, without a rounding of their own (ha_mnb_forward rounds each to f16);
    sums are f32. Operands that ha_mnb_forward's fast kernels take (K a multiple of 64, with groups of 64 of 128; codes 16-byte
    aligned with 4 bits, scales and biases 4-byte aligned) are served by fast kernels here too. Neither call allocates, synchronises or keeps anything in the handle: calls on
@@ -273,7 +273,8 @@ typedef struct ha_logprobs {
   float* top_logp;     /* device [M][top_k]: log p of those */
 } ha_logprobs;
 /* A row with a logit that is not finite gives NaN and top_ids of -1. The workspace (16-byte aligned device memory, as many bytes
-   as ha_mnb_logprobs_bytes says) is the caller's: calls that may overlap need one each. */
+   as ha_mnb_logprobs_bytes says) is the caller's and overlaps neither a nor targets nor outputs: calls that may overlap need one
+   each. */
 int ha_mnb_logprobs_bytes(const ha_mnb* w, int M, const ha_logprobs* p, size_t* bytes);
 int ha_mnb_logprobs(ha_mnb* w, int M, const void* a, const ha_logprobs* p, void* workspace, size_t bytes, void* stream);
 

@@ -20,6 +20,8 @@ bool overlap(const void* p, size_t np, const void* q, size_t nq) {
   const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
   return a < b + nq && b < a + np;
 }
+constexpr int kMaxN = 1 << 30, kMaxK = 1 << 24;  // (the kernels' 32-bit column numbers and offsets within a tile)
+constexpr long kMaxStride = 1l << 40;
 // Bytes from the first value to the end of the last row.
 size_t span(int M, long stride, int cols, size_t size) { return ((size_t)(M - 1) * stride + cols) * size; }
 
@@ -30,6 +32,7 @@ int operands(const ha_mnb* w, int M, const void* a, ha::FusedArgs* f, int* devic
   if (M < 1 || M > 1 << 20) return bad("M must be in [1, 2^20]");
   if (!a || off(a, 16)) return bad("a must be non-NULL and 16-byte aligned");
   if (off(g.q, 4) || off(g.s, 2) || (g.asym && off(g.b, 2))) return bad("the weight's codes must be 4-byte and its scales and biases 2-byte aligned");
+  if (g.N > kMaxN || g.K > kMaxK) return bad("the weight must have N up to 2^30 and K up to 2^24");
   *f = ha::FusedArgs{};
   f->M = M; f->N = g.N; f->K = g.K; f->group = g.group; f->bits = g.bits; f->asym = g.asym;
   f->a = a; f->q = g.q; f->s = g.s; f->b = g.b;
@@ -69,12 +72,14 @@ int ha_mnb_fused(ha_mnb* w, int M, const void* a, const ha_epilogue* e, void* ou
     return bad("dtypes must be HA_F32 or HA_F16");
   const size_t size = e->out_dtype == HA_F32 ? 4 : 2, rsize = e->residual_dtype == HA_F32 ? 4 : 2;
   const long stride = e->out_stride ? e->out_stride : cols, rstride = e->residual_stride ? e->residual_stride : cols;
-  if (!out || off(out, size) || stride < cols) return bad("out must be non-NULL and aligned, out_stride at least " + std::to_string(cols));
+  if (!out || off(out, size) || stride < cols || stride > kMaxStride)
+    return bad("out must be non-NULL and aligned, out_stride at least " + std::to_string(cols) + " and at most 2^40");
   if (e->bias && off(e->bias, 4)) return bad("bias must be 4-byte aligned");
   const size_t bytes = span(M, stride, cols, size);
   if (overlap(out, bytes, a, (size_t)M * f.K * 2)) return bad("out must not overlap a");
   if (e->residual) {
-    if (off(e->residual, rsize) || rstride < cols) return bad("residual must be aligned, residual_stride at least " + std::to_string(cols));
+    if (off(e->residual, rsize) || rstride < cols || rstride > kMaxStride)
+      return bad("residual must be aligned, residual_stride at least " + std::to_string(cols) + " and at most 2^40");
     const bool same = e->residual == out && rsize == size && rstride == stride;
     if (!same && overlap(out, bytes, e->residual, span(M, rstride, cols, rsize)))
       return bad("out must be the residual itself (with its type and stride) or not overlap it");
@@ -114,6 +119,11 @@ int ha_mnb_logprobs(ha_mnb* w, int M, const void* a, const ha_logprobs* p, void*
     if (off(q, 4)) return bad("targets and outputs must be 4-byte aligned");
   const size_t need = workspace_bytes(M, n_vocab, p->top_k);
   if (!workspace || off(workspace, 16) || bytes < need) return bad("the workspace must be 16-byte aligned and have " + std::to_string(need) + " bytes");
+  const struct { const void* p; size_t n; } others[] = {{a, (size_t)M * l.p.K * 2}, {p->targets, 4 * (size_t)M * p->n_targets}, {p->logp, 4 * (size_t)M * p->n_targets},
+                                                        {p->entropy, 4 * (size_t)M}, {p->lse, 4 * (size_t)M}, {p->top_ids, 4 * (size_t)M * p->top_k},
+                                                        {p->top_logp, 4 * (size_t)M * p->top_k}};
+  for (const auto& x : others)
+    if (x.p && x.n && overlap(workspace, need, x.p, x.n)) return bad("the workspace must not overlap a, the targets or an output");
   l.p.N = n_vocab;
   l.p.scale = p->scale > 0.0f ? p->scale : 1.0f;
   const bool stored = ha::fused::store_logits(M, n_vocab, p->top_k);

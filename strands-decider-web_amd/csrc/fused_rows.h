@@ -1,9 +1,10 @@
 // Products of few rows for fused.hip, gfx950: a workgroup's waves split K and meet once, at the end.
 //
-// A workgroup makes 16 MT rows x 16 NT columns (gated: 8 NT of the gate and the 8 NT of the up projection that they multiply). Its waves take the 128-k pieces w, w + SW, ... of K in 64-k halves: each copies rows of a, codes and scales of a half
-// into LDS of its own by DMA and waits for its own copies only, so there is no barrier in the loop; it reads a half into registers,
-// starts the next half's copies into the same place and multiplies. Rows of a go through LDS because lanes hold different rows: a
-// 16-byte load straight into the operands is a cache line a lane. The order of a row's sums depends on K and SW alone.
+// A workgroup makes 16 MT rows x 16 NT columns (gated: 8 NT of the gate and the 8 NT of the up projection that they multiply). Its
+// waves take the 128-k pieces w, w + SW, ... of K in 64-k halves: each copies rows of a, codes and scales of a half into LDS of its own
+// by DMA and waits for its own copies only, so there is no barrier in the loop; it reads a half into registers, starts the next half's
+// copies into the same place and multiplies. Rows of a go through LDS because lanes hold different rows: a 16-byte load straight into
+// the operands is a cache line a lane. The order of a row's sums depends on K and SW alone.
 //
 // v_mfma_f32_16x16x32_f16: lane (g = l / 16, c = l % 16) holds row c (A operand) or column c (B operand), k 8 g .. + 7 of a 32-k
 // group; D: rows 4 g + e, column c. One product is a group, and four fma add s times it.

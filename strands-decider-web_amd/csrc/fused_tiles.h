@@ -10,7 +10,9 @@
 // 128 k and scales by 128 U k, two stages each, of a wave's own columns, so only a needs the barrier. The L2 hands out whole lines
 // of 128 bytes, and a line of a column that is asked for in four parts, 64 k at a time, has left the L1 in between: four times
 // the words' bytes and, scales 4 bytes at a time, 32 times theirs were most of what a CU fetched (2048 x 248320 x 2048: 80 KB a
-// tile and workgroup, 1480 us without any arithmetic, 2415 with it).
+// tile and workgroup, 1480 us without any arithmetic, 2415 with it; now 2330).
+//
+// KS = 2: twice the waves, of which half take each half of K, with stages of their own; each half then finishes half of the row tiles.
 #pragma once
 #include <hip/hip_runtime.h>
 

@@ -6,9 +6,9 @@
 // certain token keeps the digits of what is left. Sums over threads are in 64 bits.
 //
 // The top_k largest logits stand in the top_k blocks of the largest maxima: a block further down has nothing that top_k others
-// do not exceed (with fewer blocks than that, all are looked at). Their largest columns, and every column of such a block whose second largest comes near the last of them, are
-// multiplied out again in 64 bits, and so are the given tokens: sums in f32 differ by 1e-6 of the logits, which is enough to
-// change the order of two tokens. kLpMargin more blocks are looked at, and blocks are taken by (largest value, first block), so
+// do not exceed (with fewer blocks than that, all are looked at). Their largest columns, and every column of such a block whose second
+// largest comes near the last of them, are multiplied out again in 64 bits, and so are the given tokens: sums in f32 differ by 1e-6 of
+// the logits, which is enough to change the order of two tokens. kLpMargin more blocks are looked at, and blocks are taken by (largest value, first block), so
 // that equal logits come in order too. The 64-bit values of the blocks' largest columns also replace their f32 ones in Z.
 //
 // Smaller vocabularies, where two of the top_k often share a block, or whose blocks are too few workgroups, have their logits
@@ -276,8 +276,8 @@ hipError_t launch_as(const LpArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 // Few rows: 16 waves for each, more of its loads and products at once (one row over 248320 tokens, top 8: 19 -> 12 us). Many: as
-// many rows on a CU as their blocks leave work for (2048 x 248320, 3880 blocks: 8 waves 75 us, 4 waves 92; 1431 rows of 1383 logits
-// 53 and 41).
+// many rows on a CU as their blocks leave work for (2048 x 248320, 3880 blocks: 8 waves 70 us; before the ranks were counted by waves 8
+// waves 75, 4 waves 92, and 1431 rows of 1383 logits 53 and 41).
 template <int BITS, bool ASYM, bool STORED>
 hipError_t launch_for(const LpArgs& a, hipStream_t s) {
   if (a.p.M <= 256) return launch_as<BITS, ASYM, 1024, STORED>(a, s);

@@ -100,6 +100,10 @@ int main() {
   }
   good.args.q = q + 2; BAD(ha_mnb_fused(&good, 3, a, &e, out, nullptr), "codes"); good.args.q = q;
   good.args.s = s + 1; BAD(ha_mnb_fused(&good, 3, a, &e, out, nullptr), "codes"); good.args.s = s;
+  { ha_epilogue b = e; b.out_stride = (1l << 40) + 1; BAD(ha_mnb_fused(&good, 3, a, &b, out, nullptr), "2^40"); }
+  { ha_epilogue b = e; b.residual = res; b.residual_dtype = HA_F32; b.residual_stride = 1l << 62; BAD(ha_mnb_fused(&good, 3, a, &b, out, nullptr), "2^40"); }
+  good.args.N = (1 << 30) + 2; BAD(ha_mnb_fused(&good, 1, a, &e, out, nullptr), "2^30"); good.args.N = 100;
+  good.args.K = (1 << 24) + 32; BAD(ha_mnb_fused(&good, 1, a, &e, out, nullptr), "2^24"); good.args.K = 128;
   launch_result = hipErrorInvalidValue;
   CHECK(ha_mnb_fused(&good, 3, a, &e, out, nullptr) == HA_ERR_DEVICE && current == 0);
   launch_result = hipSuccess;
@@ -123,6 +127,23 @@ int main() {
   BAD(ha_mnb_logprobs(&good, 7, a, &p, nullptr, 3000, nullptr), "workspace");
   BAD(ha_mnb_logprobs(&good, 7, a, nullptr, res, 3000, nullptr), "NULL");
   BAD(ha_mnb_logprobs(&good, 7, a + 2, &p, res, 3000, nullptr), "a must");
+  // a workspace that ends where a or an output begins, and one byte into each
+  CHECK(ha_mnb_logprobs(&good, 7, res + 2528, &p, res, 2520, nullptr) == HA_OK);
+  BAD(ha_mnb_logprobs(&good, 7, res + 2512, &p, res, 2520, nullptr), "overlap");
+  for (int i = 0; i < 6; i++) {
+    ha_logprobs b = p;
+    b.lse = (float*)(out + 512);
+    char* const at = res + 2516;
+    switch (i) {
+      case 0: b.targets = (int*)at; break;
+      case 1: b.logp = (float*)at; break;
+      case 2: b.entropy = (float*)at; break;
+      case 3: b.lse = (float*)at; break;
+      case 4: b.top_ids = (int*)at; break;
+      case 5: b.top_logp = (float*)at; break;
+    }
+    BAD(ha_mnb_logprobs(&good, 7, a, &b, res, 2520, nullptr), "overlap");
+  }
 #define WITH(field, value, text) do { ha_logprobs b = p; b.field = value; BAD(ha_mnb_logprobs(&good, 7, a, &b, res, 1 << 20, nullptr), text); } while (0)
   WITH(n_vocab, 101, "n_vocab"); WITH(n_vocab, -1, "n_vocab");
   WITH(n_targets, -1, "n_targets"); WITH(n_targets, 1025, "n_targets");

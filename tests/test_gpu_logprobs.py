@@ -263,3 +263,26 @@ def test_no_workspace_beyond_its_bytes():
     got = c(a)
     assert (c.ws[n:] == 99).all()
     check(got, fr.logprobs(a.cpu().numpy(), W, k=3), 0, 3)
+
+
+@pytest.mark.parametrize("M,V,k", [(10, 32768, 20), (64, 32700, 0), (300, 6000, 20), (260, 20000, 20), (257, 4097, 64)])
+def test_stored_logits(M, V, k):
+    """Vocabularies whose logits are stored: more of them than a thread keeps in registers, and fewer."""
+    run(M, V, 128, k=k)
+
+
+@pytest.mark.parametrize("M,V", [(3, 60000), (3, 9000), (300, 60000), (300, 3000)])
+def test_repeats_bit_for_bit(M, V):
+    """Candidates come in any order; with many equal maxima that order must not show."""
+    words, s, b, _ = fr.weight(V, 128, seed=9)
+    words[:] = words[np.arange(V) % 150]  # each logit some hundred times
+    s[:] = s[np.arange(V) % 150]
+    rng = np.random.default_rng(2)
+    a = dev(rng.standard_normal((M, 128)).astype(np.float16))
+    w = handle(words, s, b, V, 128, (4, 32, False))
+    call = Call(w, M, 0, 2, 30, targets=rng.integers(0, V, (M, 2)).astype(np.int32))
+    first = call(a)
+    for _ in range(5):
+        again = call(a)
+        assert all(first[n].tobytes() == again[n].tobytes() for n in first)
+    w.close()
