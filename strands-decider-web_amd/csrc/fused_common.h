@@ -128,7 +128,7 @@ __device__ __forceinline__ void finish(const FusedArgs& p, int m, int j, Row row
 #pragma unroll
     for (int v = 0; v < N; v++) r[v] = r[v] * sigmoid(1.5957691216057308f * fmaf(0.044715f * r[v] * r[v], r[v], r[v]));
   }
-  if (up) {
+  if (p.half) {
 #pragma unroll
     for (int v = 0; v < N; v++) r[v] *= up[v] + x.up_bias;
   }

@@ -145,7 +145,7 @@ __global__ __launch_bounds__(64 * kLanesWaves) void fused_lanes_kernel(FusedArgs
   } else {
     z = lanes_sums<LW * MR>(acc[0]);
   }
-  if (store) finish<1>(p, im, j0 + ic, one, &z, gated ? &up : nullptr, early);
+  if (store) finish<1>(p, im, j0 + ic, one, &z, &up, early);
 }
 
 template <int BITS, bool ASYM, int MR>

@@ -28,7 +28,7 @@ struct RowsLds {
   static constexpr int kBytes = SW * kStage > kSums ? SW * kStage : kSums;
 };
 
-template <int BITS, bool ASYM, int MT, int NT, int SW>
+template <int BITS, bool ASYM, int MT, int NT, int SW, bool G64>
 __global__ __launch_bounds__(64 * SW) void fused_rows_kernel(FusedArgs p) {
   using L = RowsLds<BITS, ASYM, MT, NT, SW>;
   constexpr int kUnit = BITS == 4 ? 16 : 4, kLanes = L::kW / kUnit, kUnits = (kLanes + 63) / 64;
@@ -39,7 +39,6 @@ __global__ __launch_bounds__(64 * SW) void fused_rows_kernel(FusedArgs p) {
   const int cols = gated ? p.half : p.N, wide = gated ? 8 * NT : 16 * NT;
   const int ntn = (cols + wide - 1) / wide, j0 = wide * (blockIdx.x % ntn), m0 = 16 * MT * (blockIdx.x / ntn);
   const int nh = p.K / 64, nblk = p.K / 32, ng = p.K / p.group;
-  const bool g64 = p.group == 64;
   // this wave's halves, two for each 128-k piece (one where the last piece has no second)
   const int np = (nh + 1) / 2, mine = w < np ? (np - 1 - w) / SW + 1 : 0;
   const int T = 2 * mine - ((nh & 1) && mine > 0 && (np - 1) % SW == w ? 1 : 0);
@@ -79,7 +78,7 @@ __global__ __launch_bounds__(64 * SW) void fused_rows_kernel(FusedArgs p) {
         else dma4_at(lds + L::kA + 256 * i, from);
       }
     }
-    const size_t sb = g64 ? (size_t)(h >> 1) * 4 : (size_t)h * 4;  // the half's two scales, or those of its piece's two halves
+    const size_t sb = G64 ? (size_t)(h >> 1) * 4 : (size_t)h * 4;  // the half's two scales, or those of its piece's two halves
     if (lane < 16 * NT) {
       dma4_at(lds + L::kA + L::kW, (const char*)p.s + so + sb);
       if constexpr (ASYM) dma4_at(lds + L::kA + L::kW + L::kS, (const char*)p.b + so + sb);
@@ -122,33 +121,56 @@ __global__ __launch_bounds__(64 * SW) void fused_rows_kernel(FusedArgs p) {
     }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage has been read: refill it
     if (t + 1 < T) issue(t + 1);
-    const int second = 16 * (half_of(t) & 1);  // groups of 64: which of the piece's two scales
+    const f4 zero = f4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto codes = [&](int n, int j) {
+      if constexpr (BITS == 4) return codes8<BITS>(lo[n][j], 0);
+      else return codes8<BITS>(lo[n][j] >> (16 * (g & 1)) & 0xFFFFu, hi[n][j] >> (8 * g) & 0xFFu);
+    };
+    auto add = [&](int n, int shift, const f4* d, const f4* sum) __attribute__((always_inline)) {
+      const float s = f16_bits(sw[n] >> shift);
+      float bias = 0.0f;
+      if constexpr (ASYM) bias = centred<BITS>(s, f16_bits(bw[n] >> shift));
 #pragma unroll
-    for (int j = 0; j < 2; j++) {
-      f4 sum[MT];
+      for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          acc[i][n][e] = fmaf(s, d[i][e], acc[i][n][e]);
+          if constexpr (ASYM) acc[i][n][e] = fmaf(bias, sum[i][e], acc[i][n][e]);
+        }
+    };
+    f4 sum[MT], d[MT];
+    if constexpr (G64) {  // the half is one group: both 32 k one sum, scaled once
       if constexpr (ASYM) {
 #pragma unroll
-        for (int i = 0; i < MT; i++) sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[i][j], ones8(), f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+        for (int i = 0; i < MT; i++) {
+          sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[i][0], ones8(), zero, 0, 0, 0);
+          sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[i][1], ones8(), sum[i], 0, 0, 0);
+        }
       }
 #pragma unroll
       for (int n = 0; n < NT; n++) {
-        h8 b;
-        if constexpr (BITS == 4) b = codes8<BITS>(lo[n][j], 0);
-        else b = codes8<BITS>(lo[n][j] >> (16 * (g & 1)) & 0xFFFFu, hi[n][j] >> (8 * g) & 0xFFu);
-        const int shift = g64 ? second : 16 * j;
-        const float s = f16_bits(sw[n] >> shift);
-        float bias = 0.0f;
-        if constexpr (ASYM) bias = centred<BITS>(s, f16_bits(bw[n] >> shift));
-        f4 d[MT];
 #pragma unroll
-        for (int i = 0; i < MT; i++) d[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[i][j], b, f4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+        for (int j = 0; j < 2; j++) {
+          const h8 b = codes(n, j);
 #pragma unroll
-        for (int i = 0; i < MT; i++)
+          for (int i = 0; i < MT; i++) d[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[i][j], b, j ? d[i] : zero, 0, 0, 0);
+        }
+        add(n, 16 * (half_of(t) & 1), d, sum);  // (which of the piece's two scales)
+      }
+    } else {
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            acc[i][n][e] = fmaf(s, d[i][e], acc[i][n][e]);
-            if constexpr (ASYM) acc[i][n][e] = fmaf(bias, sum[i][e], acc[i][n][e]);
-          }
+      for (int j = 0; j < 2; j++) {
+        if constexpr (ASYM) {
+#pragma unroll
+          for (int i = 0; i < MT; i++) sum[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[i][j], ones8(), zero, 0, 0, 0);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          const h8 b = codes(n, j);
+#pragma unroll
+          for (int i = 0; i < MT; i++) d[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(af[i][j], b, zero, 0, 0, 0);
+          add(n, 16 * j, d, sum);
+        }
       }
     }
   }
@@ -178,8 +200,8 @@ __global__ __launch_bounds__(64 * SW) void fused_rows_kernel(FusedArgs p) {
     const int i = q / per, col = 16 * (q % per) + c, m = m0 + 16 * i + 4 * g;
     if (col >= wide || m >= p.M || j0 + col >= cols) continue;
     const f4 z = total(i, col), up = gated ? total(i, wide + col) : f4{};
-    if constexpr (kEarly) finish<4>(p, m, j0 + col, next, (const float*)&z, gated ? (const float*)&up : nullptr, early);
-    else results<4>(p, m, j0 + col, cols, next, (const float*)&z, gated ? (const float*)&up : nullptr);
+    if constexpr (kEarly) finish<4>(p, m, j0 + col, next, (const float*)&z, (const float*)&up, early);
+    else results<4>(p, m, j0 + col, cols, next, (const float*)&z, (const float*)&up);
   }
 }
 
@@ -187,7 +209,7 @@ template <int BITS, bool ASYM, int MT, int NT, int SW>
 hipError_t launch_rows_as(const FusedArgs& p, hipStream_t s) {
   constexpr int lds = RowsLds<BITS, ASYM, MT, NT, SW>::kBytes;
   static_assert(lds <= 160 * 1024, "LDS of one CU");
-  auto k = fused_rows_kernel<BITS, ASYM, MT, NT, SW>;
+  auto k = p.group == 64 ? fused_rows_kernel<BITS, ASYM, MT, NT, SW, true> : fused_rows_kernel<BITS, ASYM, MT, NT, SW, false>;
   if (lds > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     if (e != hipSuccess) return e;

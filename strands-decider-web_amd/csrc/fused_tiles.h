@@ -42,7 +42,7 @@ struct TileShape {
   static constexpr int kWaves = RT * CT > 2 || ASYM ? 2 : BITS == 4 ? 4 : 3;  // that the registers fit
 };
 
-template <int BITS, bool ASYM, int EPI, int RT, int CT, int KS>
+template <int BITS, bool ASYM, int EPI, int RT, int CT, int KS, bool WHOLE>
 __global__ __launch_bounds__(64 * kTileWaves * KS, (TileShape<BITS, ASYM, RT, CT, KS>::kWaves)) void fused_tiles_kernel(FusedArgs p) {
   using L = TileShape<BITS, ASYM, RT, CT, KS>;
   constexpr int kRows = L::kRows, kCols = L::kCols, kA = L::kA, kW = L::kW, kS = L::kS, U = L::U, kPitch = L::kPitch;
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(64 * kTileWaves * KS, (TileShape<BITS, ASYM, RT, CT
     sp[c] = (const char*)p.s + ((size_t)first * ng + ks * kg) * 2;
     bp[c] = ASYM ? (const char*)p.b + ((size_t)first * ng + ks * kg) * 2 : sp[c];
   }
-  const bool g64 = p.group == 64;
+  const bool g64 = WHOLE || p.group == 64;
   unsigned char* const stage0 = sm + ks * L::kStaged;
   const unsigned lds_a = __builtin_amdgcn_readfirstlane(lds_addr(stage0) + 1024u * kCopiesA * w);
   const unsigned lds_w = __builtin_amdgcn_readfirstlane(lds_addr(stage0) + 2 * kA + L::kOwn * w), lds_s = lds_w + 2 * kW;
@@ -154,6 +154,7 @@ __global__ __launch_bounds__(64 * kTileWaves * KS, (TileShape<BITS, ASYM, RT, CT
     for (int c = 0; c < CT; c++) acc[i][c] = f16v{};
   const unsigned arow = (unsigned)f * 128u;
   constexpr int kPairs = RT * CT;  // (row tile, column tile) pairs of a group
+  static_assert(!WHOLE || (RT == 2 && CT == 1), "a group's sums wait in d and sum");
   f16v d[2] = {f16v{}, f16v{}}, sum[ASYM ? 2 : 1] = {};
   h8 bf[CT][2], af[2][2];
   float s[2][CT] = {}, b[2][CT] = {};
@@ -208,25 +209,26 @@ __global__ __launch_bounds__(64 * kTileWaves * KS, (TileShape<BITS, ASYM, RT, CT
     // the last tile's last), with the next row tile's reads and the next group's decoding
 #pragma unroll
     for (int t = 0; t < 2 * kPairs; t++) {
-      const int c = t % CT, v = (t / CT) & 1;
+      const int c = t % CT, v = (t / CT) & 1, before = t == 0 ? 2 * kPairs - 1 : t - 1;
+      const bool on = WHOLE && t >= kPairs, due = !WHOLE || before >= kPairs;  // (a tile is a group: its second 32 k go onto the first's sums)
       if constexpr (ASYM) {
         if (c == 0) {
-          sum[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[v][0], ones8(), f16v{}, 0, 0, 0);
+          sum[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[v][0], ones8(), on ? sum[v] : f16v{}, 0, 0, 0);
           sum[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[v][1], ones8(), sum[v], 0, 0, 0);
         }
       }
-      d[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[v][0], bf[c][0], f16v{}, 0, 0, 0);
+      d[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[v][0], bf[c][0], on ? d[t & 1] : f16v{}, 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
       if (c == 0 && t + CT < 2 * kPairs) {
         af[v ^ 1][0] = operand((t + CT) / kPairs, (t + CT) / CT % RT, 0);
         af[v ^ 1][1] = operand((t + CT) / kPairs, (t + CT) / CT % RT, 1);
       }
       if (t == CT - 1) x1 = words(ws, 2 * q + 1);
-      add(t == 0 ? 2 * kPairs - 1 : t - 1, 0);
+      if (due) add(before, 0);
       __builtin_amdgcn_sched_barrier(0);
       d[t & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(af[v][1], bf[c][1], d[t & 1], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
-      add(t == 0 ? 2 * kPairs - 1 : t - 1, 8);
+      if (due) add(before, 8);
       if (t == 0) {  // (the last tile's scales are done with)
         if constexpr (CT == 2) decode(x0, 1);
 #pragma unroll
@@ -360,7 +362,12 @@ hipError_t launch_tiles(const FusedArgs& p, hipStream_t s) {
   if (CT == 1 && gated) return hipErrorInvalidValue;  // (a pair of column tiles a wave)
   const long tiles = (long)((cols + wide - 1) / wide) * ((p.M + 32 * RT - 1) / (32 * RT));
   if (tiles > 0x7FFFFFFFl) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((fused_tiles_kernel<BITS, ASYM, EPI, RT, CT, KS>), dim3((unsigned)tiles), dim3(64 * kTileWaves * KS), 0, s, p);
+  // Groups of 64 are a tile's 64 k: where the pairs' sums have registers, both halves are one sum, scaled once
+  auto k = fused_tiles_kernel<BITS, ASYM, EPI, RT, CT, KS, false>;
+  if constexpr (RT == 2 && CT == 1) {
+    if (p.group == 64) k = fused_tiles_kernel<BITS, ASYM, EPI, RT, CT, KS, true>;
+  }
+  hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(64 * kTileWaves * KS), 0, s, p);
   return hipGetLastError();
 }
 
