@@ -34,6 +34,18 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
+// 16 + code e of a packed block, its bits straight into the mantissa: two instructions for 2 and 4 bits (a conversion to f32 and one
+// to f64 and a product took five: 2048 x 248320, top 5 75 us, now 69; 1744 x 2559 of 3 bits, top 32 114, now 104).
+template <int BITS>
+__device__ __forceinline__ double sixteen_and(const unsigned* wd, int e) {
+  auto at16 = [](unsigned v, int from) { return from <= 16 ? v << (16 - from) : v >> (from - 16); };  // bit `from` to bit 16
+  unsigned hi;
+  if constexpr (BITS == 4) hi = at16(wd[e >> 3], 4 * (e & 7)) & 0x000F0000u;
+  else hi = at16(wd[e >> 4], 2 * (e & 15)) & 0x00030000u;
+  if constexpr (BITS == 3) hi |= (e <= 18 ? wd[2] << (18 - e) : wd[2] >> (e - 18)) & 0x00040000u;
+  return __builtin_bit_cast(double, (u64)(hi | 0x40300000u) << 32);
+}
+
 // a[m] . W[n] of two rows n in 64 bits, by one wave: lanes over the packed blocks.
 template <int BITS, bool ASYM>
 __device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double* out) {
@@ -57,26 +69,19 @@ __device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double*
     double d[2] = {0.0, 0.0}, sum = 0.0;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      h8 c[2];
-#pragma unroll
-      for (int x = 0; x < 2; x++) {
-        unsigned lo, hi = 0;
-        if constexpr (BITS == 4) lo = wd[x][j];
-        else lo = wd[x][j >> 1] >> (16 * (j & 1)) & 0xFFFFu;
-        if constexpr (BITS == 3) hi = wd[x][BITS - 1] >> (8 * j) & 0xFFu;
-        c[x] = codes8<BITS>(lo, hi);
-      }
 #pragma unroll
       for (int e = 0; e < 8; e++) {
+        const double ad = (double)(float)av[j][e];
+        sum += ad;
 #pragma unroll
-        for (int x = 0; x < 2; x++) d[x] += (double)((float)av[j][e] * (float)c[x][e]);  // (15 bits: exact)
-        if constexpr (ASYM) sum += (double)(float)av[j][e];
+        for (int x = 0; x < 2; x++) d[x] = fma(ad, sixteen_and<BITS>(wd[x], 8 * j + e), d[x]);
       }
     }
+    constexpr double kMid = 1 << (BITS - 1);
 #pragma unroll
     for (int x = 0; x < 2; x++) {
-      out[x] += (double)s[x] * d[x];
-      if constexpr (ASYM) out[x] += ((double)b[x] + (1 << (BITS - 1)) * (double)s[x]) * sum;
+      out[x] += (double)s[x] * (d[x] - (16.0 + kMid) * sum);
+      if constexpr (ASYM) out[x] += ((double)b[x] + kMid * (double)s[x]) * sum;
     }
   }
 #pragma unroll
@@ -276,7 +281,7 @@ hipError_t launch_as(const LpArgs& a, hipStream_t s) {
   return hipGetLastError();
 }
 // Few rows: 16 waves for each, more of its loads and products at once (one row over 248320 tokens, top 8: 19 -> 12 us). Many: as
-// many rows on a CU as their blocks leave work for (2048 x 248320, 3880 blocks: 8 waves 70 us; before the ranks were counted by waves 8
+// many rows on a CU as their blocks leave work for (2048 x 248320, 3880 blocks: 8 waves 69 us; before the ranks were counted by waves 8
 // waves 75, 4 waves 92, and 1431 rows of 1383 logits 53 and 41).
 template <int BITS, bool ASYM, bool STORED>
 hipError_t launch_for(const LpArgs& a, hipStream_t s) {

@@ -14,15 +14,23 @@ pytestmark = pytest.mark.skipif(not os.path.exists(HIPCC), reason="hipcc is miss
 FILES = ("fused_tiles.hip", "fused_rows.hip", "fused_logits.hip")
 
 
-@pytest.fixture(scope="module", params=FILES)
-def code(request, tmp_path_factory):
-    out = tmp_path_factory.mktemp("s") / "out.s"
-    r = subprocess.run([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang",
-                        "-packed-fp32-ops", "-mllvm", "-amdgpu-mfma-vgpr-form", "-I" + os.path.join(ROOT, "include"), "-I" + CSRC,
-                        "-x", "hip", "-S", "--cuda-device-only", os.path.join(CSRC, request.param), "-o", str(out)],
-                       capture_output=True, text=True, timeout=900)
-    assert r.returncode == 0, r.stderr
-    text = out.read_text()
+@pytest.fixture(scope="module")
+def compiled(tmp_path_factory):
+    """The files' assembly, compiled side by side."""
+    d = tmp_path_factory.mktemp("s")
+    runs = {f: subprocess.Popen([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+                                 "-mllvm", "-amdgpu-mfma-vgpr-form", "-I" + os.path.join(ROOT, "include"), "-I" + CSRC, "-x", "hip", "-S",
+                                 "--cuda-device-only", os.path.join(CSRC, f), "-o", str(d / (f + ".s"))], stderr=subprocess.PIPE, text=True)
+            for f in FILES}
+    for f, r in runs.items():
+        err = r.communicate(timeout=900)[1]
+        assert r.returncode == 0, err
+    return {f: (d / (f + ".s")).read_text() for f in FILES}
+
+
+@pytest.fixture(params=FILES)
+def code(request, compiled):
+    text = compiled[request.param]
     return request.param, text, [(m.group(1), m.group(0)) for m in re.finditer(r"^(_Z\w*fused_\w*kernel\w*):.*?^\.Lfunc_end", text, re.M | re.S)]
 
 
