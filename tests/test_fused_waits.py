@@ -20,18 +20,21 @@ def compiled(tmp_path_factory):
     d = tmp_path_factory.mktemp("s")
     runs = {f: subprocess.Popen([HIPCC, "--offload-arch=gfx950", "-O3", "-std=c++17", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
                                  "-mllvm", "-amdgpu-mfma-vgpr-form", "-I" + os.path.join(ROOT, "include"), "-I" + CSRC, "-x", "hip", "-S",
-                                 "--cuda-device-only", os.path.join(CSRC, f), "-o", str(d / (f + ".s"))], stderr=subprocess.PIPE, text=True)
+                                 "--cuda-device-only", os.path.join(CSRC, f), "-o", str(d / (f + ".s"))], stderr=open(str(d / (f + ".err")), "w"))
             for f in FILES}
     for f, r in runs.items():
-        err = r.communicate(timeout=900)[1]
-        assert r.returncode == 0, err
-    return {f: (d / (f + ".s")).read_text() for f in FILES}
+        r.wait(timeout=900)
+        assert r.returncode == 0, (d / (f + ".err")).read_text()
+    out = {}
+    for f in FILES:
+        text = (d / (f + ".s")).read_text()
+        out[f] = f, text, [(m.group(1), m.group(0)) for m in re.finditer(r"^(_Z\w*fused_\w*kernel\w*):.*?^\.Lfunc_end", text, re.M | re.S)]
+    return out
 
 
 @pytest.fixture(params=FILES)
 def code(request, compiled):
-    text = compiled[request.param]
-    return request.param, text, [(m.group(1), m.group(0)) for m in re.finditer(r"^(_Z\w*fused_\w*kernel\w*):.*?^\.Lfunc_end", text, re.M | re.S)]
+    return compiled[request.param]
 
 
 def test_m0_is_written_only_by_the_copies(code):
