@@ -239,8 +239,9 @@ int ha_mnb_destroy(ha_mnb* w);
    Both take any weight of ha_mnb_create, N up to 2^30 (gated: an even one) and K up to 2^24, its codes 4-byte aligned. a is [M][K] f16, 16-byte
    aligned, M up to 2^20. Weights are what the format says, without a rounding of their own (ha_mnb_forward rounds each to f16);
    sums are f32. Operands that ha_mnb_forward's fast kernels take (K a multiple of 64, with groups of 64 of 128; codes 16-byte
-   aligned with 4 bits, scales and biases 4-byte aligned) are served by fast kernels here too. Neither call allocates, synchronises or keeps anything in the handle: calls on
-   one handle may overlap, and both can be captured into a HIP graph. */
+   aligned with 4 bits, scales and biases 4-byte aligned) are served by fast kernels here too; products of others take N up to
+   2^29 - 64. Neither call allocates, synchronises or keeps anything in the handle: calls on one handle may overlap, and both can
+   be captured into a HIP graph. */
 typedef enum ha_act { HA_ACT_NONE = 0, HA_ACT_SILU = 1, HA_ACT_GELU = 2 /* the tanh form */ } ha_act;
 typedef struct ha_epilogue {
   int act;               /* ha_act */

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstddef>
+#include <cstdint>
 #include <string>
 
 #include "ha_kernels.h"
@@ -42,6 +43,12 @@ struct FusedArgs {
   float scale;
   LpRecord* rec;       // [M][ceil(N / 64)]
 };
+
+// Whether the kernels that move whole 64-k tiles can run the operands: codes in whole words of a block's half, two scales at once.
+inline bool whole(const FusedArgs& p) {
+  const uintptr_t sb = (uintptr_t)p.s | (p.asym ? (uintptr_t)p.b : 0);
+  return p.K % 64 == 0 && (p.group == 32 || p.K % 128 == 0) && (uintptr_t)p.q % (p.bits == 4 ? 16 : 4) == 0 && sb % 4 == 0;
+}
 
 struct LpArgs {
   FusedArgs p;         // the product that the records are of

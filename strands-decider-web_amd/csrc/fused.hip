@@ -17,7 +17,7 @@ namespace {
 // v_mfma_f32_16x16x32_f16, lane (g = l / 16, c = l % 16) row c of a and column c of a tile, k 8 g .. + 7 of the group; D: rows
 // 4 g + e, column c. Operands come straight from memory, four groups a wave at a time (7 x 36 x 4000, 3 bits: 115 us with one
 // wave for all of K).
-constexpr int kAnyWaves = 8;
+constexpr int kAnyWaves = fused::kAnyThreads / 64;
 template <int BITS, bool ASYM, int EPI>
 __global__ __launch_bounds__(64 * kAnyWaves) void fused_any_kernel(FusedArgs p) {
   __shared__ f4 red[kAnyWaves][4][64];
@@ -92,7 +92,7 @@ template <int BITS, bool ASYM, int EPI>
 hipError_t launch_any_as(const FusedArgs& p, hipStream_t s) {
   const int cols = EPI == kEpiAct && p.half ? p.half : p.N, wide = EPI == kEpiAct && p.half ? 32 : 64;
   const long tiles = (long)((cols + wide - 1) / wide) * ((p.M + 15) / 16);
-  if (tiles > 0x7FFFFFFFl) return hipErrorInvalidValue;
+  if (!fused::fits(tiles, 64 * kAnyWaves)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((fused_any_kernel<BITS, ASYM, EPI>), dim3((unsigned)tiles), dim3(64 * kAnyWaves), 0, s, p);
   return hipGetLastError();
 }
@@ -110,23 +110,39 @@ hipError_t launch_any(const FusedArgs& p, hipStream_t s) {
   return hipErrorInvalidValue;
 }
 
-// Whether the kernels that move whole 64-k tiles can run the operands: codes in whole words of a block's half, two scales at once.
-bool whole(const FusedArgs& p) {
-  const uintptr_t sb = (uintptr_t)p.s | (p.asym ? (uintptr_t)p.b : 0);
-  return p.K % 64 == 0 && (p.group == 32 || p.K % 128 == 0) && (uintptr_t)p.q % (p.bits == 4 ? 16 : 4) == 0 && sb % 4 == 0;
+// Rows from .. from + M - 1 of a call.
+FusedArgs part_of(const FusedArgs& p, int from, int M) {
+  FusedArgs x = p;
+  x.M = M;
+  x.a = (const char*)p.a + (size_t)from * p.K * 2;
+  if (p.res) x.res = (const char*)p.res + (size_t)from * p.res_stride * (p.res_f32 ? 4 : 2);
+  if (p.out) x.out = (char*)p.out + (size_t)from * p.out_stride * (p.out_f32 ? 4 : 2);
+  if (p.rec) x.rec = p.rec + (size_t)from * ((p.N + kLpBlock - 1) / kLpBlock);
+  return x;
+}
+// A call that one launch cannot hold, in two parts of its rows.
+template <class Launch>
+hipError_t in_parts(const FusedArgs& p, hipStream_t s, Launch launch) {
+  const int first = fused::first_part(p.M);
+  if (!first) return hipErrorInvalidValue;
+  const hipError_t e = launch(part_of(p, 0, first), s);
+  return e == hipSuccess ? launch(part_of(p, first, p.M - first), s) : e;
 }
 
 }  // namespace
 
 hipError_t launch_fused(const FusedArgs& p, hipStream_t s) {
-  const fused::Plan plan = fused::plan({p.M, p.half ? p.half : p.N, p.K, p.half != 0, p.asym != 0, whole(p), p.K % (32 * p.group) == 0, p.bits});
+  const fused::Shape shape{p.M, p.half ? p.half : p.N, p.K, p.half != 0, p.asym != 0, whole(p), p.K % (32 * p.group) == 0, p.bits};
+  const fused::Plan plan = fused::plan(shape);
   if (plan.path == fused::kLanes) return launch_fused_lanes(p, s);
   if (plan.path == fused::kRows) return launch_fused_rows(p, plan.a, plan.b, s);
   if (plan.path == fused::kTiles) return launch_fused_tiles(p, plan.a, plan.b, plan.halves, s);
+  if (!fused::launchable(shape, plan)) return in_parts(p, s, launch_fused);
   return launch_any<kEpiAct>(p, s);
 }
 
 hipError_t launch_logit_records(const FusedArgs& p, hipStream_t s) {
+  if (!fused::logits_fit(p.M, p.N, whole(p), p.asym != 0)) return in_parts(p, s, launch_logit_records);
   return whole(p) ? launch_logit_tiles(p, s) : launch_any<kEpiLogits>(p, s);
 }
 

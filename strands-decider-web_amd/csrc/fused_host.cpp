@@ -88,6 +88,8 @@ int ha_mnb_fused(ha_mnb* w, int M, const void* a, const ha_epilogue* e, void* ou
   f.half = e->gated ? cols : 0;
   f.act = e->act; f.bias = e->bias; f.out = out; f.out_f32 = e->out_dtype == HA_F32; f.out_stride = stride;
   f.res = e->residual; f.res_f32 = e->residual_dtype == HA_F32; f.res_stride = rstride;
+  if (!ha::whole(f) && !ha::fused::fits(ha::fused::any_groups({16, cols, f.K, f.half != 0, f.asym != 0, false, false}), ha::fused::kAnyThreads))
+    return bad("a weight of more than 2^29 - 64 rows needs K and an alignment that the fast kernels take");
   ha::OnDevice on(device);
   if (on.rc != hipSuccess) return hip_error("hipSetDevice", on.rc);
   const hipError_t he = ha::launch_fused(f, (hipStream_t)stream);

@@ -17,11 +17,12 @@
 
 #include "fused.h"
 #include "fused_common.h"
+#include "fused_plan.h"
 
 namespace ha {
 namespace {
 
-constexpr int kLanesWaves = 4;
+constexpr int kLanesWaves = fused::kLanesThreads / 64;
 
 // V values of each lane (1, 2 or 4), summed over the lanes: row r = l / 16 of lanes gets that of value r % V. Pairs meet in one
 // register, so four values cost hardly more than one.
@@ -151,6 +152,7 @@ __global__ __launch_bounds__(64 * kLanesWaves) void fused_lanes_kernel(FusedArgs
 template <int BITS, bool ASYM, int MR>
 hipError_t launch_lanes_as(const FusedArgs& p, hipStream_t s) {
   const int cols = p.half ? p.half : p.N, wide = kLanesWaves * (p.half ? 1 : 2);
+  if (!fused::fits((cols + wide - 1) / wide, 64 * kLanesWaves)) return hipErrorInvalidValue;
   hipLaunchKernelGGL((fused_lanes_kernel<BITS, ASYM, MR>), dim3((unsigned)((cols + wide - 1) / wide)), dim3(64 * kLanesWaves), (size_t)MR * p.K * 2, s, p);
   return hipGetLastError();
 }

@@ -23,11 +23,33 @@ struct Plan {
   int halves = 1;
 };
 
+constexpr int kLanesRows = 2, kLanesValues = 32768;  // rows and values of a that the lanes kernel takes
+
 // Workgroups of a product with tiles of `rows` x `weights` columns of weights.
 inline long groups(const Shape& p, int rows, int weights) {
   const int wide = p.gated ? weights / 2 : weights;
   return (long)((p.cols + wide - 1) / wide) * ((p.M + rows - 1) / rows);
 }
+
+// A launch has fewer than 2^32 threads (HIP's limit).
+inline bool fits(long workgroups, int threads) { return workgroups <= ((1l << 32) - 1) / threads; }
+// Threads of a workgroup. The rows kernel splits a long K of few rows over 16 waves where its workgroups are the fewest (1 x 1 tiles of
+// 2048 x 6144: 1 row 7.0 -> 6.1 us, 16 rows 7.4 -> 7.2; 2048 x 2048, 4.1 -> 4.3).
+constexpr int kAnyThreads = 512, kLanesThreads = 256, kTileThreads = 256;
+inline int rows_waves(int M, int K, int a, int b) { return a == 1 && b == 1 && K >= 4096 && M <= 16 ? 16 : 8; }
+inline long any_groups(const Shape& p) { return groups(p, 16, 64); }
+inline long lanes_groups(const Shape& p) { return groups(p, kLanesRows, 8); }
+inline bool launchable(const Shape& p, const Plan& x) {
+  switch (x.path) {
+    case kAny: return fits(any_groups(p), kAnyThreads);
+    case kLanes: return fits(lanes_groups(p), kLanesThreads);
+    case kRows: return fits(groups(p, 16 * x.a, 16 * x.b), 64 * rows_waves(p.M, p.K, x.a, x.b));
+    case kTiles: return fits(groups(p, 32 * x.a, 128 * x.b), x.halves * kTileThreads);
+  }
+  return false;
+}
+// Rows of the first of two launches for a call that no kernel takes in one (0: it cannot be parted).
+inline int first_part(int M) { return M > 16 ? (M / 2 + 15) / 16 * 16 : 0; }
 
 // What asymmetric weights and 3 bits cost where arithmetic counts: 1744 x 2560 x 2560, us, rows 4 x 2 and tiles 2 x 1, 4 bits 56 and 49,
 // asymmetric 75 and 74, 3 bits 74 and 58, both 84 and 88 (2 bits as 4).
@@ -63,19 +85,24 @@ inline float halves_us(const Shape& p) {
 }
 // The lanes kernel (one or two rows that fit 64 KiB of LDS; any alignment). Times in fused_lanes.h; each 2048 k are a step, each 2048
 // columns a wave on every SIMD.
-constexpr int kLanesRows = 2, kLanesValues = 32768;
 inline float lanes_us(const Shape& p) {
   const float x = std::max(1.0f, p.K / 2048.0f), n = std::max(1.0f, p.cols * (p.gated ? 2.0f : 1.0f) / 2048.0f);
   return p.M == 1 ? 2.1f + 0.75f * x + 0.6f * (n - 1.0f) * x : 2.2f + x + 0.85f * (n - 1.0f) * x;
 }
 
-inline Plan plan(const Shape& p) {
+// The fastest kernel, or the fastest of those that one launch suffices for.
+inline Plan fastest(const Shape& p, bool one_launch) {
   const bool lanes = p.M <= kLanesRows && p.M * p.K <= kLanesValues;
-  if (!p.whole) return {lanes ? kLanes : kAny, 0, 0, 0.0f};
   Plan best{kAny, 0, 0, 1e30f};
-  auto look = [&](Path path, int a, int b, float us) {
-    if (us < best.us) best = {path, a, b, us};
+  auto look = [&](Path path, int a, int b, float us, int halves = 1) {
+    const Plan x{path, a, b, us, halves};
+    if (us < best.us && (!one_launch || launchable(p, x))) best = x;
   };
+  if (!p.whole) {
+    if (lanes) look(kLanes, 0, 0, 0.0f);
+    else best.us = 0.0f;
+    return best;
+  }
   if (lanes) look(kLanes, 0, 0, lanes_us(p));
   for (int a : {1, 2, 4})
     for (int b : {1, 2, 3, 4}) look(kRows, a, b, rows_us(p, a, b));
@@ -83,11 +110,12 @@ inline Plan plan(const Shape& p) {
     for (int b : {1, 2})
       if ((!p.gated || b == 2) && !(p.asym && a * b > 4)) look(kTiles, a, b, tiles_us(p, a, b));  // (asymmetric 3 x 2, 4 x 2: too many registers)
   // (asymmetric: one such workgroup fits a CU)
-  if (p.halves && !p.gated && (!p.asym || groups(p, 64, 128) <= 256)) {
-    const float us = halves_us(p);
-    if (us < best.us) best = {kTiles, 2, 1, us, 2};
-  }
+  if (p.halves && !p.gated && (!p.asym || groups(p, 64, 128) <= 256)) look(kTiles, 2, 1, halves_us(p), 2);
   return best;
+}
+inline Plan plan(const Shape& p) {
+  const Plan best = fastest(p, false);
+  return launchable(p, best) ? best : fastest(p, true);
 }
 
 // The tile kernel's shape for logits, of so many columns that rounds of workgroups count for little: base + each for every 32 a rows.
@@ -102,6 +130,14 @@ inline Plan logit_tiles(int M, bool asym) {
     if (us < best.us && !(asym && x.b == 2)) best = {kTiles, x.a, x.b, us};
   }
   return best;
+}
+
+// Whether one launch makes a call's records. Vocabularies are up to 2^20: 16 rows always fit.
+inline bool logits_fit(int M, int n_vocab, bool whole, bool asym) {
+  const Shape p{M, n_vocab, 64, false, asym, whole, false};
+  if (!whole) return fits(any_groups(p), kAnyThreads);
+  const Plan x = logit_tiles(M, asym);
+  return fits(groups(p, 32 * x.a, 128 * x.b), kTileThreads);
 }
 
 // Whether log probabilities store the logits (f32) and read them back rather than leave records of 64 columns: in vocabularies up

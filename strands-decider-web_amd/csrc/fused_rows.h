@@ -15,6 +15,7 @@
 
 #include "fused.h"
 #include "fused_common.h"
+#include "fused_plan.h"
 #include "lds_dma.h"
 
 namespace ha {
@@ -216,7 +217,7 @@ hipError_t launch_rows_as(const FusedArgs& p, hipStream_t s) {
   }
   const int cols = p.half ? p.half : p.N, wide = p.half ? 8 * NT : 16 * NT;
   const long tiles = (long)((cols + wide - 1) / wide) * ((p.M + 16 * MT - 1) / (16 * MT));
-  if (tiles > 0x7FFFFFFFl) return hipErrorInvalidValue;
+  if (!fused::fits(tiles, 64 * SW)) return hipErrorInvalidValue;
   hipLaunchKernelGGL(k, dim3((unsigned)tiles), dim3(64 * SW), lds, s, p);
   return hipGetLastError();
 }

@@ -7,10 +7,7 @@ namespace {
 template <int BITS, bool ASYM>
 hipError_t launch(const FusedArgs& p, int mt, int nt, hipStream_t s) {
   switch (8 * mt + nt) {
-    case 9:
-      // The fewest workgroups that a long K is split over: 16 waves (2048 x 6144: 1 row 7.0 -> 6.1 us, 16 rows 7.4 -> 7.2; 2048 x
-      // 2048, 4.1 -> 4.3)
-      return p.K >= 4096 && p.M <= 16 ? launch_rows_as<BITS, ASYM, 1, 1, 16>(p, s) : launch_rows_as<BITS, ASYM, 1, 1, 8>(p, s);
+    case 9: return fused::rows_waves(p.M, p.K, 1, 1) == 16 ? launch_rows_as<BITS, ASYM, 1, 1, 16>(p, s) : launch_rows_as<BITS, ASYM, 1, 1, 8>(p, s);
     case 10: return launch_rows_as<BITS, ASYM, 1, 2, 8>(p, s);
     case 11: return launch_rows_as<BITS, ASYM, 1, 3, 8>(p, s);
     case 12: return launch_rows_as<BITS, ASYM, 1, 4, 8>(p, s);

@@ -20,13 +20,14 @@
 
 #include "fused.h"
 #include "fused_common.h"
+#include "fused_plan.h"
 #include "lds_dma.h"
 
 namespace ha {
 namespace {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
-constexpr int kTileWaves = 4;
+constexpr int kTileWaves = fused::kTileThreads / 64;
 
 // A workgroup's LDS and waves a SIMD. U: 128-k pieces whose scales come together.
 template <int BITS, bool ASYM, int RT, int CT, int KS>
@@ -361,7 +362,7 @@ hipError_t launch_tiles(const FusedArgs& p, hipStream_t s) {
   const int cols = gated ? p.half : p.N, wide = kTileWaves * (gated ? 32 : 32 * CT);
   if (CT == 1 && gated) return hipErrorInvalidValue;  // (a pair of column tiles a wave)
   const long tiles = (long)((cols + wide - 1) / wide) * ((p.M + 32 * RT - 1) / (32 * RT));
-  if (tiles > 0x7FFFFFFFl) return hipErrorInvalidValue;
+  if (!fused::fits(tiles, 64 * kTileWaves * KS)) return hipErrorInvalidValue;
   // Groups of 64 are a tile's 64 k: where the pairs' sums have registers, both halves are one sum, scaled once
   auto k = fused_tiles_kernel<BITS, ASYM, EPI, RT, CT, KS, false>;
   if constexpr (RT == 2 && CT == 1) {

@@ -1,0 +1,60 @@
+"""What the products whose results are not stored as they are launch, on the CPU (tests/fused_launches.py)."""
+import os
+
+import pytest
+
+from fused_launches import CXX, HIPCC, ask, fused, logprobs
+
+pytestmark = pytest.mark.skipif(not (os.path.exists(HIPCC) and os.path.exists(CXX)), reason="hipcc is missing")
+ROWS = [1, 2, 3, 16, 17, 33, 100, 1000, 65537, 1 << 20]
+
+
+def parts(launches, M):
+    """The launches take each of M rows once, in order."""
+    assert sum(x.rows for x in launches) == M
+    at = 0
+    for x in launches:
+        yield x, at
+        at += x.rows
+
+
+def small(x):
+    return 0 < x.groups * x.threads < 1 << 32
+
+
+def test_threads_of_products():
+    """HIP takes launches of fewer than 2^32 threads: calls of more are parted by rows, or go to a kernel with fewer."""
+    calls = [(M, N, K, fmt, gated, q_at) for M in ROWS for N in (2, 1000, 12288, 248320, 1 << 24, 1 << 27, (1 << 29) - 64, 1 << 30)
+             for K in (32, 64, 2048, 2080, 4096) for fmt in ((4, 32, False), (3, 32, True)) for gated in (False, True) for q_at in (0, 2 * 4) if M * N <= 1 << 40]
+    parted = 0
+    for (M, N, K, fmt, gated, q_at), got in zip(calls, ask([fused(*c[:5], q_at=c[5]) for c in calls])):
+        case = (M, N, K, fmt, gated, q_at)
+        fast = K % 64 == 0 and (q_at == 0 or fmt[0] != 4)
+        if N > (1 << 29) - 64 and not fast:
+            assert got.status == -1 and "2^29" in got.refusal and not got.launches, case
+            continue
+        assert got.status == 0, (case, got)
+        cols = N // 2 if gated else N
+        for x, row in parts(got.launches, M):
+            assert small(x), (case, x)
+            assert (x.a, x.out, x.residual) == (row * K * 2, row * cols * 4, row * cols * 2), (case, x)
+        parted += len(got.launches) > 1
+    assert parted
+
+
+def test_threads_of_log_probabilities():
+    calls = [(M, V, K, fmt) for M in ROWS + [20000, 40000] for V in (1, 100, 5000, 32768, 32769, 248320, 1 << 20) for K in (32, 64, 256, 2080)
+             for fmt in ((4, 32, False), (2, 64, True)) if K % fmt[1] == 0]
+    parted = 0
+    for (M, V, K, fmt), got in zip(calls, ask([logprobs(*c, targets=2, top_k=1) for c in calls])):
+        case = (M, V, K, fmt)
+        assert got.status == 0, (case, got)
+        records = [x for x in got.launches if "logprobs_kernel" not in x.kernel]
+        joins = [x for x in got.launches if "logprobs_kernel" in x.kernel]
+        assert all(small(x) for x in got.launches), case
+        for x, row in parts(joins, M):
+            assert (x.groups, x.a, x.logp, x.lse, x.top_ids) == (x.rows, row * K * 2, row * 8, row * 4, row * 4), (case, x)
+        for x, row in parts(records, M):
+            assert x.a == row * K * 2 and (x.records < 0 or x.records == row * -(-V // 64) * 16), (case, x)
+        parted += len(records) > len(joins)
+    assert parted
