@@ -14,6 +14,7 @@ namespace ha {
 constexpr int kLpBlock = 64;     // columns of a block of logits (a record of its own)
 constexpr int kLpMargin = 8;     // blocks looked at beyond the top_k largest
 constexpr int kLpMaxTop = 64;    // top_k, at most
+constexpr int kLpMaxTargets = 1024;
 constexpr int kLpMaxVocab = 1 << 20;
 
 // What a 64-column block of a row's scaled logits comes to: its largest value, over the other columns the sums of e^(z - max)

@@ -45,7 +45,7 @@ int check_logprobs(const ha_logprobs* p, int N, int* n_vocab) {
   *n_vocab = p->n_vocab ? p->n_vocab : N;
   if (*n_vocab < 1 || *n_vocab > N) return bad("n_vocab must be in [1, " + std::to_string(N) + "], the table's rows");
   if (*n_vocab > ha::kLpMaxVocab) return bad("n_vocab must be at most 2^20");
-  if (p->n_targets < 0 || p->n_targets > 1024) return bad("n_targets must be in [0, 1024]");
+  if (p->n_targets < 0 || p->n_targets > ha::kLpMaxTargets) return bad("n_targets must be in [0, 1024]");
   if (p->top_k < 0 || p->top_k > ha::kLpMaxTop || p->top_k > *n_vocab) return bad("top_k must be in [0, 64] and at most n_vocab");
   if (!(p->scale >= 0.0f && p->scale <= 1e6f)) return bad("scale must be in [0, 1e6] (0: 1)");
   return HA_OK;

@@ -145,9 +145,10 @@ inline bool logits_fit(int M, int n_vocab, bool whole, bool asym) {
 // of the top_k largest, which costs 62 products in 64 bits each. Measured, us, records : stored: 1431 x 1383 x 256 top 20 1125 :
 // 51, 1 x 4284 x 640 (3 bits) top 32 178 : 25, 187 x 2507 x 4096 (3 bits) 114 : 35, 605 x 20658 x 192 top 20 108 : 106; the other
 // way, 2048 x 32768 x 2048 top 5 372, stored (top 30) 616; 1024 x 8192 x 2048 top 5 98, stored (top 12) 97.
+constexpr int kStoredVocab = 32768;
 inline bool store_logits(int M, int n_vocab, int top_k) {
   const int nb = (n_vocab + 63) / 64;
-  return nb <= 512 && (M <= 64 || top_k * top_k > nb || (long)((n_vocab + 255) / 256) * ((M + 127) / 128) < 256);
+  return n_vocab <= kStoredVocab && (M <= 64 || top_k * top_k > nb || (long)((n_vocab + 255) / 256) * ((M + 127) / 128) < 256);
 }
 
 }  // namespace fused

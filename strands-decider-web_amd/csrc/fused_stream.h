@@ -184,8 +184,8 @@ template <int BITS, bool ASYM, bool G64>
 hipError_t launch_stream_as(const FusedArgs& p, hipStream_t s) {
   const int lds = p.M * p.K * 2, nb = (p.N + kLpBlock - 1) / kLpBlock;
   auto k = fused_stream_kernel<BITS, ASYM, G64>;
-  if (lds > 48 * 1024) {
-    const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+  if (lds > 48 * 1024) {  // (the same limit for every call: it is the function's, not the launch's, and calls may overlap)
+    const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, kStreamLds);
     if (e != hipSuccess) return e;
   }
   hipLaunchKernelGGL(k, dim3((nb + kStreamWaves - 1) / kStreamWaves), dim3(64 * kStreamWaves), lds, s, p);

@@ -19,6 +19,7 @@
 
 #include "fused.h"
 #include "fused_common.h"
+#include "fused_plan.h"
 
 namespace ha {
 namespace {
@@ -265,16 +266,25 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
   }
 }
 
+// Dynamic LDS: keys and maxima of the list, values and columns of the candidates, targets. At most, over all vocabularies:
+constexpr int kLpLds = 128 * 1024;
+constexpr size_t lds_bytes(int list, int cand, int targets) { return 12 * (size_t)list + 12 * (size_t)cand + 4 * (size_t)targets; }
+constexpr int list_most(int T, bool stored) {
+  return (kLpMaxTop + kLpMargin) * (T / kLpSets) * (((stored ? fused::kStoredVocab : kLpMaxVocab / kLpBlock) + T - 1) / T);
+}
+constexpr int cand_most(bool stored) { return (kLpMaxTop + kLpMargin) * (stored ? 1 : kLpBlock) + kLpMaxTargets; }
+
 template <int BITS, bool ASYM, int T, bool STORED>
 hipError_t launch_as(const LpArgs& a, hipStream_t s) {
   const int nb = STORED ? a.p.N : (a.p.N + kLpBlock - 1) / kLpBlock, kk = std::min(a.top_k + kLpMargin, nb);
   // the kk sets of T / kLpSets threads that hold a key from the cut on (where there are fewer sets, all of them)
   const int list_cap = std::min(nb, kk * (T / kLpSets) * ((nb + T - 1) / T));
   const int cand_cap = (a.top_k > 0 && !STORED ? kk * kLpBlock : kk) + a.n_targets;
-  const size_t lds = 12 * (size_t)list_cap + 12 * (size_t)cand_cap + 4 * (size_t)a.n_targets;
+  const size_t lds = lds_bytes(list_cap, cand_cap, a.n_targets);
+  static_assert(lds_bytes(list_most(T, STORED), cand_most(STORED), kLpMaxTargets) <= kLpLds, "what a call may need");
   auto k = logprobs_kernel<BITS, ASYM, T, STORED>;
-  if (lds > 48 * 1024) {
-    const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (lds > 48 * 1024) {  // (the same limit for every call: it is the function's, not the launch's, and calls may overlap)
+    const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, kLpLds);
     if (e != hipSuccess) return e;
   }
   hipLaunchKernelGGL(k, dim3(a.p.M), dim3(T), lds, s, a, nb, list_cap, cand_cap);

@@ -58,3 +58,20 @@ def test_threads_of_log_probabilities():
             assert x.a == row * K * 2 and (x.records < 0 or x.records == row * -(-V // 64) * 16), (case, x)
         parted += len(records) > len(joins)
     assert parted
+
+
+def test_lds_limits_are_constants():
+    """A kernel's limit on dynamic LDS is the function's, in every thread: a call that set one of its own could take it from another
+    call's launch. So each kernel has one, which no launch exceeds."""
+    calls = [logprobs(M, V, K, fmt, targets=T, top_k=k) for M in (1, 7, 16, 40, 300, 3000) for V in (64, 2000, 5000, 32768, 40000, 248320, 1 << 20)
+             for K in (256, 2048, 4096, 8192) for T in (0, 1, 1024) for k in (0, 5, 64) for fmt in ((4, 32, False), (3, 64, True))]
+    limits, most = {}, {}
+    for got in ask(calls):
+        assert got.status == 0
+        for name, n in got.limits:
+            limits.setdefault(name, set()).add(n)
+        for x in got.launches:
+            most[x.kernel] = max(most.get(x.kernel, 0), x.lds)
+    assert len([n for n in most if "stream" in n and n in limits]) and len([n for n in most if "logprobs" in n and n in limits])
+    for name, n in most.items():
+        assert n <= 48 * 1024 or len(limits[name]) == 1 and n <= min(limits[name]) <= 128 * 1024, (name, n, limits[name])
