@@ -275,7 +275,8 @@ typedef struct ha_logprobs {
 } ha_logprobs;
 /* A row with a logit that is not finite gives NaN and top_ids of -1. The workspace (16-byte aligned device memory, as many bytes
    as ha_mnb_logprobs_bytes says) is the caller's and overlaps neither a nor targets nor outputs: calls that may overlap need one
-   each. */
+   each. Outputs overlap neither a nor targets (refused; logp alone may be the targets' own memory) nor each other (what is written there last
+   stays). */
 int ha_mnb_logprobs_bytes(const ha_mnb* w, int M, const ha_logprobs* p, size_t* bytes);
 int ha_mnb_logprobs(ha_mnb* w, int M, const void* a, const ha_logprobs* p, void* workspace, size_t bytes, void* stream);
 

@@ -1,6 +1,7 @@
 // Host side of the products whose results are not stored as they are (ha_mnb_fused, ha_mnb_logprobs, include/ha.h): checks of
 // arguments, launches of fused.hip and logprobs.hip. No counterpart in the reference.
 #include <cstdint>
+#include <iterator>
 #include <string>
 
 #include "fused.h"
@@ -121,11 +122,19 @@ int ha_mnb_logprobs(ha_mnb* w, int M, const void* a, const ha_logprobs* p, void*
     if (off(q, 4)) return bad("targets and outputs must be 4-byte aligned");
   const size_t need = workspace_bytes(M, n_vocab, p->top_k);
   if (!workspace || off(workspace, 16) || bytes < need) return bad("the workspace must be 16-byte aligned and have " + std::to_string(need) + " bytes");
-  const struct { const void* p; size_t n; } others[] = {{a, (size_t)M * l.p.K * 2}, {p->targets, 4 * (size_t)M * p->n_targets}, {p->logp, 4 * (size_t)M * p->n_targets},
+  // A row's results are written while other rows still read a and the targets
+  const struct Span { const void* p; size_t n; } others[] = {{a, (size_t)M * l.p.K * 2}, {p->targets, 4 * (size_t)M * p->n_targets}, {p->logp, 4 * (size_t)M * p->n_targets},
                                                         {p->entropy, 4 * (size_t)M}, {p->lse, 4 * (size_t)M}, {p->top_ids, 4 * (size_t)M * p->top_k},
                                                         {p->top_logp, 4 * (size_t)M * p->top_k}};
   for (const auto& x : others)
     if (x.p && x.n && overlap(workspace, need, x.p, x.n)) return bad("the workspace must not overlap a, the targets or an output");
+  const Span &rows = others[0], &targets = others[1];
+  for (const Span* x = others + 2; x != std::end(others); x++) {
+    if (!x->p || !x->n) continue;
+    if (overlap(x->p, x->n, rows.p, rows.n)) return bad("an output must not overlap a");
+    const bool in_place = x == others + 2 && x->p == targets.p;  // (a row's targets are read before its logp is written)
+    if (targets.p && targets.n && !in_place && overlap(x->p, x->n, targets.p, targets.n)) return bad("an output must not overlap the targets (logp may be them)");
+  }
   l.p.N = n_vocab;
   l.p.scale = p->scale > 0.0f ? p->scale : 1.0f;
   const bool stored = ha::fused::store_logits(M, n_vocab, p->top_k);

@@ -66,8 +66,12 @@ def ask(lines):
             status, nbytes = map(int, rest.split())
             answers.append(Answer(status, nbytes, refusal, launches, limits))
             launches, limits, refusal = [], [], ""
-    assert len(answers) == len(lines)
+    assert len(answers) == sum(l[0] != "put" for l in lines)
     return answers
+
+
+def put(output, base, at):
+    return ("put", output, base, at)
 
 
 def fused(M, N, K, fmt=(4, 32, False), gated=False, q_at=0, s_at=0):

@@ -3,6 +3,7 @@
 //   fused M N K bits group asym gated q_at s_at               (q_at, s_at: bytes past an aligned address)
 //   logprobs M V K bits group asym n_vocab targets top_k q_at bytes   (bytes: of the workspace; -1: as many as the call asks for)
 //   bytes M V K n_vocab targets top_k
+//   put <output> <a | targets> <bytes>           (the next call's output of that name stands there)
 // For each, the launches ("launch <kernel> <workgroups> <threads> <lds> <rows> <bytes from a, out, residual, records, logp, lse,
 // top_ids of the first row's>"), the functions' LDS limits that were set ("limit <kernel> <bytes>"), and "done <status> <bytes>".
 #include <hip/hip_runtime.h>
@@ -56,9 +57,14 @@ hipError_t hipLaunchKernel(const void* f, dim3 g, dim3 b, void** args, size_t ld
 }
 
 int main() {
-  char line[256], what[16];
+  char line[256], what[16], name[16], base[16];
+  std::map<std::string, void*> put;
   while (fgets(line, sizeof line, stdin)) {
     long v[11] = {};
+    if (sscanf(line, "put %15s %15s %ld", name, base, v) == 3) {
+      put[name] = (strcmp(base, "a") ? kTargets : kA) + v[0];
+      continue;
+    }
     if (sscanf(line, "%15s %ld %ld %ld %ld %ld %ld %ld %ld %ld %ld %ld", what, v, v + 1, v + 2, v + 3, v + 4, v + 5, v + 6, v + 7, v + 8, v + 9, v + 10) < 2) continue;
     ha::MnbArgs& w = weight.args;
     w = {};
@@ -69,6 +75,12 @@ int main() {
       ha_logprobs p = {};
       p.n_vocab = n_vocab; p.n_targets = targets; p.top_k = top_k;
       p.targets = (int*)kTargets; p.logp = (float*)kLogp; p.lse = (float*)kLse; p.top_ids = (int*)kIds; p.top_logp = (float*)kTop;
+      if (put.count("logp")) p.logp = (float*)put["logp"];
+      if (put.count("entropy")) p.entropy = (float*)put["entropy"];
+      if (put.count("lse")) p.lse = (float*)put["lse"];
+      if (put.count("top_ids")) p.top_ids = (int*)put["top_ids"];
+      if (put.count("top_logp")) p.top_logp = (float*)put["top_logp"];
+      put.clear();
       return p;
     };
     if (!strcmp(what, "bytes")) {

@@ -3,7 +3,7 @@ import os
 
 import pytest
 
-from fused_launches import CXX, HIPCC, ask, fused, logprobs
+from fused_launches import CXX, HIPCC, ask, fused, logprobs, put
 
 pytestmark = pytest.mark.skipif(not (os.path.exists(HIPCC) and os.path.exists(CXX)), reason="hipcc is missing")
 ROWS = [1, 2, 3, 16, 17, 33, 100, 1000, 65537, 1 << 20]
@@ -75,3 +75,22 @@ def test_lds_limits_are_constants():
     assert len([n for n in most if "stream" in n and n in limits]) and len([n for n in most if "logprobs" in n and n in limits])
     for name, n in most.items():
         assert n <= 48 * 1024 or len(limits[name]) == 1 and n <= min(limits[name]) <= 128 * 1024, (name, n, limits[name])
+
+
+def test_outputs_over_what_is_read():
+    """Rows are written while others read a and the targets: an output that overlaps them by a value is refused, one that ends where
+    they begin, or begins where they end, is not. logp may be the targets' own memory: a row reads its targets first."""
+    M, K, T, k = 7, 96, 3, 5
+    size = {"logp": 4 * M * T, "entropy": 4 * M, "lse": 4 * M, "top_ids": 4 * M * k, "top_logp": 4 * M * k}
+    read = {"a": 2 * M * K, "targets": 4 * M * T}
+    for V in (1000, 40000):
+        for name, n in size.items():
+            for base, m in read.items():
+                call = logprobs(M, V, K, targets=T, top_k=k)
+                at = {-n: True, -n + 4: False, 0: (name, base) == ("logp", "targets"), 4: False, m - 4: False, m: True}
+                for (x, fine), got in zip(at.items(), ask([y for x in at for y in (put(name, base, x), call)])):
+                    case = (V, name, base, x, got)
+                    if fine:
+                        assert got.status == 0 and len(got.launches) == 2, case
+                    else:
+                        assert got.status == -1 and "overlap" in got.refusal and not got.launches, case
