@@ -260,7 +260,8 @@ int ha_mnb_fused(ha_mnb* w, int M, const void* a, const ha_epilogue* e, void* ou
 
 /* Log probabilities over a vocabulary, from the final norm's rows and the table (an embedding table, where model and vocabulary
    share one): z[m][n] = scale a[m] . W[n] for n < n_vocab, p[m] = softmax(z[m]). Of larger vocabularies no logit is stored: the workspace
-   holds a few numbers for each 64 of them; where that is less work it holds the f32 logits of a smaller one. */
+   holds a few numbers for each 64 of them; where that is less work it holds the f32 logits of a smaller one, up to 1 GiB of them at a
+   time. */
 typedef struct ha_logprobs {
   int n_vocab;         /* the table's first n_vocab rows are tokens, up to 2^20 (0: all N; rows behind them are padding) */
   float scale;         /* of the logits, one over the temperature, up to 1e6 (0: 1) */
@@ -274,7 +275,7 @@ typedef struct ha_logprobs {
   float* top_logp;     /* device [M][top_k]: log p of those */
 } ha_logprobs;
 /* A row with a logit that is not finite gives NaN and top_ids of -1. The workspace (16-byte aligned device memory, as many bytes
-   as ha_mnb_logprobs_bytes says) is the caller's and overlaps neither a nor targets nor outputs: calls that may overlap need one
+   as ha_mnb_logprobs_bytes says, which suffice for every call of up to M rows of the same n_vocab and top_k) is the caller's and overlaps neither a nor targets nor outputs: calls that may overlap need one
    each. Outputs overlap neither a nor targets (refused; logp alone may be the targets' own memory) nor each other (what is written there last
    stays). */
 int ha_mnb_logprobs_bytes(const ha_mnb* w, int M, const ha_logprobs* p, size_t* bytes);

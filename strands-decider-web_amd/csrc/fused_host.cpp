@@ -1,5 +1,6 @@
 // Host side of the products whose results are not stored as they are (ha_mnb_fused, ha_mnb_logprobs, include/ha.h): checks of
 // arguments, launches of fused.hip and logprobs.hip. No counterpart in the reference.
+#include <algorithm>
 #include <cstdint>
 #include <iterator>
 #include <string>
@@ -52,11 +53,6 @@ int check_logprobs(const ha_logprobs* p, int N, int* n_vocab) {
   return HA_OK;
 }
 
-size_t workspace_bytes(int M, int n_vocab, int top_k) {
-  if (ha::fused::store_logits(M, n_vocab, top_k)) return (size_t)M * n_vocab * sizeof(float);
-  return (size_t)M * ((n_vocab + ha::kLpBlock - 1) / ha::kLpBlock) * sizeof(ha::LpRecord);
-}
-
 }  // namespace
 
 extern "C" {
@@ -105,7 +101,7 @@ int ha_mnb_logprobs_bytes(const ha_mnb* w, int M, const ha_logprobs* p, size_t* 
   if (!ha::mnb_weight(w, &g, &device)) return set_error(HA_ERR_HANDLE, "invalid MatMulNBits handle");
   if (M < 1 || M > 1 << 20) return bad("M must be in [1, 2^20]");
   if (int rc = check_logprobs(p, g.N, &n_vocab)) return rc;
-  *bytes = workspace_bytes(M, n_vocab, p->top_k);
+  *bytes = ha::fused::most_logits_bytes(M, n_vocab, p->top_k);
   return HA_OK;
 }
 
@@ -120,7 +116,7 @@ int ha_mnb_logprobs(ha_mnb* w, int M, const void* a, const ha_logprobs* p, void*
   for (const void* q : {(const void*)p->targets, (const void*)p->logp, (const void*)p->entropy, (const void*)p->lse, (const void*)p->top_ids,
                         (const void*)p->top_logp})
     if (off(q, 4)) return bad("targets and outputs must be 4-byte aligned");
-  const size_t need = workspace_bytes(M, n_vocab, p->top_k);
+  const size_t need = ha::fused::logits_bytes(M, n_vocab, p->top_k);
   if (!workspace || off(workspace, 16) || bytes < need) return bad("the workspace must be 16-byte aligned and have " + std::to_string(need) + " bytes");
   // A row's results are written while other rows still read a and the targets
   const struct Span { const void* p; size_t n; } others[] = {{a, (size_t)M * l.p.K * 2}, {p->targets, 4 * (size_t)M * p->n_targets}, {p->logp, 4 * (size_t)M * p->n_targets},
@@ -149,8 +145,18 @@ int ha_mnb_logprobs(ha_mnb* w, int M, const void* a, const ha_logprobs* p, void*
   l.top_k = p->top_k; l.top_ids = p->top_ids; l.top_logp = p->top_logp;
   ha::OnDevice on(device);
   if (on.rc != hipSuccess) return hip_error("hipSetDevice", on.rc);
-  hipError_t he = stored ? ha::launch_fused(l.p, (hipStream_t)stream) : ha::launch_logit_records(l.p, (hipStream_t)stream);
-  if (he == hipSuccess) he = ha::launch_logprobs(l, (hipStream_t)stream);
+  hipError_t he = hipSuccess;
+  for (int left = M; left > 0 && he == hipSuccess;) {  // (parts of stored logits stand in the same place)
+    const int part = l.p.M = stored ? std::min(left, ha::fused::stored_part(n_vocab)) : left;
+    he = stored ? ha::launch_fused(l.p, (hipStream_t)stream) : ha::launch_logit_records(l.p, (hipStream_t)stream);
+    if (he == hipSuccess) he = ha::launch_logprobs(l, (hipStream_t)stream);
+    l.p.a = (const char*)l.p.a + (size_t)part * l.p.K * 2;
+    if (l.n_targets) l.targets += (size_t)part * l.n_targets, l.logp += (size_t)part * l.n_targets;
+    if (l.entropy) l.entropy += part;
+    if (l.lse) l.lse += part;
+    if (l.top_k) l.top_ids += (size_t)part * l.top_k, l.top_logp += (size_t)part * l.top_k;
+    left -= part;
+  }
   return he == hipSuccess ? HA_OK : hip_error("log probabilities", he);
 }
 

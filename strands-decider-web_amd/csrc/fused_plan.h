@@ -2,6 +2,7 @@
 // formats alone (no HIP, so that a test can compile it by itself).
 #pragma once
 #include <algorithm>
+#include <cstddef>
 
 namespace ha {
 namespace fused {
@@ -146,9 +147,25 @@ inline bool logits_fit(int M, int n_vocab, bool whole, bool asym) {
 // 51, 1 x 4284 x 640 (3 bits) top 32 178 : 25, 187 x 2507 x 4096 (3 bits) 114 : 35, 605 x 20658 x 192 top 20 108 : 106; the other
 // way, 2048 x 32768 x 2048 top 5 372, stored (top 30) 616; 1024 x 8192 x 2048 top 5 98, stored (top 12) 97.
 constexpr int kStoredVocab = 32768;
-inline bool store_logits(int M, int n_vocab, int top_k) {
-  const int nb = (n_vocab + 63) / 64;
-  return n_vocab <= kStoredVocab && (M <= 64 || top_k * top_k > nb || (long)((n_vocab + 255) / 256) * ((M + 127) / 128) < 256);
+// The rows of a call up to which that is (0: none).
+inline int stored_rows(int n_vocab, int top_k) {
+  if (n_vocab > kStoredVocab) return 0;
+  if (top_k * top_k > (n_vocab + 63) / 64) return 0x7FFFFFFF;
+  return 255 / ((n_vocab + 255) / 256) * 128;  // fewer than 256 tiles of 128 x 256
+}
+inline bool store_logits(int M, int n_vocab, int top_k) { return M <= stored_rows(n_vocab, top_k); }
+// Rows whose logits are stored at a time: 1 GiB of them, whole tiles.
+inline int stored_part(int n_vocab) { return (1 << 28) / n_vocab / 128 * 128; }
+
+// Bytes that a call's logits or records take.
+inline size_t logits_bytes(int M, int n_vocab, int top_k) {
+  if (store_logits(M, n_vocab, top_k)) return (size_t)std::min(M, stored_part(n_vocab)) * n_vocab * 4;
+  return (size_t)M * ((n_vocab + 63) / 64) * 16;
+}
+// The most that a call of up to M rows takes: logits are 16 times the records' bytes, so fewer rows, where they are stored, may take more.
+inline size_t most_logits_bytes(int M, int n_vocab, int top_k) {
+  const int stored = std::min(M, stored_rows(n_vocab, top_k));
+  return std::max(logits_bytes(M, n_vocab, top_k), stored > 0 ? logits_bytes(stored, n_vocab, top_k) : 0);
 }
 
 }  // namespace fused

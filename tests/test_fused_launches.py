@@ -94,3 +94,22 @@ def test_outputs_over_what_is_read():
                         assert got.status == 0 and len(got.launches) == 2, case
                     else:
                         assert got.status == -1 and "overlap" in got.refusal and not got.launches, case
+
+
+def test_workspaces_serve_fewer_rows():
+    """The bytes asked for M rows never fall with M, and are taken by every call of fewer rows, although small calls store logits
+    where larger ones leave records of a sixteenth; stored logits are 1 GiB at most, in parts of the rows."""
+    rows = [1, 2, 16, 64, 65, 127, 128, 129, 255, 256, 257, 300, 1000, 8192, 8193, 20000, 32640, 32641, 1 << 20]
+    for V, k in [(1, 0), (255, 1), (1000, 3), (1000, 4), (5000, 5), (32000, 5), (32000, 22), (32000, 23), (32768, 0), (32768, 64), (32769, 64), (248320, 20)]:
+        need = [x.bytes for x in ask([("bytes", M, V, 64, 0, 0, k) for M in rows])]
+        assert need == sorted(need), (V, k, need)
+        assert all(n <= max(1 << 30, M * -(-V // 64) * 16) for M, n in zip(rows, need)), (V, k)
+        for M, got in zip(rows, ask([logprobs(M, V, 64, targets=1, top_k=k, workspace=need[-1]) for M in rows])):
+            assert got.status == 0, (V, k, M, got.refusal)
+        for i in range(1, len(rows)):
+            for M, got in zip(rows[:i + 1], ask([logprobs(M, V, 64, targets=1, top_k=k, workspace=need[i]) for M in rows[:i + 1]])):
+                assert got.status == 0, (V, k, M, rows[i], got.refusal)
+                joins = [x for x in got.launches if "logprobs_kernel" in x.kernel]
+                for x, row in parts(joins, M):
+                    assert (x.a, x.logp, x.lse, x.top_ids) == (row * 128, row * 4, row * 4, row * 4 * k if k else 0), (V, k, M, x)
+                    assert x.records >= 0 or x.out == 0 and x.rows * V * 4 <= min(need[i], 1 << 30), (V, k, M, x)

@@ -42,3 +42,19 @@ def test_log_probabilities():
     assert all(np.isfinite(x).all() for x in got.values())
     rows = some(M)
     tl.check({n: x[rows] for n, x in got.items()}, fr.logprobs(a[rows], W, 1.0, targets[rows], 5), 2, 5)
+
+
+def test_stored_logits_in_parts():
+    """More rows than have their logits in the workspace at a time."""
+    import torch
+    M, V, K, k = 8333, 32768, 64, 23
+    words, s, b, W = fr.weight(V, K, seed=34, std=2 / np.sqrt(K))
+    rng = np.random.default_rng(35)
+    a = rng.standard_normal((M, K)).astype(np.float16)
+    targets = rng.integers(0, V, (M, 2)).astype(np.int32)
+    c = tl.Call(tf.handle(words, s, b, V, K, (4, 32, False)), M, 0, 2, k, 0.0, targets)
+    assert c.ws.numel() == 1 << 30
+    got = c(torch.from_numpy(a).to(tf.DEV))
+    assert all(np.isfinite(x).all() for x in got.values())
+    rows = sorted({*some(M), 8191, 8192, 8193})
+    tl.check({n: x[rows] for n, x in got.items()}, fr.logprobs(a[rows], W, 1.0, targets[rows], k), 2, k)
