@@ -319,10 +319,11 @@ class MnbWeight:
         if M > 0:
             p._check(M, self._device)
             a = _kv_ptr(a, "a", _torch_type(F16), M * self.K, self._device)
-            if workspace_bytes is None and hasattr(workspace, "is_contiguous"):
-                if not (workspace.is_cuda and workspace.device.index == self._device and workspace.is_contiguous()):
-                    raise TypeError("workspace must be a contiguous tensor on GPU %d" % self._device)
-                workspace_bytes = workspace.numel() * workspace.element_size()
+            if hasattr(workspace, "is_contiguous"):
+                have = workspace.numel() * workspace.element_size()
+                workspace_bytes = have if workspace_bytes is None else workspace_bytes
+                if not (workspace.is_cuda and workspace.device.index == self._device and workspace.is_contiguous() and workspace_bytes <= have):
+                    raise TypeError("workspace must be a contiguous tensor of %d bytes on GPU %d" % (workspace_bytes, self._device))
         _check(_lib.ha_mnb_logprobs(self._h, M, _ptr(a), p._ref, _ptr(workspace), workspace_bytes or 0, _st(stream)))
 
     def close(self):
