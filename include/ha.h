@@ -298,7 +298,7 @@ int ha_embed(const ha_mnb* table, int L, const void* ids, void* x, void* stream)
    if y != NULL first x[s] += y[s] (f32 += f16, written back), then
    h[r] = x[s] * (mean(x[s]^2) + eps)^-1/2 * w   (w: D f32, already 1 + w where the model says so),
    h f16, or f32 when out_f32 (the final norm, engine.js:283-284, 342). x has nx rows of D (D % 8 == 0, D <= 8192);
-   a source row >= nx gives a NaN output row. */
+   a source row >= nx gives a NaN output row. With y a source row is listed once at most: each output row adds to its own. */
 int ha_add_norm(int R, int D, int nx, void* x, const void* y, const float* w, void* h, int out_f32,
                 const void* rows, float eps, int device, void* stream);
 

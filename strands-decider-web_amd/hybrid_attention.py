@@ -718,7 +718,9 @@ class Torso:
             o = torch.empty(L, D, dtype=f16, device=self.dev)
             y = torch.empty(L, D, dtype=f16, device=self.dev)
             mid = torch.empty(L, I, dtype=f16, device=self.dev)
-            rd = torch.as_tensor(np.asarray(rows or [0], np.uint32).view(np.int32)).to(self.dev)
+            rows_on = lambda r: torch.as_tensor(np.asarray(r or [0], np.uint32).view(np.int32)).to(self.dev)  # noqa: E731
+            rd, once = rows_on(rows), list(dict.fromkeys(rows))
+            rd_once = rows_on(once) if len(once) < len(rows) else None
             out = torch.empty(len(rows), D, dtype=f16 if ask else f32, device=self.dev)
             add = Epilogue(residual=x, out_dtype=F32) if self.fused else None  # x += the product
             gate = Epilogue("silu", gated=True)
@@ -759,8 +761,12 @@ class Torso:
                     step(S + "silu", lambda: silu_mul(L, I, big, mid, device=self.device, stream=st))
                 step(S + "down", lambda: onto(p + "down", mid))
             if rows:
-                step("final_norm", lambda: add_norm(len(rows), D, L, x, left, self.v["final_norm"], out, out_f32=not ask,
-                                                    rows=rd, device=self.device, stream=st))
+                norm = lambda R, rd, left: add_norm(R, D, L, x, left, self.v["final_norm"], out, out_f32=not ask, rows=rd,  # noqa: E731
+                                                    device=self.device, stream=st)
+                if left is not None and rd_once is not None:  # a row that is asked for twice gets its sum once
+                    step("final_norm", lambda: norm(len(once), rd_once, left))
+                    left = None
+                step("final_norm", lambda: norm(len(rows), rd, left))
             if ask:
                 out = self._score(len(rows), out, ask)
             if timer:

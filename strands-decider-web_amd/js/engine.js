@@ -630,6 +630,12 @@ class Torso {
       const out = new Float32Array(ask ? 0 : R.length * D);
       if (R.length) {
         bufs.rows.upload(Uint32Array.from(R));
+        const once = Array.from(new Set(R));
+        if (left && once.length < R.length) {  // a row that is asked for twice gets its sum once
+          const at = this._buf('rows_once', 4 * once.length).upload(Uint32Array.from(once));
+          this._step('final_norm', () => this._norm(once.length, L, bufs.x, left, 'final_norm', bufs.out, !ask, at));
+          left = null;
+        }
         this._step('final_norm', () => this._norm(R.length, L, bufs.x, left, 'final_norm', bufs.out, !ask, bufs.rows));
       }
       const done = () => { if (timer) native.timerMark(timer, 1, this.lead._h); };

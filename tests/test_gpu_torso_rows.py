@@ -1,0 +1,63 @@
+"""A torso asked for the same row more than once, in both hosts: each time the row that a single request gives, bit for bit."""
+import json
+import os
+import shutil
+import subprocess
+
+import numpy as np
+import pytest
+
+import test_gpu_torso_model as tm
+from test_gpu_torso_model import D, I, TYPES, VOCAB
+
+pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+ROWS = [7, 3] + [7] * 4000 + [0, 3, 8, 8]  # more output rows than run at once
+
+
+@pytest.fixture(scope="module")
+def model():
+    return tm._model()
+
+
+@pytest.fixture(scope="module")
+def ids():
+    return np.random.default_rng(6).integers(0, VOCAB, 9).astype(np.uint32)
+
+
+@pytest.mark.parametrize("fused", [False, True])
+def test_rows(model, ids, fused, tmp_path):
+    W, V, Mx = model
+    t = tm._torso(W, V, Mx)
+    t.fused = fused
+    single, _ = t.forward(ids)
+    scores, _ = t.score(ids, top_k=3)
+    got, _ = t.forward(ids, ROWS)
+    assert np.array_equal(got, single[ROWS])
+    got, _ = t.score(ids, ROWS[:2] + ROWS[-4:], top_k=3)
+    for n, x in got.items():
+        assert np.array_equal(x, scores[n][ROWS[:2] + ROWS[-4:]]), n
+    again, _ = t.forward(ids, [8, 8])
+    assert np.array_equal(again, single[[8, 8]])
+    node = shutil.which("node")
+    if node is None:
+        pytest.skip("node is not installed")
+    d = str(tmp_path)
+    spec = {"types": TYPES, "D": D, "I": I, "rows": ROWS, "fused": fused, "weights": {k: {"N": v[2], "K": v[3]} for k, v in W.items()},
+            "vectors": sorted(V), "mixer": [[i, k] for i, k, _ in Mx]}
+    for name, (words, s, _, _) in W.items():
+        words.tofile(os.path.join(d, "w_%s.q" % name))
+        s.tofile(os.path.join(d, "w_%s.s" % name))
+    for name, v in V.items():
+        v.tofile(os.path.join(d, "v_%s.bin" % name))
+    for i, k, v in Mx:
+        v.tofile(os.path.join(d, "m_%d_%s.bin" % (i, k)))
+    ids.tofile(os.path.join(d, "ids.bin"))
+    with open(os.path.join(d, "spec.json"), "w") as f:
+        json.dump(spec, f)
+    r = subprocess.run([node, os.path.join(ROOT, "tests", "js", "napi_rows.js"), d], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert np.array_equal(np.fromfile(os.path.join(d, "hidden.bin"), np.float32).reshape(len(ROWS), D), single[ROWS])
+    many, _ = t.score(ids, ROWS, top_k=3)
+    assert np.array_equal(np.fromfile(os.path.join(d, "lse.bin"), np.float32), many["lse"])
+    assert np.array_equal(np.fromfile(os.path.join(d, "topIds.bin"), np.int32).reshape(-1, 3), many["top_ids"])
