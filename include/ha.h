@@ -271,10 +271,14 @@ typedef struct ha_logprobs {
   float* logp;         /* device [M][n_targets]: log p of the targets */
   float* entropy;      /* device [M] or NULL: -sum p log p, in nats */
   float* lse;          /* device [M] or NULL: log sum e^z */
-  int* top_ids;        /* device [M][top_k]: the largest first, equal ones by their number. In the order of the logits in 64 bits */
+  int* top_ids;        /* device [M][top_k]: the largest first, equal ones by their number, in the order of the logits in 64 bits (below) */
   float* top_logp;     /* device [M][top_k]: log p of those */
 } ha_logprobs;
-/* A row with a logit that is not finite gives NaN and top_ids of -1. The workspace (16-byte aligned device memory, as many bytes
+/* The largest tokens are found by f32 sums, which may be off by some 2^-23 (K / 16 + 40) of sum |a| |W|, and put in order by products in
+   64 bits. So top_ids are the largest by their logits in 64 bits as long as at most 8 tokens behind the top_k (where no logits are stored, at
+   most 8 blocks of 64 tokens behind the top_k largest blocks) come that near to the last of them, and no row of the table is many
+   times larger than those that are found.
+   A row with a logit that is not finite gives NaN and top_ids of -1. The workspace (16-byte aligned device memory, as many bytes
    as ha_mnb_logprobs_bytes says, which suffice for every call of up to M rows of the same n_vocab and top_k) is the caller's and overlaps neither a nor targets nor outputs: calls that may overlap need one
    each. Outputs overlap neither a nor targets (refused; logp alone may be the targets' own memory) nor each other (what is written there last
    stays). */

@@ -8,8 +8,10 @@
 // The top_k largest logits stand in the top_k blocks of the largest maxima: a block further down has nothing that top_k others
 // do not exceed (with fewer blocks than that, all are looked at). Their largest columns, and every column of such a block whose second
 // largest comes near the last of them, are multiplied out again in 64 bits, and so are the given tokens: sums in f32 differ by 1e-6 of
-// the logits, which is enough to change the order of two tokens. kLpMargin more blocks are looked at, and blocks are taken by (largest value, first block), so
-// that equal logits come in order too. The 64-bit values of the blocks' largest columns also replace their f32 ones in Z.
+// the logits, which is enough to change the order of two tokens. Near: within what f32 sums may be off, which goes with sum |a| |w| and
+// not with the logit (terms may cancel), so the chosen columns' own such sums are taken along. kLpMargin more blocks are looked at, and
+// blocks are taken by (largest value, first block), so that equal logits come in order too. The 64-bit values of the blocks' largest
+// columns also replace their f32 ones in Z.
 //
 // Smaller vocabularies, where two of the top_k often share a block, or whose blocks are too few workgroups, have their logits
 // stored in f32 by a product (fused.hip) and read here in the records' place (fused_plan.h says when).
@@ -47,12 +49,14 @@ __device__ __forceinline__ double sixteen_and(const unsigned* wd, int e) {
   return __builtin_bit_cast(double, (u64)(hi | 0x40300000u) << 32);
 }
 
-// a[m] . W[n] of two rows n in 64 bits, by one wave: lanes over the packed blocks.
+// a[m] . W[n] of two rows n in 64 bits, by one wave: lanes over the packed blocks. size: a bound on the larger sum |a| |w| (codes at their
+// largest: within some four times).
 template <int BITS, bool ASYM>
-__device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double* out) {
+__device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double* out, float* size) {
   const int nblk = p.K / 32, ng = p.K / p.group, gl = p.group == 64 ? 1 : 0;
   gptr<h8> ap = (gptr<h8>)(gp<_Float16>(p.a) + (size_t)m * p.K);
   out[0] = out[1] = 0.0;
+  float most = 0.0f;
   for (int k = lane; k < nblk; k += 64) {
     unsigned wd[2][BITS];
     float s[2], b[2] = {0.0f, 0.0f};
@@ -68,12 +72,15 @@ __device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double*
 #pragma unroll
     for (int j = 0; j < 4; j++) av[j] = ap[4 * k + j];
     double d[2] = {0.0, 0.0}, sum = 0.0;
+    float abs_sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
 #pragma unroll
       for (int e = 0; e < 8; e++) {
-        const double ad = (double)(float)av[j][e];
+        const float af = (float)av[j][e];
+        const double ad = (double)af;
         sum += ad;
+        abs_sum += fabsf(af);
 #pragma unroll
         for (int x = 0; x < 2; x++) d[x] = fma(ad, sixteen_and<BITS>(wd[x], 8 * j + e), d[x]);
       }
@@ -84,9 +91,14 @@ __device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double*
       out[x] += (double)s[x] * (d[x] - (16.0 + kMid) * sum);
       if constexpr (ASYM) out[x] += ((double)b[x] + kMid * (double)s[x]) * sum;
     }
+    constexpr float kCodes = ASYM ? 2 * kMid : kMid;
+    most = fmaf(fmaxf(kCodes * fabsf(s[0]) + fabsf(b[0]), kCodes * fabsf(s[1]) + fabsf(b[1])), abs_sum, most);
   }
 #pragma unroll
   for (int x = 0; x < 2; x++) out[x] = wave_sum(out[x]);
+#pragma unroll
+  for (int d = 32; d >= 1; d /= 2) most += __shfl_xor(most, d);
+  *size = most;
 }
 
 // A workgroup of T threads for a row. Dynamic LDS: list_cap keys, cand_cap values, their columns, the targets, list_cap maxima. STORED: the row's
@@ -100,6 +112,7 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
   __shared__ double red[2][kWaves];
   __shared__ int chosen[kLpMaxTop + kLpMargin];
   __shared__ int n_list, n_cand;
+  __shared__ unsigned most;  // bits of the largest bound on a chosen column's sum |a| |w|
   u64* list = (u64*)sm;
   double* val = (double*)(list + list_cap);
   int* ids = (int*)(val + cand_cap);
@@ -127,19 +140,19 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
 #pragma unroll 4
     for (int i = tid + kKeep * T; i < nb; i += T) f(record(i), i);
   };
-  float most = kNoLogit;
+  float top = kNoLogit;
   int at = -1;
   bool bad = false;
   each([&](const LpRecord& r, int i) {
     bad |= !(fabsf(r.max) <= 3.4e38f && fabsf(r.rest) <= 3.4e38f && fabsf(r.rest_z) <= 3.4e38f);
-    if (r.max > most) most = r.max, at = i;
+    if (r.max > top) top = r.max, at = i;
   });
-  u64 mine = at < 0 ? 0 : key_of(most, at);
+  u64 mine = at < 0 ? 0 : key_of(top, at);
   // the largest key of every T / kLpSets threads (0: no block)
 #pragma unroll
   for (int d = 1; d < T / kLpSets; d *= 2) mine = max(mine, (u64)__shfl_xor((long long)mine, d));
   if (tid % (T / kLpSets) == 0) best[tid / (T / kLpSets)] = mine;
-  if (tid == 0) n_list = 0, n_cand = 0;
+  if (tid == 0) n_list = 0, n_cand = 0, most = 0;
   if (__syncthreads_or(bad)) {  // a logit that is not finite
     const float nan = __builtin_nanf("");
     for (int t = tid; t < nt; t += T) a.logp[(size_t)m * nt + t] = nan;
@@ -201,42 +214,58 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
   zx = wave_sum(zx);
   if (lane == 0) red[0][w] = z, red[1][w] = zx;
   __syncthreads();
-  // candidates: the chosen blocks' largest columns, and blocks whose second largest may be among the top_k
+  // candidates: the chosen blocks' largest columns, then all others of blocks whose second largest may be among the top_k. Their values
+  // stand behind those of the targets.
+  unsigned second = 0;
+  int arg = 0;
+  float last = 0.0f;
   if (STORED && tid < kk) ids[tid] = chosen[tid];
   if (!STORED && tid < kk) {
-    const int i = chosen[tid];
-    const LpRecord r = rec[i];
-    const int arg = (int)(r.second & 63u);
-    ids[tid] = kLpBlock * i + arg;
-    if (k > 0) {
-      const float last = rec[chosen[min(k, kk) - 1]].max;
-      const float near = last - fmaxf(fabsf(M), fabsf(last)) * 0x1p-12f;
-      if (kk < k || unordered(r.second & ~63u) >= near) {
-        const int cols = min(kLpBlock, n_vocab - kLpBlock * i);
-        int at = kk + atomicAdd(&n_cand, cols - 1);
-        for (int c = 0; c < cols; c++)
-          if (c != arg) ids[at++] = kLpBlock * i + c;
+    const LpRecord r = rec[chosen[tid]];
+    arg = (int)(r.second & 63u);
+    second = r.second & ~63u;
+    ids[tid] = kLpBlock * chosen[tid] + arg;
+    if (k > 0) last = rec[chosen[min(k, kk) - 1]].max;
+  }
+  __syncthreads();
+  int from = 0, to = kk + nt;
+#pragma unroll 1
+  while (true) {
+    for (int i = from + 2 * w; i < to; i += 2 * kWaves) {
+      int n[2];
+      bool token[2];
+#pragma unroll
+      for (int x = 0; x < 2; x++) {
+        const int at = min(i + x, to - 1), id = at < kk ? ids[at] : at < kk + nt ? wanted[at - kk] : ids[at - nt];
+        token[x] = (unsigned)id < (unsigned)n_vocab;  // (no token: its log probability is NaN)
+        n[x] = token[x] ? id : 0;
       }
+      double d[2];
+      float size;
+      dot64<BITS, ASYM>(a.p, m, n, lane, d, &size);
+#pragma unroll
+      for (int x = 0; x < 2; x++)
+        if (lane == 0 && i + x < to) val[i + x] = token[x] ? (double)a.p.scale * d[x] : __builtin_nan("");
+      if (!STORED && lane == 0 && i < kk) atomicMax(&most, __builtin_bit_cast(unsigned, size));
     }
+    __syncthreads();
+    if (STORED || k == 0 || from > 0) break;
+    // Two f32 sums of K / 32 groups: K / 32 additions and as many products, 40 within groups and reductions, each off by 2^-23 of
+    // sum |a| |w| at most
+    const float off = 2.0f * ((float)a.p.K / 16.0f + 40.0f) * 0x1p-23f * a.p.scale * __builtin_bit_cast(float, most);
+    if (tid < kk && (kk < k || unordered(second) >= last - off)) {
+      const int base = kLpBlock * chosen[tid], cols = min(kLpBlock, n_vocab - base);
+      int at = kk + atomicAdd(&n_cand, cols - 1);
+      for (int c = 0; c < cols; c++)
+        if (c != arg) ids[at++] = base + c;
+    }
+    __syncthreads();
+    if (n_cand == 0) break;
+    from = to;
+    to += n_cand;
   }
-  __syncthreads();
   const int nc = kk + n_cand;
-  for (int i = 2 * w; i < nc + nt; i += 2 * kWaves) {
-    int n[2];
-    bool token[2];
-#pragma unroll
-    for (int x = 0; x < 2; x++) {
-      const int at = min(i + x, nc + nt - 1), id = at < nc ? ids[at] : wanted[at - nc];
-      token[x] = (unsigned)id < (unsigned)n_vocab;  // (no token: its log probability is NaN)
-      n[x] = token[x] ? id : 0;
-    }
-    double d[2];
-    dot64<BITS, ASYM>(a.p, m, n, lane, d);
-#pragma unroll
-    for (int x = 0; x < 2; x++)
-      if (lane == 0 && i + x < nc + nt) val[i + x] = token[x] ? (double)a.p.scale * d[x] : __builtin_nan("");
-  }
-  __syncthreads();
+  auto value = [&](int i) { return val[i < kk ? i : i + nt]; };  // of candidate i
   // every wave: the sums, with the chosen blocks' largest columns from 64 bits
   z = lane < kWaves ? red[0][lane] : 0.0;
   zx = lane < kWaves ? red[1][lane] : 0.0;
@@ -251,15 +280,15 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
   auto logp = [&](double v) { return (float)((v - (double)M) - log_z); };
   if (tid == 0 && a.entropy) a.entropy[m] = (float)(log_z - zx / z);
   if (tid == 0 && a.lse) a.lse[m] = (float)((double)M + log_z);
-  for (int t = tid; t < nt; t += T) a.logp[(size_t)m * nt + t] = logp(val[nc + t]);
+  for (int t = tid; t < nt; t += T) a.logp[(size_t)m * nt + t] = logp(val[kk + t]);
   if (k > 0) {
     for (int i = w; i < nc; i += kWaves) {
-      const double v = val[i];
+      const double v = value(i);
       const int id = ids[i];
       int rank = 0;
       for (int j = 0; j < nc; j += 64) {
         const int at = min(j + lane, nc - 1);
-        rank += __popcll(__ballot(j + lane < nc && (val[at] > v || (val[at] == v && ids[at] < id))));
+        rank += __popcll(__ballot(j + lane < nc && (value(at) > v || (value(at) == v && ids[at] < id))));
       }
       if (lane == 0 && rank < k) a.top_ids[(size_t)m * k + rank] = id, a.top_logp[(size_t)m * k + rank] = logp(v);
     }
