@@ -70,6 +70,12 @@ def ask(lines):
     return answers
 
 
+def kernels():
+    """All kernels of the compiled files."""
+    r = subprocess.run([program()], input="kernels\n", capture_output=True, text=True, timeout=60)
+    return {kernel(l.split()[1]) for l in r.stdout.splitlines()}
+
+
 def put(output, base, at):
     return ("put", output, base, at)
 

@@ -4,6 +4,7 @@
 //   logprobs M V K bits group asym n_vocab targets top_k q_at bytes   (bytes: of the workspace; -1: as many as the call asks for)
 //   bytes M V K n_vocab targets top_k
 //   put <output> <a | targets> <bytes>           (the next call's output of that name stands there)
+//   kernels                                      (lines "kernel <name>" of all there are)
 // For each, the launches ("launch <kernel> <workgroups> <threads> <lds> <rows> <bytes from a, out, residual, records, logp, lse,
 // top_ids of the first row's>"), the functions' LDS limits that were set ("limit <kernel> <bytes>"), and "done <status> <bytes>".
 #include <hip/hip_runtime.h>
@@ -61,6 +62,10 @@ int main() {
   std::map<std::string, void*> put;
   while (fgets(line, sizeof line, stdin)) {
     long v[11] = {};
+    if (!strncmp(line, "kernels", 7)) {
+      for (const auto& x : names()) printf("kernel %s\n", x.second.c_str());
+      continue;
+    }
     if (sscanf(line, "put %15s %15s %ld", name, base, v) == 3) {
       put[name] = (strcmp(base, "a") ? kTargets : kA) + v[0];
       continue;

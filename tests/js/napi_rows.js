@@ -1,7 +1,7 @@
 'use strict';
 // A Torso of the Node host asked for rows more than once. The directory named by the first argument holds the model as
 // tests/js/napi_fused.js reads it (spec.json {types, D, I, rows, fused, weights, vectors, mixer}, w_<name>.q / .s, v_<name>.bin,
-// m_<i>_<name>.bin, ids.bin); writes hidden.bin and lse.bin, topIds.bin of its score.
+// m_<i>_<name>.bin, ids.bin); writes hidden.bin and, of its score (of spec.ask where there is one), lse.bin, topIds.bin, logp.bin.
 const fs = require('fs');
 const path = require('path');
 const ha = require(path.join(__dirname, '..', '..', 'strands-decider-web_amd', 'js', 'engine.js'));
@@ -19,9 +19,8 @@ spec.vectors.forEach((name) => torso.setParam(name, new Float32Array(raw('v_' + 
 spec.mixer.forEach(([i, name]) => torso.setParam('layers.' + i + '.' + name, new Float32Array(raw('m_' + i + '_' + name + '.bin'))));
 const ids = Array.from(new Uint32Array(raw('ids.bin')));
 save('hidden.bin', torso.forward(ids, spec.rows).hidden);
-const s = torso.score(ids, spec.rows, { topK: 3 });
-save('lse.bin', s.lse);
-save('topIds.bin', s.topIds);
+const s = torso.score(ids, spec.rows, spec.ask || { topK: 3 });
+['lse', 'topIds', 'logp'].forEach((k) => save(k + '.bin', s[k]));
 torso.dropWeights();
 keep.forEach((b) => b.free());
 torso.destroy();

@@ -43,3 +43,24 @@ def test_calls_of_many_sizes():
     for (c, _), x in zip(calls, want):
         for n in x:
             assert np.array_equal(getattr(c, n).cpu().numpy(), x[n], equal_nan=True), n
+
+
+def test_a_graph_of_a_call_with_much_lds():
+    """Captured and replayed with the program's own calls between: 128 KiB of rows in LDS, 1024 targets and the 64 largest in the join."""
+    import torch
+    K, V, M = 4096, 40000, 16
+    words, s, b, _ = fr.weight(V, K, seed=52)
+    w = tl.handle(words, s, b, V, K, (4, 32, False))
+    targets = np.random.default_rng(53).integers(0, V, (M, 1024)).astype(np.int32)
+    a = torch.randn(M, K, device=tl.DEV).half()
+    one, two = (tl.Call(w, M, 0, 1024, 64, 0.0, targets) for _ in range(2))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):  # (nothing ran before it)
+        w.logprobs(M, a, two.p, two.ws, stream=torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        a.copy_(torch.randn(M, K, device=tl.DEV).half())
+        g.replay()
+        torch.cuda.synchronize()
+        want = one(a)
+        for n in want:
+            assert np.array_equal(getattr(two, n).cpu().numpy(), want[n]), n
