@@ -12,6 +12,8 @@
 // not with the logit (terms may cancel), so the chosen columns' own such sums are taken along. kLpMargin more blocks are looked at, and
 // blocks are taken by (largest value, first block), so that equal logits come in order too. The 64-bit values of the blocks' largest
 // columns also replace their f32 ones in Z.
+// (The sizes cost 1 us of 78 to 90 for 8 rows x 248320, top 20, and 2 where a block is multiplied out, behind the other products; those that
+// come within 2^-12 of the largest logits at once, beside the others, gains nothing.)
 //
 // Smaller vocabularies, where two of the top_k often share a block, or whose blocks are too few workgroups, have their logits
 // stored in f32 by a product (fused.hip) and read here in the records' place (fused_plan.h says when).
@@ -49,10 +51,10 @@ __device__ __forceinline__ double sixteen_and(const unsigned* wd, int e) {
   return __builtin_bit_cast(double, (u64)(hi | 0x40300000u) << 32);
 }
 
-// a[m] . W[n] of two rows n in 64 bits, by one wave: lanes over the packed blocks. size: a bound on the larger sum |a| |w| (codes at their
-// largest: within some four times).
-template <int BITS, bool ASYM>
-__device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double* out, float* size) {
+// a[m] . W[n] of two rows n in 64 bits, by one wave: lanes over the packed blocks. SIZE: returns a bound on the larger sum |a| |w| (codes
+// at their largest: within some four times), else 0.
+template <int BITS, bool ASYM, bool SIZE>
+__device__ float dot64(const FusedArgs& p, int m, const int* n, int lane, double* out) {
   const int nblk = p.K / 32, ng = p.K / p.group, gl = p.group == 64 ? 1 : 0;
   gptr<h8> ap = (gptr<h8>)(gp<_Float16>(p.a) + (size_t)m * p.K);
   out[0] = out[1] = 0.0;
@@ -80,7 +82,7 @@ __device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double*
         const float af = (float)av[j][e];
         const double ad = (double)af;
         sum += ad;
-        abs_sum += fabsf(af);
+        if constexpr (SIZE) abs_sum += fabsf(af);
 #pragma unroll
         for (int x = 0; x < 2; x++) d[x] = fma(ad, sixteen_and<BITS>(wd[x], 8 * j + e), d[x]);
       }
@@ -92,13 +94,15 @@ __device__ void dot64(const FusedArgs& p, int m, const int* n, int lane, double*
       if constexpr (ASYM) out[x] += ((double)b[x] + kMid * (double)s[x]) * sum;
     }
     constexpr float kCodes = ASYM ? 2 * kMid : kMid;
-    most = fmaf(fmaxf(kCodes * fabsf(s[0]) + fabsf(b[0]), kCodes * fabsf(s[1]) + fabsf(b[1])), abs_sum, most);
+    if constexpr (SIZE) most = fmaf(fmaxf(kCodes * fabsf(s[0]) + fabsf(b[0]), kCodes * fabsf(s[1]) + fabsf(b[1])), abs_sum, most);
   }
 #pragma unroll
   for (int x = 0; x < 2; x++) out[x] = wave_sum(out[x]);
+  if constexpr (SIZE) {
 #pragma unroll
-  for (int d = 32; d >= 1; d /= 2) most += __shfl_xor(most, d);
-  *size = most;
+    for (int d = 32; d >= 1; d /= 2) most += __shfl_xor(most, d);
+  }
+  return most;
 }
 
 // A workgroup of T threads for a row. Dynamic LDS: list_cap keys, cand_cap values, their columns, the targets, list_cap maxima. STORED: the row's
@@ -241,8 +245,9 @@ __global__ __launch_bounds__(T) void logprobs_kernel(LpArgs a, int nb, int list_
         n[x] = token[x] ? id : 0;
       }
       double d[2];
-      float size;
-      dot64<BITS, ASYM>(a.p, m, n, lane, d, &size);
+      float size = 0.0f;
+      if (!STORED && from == 0) size = dot64<BITS, ASYM, true>(a.p, m, n, lane, d);
+      else dot64<BITS, ASYM, false>(a.p, m, n, lane, d);
 #pragma unroll
       for (int x = 0; x < 2; x++)
         if (lane == 0 && i + x < to) val[i + x] = token[x] ? (double)a.p.scale * d[x] : __builtin_nan("");
@@ -319,9 +324,9 @@ hipError_t launch_as(const LpArgs& a, hipStream_t s) {
   hipLaunchKernelGGL(k, dim3(a.p.M), dim3(T), lds, s, a, nb, list_cap, cand_cap);
   return hipGetLastError();
 }
-// Few rows: 16 waves for each, more of its loads and products at once (one row over 248320 tokens, top 8: 19 -> 12 us). Many: as
-// many rows on a CU as their blocks leave work for (2048 x 248320, 3880 blocks: 8 waves 69 us; before the ranks were counted by waves 8
-// waves 75, 4 waves 92, and 1431 rows of 1383 logits 53 and 41).
+// Few rows: 16 waves for each, more of its loads and products at once (one row over 248320 tokens, top 8: 19 -> 12 us, 13 with the columns'
+// sizes). Many: as many rows on a CU as their blocks leave work for (2048 x 248320, 3880 blocks: 8 waves 71 us; before the ranks were
+// counted by waves 8 waves 75, 4 waves 92, and 1431 rows of 1383 logits 53 and 41).
 template <int BITS, bool ASYM, bool STORED>
 hipError_t launch_for(const LpArgs& a, hipStream_t s) {
   if (a.p.M <= 256) return launch_as<BITS, ASYM, 1024, STORED>(a, s);
