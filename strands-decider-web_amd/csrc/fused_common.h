@@ -2,7 +2,7 @@
 //
 // Weights stay exact. A code less 2^(bits-1) is a small integer, which f16 holds; the matrix unit sums its products with the 32
 // f16 values of a in f32, and the group's f16 scale multiplies that sum in f32 (one fma a sum). Against weights rounded to f16
-// before the product (mnb_common.h: 2^-12 of each weight) the sums are some 500 times nearer to 64 bits (3e-7 against 1.4e-4 of
+// before the product (mnb_common.h: up to 2^-11 of each weight) the sums are some 500 times nearer to 64 bits (3e-7 against 1.4e-4 of
 // their size at K = 2048), which results in f32 show, and the decoding has no multiplications. Asymmetric weights s c + b are
 // s (c - 2^(bits-1)) + b', b' = b + 2^(bits-1) s: b' times the group's sum of a, which a product with ones gives.
 #pragma once
@@ -167,7 +167,8 @@ __device__ __forceinline__ unsigned pack_second(float second, int arg) {
   return (min(ordered(second) >> 6, (1u << 26) - 2) + 1) << 6 | (unsigned)arg;
 }
 
-// What stands for a column that is none: below every logit (|z| < 10^23: f16 rows and scales, fused_host.cpp bounds the factor).
+// What stands for a column that is none: below every logit (|z| < 2 10^24: f16 rows, scales and biases, K up to 2^24 and the factor up
+// to 10^6, which fused_host.cpp sees to).
 constexpr float kNoLogit = -3e38f;
 
 // The record of a row's block of which this lane has the N columns col(0) < col(1) < ..., and the lanes at distance D, 2 D, ...

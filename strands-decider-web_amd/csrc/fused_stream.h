@@ -5,12 +5,12 @@
 // blocks 2 g and 2 g + 1 of column c, so that four lanes read whole 128-byte lines, and swaps of lane groups turn them into the operands
 // of v_mfma_f32_16x16x32_f16, of which lane (g, c) holds k 8 g .. + 7 of one 32-k group of column c: a 4 x 4 transposition of (lane
 // group, word). Four parts are on their way at any time. Along K first: the eight parts that share a column's line of scales follow
-// each other (16 columns after another for each 256 k, which shares the operands of a, fetched those lines again: 74 us for 63).
+// each other (16 columns after another for each 256 k, which shares the operands of a, fetched those lines again: a sixth slower).
 //
 // a stands in LDS, 16-byte chunk j of row r in slot j ^ (r & 15) of its 16.
 //
-// Bound: the table's bytes: 63 us for one row over 248320 tokens of 2048 (4 bits, groups of 32), 4.5 TB/s, 57 with groups of 64; with 3
-// and 2 bits (82 and 53) the vector unit: decoding, a swap a word, four fma a group. Products of up to 16 rows, with K split over the
+// Bound: the table's bytes: 67 us (65 at best) for one row over 248320 tokens of 2048 (4 bits, groups of 32), 4.3 TB/s, 57 with groups of
+// 64; with 3 and 2 bits (83 and 54) the vector unit: decoding, a swap a word, four fma a group. Products of up to 16 rows, with K split over the
 // waves of a workgroup, gained nothing on the rows kernel this way (1 x 12288 x 2048 7.5 : 7.4 us, 8 rows 8.3 : 7.2).
 #pragma once
 #include <hip/hip_runtime.h>
