@@ -264,7 +264,7 @@ int ha_mnb_fused(ha_mnb* w, int M, const void* a, const ha_epilogue* e, void* ou
    time. */
 typedef struct ha_logprobs {
   int n_vocab;         /* the table's first n_vocab rows are tokens, up to 2^20 (0: all N; rows behind them are padding) */
-  float scale;         /* of the logits, one over the temperature, up to 1e6 (0: 1) */
+  float scale;         /* of the logits, one over the temperature, up to 1e6 (0: 1). Below 1e-20 their f32 forms may underflow */
   int n_targets;       /* tokens asked for in each row, up to 1024 */
   const int* targets;  /* device [M][n_targets]; a number outside [0, n_vocab) gives NaN */
   int top_k;           /* largest tokens of each row, up to 64 and n_vocab */

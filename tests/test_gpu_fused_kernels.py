@@ -24,23 +24,21 @@ DEEP = [(1, 26, 1088, False), (2, 26, 1088, False), (5, 26, 1088, False), (5, 26
         (1000, 12290, 1152, False), (1100, 1998, 1152, False)]
 
 
+def in_formats(sizes):
+    return [(M, N, K, fmt, gated) for M, N, K, gated in sizes for fmt in FORMATS if K % fmt[1] == 0]
+
+
 def cases():
-    return [(M, N, K, fmt, gated) for fmt in FORMATS for M, N, K, gated in SHALLOW + DEEP if K % fmt[1] == 0]
+    return in_formats(SHALLOW + DEEP)
 
 
-@pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("M,N,K,gated", SHALLOW)
-def test_shallow(M, N, K, gated, fmt):
-    if K % fmt[1]:
-        pytest.skip("K is not whole groups")
+@pytest.mark.parametrize("M,N,K,fmt,gated", in_formats(SHALLOW))
+def test_shallow(M, N, K, fmt, gated):
     tf.run(M, N, K, fmt, act="silu" if gated else None, gated=gated, bias=True, residual=ha.F32, out=ha.F32, pad=3, inplace=True)
 
 
-@pytest.mark.parametrize("fmt", FORMATS)
-@pytest.mark.parametrize("M,N,K,gated", DEEP)
-def test_deep(M, N, K, gated, fmt):
-    if K % fmt[1]:
-        pytest.skip("K is not whole groups")
+@pytest.mark.parametrize("M,N,K,fmt,gated", in_formats(DEEP))
+def test_deep(M, N, K, fmt, gated):
     tf.run(M, N, K, fmt, act="gelu" if gated else None, gated=gated, out=ha.F32)
 
 

@@ -15,9 +15,10 @@ def some(M):
     return sorted({0, 1, M // 2 - 1, M // 2, M // 2 + 1, M - 17, M - 1})
 
 
-def test_product():
+@pytest.mark.parametrize("M", [98307, (1 << 17) + 5])  # (3.2 10^9 threads at once, and more than a launch holds)
+def test_product(M):
     import torch
-    M, N, K = (1 << 17) + 5, 65536, 96  # (K is not of 64: the general kernel, 512 threads for 16 x 64 results)
+    N, K = 65536, 96  # (K is not of 64: the general kernel, 512 threads for 16 x 64 results)
     words, s, b, W = fr.weight(N, K, seed=30)
     rng = np.random.default_rng(31)
     a = torch.from_numpy(rng.standard_normal((M, K)).astype(np.float16)).to(tf.DEV)
