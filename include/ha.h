@@ -278,10 +278,10 @@ typedef struct ha_logprobs {
    64 bits. So top_ids are the largest by their logits in 64 bits as long as at most 8 tokens behind the top_k (where no logits are stored, at
    most 8 blocks of 64 tokens behind the top_k largest blocks) come that near to the last of them, and no row of the table is many
    times larger than those that are found.
-   A row with a logit that is not finite gives NaN and top_ids of -1. The workspace (16-byte aligned device memory, as many bytes
-   as ha_mnb_logprobs_bytes says, which suffice for every call of up to M rows of the same n_vocab and top_k) is the caller's and overlaps neither a nor targets nor outputs: calls that may overlap need one
-   each. Outputs overlap neither a nor targets (refused; logp alone may be the targets' own memory) nor each other (what is written there last
-   stays). */
+   A row with a logit that is not finite gives NaN and top_ids of -1. The workspace is 16-byte aligned device memory, as many bytes
+   as ha_mnb_logprobs_bytes says, which suffice for every call of up to M rows of the same n_vocab and top_k. It is the caller's and
+   overlaps neither a nor targets nor outputs: calls that may overlap need one each. Outputs overlap neither a nor targets (refused;
+   logp alone may be the targets' own memory) nor each other (what is written there last stays). */
 int ha_mnb_logprobs_bytes(const ha_mnb* w, int M, const ha_logprobs* p, size_t* bytes);
 int ha_mnb_logprobs(ha_mnb* w, int M, const void* a, const ha_logprobs* p, void* workspace, size_t bytes, void* stream);
 
